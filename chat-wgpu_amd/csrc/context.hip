@@ -269,6 +269,7 @@ int cw_ctx_destroy(cw_ctx *ctx) {
         (void)hipFree(t.cos_t);
         (void)hipFree(t.sin_t);
     }
+    for (auto &t : ctx->rope_turns) (void)hipFree(t.turns);
     for (hipEvent_t e : ctx->event_pool) (void)hipEventDestroy(e);
     (void)hipStreamDestroy(ctx->stream);
     delete ctx;

@@ -119,6 +119,13 @@ struct cw_ctx {
     // RoPE tables; a deque, so a table's address stays valid as others are added
     std::deque<cw_rope_tab> ropes;
 
+    // frequencies of cw_rope_spec's, one device table each (paged.hip)
+    struct RopeTurns {
+        cw_rope_spec spec;
+        double *turns;
+    };
+    std::deque<RopeTurns> rope_turns;
+
     // a cw_graph_begin .. cw_graph_end recording is open on the stream
     bool capturing = false;
 

@@ -56,6 +56,29 @@ class ModelConfig(C.Structure):
                 ("max_seq", _I), ("kv_dtype", _I)]
 
 
+# rotary layouts and scalings, block-table status bits (include/chat_wgpu.h)
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN, ROPE_BANDS = 0, 1, 2, 3
+BLOCKS_BAD, BLOCKS_ROWS, BLOCKS_TABLE, BLOCKS_FREE = 1, 2, 4, 8
+
+
+class RopeSpec(C.Structure):
+    _fields_ = [("rot_dim", _I), ("layout", _I), ("scaling", _I), ("trained", _I),
+                ("theta", C.c_double), ("factor", C.c_double),
+                ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+                ("low_turns", C.c_double), ("high_turns", C.c_double), ("gain", C.c_double)]
+
+
+class KvPages(C.Structure):
+    _fields_ = [("k", _P), ("v", _P), ("kv_dtype", _I), ("n_kv_heads", _I), ("head_dim", _I),
+                ("page", _I), ("n_blocks", _I)]
+
+
+class Batch(C.Structure):
+    _fields_ = [("cached", _P), ("n_seq", _I), ("rows", _I), ("first_row", _P), ("tables", _P),
+                ("max_blocks", _I), ("mask", _P), ("mask_words", _I)]
+
+
 # name -> (restype, argtypes); every declaration of include/chat_wgpu.h
 _SIGS = {
     "cw_ctx_create": (_I, [_I, C.POINTER(_P)]),
@@ -89,6 +112,13 @@ _SIGS = {
     "cw_kv_write": (_I, [_P, _P, _P, _I, _I, _I, _P, _P]),
     "cw_embed": (_I, [_P, _P, _I, _I, _P, _P]),
     "cw_hbm_read_probe": (_I, [_P, _P, _SZ, _I, _P]),
+    "cw_rope_rows": (_I, [_P, C.POINTER(RopeSpec), _P, _SZ, _P, _I, _I, _I, _P, _SZ]),
+    "cw_rope_kv_rows": (_I, [_P, C.POINTER(RopeSpec), C.POINTER(KvPages), _P, _SZ, _P, _P, _I,
+                             _I, _P, _SZ]),
+    "cw_block_tables": (_I, [_P, C.POINTER(KvPages), C.POINTER(Batch), _P, _P, _P, _P, _P, _P,
+                             _P, _P, _P]),
+    "cw_attention_tree": (_I, [_P, C.POINTER(KvPages), C.POINTER(Batch), _P, _SZ, _I, _P, _SZ]),
+    "cw_kv_accept": (_I, [_P, C.POINTER(KvPages), C.POINTER(Batch), _P, _I, _P, _P]),
     "cw_q4_quantize": (_I, [_P, _SZ, _SZ, _P, _P]),
     "cw_q4_split_blocks": (_I, [_P, _SZ, _P, _P]),
     "cw_synth_key": (_U64, [_U64, C.c_char_p]),
@@ -165,6 +195,31 @@ def check(rc):
 
 def _ptr(a):
     return a.ctypes.data_as(_P) if isinstance(a, np.ndarray) else a
+
+
+# ---------------------------------------------------------------- a paged cache and its batch
+
+def rope_spec(rot_dim, theta, layout=ROPE_HALVES, scaling=ROPE_PLAIN, factor=1.0, trained=0,
+              beta_fast=32.0, beta_slow=1.0, low_turns=1.0, high_turns=4.0, gain=0.0):
+    return RopeSpec(rot_dim, layout, scaling, trained, theta, factor, beta_fast, beta_slow,
+                    low_turns, high_turns, gain)
+
+
+def _opt(a):
+    return a.ptr if a is not None else None
+
+
+def kv_pages(k, v, kv_dtype, n_kv_heads, head_dim, page, n_blocks):
+    """A cache of n_blocks blocks of `page` positions (k, v: device arrays
+    [n_blocks * page, n_kv_heads * head_dim])."""
+    return KvPages(_opt(k), _opt(v), kv_dtype, n_kv_heads, head_dim, page, n_blocks)
+
+
+def batch(cached, n_seq, rows, first_row, tables, max_blocks, mask=None, mask_words=0):
+    """The requests of a step (device arrays; first_row [n_seq + 1], tables
+    [n_seq, max_blocks] or None, mask [rows, mask_words] or None)."""
+    return Batch(_opt(cached), n_seq, rows, _opt(first_row), _opt(tables), max_blocks,
+                 _opt(mask), mask_words)
 
 
 # ---------------------------------------------------------------- host-side helpers
@@ -475,6 +530,45 @@ class Context:
         o = self.empty(dim)
         check(lib().cw_embed(self.h, table.ptr, vocab, dim, token_dev.ptr, o.ptr))
         return o
+
+    # ---- several requests in one paged cache
+    def rope_rows(self, spec, x, positions, rows, heads, head_dim, x_stride=None, y=None,
+                  y_stride=None):
+        width = heads * head_dim
+        y = y if y is not None else self.empty((rows, width))
+        check(lib().cw_rope_rows(self.h, spec, x.ptr, x_stride or width, positions.ptr, rows,
+                                 heads, head_dim, y.ptr, y_stride or width))
+        return y
+
+    def rope_kv_rows(self, spec, kv, qkv, positions, slots, rows, n_heads, stride=None,
+                     q_out=None, q_stride=None):
+        width = n_heads * kv.head_dim
+        if q_out is None and n_heads:
+            q_out = self.empty((rows, width))
+        check(lib().cw_rope_kv_rows(self.h, spec, kv, qkv.ptr,
+                                    stride or width + 2 * kv.n_kv_heads * kv.head_dim,
+                                    positions.ptr, slots.ptr, rows, n_heads, _opt(q_out),
+                                    q_stride or width))
+        return q_out
+
+    def block_tables(self, kv, batch, fresh, held, held_out, free_list, n_free, n_free_out,
+                     positions, slots, status):
+        """Fills batch's first_row and tables, positions and slots; status
+        holds BLOCKS_* bits (device arrays, all int32)."""
+        check(lib().cw_block_tables(self.h, kv, batch, fresh.ptr, held.ptr, held_out.ptr,
+                                    free_list.ptr, n_free.ptr, n_free_out.ptr, positions.ptr,
+                                    slots.ptr, status.ptr))
+
+    def attention_tree(self, kv, batch, q, n_heads, q_stride=None, out=None, out_stride=None):
+        width = n_heads * kv.head_dim
+        out = out if out is not None else self.empty((batch.rows, width))
+        check(lib().cw_attention_tree(self.h, kv, batch, q.ptr, q_stride or width, n_heads,
+                                      out.ptr, out_stride or width))
+        return out
+
+    def kv_accept(self, kv, batch, path, max_path, path_len, cached_out=None):
+        check(lib().cw_kv_accept(self.h, kv, batch, path.ptr, max_path, path_len.ptr,
+                                 _opt(cached_out)))
 
     def graph_begin(self):
         """Record the following launches (cw_graph_begin)."""

@@ -170,6 +170,137 @@ int cw_q4_gemm(cw_ctx *ctx, const float *x, int m, const uint16_t *scales, const
                int in_f, int out_f, float *y);
 
 /* ---------------------------------------------------------------- */
+/* Several requests in one paged KV cache, with drafted tokens.  No     */
+/* counterpart in the reference, which runs one request over one cache. */
+/*                                                                    */
+/* A step of such a server: cw_block_tables gives every new row (token) */
+/* its request, position and cache slot; per layer cw_rope_kv_rows      */
+/* writes the rows' K and V there and cw_attention_tree attends; once   */
+/* drafted tokens are verified, cw_kv_accept moves the accepted path's  */
+/* rows to the positions that follow the cached ones.  Lengths, tables, */
+/* positions and masks are device arrays, read when a kernel runs: the  */
+/* same calls can be recorded (cw_graph_begin) and replayed as they     */
+/* change.  Device values are checked on the device: a row, slot, block */
+/* or request out of its range is left out, never read or written       */
+/* (which result says so is stated below).                              */
+/* ---------------------------------------------------------------- */
+
+/* which elements of a head form a rotated pair */
+#define CW_ROPE_HALVES 0  /* i and i + rot_dim/2 (cw_rope's) */
+#define CW_ROPE_PAIRS 1   /* 2i and 2i + 1 */
+/* how the frequencies f_i = theta^(-2i/rot_dim) are scaled for contexts
+ * `factor` times the trained length */
+#define CW_ROPE_PLAIN 0
+#define CW_ROPE_LINEAR 1  /* f / factor */
+#define CW_ROPE_YARN 2    /* f / factor * r + f * (1 - r): r rises from 0 at the pair that turns
+                             beta_fast times over the trained length to 1 at beta_slow (pair
+                             numbers rounded outwards); cos and sin times `gain` */
+#define CW_ROPE_BANDS 3   /* pairs of at most low_turns over the trained length: f / factor, of
+                             high_turns or more: f, linear in the turns between */
+
+typedef struct cw_rope_spec {
+    int rot_dim;  /* leading elements of a head that are rotated (even); the others are copied */
+    int layout;   /* CW_ROPE_HALVES or CW_ROPE_PAIRS */
+    int scaling;  /* CW_ROPE_PLAIN, _LINEAR, _YARN or _BANDS; what it does not use is ignored */
+    int trained;  /* positions the model was trained on (yarn, bands) */
+    double theta;
+    double factor;
+    double beta_fast, beta_slow;  /* yarn */
+    double low_turns, high_turns; /* bands */
+    double gain;                  /* yarn: 0 stands for 0.1 ln(factor) + 1 */
+} cw_rope_spec;
+
+/* A cache of n_blocks blocks of `page` positions; slot s is row s of k and of
+ * v, block s / page.  With block tables page is a power of two from 16 on;
+ * without (tables NULL in cw_batch) request b owns the slots b*page ..
+ * b*page + page - 1, for any page.  At most 2^31 - 1 slots. */
+typedef struct cw_kv_pages {
+    void *k, *v;   /* [n_blocks*page][n_kv_heads*head_dim], 16-byte aligned */
+    int kv_dtype;  /* CW_F32 or CW_F16 */
+    int n_kv_heads, head_dim; /* head_dim in {16,32,64,128,256} */
+    int page, n_blocks;
+} cw_kv_pages;
+
+/* The requests of a step.  Request b has cached[b] positions in the cache and
+ * the rows first_row[b] .. first_row[b+1]-1; row i of them (its node i) has
+ * its K and V at position cached[b] + i.  rows is the arrays' capacity: rows
+ * behind first_row[n_seq] belong to nobody and are left as they are.
+ * A request whose row range, length or cached count is out of range has no rows. */
+typedef struct cw_batch {
+    const int *cached;     /* [n_seq] */
+    int n_seq, rows;
+    int *first_row;        /* [n_seq+1] */
+    int *tables;           /* [n_seq][max_blocks]: block of positions j*page .. or NULL */
+    int max_blocks;
+    const uint32_t *mask;  /* [rows][mask_words]: bit j of a row: it sees its request's node j.
+                              Nodes behind the last bit are not seen.  NULL: every node sees
+                              itself and the nodes before it */
+    int mask_words;
+} cw_batch;
+
+/* Rotary positions for rows of their own positions: y[r][h] = x[r][h] rotated
+ * at positions[r], row r of x at x + r*x_stride floats, its heads contiguous.
+ * Angles are evaluated in f64 for any position (int32).  A row of a negative
+ * position is padding: not written.  y may be x with the same stride (in
+ * place); otherwise the rows must not overlap.  head_dim at most 256. */
+int cw_rope_rows(cw_ctx *ctx, const cw_rope_spec *spec, const float *x, size_t x_stride,
+                 const int *positions, int rows, int heads, int head_dim, float *y,
+                 size_t y_stride);
+/* Rows of [q | k | v] (n_heads*head_dim, then twice n_kv_heads*head_dim floats,
+ * `stride` apart): q rotated into q_out (n_heads*head_dim floats, q_stride
+ * apart; q_out may be qkv with the same stride), k rotated and v as it is
+ * into the cache row slots[r], rounded to nearest even for CW_F16.  n_heads 0
+ * (q_out NULL) writes the cache alone.  A row of a negative position is
+ * padding; one whose slot is not in the cache only has its q rotated.  Slots
+ * of a call are distinct. */
+int cw_rope_kv_rows(cw_ctx *ctx, const cw_rope_spec *spec, const cw_kv_pages *kv,
+                    const float *qkv, size_t stride, const int *positions, const int *slots,
+                    int rows, int n_heads, float *q_out, size_t q_stride);
+
+/* bits of cw_block_tables's status */
+#define CW_BLOCKS_BAD 1    /* a length, held count or free count out of its range */
+#define CW_BLOCKS_ROWS 2   /* more new rows than b->rows */
+#define CW_BLOCKS_TABLE 4  /* a request needs more than max_blocks blocks */
+#define CW_BLOCKS_FREE 8   /* the free list is too short */
+/* Blocks, positions and slots of a step's new rows from the requests' lengths.
+ * Request b adds fresh[b] >= 0 rows to its cached[b] positions; fresh[b] < 0:
+ * it has ended, and its held[b] blocks return to the free list.  free_list
+ * [n_blocks] holds n_free[0] free blocks; returned ones are put behind them in
+ * request order, needed ones taken from the end, again in request order
+ * (max(0, ceil((cached+fresh)/page) - held) for each, entered in tables from
+ * entry held[b] on).  Of kv only page and n_blocks are used.  Writes held_out,
+ * n_free_out (which may be held and n_free), b->first_row and, for every row
+ * up to b->rows, positions (cached + i; with a mask cached + the number of
+ * nodes row i sees - 1, the depth of a tree's node) and slots, -1 both for
+ * rows behind the last request's.  status[0] = 0; or CW_BLOCKS_* bits (only
+ * _BAD if that is one): then no block changes hands, held_out and n_free_out
+ * repeat held and n_free, and there are no rows (first_row 0, the rest -1).
+ * An entry of tables or free_list that is no block gives slot -1. */
+int cw_block_tables(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const int *fresh,
+                    const int *held, int *held_out, int *free_list, const int *n_free,
+                    int *n_free_out, int *positions, int *slots, int *status);
+/* Attention of every row over its request's cached positions and the nodes of
+ * its request that its mask shows: out[r][h] = sum_p softmax_p(q.k_p /
+ * sqrt(head_dim)) v_p, kv head h / (n_heads / n_kv_heads), rows of q and out
+ * q_stride and out_stride floats apart (multiples of 4, 16-byte aligned).
+ * K and V of positions that a row does not see do not reach it, whatever they
+ * hold.  A row that sees nothing (or only scores of -inf) gives zeros; the
+ * rows of a request with positions whose block is not in the cache give NaN.
+ * cached[b] + rows of b is at most 2^30.  out must not overlap q.  Covers a
+ * decode step (one row each, mask NULL), pieces of prompts (mask NULL) and
+ * trees of drafted tokens. */
+int cw_attention_tree(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const float *q,
+                      size_t q_stride, int n_heads, float *out, size_t out_stride);
+/* Keeps the accepted nodes of each request: for i < path_len[b] the K and V of
+ * node path[b*max_path + i] (increasing in i) move to position cached[b] + i,
+ * and cached_out[b] = cached[b] + path_len[b] (NULL: not wanted; it must not
+ * be b->cached).  Of b only cached, n_seq, tables and max_blocks are used.  A
+ * path_len outside 0 .. max_path counts as the nearer of the two; a move from
+ * or to a position that has no block is left out. */
+int cw_kv_accept(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const int *path,
+                 int max_path, const int *path_len, int *cached_out);
+
+/* ---------------------------------------------------------------- */
 /* Host-side Q4 helpers                                              */
 /* ---------------------------------------------------------------- */
 
