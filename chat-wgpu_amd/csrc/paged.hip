@@ -508,7 +508,7 @@ int cw_rope_rows(cw_ctx *ctx, const cw_rope_spec *spec, const float *x, size_t x
     const bool in_place = x == y && x_stride == y_stride;
     CW_CHECK_ARG(in_place || rows_apart(rows, x, x_stride, width, y, y_stride, width),
                  "cw_rope_rows: rows of x and y overlap");
-    DeviceGuard guard(ctx->device);
+    CW_HIP(hipSetDevice(ctx->device));
     RopeArgs a{};
     CW_TRY(ctx_rope_turns(ctx, "cw_rope_rows", *spec, &a.turns));
     a.gain = spec_gain(*spec);
@@ -549,7 +549,7 @@ int cw_rope_kv_rows(cw_ctx *ctx, const cw_rope_spec *spec, const cw_kv_pages *kv
     CW_CHECK_ARG(!n_heads || in_place ||
                      rows_apart(rows, qkv, stride, width, q_out, q_stride, q_width),
                  "cw_rope_kv_rows: rows of qkv and q_out overlap");
-    DeviceGuard guard(ctx->device);
+    CW_HIP(hipSetDevice(ctx->device));
     RopeArgs a{};
     CW_TRY(ctx_rope_turns(ctx, "cw_rope_kv_rows", *spec, &a.turns));
     a.gain = spec_gain(*spec);
@@ -586,7 +586,7 @@ int cw_block_tables(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const
     CW_TRY(check_pages("cw_block_tables", kv, b, false, &map));
     CW_CHECK_ARG(b->rows > 0 && b->rows <= kMaxRows, "cw_block_tables: rows=%d (1 .. 2^23)", b->rows);
     CW_CHECK_ARG(!b->mask || b->mask_words > 0, "cw_block_tables: mask_words=%d", b->mask_words);
-    DeviceGuard guard(ctx->device);
+    CW_HIP(hipSetDevice(ctx->device));
     const size_t n = (size_t)b->n_seq + 1;
     void *scratch = nullptr;
     CW_TRY(ctx_scratch(ctx, 3 * n * sizeof(int), &scratch));
@@ -609,7 +609,7 @@ int cw_kv_accept(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const in
     PageMap map;
     CW_TRY(check_pages("cw_kv_accept", kv, b, true, &map));
     CW_CHECK_ARG(cached_out != b->cached, "cw_kv_accept: cached_out is cached");
-    DeviceGuard guard(ctx->device);
+    CW_HIP(hipSetDevice(ctx->device));
     const int row_u4 = kv->n_kv_heads * kv->head_dim * (kv->kv_dtype == CW_F16 ? 2 : 4) / 16;
     const dim3 grid((2 * row_u4 + kThreads - 1) / kThreads, b->n_seq);
     return launch(ctx, "kv_accept", accept_kernel, grid, dim3(kThreads), 0, map,

@@ -47,19 +47,4 @@ __device__ __forceinline__ SeqRows seq_rows(const int *first_row, const int *cac
     return SeqRows{ok ? r0 : 0, ok ? r1 - r0 : 0, ok ? c : 0};
 }
 
-// The context's device as the current one for the time of a call.
-struct DeviceGuard {
-    int old = -1;
-    explicit DeviceGuard(int device) {
-        int d = 0;
-        if (hipGetDevice(&d) == hipSuccess && d != device && hipSetDevice(device) == hipSuccess)
-            old = d;
-    }
-    ~DeviceGuard() {
-        if (old >= 0) (void)hipSetDevice(old);
-    }
-    DeviceGuard(const DeviceGuard &) = delete;
-    DeviceGuard &operator=(const DeviceGuard &) = delete;
-};
-
 }  // namespace cwi

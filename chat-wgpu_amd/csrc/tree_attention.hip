@@ -136,7 +136,7 @@ extern "C" int cw_attention_tree(cw_ctx *ctx, const cw_kv_pages *kv, const cw_ba
                  "cw_attention_tree: q and out must be 16-byte aligned");
     CW_CHECK_ARG(rows_apart(b->rows, q, q_stride, width, out, out_stride, width),
                  "cw_attention_tree: rows of q and out overlap");
-    DeviceGuard guard(ctx->device);
+    CW_HIP(hipSetDevice(ctx->device));
     TreeArgs a{q, q_stride, out, out_stride, kv->k, kv->v, map, b->first_row, b->cached, b->n_seq,
                b->rows, b->mask, b->mask_words, n_heads, kv->n_kv_heads,
                (float)(1.4426950408889634 / std::sqrt((double)kv->head_dim))};

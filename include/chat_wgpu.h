@@ -182,7 +182,8 @@ int cw_q4_gemm(cw_ctx *ctx, const float *x, int m, const uint16_t *scales, const
 /* same calls can be recorded (cw_graph_begin) and replayed as they     */
 /* change.  Device values are checked on the device: a row, slot, block */
 /* or request out of its range is left out, never read or written       */
-/* (which result says so is stated below).                              */
+/* (which result says so is stated below).  The calls leave the context's */
+/* device current, as cw_ctx_create does.                               */
 /* ---------------------------------------------------------------- */
 
 /* which elements of a head form a rotated pair */
