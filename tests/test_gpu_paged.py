@@ -380,6 +380,13 @@ SHAPES = [
     ([257], [130], 2, 2, 64, 256), ([33, 120], [20, 1], 4, 2, 256, 16),
     ([0, 70], [65, 2], 5, 5, 256, 32), ([18, 3, 200], [7, 1, 30], 4, 2, 16, 16),
     ([50, 129], [33, 2], 3, 1, 32, 64), ([1000, 1, 400, 0, 64], [1, 1, 1, 1, 1], 32, 8, 128, 64),
+    # more tiles than workgroups: runs over several requests and heads
+    ([1300, 700, 0, 999, 64, 411, 1280, 850, 37, 600], [1, 3, 2, 1, 5, 4, 1, 2, 3, 1], 16, 8, 128,
+     32),
+    ([500, 800, 300, 1000, 64, 640], [7, 6, 8, 7, 5, 9], 32, 8, 128, 64),
+    ([900, 1300, 250, 700, 1100, 30], [20, 9, 33, 14, 25, 40], 16, 8, 128, 16),
+    ([1500, 800], [61, 40], 32, 8, 128, 16), ([2000, 1500], [40, 9], 8, 8, 64, 32),
+    ([1000, 1200, 500], [6, 2, 9], 16, 8, 256, 16),
 ]
 
 
