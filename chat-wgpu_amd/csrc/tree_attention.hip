@@ -6,6 +6,7 @@
 // its mask shows.
 
 #include <cmath>
+#include <type_traits>
 
 #include "paged_device.hpp"
 #include "prompt_device.hpp"
@@ -137,79 +138,17 @@ __global__ __launch_bounds__(kThreads) void tree_row_kernel(TreeArgs a) {
 // A[li][8 lg + j], B[8 lg + j][li]; 16x16x16 f16 A[li][4 lg + j], B[4 lg + j][li];
 // 16x16x4 f32 A[li][lg], B[lg][li]; all D[4 lg + r][li].
 
-// KT positions a tile, QT tiles of 16 rows a wave.  SPLIT: the four waves share
-// the rows and take 16 of the tile's 64 positions each; else they share the
-// positions and take 16 QT rows each.
-template <typename KVT, int HD_, int QT_, bool SPLIT_>
-struct TC {
-    static constexpr int HD = HD_, QT = QT_, ES = (int)sizeof(KVT);
-    static constexpr bool SPLIT = SPLIT_, F16 = ES == 2;
-    static constexpr int ROWB = HD * ES;    // bytes of a row of one kv head
-    static constexpr int CPR = ROWB / 16;   // 16-byte chunks of it
-    static constexpr int SWZ = CPR < 16 ? CPR - 1 : 15;
-    static constexpr int KT = SPLIT || ROWB <= 256 ? 64 : 32;
-    static constexpr int TILE = KT * ROWB;  // bytes of a K (or V) tile
-    static constexpr int GROUPB = 16 * ROWB;
-    static constexpr int ST = SPLIT ? 1 : KT / 16;       // score tiles of a wave
-    static constexpr int RT = 16 * QT * (SPLIT ? 1 : 4); // rows of a workgroup
-    static constexpr int NU = ROWB / 64;                 // DMAs of 16 rows
-    static constexpr int GPW = 2 * KT / 64;              // groups of 16 rows a wave loads a tile
-    static constexpr int NLD = GPW * NU;                 // DMAs a wave issues a tile
-    static constexpr int LDS = 4 * TILE;                 // two buffers of K and V
-    static constexpr float UP = F16 ? 15.0f : 0.0f;
-    static_assert(!SPLIT || 4 * RT * HD * 4 <= LDS, "the waves' o must fit the tiles");
-    static_assert(LDS + 4096 <= 160 * 1024, "tiles must fit a CU");
-};
-
-// The units of a request: a unit is one tile of positions for one row block of
-// one kv head; a request's are ordered (kv head, row block, tile).
-struct Work {
-    int tiles, blocks;
-    long long units;
-};
-__device__ __forceinline__ Work work_of(const SeqRows &s, int group, int n_kv, int kt, int rt) {
-    if (!s.n) return Work{0, 0, 0};
-    const int t = (s.cached + s.n + kt - 1) / kt, rb = (int)(((long long)s.n * group + rt - 1) / rt);
-    return Work{t, rb, (long long)n_kv * rb * t};
-}
-
-__device__ __forceinline__ long long wave_scan(long long v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-
-// All units are dealt to `wgs` workgroups in runs of q or q + 1.
-struct Deal {
-    long long q;
-    int rem;
-    __device__ Deal(long long units, int wgs) {
-        q = units / wgs;
-        rem = (int)(units - q * wgs);
-    }
-    __device__ long long start(int w) const { return q * w + min(w, rem); }
-    __device__ int owner(long long u) const {
-        const long long big = (q + 1) * rem;
-        return u < big ? (int)(u / (q + 1)) : rem + (int)((u - big) / q);
-    }
-};
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ long long uniform(long long v) {
     return (long long)(uint32_t)uniform((int)v) | (long long)uniform((int)(v >> 32)) << 32;
 }
-
 __device__ __forceinline__ SeqRows uniform(SeqRows s) {
     return SeqRows{uniform(s.r0), uniform(s.n), uniform(s.cached)};
 }
-
-typedef const __attribute__((address_space(4))) int *const_i32;
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 template <int N>
 __device__ __forceinline__ void wait_vm() {
@@ -231,346 +170,737 @@ __device__ __forceinline__ void lds_barrier() {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
+// Over the lanes li, li + 16, li + 32, li + 48: a row of the transposed products.
+// (Elements of a vector are copied before a bit cast: of the element itself it
+// would take the vector's first.)
+template <typename F>
+__device__ __forceinline__ float over_groups(float v, F f) {
+    const uint32_t v0 = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(v0, v0, false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    const uint32_t v1 = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+    const auto b = __builtin_amdgcn_permlane32_swap(v1, v1, false, false);
+    const uint32_t b0 = b[0], b1 = b[1];
+    v = f(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+    // keeps the swaps here: moved into a branch that fewer lanes take they
+    // would swap with none
+    asm volatile("" : "+v"(v));
+    return v;
+}
+__device__ __forceinline__ float group_max(float v) {
+    return over_groups(v, [](float x, float y) { return fmaxf(x, y); });
+}
+__device__ __forceinline__ float group_sum(float v) {
+    return over_groups(v, [](float x, float y) { return x + y; });
+}
+
 // v = hi + lo in f16 (22 bits)
 __device__ __forceinline__ void split_f16(float v, _Float16 &hi, _Float16 &lo) {
     hi = (_Float16)v;
     lo = (_Float16)(v - (float)hi);
 }
 
-template <typename KVT, int HD, int QT, bool SPLIT>
-__global__ __launch_bounds__(256, (TC<KVT, HD, QT, SPLIT>::LDS <= 72 * 1024 ? 2 : 1)) void tree_kernel(TreeArgs a) {
-    using C = TC<KVT, HD, QT, SPLIT>;
-    constexpr int KT = C::KT, ST = C::ST, RT = C::RT, ROWB = C::ROWB, DT = HD / 16;
-    constexpr bool F16 = C::F16;
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
-    __shared__ float w_ml[SPLIT ? 4 : 1][SPLIT ? RT : 1][2];
-    __shared__ int bad_seg;
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const int li = lane & 15, lg = lane >> 4;
-    const int group = a.n_heads / a.n_kv;
-    const size_t row_b = (size_t)a.n_kv * ROWB;
+// ---- who does what.  A unit is one tile of kt positions for one block of rt
+// rows (a row: a node and one of its query heads) of one kv head; the units of
+// a request are ordered (kv head, row block, tile), all of them dealt to the
+// workgroups in runs of q or q + 1, so that requests of any lengths share the
+// chip evenly.  A run's piece of a (kv head, row block) is a segment; what no
+// workgroup has whole is joined by tree_merge_kernel.
 
-    // the units of all requests, and the request where this workgroup begins
-    auto lane_units = [&](int b) {
+struct Work {
+    int tiles, blocks;
+    long long units;
+};
+__device__ __forceinline__ Work work_of(const SeqRows &s, int group, int n_kv, int kt, int rt) {
+    if (!s.n) return Work{0, 0, 0};
+    const int t = (s.cached + s.n + kt - 1) / kt, rb = (int)(((long long)s.n * group + rt - 1) / rt);
+    return Work{t, rb, (long long)n_kv * rb * t};
+}
+
+__device__ __forceinline__ long long wave_scan(long long v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+struct Deal {
+    long long q;
+    int rem;
+    __device__ Deal(long long units, int wgs) {
+        q = units / wgs;
+        rem = (int)(units - q * wgs);
+    }
+    __device__ long long start(int w) const { return q * w + min(w, rem); }
+    __device__ int owner(long long u) const {
+        const long long big = (q + 1) * rem;
+        return u < big ? (int)(u / (q + 1)) : rem + (int)((u - big) / q);
+    }
+};
+
+// A segment, and where the next one begins
+struct Seg {
+    SeqRows s;
+    int b, h, rb, t0, t1, nrows, last, part;  // part: its place among the partials
+    bool whole, lost;                         // lost: positions that no table entry covers
+};
+struct Cursor {
+    long long u, end, base;  // next unit, end of the run, first unit of request b
+    int b;
+};
+
+// The workgroup's run
+template <int KT, int RT>
+__device__ __forceinline__ Cursor first_unit(const TreeArgs &a, int group, int lane) {
+    auto units = [&](int b) {
         return b < a.n_seq ? work_of(seq_rows(a.first_row, a.cached, a.rows, b), group, a.n_kv, KT,
                                      RT).units : 0;
     };
-    long long total = 0;
-    for (int b = 0; b < a.n_seq; b += 64) total += __shfl(wave_scan(lane_units(b + lane), lane), 63);
-    total = uniform(total);
-    const Deal deal(total, a.wgs);
-    const long long u_end = deal.start(blockIdx.x + 1);
-    long long u = deal.start(blockIdx.x);
-    if (u >= u_end) return;
-    int b = 0;
-    long long base = 0;
-    for (int c = 0; c < a.n_seq; c += 64) {
-        const long long v = lane_units(c + lane), inc = wave_scan(v, lane) + base;
-        const unsigned long long hit = __ballot(inc > u);
+    const long long v0 = units(lane), inc0 = wave_scan(v0, lane);
+    long long total = __shfl(inc0, 63);
+    for (int c = 64; c < a.n_seq; c += 64) total += __shfl(wave_scan(units(c + lane), lane), 63);
+    const Deal deal(uniform(total), a.wgs);
+    Cursor cur{deal.start(blockIdx.x), deal.start(blockIdx.x + 1), 0, 0};
+    if (cur.u >= cur.end) return cur;
+    long long v = v0, inc = inc0;
+    for (int c = 0;;) {
+        const unsigned long long hit = __ballot(inc > cur.u);
         if (hit) {
             const int at = __ffsll((long long)hit) - 1;
-            b = uniform(c + at);
-            base = uniform(__shfl(inc - v, at));
-            break;
+            cur.b = c + at;
+            cur.base = uniform(__shfl(inc - v, at));
+            return cur;
         }
-        base = uniform(__shfl(inc, 63));
+        const long long before = __shfl(inc, 63);
+        c += 64;
+        if (c >= a.n_seq) break;
+        v = units(c + lane);
+        inc = wave_scan(v, lane) + before;
     }
+    cur.end = cur.u;  // (not reached: u is below the total)
+    return cur;
+}
 
-    if (tid == 0) bad_seg = 0;
-    int seg = 0;
-    while (u < u_end && b < a.n_seq) {
-        const SeqRows s = uniform(seq_rows(a.first_row, a.cached, a.rows, b));
-        const Work wk = work_of(s, group, a.n_kv, KT, RT);
-        if (u >= base + wk.units) {  // (requests without rows have no units)
-            base += wk.units;
-            ++b;
+template <int KT, int RT>
+__device__ __forceinline__ bool next_segment(const TreeArgs &a, int group, Cursor &cur, Seg &g) {
+    while (cur.u < cur.end && cur.b < a.n_seq) {
+        g.s = uniform(seq_rows(a.first_row, a.cached, a.rows, cur.b));
+        const Work wk = work_of(g.s, group, a.n_kv, KT, RT);
+        if (cur.u >= cur.base + wk.units) {
+            cur.base += wk.units;
+            ++cur.b;
             continue;
         }
-        ++seg;
-        const long long local = u - base;
-        const int hr = uniform((int)(local / wk.tiles)), t0 = uniform((int)(local - (long long)hr * wk.tiles));
-        const int t1 = (int)min((long long)wk.tiles, t0 + (u_end - u));
-        const int h = uniform(hr / wk.blocks), rb = hr - h * wk.blocks;
-        const bool whole = t0 == 0 && t1 == wk.tiles;
-        const int slot_part = blockIdx.x * 2 + (t0 > 0 ? 0 : 1);
-        u += t1 - t0;
-        const int last = s.cached + s.n - 1, nrows = s.n * group;
-        const char *const kc = static_cast<const char *>(a.kc) + (size_t)h * ROWB;
-        const char *const vc = static_cast<const char *>(a.vc) + (size_t)h * ROWB;
-        lds_barrier();  // the last segment's reads of LDS are done, bad_seg is set up
+        const long long local = cur.u - cur.base;
+        const int hr = uniform((int)(local / wk.tiles));
+        g.b = cur.b;
+        g.t0 = uniform((int)(local - (long long)hr * wk.tiles));
+        g.t1 = uniform((int)min((long long)wk.tiles, g.t0 + (cur.end - cur.u)));
+        g.h = uniform(hr / wk.blocks);
+        g.rb = uniform(hr - g.h * wk.blocks);
+        g.nrows = g.s.n * group;
+        g.last = g.s.cached + g.s.n - 1;
+        g.whole = g.t0 == 0 && g.t1 == wk.tiles;
+        g.part = blockIdx.x * 2 + (g.t0 > 0 ? 0 : 1);
+        g.lost = a.map.tables ? (g.last >> a.map.shift) >= a.map.max_blocks
+                              : g.b >= a.map.n_blocks || g.last >= a.map.page;
+        cur.u += g.t1 - g.t0;
+        return true;
+    }
+    return false;
+}
 
-        // first slot of the 16 positions of group gi; -1: they have no block
-        auto slot16 = [&](int gi) -> int {
-            const int p0 = min(gi, last >> 4) << 4;
-            bool bad;
-            int slot;
-            if (a.map.tables) {
-                const int e = p0 >> a.map.shift;
-                const const_i32 tab = (const_i32)(uintptr_t)(a.map.tables + (size_t)b * a.map.max_blocks);
-                const int id = tab[uniform(min(e, a.map.max_blocks - 1))];
-                bad = e >= a.map.max_blocks || (unsigned)id >= (unsigned)a.map.n_blocks;
-                slot = bad ? -1 : (id << a.map.shift) + (p0 & (a.map.page - 1));
-            } else {
-                bad = min(p0 + 15, last) >= a.map.page;
-                slot = bad ? -1 : b * a.map.page + p0;
-            }
-            if (bad && lane == 0) bad_seg = seg;
-            return uniform(slot);
-        };
-        // a wave's groups of a tile: K and V of group `wave`, or (32 positions)
-        // group wave % 2 of K or V
-        const int my_group = C::GPW == 2 ? wave : wave & 1;
-        auto load = [&](int t, int slot, unsigned char *buf) {
-            const int p0 = min(t * (KT / 16) + my_group, last >> 4) << 4;
-            const int rows = slot < 0 ? 0 : last - p0;  // (without a block: slot 0, results are NaN)
-            slot = max(slot, 0);
-#pragma unroll
-            for (int x = 0; x < C::GPW; ++x) {
-                const bool is_v = C::GPW == 2 ? x == 1 : wave >= 2;
-                const char *src = (is_v ? vc : kc) + (size_t)slot * row_b;
-                unsigned char *dst = buf + (is_v ? C::TILE : 0) + my_group * C::GROUPB;
-#pragma unroll
-                for (int n = 0; n < C::NU; ++n) {
-                    // chunk c of row r lies at slot c ^ (r & SWZ) of its row, so that
-                    // the fragment reads spread over the banks; rows behind the
-                    // last position repeat it
-                    const int r = n * (64 / C::CPR) + lane / C::CPR;
-                    const int c = (lane % C::CPR) ^ (r & C::SWZ);
-                    dma16(src, (uint32_t)min(r, rows) * (uint32_t)row_b + c * 16, dst + n * 1024);
-                }
-            }
-        };
-        const int per_tile = KT / 16;
-        int slot = slot16(t0 * per_tile + my_group);
-        load(t0, slot, lds);
-        slot = slot16((t0 + 1) * per_tile + my_group);
+// The first slot of the 16 positions of group gi of the request (a block holds
+// all 16); -1 where the table names no block
+__device__ __forceinline__ int slot16(const TreeArgs &a, const Seg &g, int gi) {
+    const int p0 = min(gi, g.last >> 4) << 4;
+    if (!a.map.tables) return g.b * a.map.page + p0;
+    const int id = a.map.tables[(size_t)g.b * a.map.max_blocks + (p0 >> a.map.shift)];
+    return (unsigned)id < (unsigned)a.map.n_blocks ? (id << a.map.shift) + (p0 & (a.map.page - 1)) : -1;
+}
 
-        // q of this lane's rows (B operands), as two f16 of q times a power of
-        // two that brings the row's largest below 2^15
-        const int w_row = rb * RT + (SPLIT ? 0 : wave * 16 * QT);
-        int node[QT], head[QT];
-        f16x8 qh[F16 ? QT : 1][HD / 32], ql[F16 ? QT : 1][HD / 32];
-        f32x4 qf[F16 ? 1 : QT][HD / 16];
-        float qs[QT];
+// Four elements of a row's result: the output where the segment has every
+// tile, else a partial
+template <int HD, int RT>
+__device__ __forceinline__ void put(const TreeArgs &a, const Seg &g, int group, int row, int col,
+                                    f32x4 v, float m, float l) {
+    if (g.whole) {
+        const int rr = g.rb * RT + row, node = rr / group;
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = l == 0.0f ? 0.0f : v[e] * f;
+        *reinterpret_cast<f32x4 *>(a.out + (size_t)(g.s.r0 + node) * a.out_stride +
+                                   (size_t)(g.h * group + rr - node * group) * HD + col) = v;
+    } else {
+        const size_t at = (size_t)g.part * RT + row;
+        *reinterpret_cast<f32x4 *>(a.part + at * HD + col) = v;
+        if (col == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(m, l);
+    }
+}
+
+// A segment whose nodes have a V that is no finite number: as 0 * V it would
+// reach rows that do not see it, so the products are taken one by one, a wave a
+// row, a lane HD / 64 elements.  (up: the tiles' weights carry 2^up.)
+template <typename KVT, int HD, int RT>
+__device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, float up) {
+    constexpr int E = HD / 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const KVT *kc = static_cast<const KVT *>(a.kc), *vc = static_cast<const KVT *>(a.vc);
+    for (int row = wave; row < RT && g.rb * RT + row < g.nrows; row += 4) {
+        const int rr = g.rb * RT + row, node = rr / group;
+        const size_t head = (size_t)(g.h * group + rr - node * group) * HD + lane * E;
+        float q[E], o[E] = {}, m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[e] = a.q[(size_t)(g.s.r0 + node) * a.q_stride + head + e];
+        for (int p = g.t0 * kt; p < min(g.t1 * kt, g.last + 1); ++p) {
+            const int slot = slot_of(a.map, g.b, p);
+            const int j = p - g.s.cached;
+            if (slot < 0 || (j >= 0 && !sees(a, g.s.r0 + node, node, j))) continue;
+            const size_t at = ((size_t)slot * a.n_kv + g.h) * HD + lane * E;
+            float d = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) d = __builtin_fmaf(q[e], (float)kc[at + e], d);
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) d += __shfl_xor(d, off);
+            d *= a.scale;
+            const float mn = fmaxf(m, d), ref = mn == -INFINITY ? 0.0f : mn;
+            const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(d - ref + up);
+            m = mn;
+            l = __builtin_fmaf(l, f, w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(o[e], f, w * (float)vc[at + e]);
+        }
+        const size_t part = (size_t)g.part * RT + row;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (g.whole)
+                a.out[(size_t)(g.s.r0 + node) * a.out_stride + head + e] = l == 0.0f ? 0.0f : o[e] / l;
+            else
+                a.part[part * HD + lane * E + e] = o[e];
+        }
+        if (!g.whole && lane == 0) *reinterpret_cast<float2 *>(a.ml + part * 2) = make_float2(m, l);
+    }
+}
+
+// whether one of the register's f16 pair, or its f32, is no finite number
+template <bool F16>
+__device__ __forceinline__ int not_finite(uint32_t w) {
+    constexpr uint32_t E = F16 ? 0x7c00u : 0x7f800000u;
+    return (int)((w & E) == E) | (int)(F16 && (w >> 16 & E) == E);
+}
+
+// ---- operands that both kernels read: rows of one kv head in LDS, 16-byte
+// chunk c of row r at slot c ^ (r & SWZ) of its row, so that the fragment reads
+// spread over the banks
+template <typename KVT, int HD_>
+struct Tile {
+    static constexpr int HD = HD_, ES = (int)sizeof(KVT);
+    static constexpr bool F16 = ES == 2;
+    static constexpr int ROWB = HD * ES, CPR = ROWB / 16;
+    static constexpr int SWZ = CPR < 16 ? CPR - 1 : 15;
+    static constexpr int GROUPB = 16 * ROWB;  // 16 positions
+    static constexpr int NU = ROWB / 64;      // DMAs of them
+    static constexpr int DT = HD / 16;        // 16 x 16 tiles of o^T
+    static constexpr int KS = F16 ? HD / 32 : HD / 16;  // 16-byte reads of a K fragment
+    // weights carry 2^UP (it cancels in o / sum), so that small ones keep their
+    // bits as f16 hi + lo: 22 bits down to 2^-18 of the largest
+    static constexpr float UP = F16 ? 15.0f : 0.0f;
+    typedef typename std::conditional<F16, f16x8, f32x4>::type frag;
+};
+
+// 16 positions of a kv head from slot `slot` on into LDS, 1 KB a DMA; rows
+// behind `rows` repeat it.  off: this lane's offsets where all 16 are there.
+template <typename T>
+__device__ __forceinline__ void dma_offsets(uint32_t (&off)[T::NU], uint32_t row_b, int lane) {
+#pragma unroll
+    for (int n = 0; n < T::NU; ++n) {
+        const int r = n * (64 / T::CPR) + lane / T::CPR;
+        off[n] = r * row_b + (((lane % T::CPR) ^ (r & T::SWZ)) << 4);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void dma_group(const char *src, unsigned char *dst, int rows,
+                                          const uint32_t (&off)[T::NU], uint32_t row_b, int lane) {
+    if (rows >= 15) {
+#pragma unroll
+        for (int n = 0; n < T::NU; ++n) dma16(src, off[n], dst + n * 1024);
+    } else {
+#pragma unroll
+        for (int n = 0; n < T::NU; ++n) {
+            const int r = n * (64 / T::CPR) + lane / T::CPR;
+            dma16(src, off[n] - (uint32_t)max(r - rows, 0) * row_b, dst + n * 1024);
+        }
+    }
+}
+
+// q of QT tiles of 16 rows (B operands): f16 as hi + lo of q times the power of
+// two that brings the row's largest to 2^14 .. 2^15, qs the scores' factor
+template <typename T, int QT>
+struct Query {
+    f16x8 hi[T::F16 ? QT : 1][T::F16 ? T::HD / 32 : 1], lo[T::F16 ? QT : 1][T::F16 ? T::HD / 32 : 1];
+    f32x4 f[T::F16 ? 1 : QT][T::F16 ? 1 : T::HD / 16];
+    float qs[QT];
+    int node[QT];
+
+    __device__ void load(const TreeArgs &a, const Seg &g, int group, int w_row, int li, int lg) {
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
-            const int rr = min(w_row + i * 16 + li, nrows - 1);
+            const int rr = min(w_row + i * 16 + li, g.nrows - 1);
             node[i] = rr / group;
-            head[i] = h * group + rr % group;
-            const float *qr = a.q + (size_t)(s.r0 + node[i]) * a.q_stride + (size_t)head[i] * HD;
+            const float *qr = a.q + (size_t)(g.s.r0 + node[i]) * a.q_stride +
+                              (size_t)(g.h * group + rr - node[i] * group) * T::HD;
             qs[i] = a.scale;
-            if constexpr (F16) {
-                f32x4 v[HD / 32][2];
+            if constexpr (T::F16) {
+                f32x4 v[T::HD / 32][2];
                 float mx = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < HD / 32; ++ks)
+                for (int ks = 0; ks < T::HD / 32; ++ks)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
+                    for (int x = 0; x < 2; ++x)
                         v[ks][x] = *reinterpret_cast<const f32x4 *>(qr + 32 * ks + 8 * lg + 4 * x);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fabsf(v[ks][x][j]));
-                    }
-                mx = fmaxf(mx, __shfl_xor(mx, 16));
-                mx = fmaxf(mx, __shfl_xor(mx, 32));
-                // mx in [2^(e-1), 2^e)
-                const int e = max(__builtin_amdgcn_frexp_expf(mx), -110);
+                for (int ks = 0; ks < T::HD / 32; ++ks)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(v[ks][j / 4][j % 4]));
+                mx = group_max(mx);
+                const int e = max(__builtin_amdgcn_frexp_expf(mx), -110);  // mx in [2^(e-1), 2^e)
                 const bool fin = mx > 0.0f && mx < INFINITY;
                 const float up = fin ? ldexpf(1.0f, 15 - e) : 1.0f;
                 qs[i] = fin ? ldexpf(a.scale, e - 15) : a.scale;
 #pragma unroll
-                for (int ks = 0; ks < HD / 32; ++ks)
+                for (int ks = 0; ks < T::HD / 32; ++ks)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        _Float16 hi, lo;
-                        split_f16(v[ks][j / 4][j % 4] * up, hi, lo);
-                        qh[i][ks][j] = hi;
-                        ql[i][ks][j] = lo;
+                        _Float16 h, l;
+                        split_f16(v[ks][j / 4][j % 4] * up, h, l);
+                        hi[i][ks][j] = h;
+                        lo[i][ks][j] = l;
                     }
             } else {
 #pragma unroll
-                for (int x = 0; x < HD / 16; ++x)
-                    qf[i][x] = *reinterpret_cast<const f32x4 *>(qr + 16 * x + 4 * lg);
+                for (int x = 0; x < T::HD / 16; ++x)
+                    f[i][x] = *reinterpret_cast<const f32x4 *>(qr + 16 * x + 4 * lg);
             }
         }
+    }
+};
 
-        f32x4 o[QT][DT];  // o^T: dims 16 d + 4 lg + r of row li
-        float mrow[QT], lsum[QT];
+// K fragment x of the 16 rows at Ks
+template <typename T>
+__device__ __forceinline__ typename T::frag k_frag(const unsigned char *Ks, int x, int li, int lg) {
+    return *reinterpret_cast<const typename T::frag *>(Ks + li * T::ROWB + (((4 * x + lg) ^ (li & T::SWZ)) << 4));
+}
+
+// s^T = K q^T of 16 positions, K's fragments in registers
+template <typename T, int QT>
+__device__ __forceinline__ f32x4 scores(const typename T::frag (&kf)[T::KS], const Query<T, QT> &q, int i) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f}, t = s;  // two chains
+    if constexpr (T::F16) {
+#pragma unroll
+        for (int x = 0; x < T::KS; ++x) {
+            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x], q.hi[i][x], s, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x], q.lo[i][x], t, 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < T::KS; ++x) {
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][0], q.f[i][x][0], s, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][1], q.f[i][x][1], t, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][2], q.f[i][x][2], s, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][3], q.f[i][x][3], t, 0, 0, 0);
+        }
+    }
+    return s + t;
+}
+
+// Running softmax of one row (this lane's: li) over N tiles of 16 scores, which
+// become the weights; returns the factor of what was summed before.
+template <int N>
+__device__ __forceinline__ float soften(f32x4 (&s)[N], float qs, float up, float &m, float &l) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[n][r]);
+    const float mnew = fmaxf(m, group_max(mx) * qs);
+    // a row that has seen nothing keeps -inf: its weights are 2^-inf = 0
+    const float ref = mnew == -INFINITY ? 0.0f : mnew;
+    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = mnew;
+    float ls = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], qs, up - ref));
+            ls += s[n][r];
+        }
+    l = l * alpha + ls;
+    return alpha;
+}
+
+// Element 4 col .. 4 col + 3 of row li of o^T, in registers as the products
+// leave it: f16 tile d has elements 16 d + 4 lg + r; f32 tile 4 c + e has
+// elements 64 c + 16 lg + 4 r + e (its V fragments are four elements wide)
+template <typename T>
+__device__ __forceinline__ f32x4 o_quad(const f32x4 (&o)[T::DT], int n) {
+    if constexpr (T::F16) return o[n];
+    const int c = n / 4 * 4, r = n % 4;
+    return f32x4{o[c][r], o[c + 1][r], o[c + 2][r], o[c + 3][r]};
+}
+template <typename T>
+__device__ __forceinline__ int o_col(int n, int lg) {
+    return T::F16 ? 16 * n + 4 * lg : n / 4 * 64 + 16 * lg + n % 4 * 4;
+}
+
+// ---- few rows of a kv head (at most 32): a workgroup's four waves share them
+// and take 16 of a tile's 64 positions each, through LDS of their own, so
+// nothing waits for another wave before the end of a segment.
+template <typename KVT, int HD, int QT>
+struct SplitCfg : Tile<KVT, HD> {
+    typedef Tile<KVT, HD> T;
+    static constexpr int KT = 64, RT = 16 * QT;
+    static constexpr int STAGE = 2 * T::GROUPB;  // K and V of a wave's 16 positions
+    static constexpr int LDS = 4 * 2 * STAGE;
+    static constexpr int PER_CU = LDS <= 72 * 1024 ? 2 : 1;
+    static_assert(4 * RT * HD * 4 <= LDS, "the waves' o must fit the stages");
+    static_assert(LDS + 4096 <= 160 * 1024, "stages must fit a CU");
+};
+
+template <typename KVT, int HD, int QT>
+__global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_split_kernel(TreeArgs a) {
+    using C = SplitCfg<KVT, HD, QT>;
+    using T = Tile<KVT, HD>;
+    constexpr int KT = C::KT, RT = C::RT, DT = T::DT;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
+    __shared__ float w_ml[4][RT][2];
+    __shared__ int w_odd[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int li = lane & 15, lg = lane >> 4;
+    const int group = a.n_heads / a.n_kv;
+    const uint32_t row_b = (uint32_t)a.n_kv * T::ROWB;
+    unsigned char *const mine = lds + wave * 2 * C::STAGE;
+    uint32_t off[T::NU];
+    dma_offsets<T>(off, row_b, lane);
+    Cursor cur = first_unit<KT, RT>(a, group, lane);
+    Seg g;
+    while (next_segment<KT, RT>(a, group, cur, g)) {
+        lds_barrier();  // the last segment's reads of LDS are done
+        const char *const kc = static_cast<const char *>(a.kc) + (size_t)g.h * T::ROWB;
+        const char *const vc = static_cast<const char *>(a.vc) + (size_t)g.h * T::ROWB;
+        bool bad = g.lost, odd = false;
+        int slots = 0, tb = g.t0;  // of this wave's positions of tile tb + lane
+        auto look_up = [&]() {
+            slots = slot16(a, g, (tb + lane) * 4 + wave);
+            bad |= __any(slots < 0 && tb + lane < g.t1);
+            slots = max(slots, 0);  // a block has 16 positions: in the cache, and the row is lost
+        };
+        auto load = [&](int t) {
+            const size_t at = (size_t)(uint32_t)__builtin_amdgcn_readlane(slots, t - tb) * row_b;
+            const int rows = g.last - (min(t * 4 + wave, g.last >> 4) << 4);
+            unsigned char *const dst = mine + (t & 1) * C::STAGE;
+            dma_group<T>(kc + at, dst, rows, off, row_b, lane);
+            dma_group<T>(vc + at, dst + T::GROUPB, rows, off, row_b, lane);
+        };
+        const int t1 = g.lost ? g.t0 : g.t1;
+        if (g.t0 < t1) {
+            look_up();
+            load(g.t0);
+        }
+        Query<T, QT> q;
+        q.load(a, g, group, g.rb * RT, li, lg);
+        f32x4 o[QT][DT];
+        float m[QT], l[QT];
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
-            mrow[i] = -INFINITY;
-            lsum[i] = 0.0f;
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        const int ka = li * ROWB + ((lg ^ (li & C::SWZ)) << 4);
-        const int vrow = 4 * lg + (li >> 2);
-        const int va = vrow * ROWB + ((((li & 3) >> 1) ^ (vrow & C::SWZ)) << 4) + (li & 1) * 8;
-
-        for (int t = t0; t < t1; ++t) {
-            unsigned char *const buf = lds + ((t - t0) & 1) * 2 * C::TILE;
-            unsigned char *const next = lds + ((t - t0 + 1) & 1) * 2 * C::TILE;
-            if constexpr (SPLIT) {
-                // each wave reads only what it loaded: no barrier
-                if (t + 1 < t1) {
-                    wait_lds();  // of the tile before, whose place this takes
-                    load(t + 1, slot, next);
-                    slot = slot16((t + 2) * per_tile + my_group);
-                    wait_vm<C::NLD>();
-                } else {
-                    wait_vm<0>();
+        for (int t = g.t0; t < t1; ++t) {
+            if (t + 1 < t1) {
+                if (t + 1 - tb == 64) {
+                    tb += 64;
+                    look_up();
                 }
+                wait_lds();  // reads of the tile before, whose place this takes
+                load(t + 1);
+                wait_vm<2 * T::NU>();
             } else {
                 wait_vm<0>();
-                lds_barrier();  // tile t is there, the other buffer free
-                if (t + 1 < t1) {
-                    load(t + 1, slot, next);
-                    slot = slot16((t + 2) * per_tile + my_group);
-                }
-                if (w_row >= nrows) continue;
             }
-            const int k0 = t * KT + (SPLIT ? wave * 16 : 0);  // this wave's first position
-            const unsigned char *const Ks = buf + (SPLIT ? wave * C::GROUPB : 0);
-            const unsigned char *const Vs = Ks + C::TILE;
-
-            f32x4 sc[QT][ST];
+            const unsigned char *const Ks = mine + (t & 1) * C::STAGE, *const Vs = Ks + T::GROUPB;
+            // every fragment is requested before the first is used
+            typename T::frag kf[T::KS];
 #pragma unroll
-            for (int kt = 0; kt < ST; ++kt) {
+            for (int x = 0; x < T::KS; ++x) kf[x] = k_frag<T>(Ks, x, li, lg);
+            f16x4 vh[T::F16 ? DT : 1];
+            f32x4 vf[T::F16 ? 1 : 4][T::F16 ? 1 : HD / 64];
+            if constexpr (T::F16) {
+                // V^T: within 16 lanes, lane i receives element i % 4 of the 8
+                // bytes at lane 4 j + i / 4's address: element 16 d + i of rows 4 lg + j
+                const int row = 4 * lg + (li >> 2), c = (li & 3) >> 1;
 #pragma unroll
-                for (int i = 0; i < QT; ++i) sc[i][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if constexpr (F16) {
+                for (int d = 0; d < DT; ++d)
+                    vh[d] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(
+                        Vs + row * T::ROWB + (((2 * d + c) ^ (row & T::SWZ)) << 4) + (li & 1) * 8)));
+            } else {
 #pragma unroll
-                    for (int ks = 0; ks < HD / 32; ++ks) {
-                        const f16x8 kf = *reinterpret_cast<const f16x8 *>(Ks + ((ka ^ (ks << 6)) + kt * C::GROUPB));
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int i = 0; i < QT; ++i)
-                            sc[i][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[i][ks], sc[i][kt], 0, 0, 0);
+                    for (int c = 0; c < HD / 64; ++c) {
+                        const int row = 4 * lg + r;
+                        vf[r][c] = *reinterpret_cast<const f32x4 *>(
+                            Vs + row * T::ROWB + (((16 * c + li) ^ (row & T::SWZ)) << 4));
+                    }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            f32x4 s[QT][1];
 #pragma unroll
-                        for (int i = 0; i < QT; ++i)
-                            sc[i][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[i][ks], sc[i][kt], 0, 0, 0);
+            for (int i = 0; i < QT; ++i) s[i][0] = scores<T, QT>(kf, q, i);
+            const int k0 = t * KT + wave * 16;
+            if (k0 + 16 > g.s.cached) {  // nodes: by the mask
+#pragma unroll
+                for (int i = 0; i < QT; ++i) {
+                    const uint32_t vis = sees4(a, g.s.r0 + q.node[i], q.node[i], g.s.n, k0 + 4 * lg - g.s.cached);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[i][0][r] = vis >> r & 1 ? s[i][0][r] : -INFINITY;
+                }
+                int x = 0;
+                if constexpr (T::F16) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        const uint2 w = __builtin_bit_cast(uint2, vh[d]);
+                        x |= not_finite<true>(w.x) | not_finite<true>(w.y);
                     }
                 } else {
 #pragma unroll
-                    for (int x = 0; x < HD / 16; ++x) {
-                        const f32x4 kf = *reinterpret_cast<const f32x4 *>(Ks + ((ka ^ (x << 6)) + kt * C::GROUPB));
+                    for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
+                        for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
-                            for (int i = 0; i < QT; ++i)
-                                sc[i][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[r], qf[i][x][r], sc[i][kt], 0, 0, 0);
-                    }
+                            for (int e = 0; e < 4; ++e) {
+                                const float w = vf[r][c][e];
+                                x |= not_finite<false>(__builtin_bit_cast(uint32_t, w));
+                            }
                 }
+                odd |= __any(x);
             }
-            // what a row sees: every cached position; of the nodes by the mask
-            const bool tail = k0 + 16 * ST > s.cached;
-            if (tail) {
-#pragma unroll
-                for (int i = 0; i < QT; ++i)
-#pragma unroll
-                    for (int kt = 0; kt < ST; ++kt) {
-                        const uint32_t vis = sees4(a, s.r0 + node[i], node[i], s.n,
-                                                   k0 + kt * 16 + 4 * lg - s.cached);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            sc[i][kt][r] = vis >> r & 1 ? sc[i][kt][r] : -INFINITY;
-                    }
-            }
-            float alpha[QT];
-            bool grew = false;
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
-                float mx = sc[i][0][0];
-#pragma unroll
-                for (int kt = 0; kt < ST; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[i][kt][r]);
-                mx = fmaxf(mx, __shfl_xor(mx, 16));
-                mx = fmaxf(mx, __shfl_xor(mx, 32));
-                const float mnew = fmaxf(mrow[i], mx * qs[i]);
-                const float ref = mnew == -INFINITY ? 0.0f : mnew;
-                alpha[i] = __builtin_amdgcn_exp2f(mrow[i] - ref);
-                grew |= mnew > mrow[i];
-                mrow[i] = mnew;
-                float ls = 0.0f;
-#pragma unroll
-                for (int kt = 0; kt < ST; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i][kt][r], qs[i], C::UP - ref));
-                        sc[i][kt][r] = p;
-                        ls += p;
-                    }
-                lsum[i] = lsum[i] * alpha[i] + ls;
-            }
-            if (__any(grew)) {
-#pragma unroll
-                for (int i = 0; i < QT; ++i)
+                const float before = m[i];
+                const float alpha = soften<1>(s[i], q.qs[i], T::UP, m[i], l[i]);
+                if (__any(m[i] > before)) {
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) o[i][d][r] *= alpha[i];
-            }
-            // a V that is no finite number would reach rows that do not see it
-            // as 0 * V: such a tile's products are taken one by one
-            bool odd = false;
-            if (tail) {
-#pragma unroll
-                for (int n = 0; n < 16 * ST * C::CPR / 64; ++n) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(Vs + n * 1024 + lane * 16);
-                    constexpr uint32_t E = F16 ? 0x7c00u : 0x7f800000u;
-                    for (uint32_t x : {w.x, w.y, w.z, w.w})
-                        odd |= (x & E) == E || (F16 && (x >> 16 & E) == E);
+                        for (int r = 0; r < 4; ++r) o[i][d][r] *= alpha;
                 }
-            }
-            if (__any(odd)) {
-#pragma unroll 1
-                for (int key = 0; key < 16 * ST; ++key) {
-                    const int kt = key >> 4, r = key & 3, from = li + 4 * (key & 12);
+                if constexpr (T::F16) {
+                    f16x4 ph, pl;
 #pragma unroll
-                    for (int i = 0; i < QT; ++i) {
-                        float p = 0.0f;
+                    for (int r = 0; r < 4; ++r) {
+                        _Float16 h, w;
+                        split_f16(s[i][0][r], h, w);
+                        ph[r] = h;
+                        pl[r] = w;
+                    }
 #pragma unroll
-                        for (int x = 0; x < ST; ++x)
+                    for (int d = 0; d < DT; ++d)
+                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vh[d], ph, o[i][d], 0, 0, 0);
 #pragma unroll
-                            for (int y = 0; y < 4; ++y)
-                                if (x == kt && y == r) p = sc[i][x][y];
-                        p = __shfl(p, from);
+                    for (int d = 0; d < DT; ++d)
+                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vh[d], pl, o[i][d], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
 #pragma unroll
                         for (int d = 0; d < DT; ++d)
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) {
-                                const int e = 16 * d + 4 * lg + y;
-                                const int c = e * C::ES / 16;
-                                const float v = (float)*reinterpret_cast<const KVT *>(
-                                    Vs + key * ROWB + ((c ^ (key & C::SWZ)) << 4) + e * C::ES % 16);
-                                if (p != 0.0f) o[i][d][y] = __builtin_fmaf(p, v, o[i][d][y]);
-                            }
-                    }
+                            o[i][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[r][d / 4][d % 4], s[i][0][r], o[i][d], 0, 0, 0);
                 }
-            } else if constexpr (F16 && ST == 1) {
-                f16x4 ph[QT], pl[QT];
+            }
+        }
+        // join the waves
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+            l[i] = group_sum(l[i]);
+            if (lg == 0) {
+                w_ml[wave][i * 16 + li][0] = m[i];
+                w_ml[wave][i * 16 + li][1] = bad ? NAN : l[i];
+            }
+        }
+        if (lane == 0) w_odd[wave] = odd;
+        lds_barrier();  // and every wave is done with its stages
+        if (uniform(w_odd[0] | w_odd[1] | w_odd[2] | w_odd[3])) {
+            one_by_one<KVT, HD, RT>(a, g, group, KT, T::UP);
+            continue;
+        }
+        constexpr int OS = HD / 4 < 16 ? HD / 4 - 1 : 15;
+        f32x4 *const ow = reinterpret_cast<f32x4 *>(lds);
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+            const int row = i * 16 + li;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, w_ml[w][row][0]);
+            const float f = __builtin_amdgcn_exp2f(m[i] - (M == -INFINITY ? 0.0f : M));
+#pragma unroll
+            for (int n = 0; n < DT; ++n) {
+                f32x4 v = o_quad<T>(o[i], n);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] *= f;
+                ow[(wave * RT + row) * (HD / 4) + ((o_col<T>(n, lg) / 4) ^ (row & OS))] = v;
+            }
+        }
+        lds_barrier();
+        for (int x = tid; x < RT * (HD / 4); x += 256) {
+            const int row = x / (HD / 4), c4 = x % (HD / 4);
+            if (g.rb * RT + row >= g.nrows) continue;
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, w_ml[w][row][0]);
+            const float ref = M == -INFINITY ? 0.0f : M;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                L += w_ml[w][row][1] * __builtin_amdgcn_exp2f(w_ml[w][row][0] - ref);
+                v += ow[(w * RT + row) * (HD / 4) + (c4 ^ (row & OS))];
+            }
+            put<HD, RT>(a, g, group, row, 4 * c4, v, M, L);
+        }
+    }
+}
+
+// ---- more rows: the four waves take 16 QT rows each, and share the tile's
+// positions in LDS.
+template <typename KVT, int HD, int QT>
+struct TileCfg : Tile<KVT, HD> {
+    typedef Tile<KVT, HD> T;
+    static constexpr int KT = T::ROWB <= 256 ? 64 : 32, RT = 64 * QT;
+    static constexpr int ST = KT / 16;
+    static constexpr int TILE = KT * T::ROWB;
+    static constexpr int LDS = 4 * TILE;  // two buffers of K and V
+    static constexpr int PER_CU = LDS <= 72 * 1024 ? 2 : 1;
+    static constexpr int GPW = KT / 32;   // groups of 16 rows that a wave loads a tile
+    static_assert(LDS + 4096 <= 160 * 1024, "tiles must fit a CU");
+};
+
+template <typename KVT, int HD, int QT>
+__global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile_kernel(TreeArgs a) {
+    using C = TileCfg<KVT, HD, QT>;
+    using T = Tile<KVT, HD>;
+    constexpr int KT = C::KT, RT = C::RT, DT = T::DT, ST = C::ST;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
+    __shared__ int bad_seg;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int li = lane & 15, lg = lane >> 4;
+    const int group = a.n_heads / a.n_kv;
+    const uint32_t row_b = (uint32_t)a.n_kv * T::ROWB;
+    // a wave's groups of a tile: K and V of group `wave`, or (32 positions)
+    // group wave % 2 of K or V
+    const int my_group = C::GPW == 2 ? wave : wave & 1;
+    uint32_t off[T::NU];
+    dma_offsets<T>(off, row_b, lane);
+    Cursor cur = first_unit<KT, RT>(a, group, lane);
+    if (tid == 0) bad_seg = 0;
+    int seg = 0;
+    Seg g;
+    while (next_segment<KT, RT>(a, group, cur, g)) {
+        ++seg;
+        lds_barrier();  // the last segment's reads of LDS are done, bad_seg is set up
+        const char *const kc = static_cast<const char *>(a.kc) + (size_t)g.h * T::ROWB;
+        const char *const vc = static_cast<const char *>(a.vc) + (size_t)g.h * T::ROWB;
+        int slots = 0, tb = g.t0;
+        auto look_up = [&]() {
+            slots = slot16(a, g, (tb + lane) * (KT / 16) + my_group);
+            if (__any(slots < 0 && tb + lane < g.t1)) bad_seg = seg;
+            slots = max(slots, 0);  // a block has 16 positions: in the cache, and the row is lost
+        };
+        auto load = [&](int t) {
+            const size_t at = (size_t)(uint32_t)__builtin_amdgcn_readlane(slots, t - tb) * row_b;
+            const int rows = g.last - (min(t * (KT / 16) + my_group, g.last >> 4) << 4);
+            unsigned char *const dst = lds + (t & 1) * 2 * C::TILE + my_group * T::GROUPB;
+            if (C::GPW == 2 || wave < 2) dma_group<T>(kc + at, dst, rows, off, row_b, lane);
+            if (C::GPW == 2 || wave >= 2) dma_group<T>(vc + at, dst + C::TILE, rows, off, row_b, lane);
+        };
+        const int t1 = g.lost ? g.t0 : g.t1;
+        if (g.t0 < t1) {
+            look_up();
+            load(g.t0);
+        }
+        const int w_row = g.rb * RT + wave * 16 * QT;
+        Query<T, QT> q;
+        q.load(a, g, group, w_row, li, lg);
+        f32x4 o[QT][DT];
+        float m[QT], l[QT];
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        for (int t = g.t0; t < t1; ++t) {
+            wait_vm<0>();
+            lds_barrier();  // tile t is there, the other buffer free
+            if (t + 1 < t1) {
+                if (t + 1 - tb == 64) {
+                    tb += 64;
+                    look_up();
+                }
+                load(t + 1);
+            }
+            const int k0 = t * KT;
+            const unsigned char *const Ks = lds + (t & 1) * 2 * C::TILE, *const Vs = Ks + C::TILE;
+            const bool tail = k0 + KT > g.s.cached;
+            if (tail) {
+                int x = 0;
+#pragma unroll
+                for (int n = 0; n < C::TILE / 1024; ++n) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(Vs + n * 1024 + lane * 16);
+                    x |= not_finite<T::F16>(w.x) | not_finite<T::F16>(w.y) | not_finite<T::F16>(w.z) |
+                         not_finite<T::F16>(w.w);
+                }
+                odd |= __any(x);
+            }
+            if (w_row >= g.nrows) continue;
+            f32x4 s[QT][ST];
+#pragma unroll
+            for (int n = 0; n < ST; ++n) {
+                typename T::frag kf[T::KS];
+#pragma unroll
+                for (int x = 0; x < T::KS; ++x) kf[x] = k_frag<T>(Ks + n * T::GROUPB, x, li, lg);
+#pragma unroll
+                for (int i = 0; i < QT; ++i) s[i][n] = scores<T, QT>(kf, q, i);
+            }
+            if (tail) {  // nodes: by the mask
 #pragma unroll
                 for (int i = 0; i < QT; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        _Float16 hi, lo;
-                        split_f16(sc[i][0][r], hi, lo);
-                        ph[i][r] = hi;
-                        pl[i][r] = lo;
+                    for (int n = 0; n < ST; ++n) {
+                        const uint32_t vis = sees4(a, g.s.r0 + q.node[i], q.node[i], g.s.n,
+                                                   k0 + n * 16 + 4 * lg - g.s.cached);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[i][n][r] = vis >> r & 1 ? s[i][n][r] : -INFINITY;
                     }
+            }
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    // V^T: within 16 lanes, lane i receives element i % 4 of the 8
-                    // bytes at lane 4 j + i / 4's address: dim 16 d + i of keys 4 lg + j
-                    const f16x4 vf = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s16x4 *)(Vs + (va ^ (d << 5)))));
+            for (int i = 0; i < QT; ++i) {
+                const float before = m[i];
+                const float alpha = soften<ST>(s[i], q.qs[i], T::UP, m[i], l[i]);
+                if (__any(m[i] > before)) {
 #pragma unroll
-                    for (int i = 0; i < QT; ++i)
-                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vf, ph[i], o[i][d], 0, 0, 0);
+                    for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int i = 0; i < QT; ++i)
-                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vf, pl[i], o[i][d], 0, 0, 0);
+                        for (int r = 0; r < 4; ++r) o[i][d][r] *= alpha;
                 }
-            } else if constexpr (F16) {
+            }
+            if constexpr (T::F16) {
+                const int row = 4 * lg + (li >> 2), c = (li & 3) >> 1;
 #pragma unroll
                 for (int kk = 0; kk < ST / 2; ++kk) {
                     f16x8 ph[QT], pl[QT];
@@ -578,17 +908,19 @@ __global__ __launch_bounds__(256, (TC<KVT, HD, QT, SPLIT>::LDS <= 72 * 1024 ? 2 
                     for (int i = 0; i < QT; ++i)
 #pragma unroll
                         for (int r = 0; r < 8; ++r) {
-                            _Float16 hi, lo;
-                            split_f16(sc[i][2 * kk + r / 4][r % 4], hi, lo);
-                            ph[i][r] = hi;
-                            pl[i][r] = lo;
+                            _Float16 h, w;
+                            split_f16(s[i][2 * kk + r / 4][r % 4], h, w);
+                            ph[i][r] = h;
+                            pl[i][r] = w;
                         }
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
-                        const unsigned char *p = Vs + ((va ^ (d << 5)) + kk * 2 * C::GROUPB);
-                        const uint2 r0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
-                        const uint2 r1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + C::GROUPB)));
-                        const f16x8 vf = __builtin_bit_cast(f16x8, make_uint4(r0.x, r0.y, r1.x, r1.y));
+                        // the k order of the fragments: rows 4 lg + j of both groups
+                        const unsigned char *p = Vs + kk * 2 * T::GROUPB + row * T::ROWB +
+                                                 (((2 * d + c) ^ (row & T::SWZ)) << 4) + (li & 1) * 8;
+                        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
+                        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + T::GROUPB)));
+                        const f16x8 vf = __builtin_bit_cast(f16x8, make_uint4(x.x, x.y, y.x, y.y));
 #pragma unroll
                         for (int i = 0; i < QT; ++i)
                             o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[i], o[i][d], 0, 0, 0);
@@ -599,101 +931,51 @@ __global__ __launch_bounds__(256, (TC<KVT, HD, QT, SPLIT>::LDS <= 72 * 1024 ? 2 
                 }
             } else {
 #pragma unroll
-                for (int kt = 0; kt < ST; ++kt)
+                for (int n = 0; n < ST; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int row = 4 * lg + r;
-                        const int vb = row * ROWB + (((li >> 2) ^ (row & C::SWZ)) << 4) + (li & 3) * 4;
 #pragma unroll
-                        for (int d = 0; d < DT; ++d) {
-                            const float vf = *reinterpret_cast<const float *>(Vs + ((vb ^ (d << 6)) + kt * C::GROUPB));
+                        for (int c = 0; c < HD / 64; ++c) {
+                            const f32x4 vf = *reinterpret_cast<const f32x4 *>(
+                                Vs + n * T::GROUPB + row * T::ROWB + (((16 * c + li) ^ (row & T::SWZ)) << 4));
 #pragma unroll
-                            for (int i = 0; i < QT; ++i)
-                                o[i][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, sc[i][kt][r], o[i][d], 0, 0, 0);
+                            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                                for (int i = 0; i < QT; ++i)
+                                    o[i][4 * c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                        vf[e], s[i][n][r], o[i][4 * c + e], 0, 0, 0);
                         }
                     }
             }
         }
-
-        // the segment's result: the output where it has every tile, else a partial
-        auto put = [&](int row_in, int nd, int hd_, int col, f32x4 v, float m, float l) {
-            if (whole) {
-                const float f = l == 0.0f ? 0.0f : 1.0f / l;
-                f32x4 y;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = l == 0.0f ? 0.0f : v[r] * f;
-                *reinterpret_cast<f32x4 *>(a.out + (size_t)(s.r0 + nd) * a.out_stride + (size_t)hd_ * HD + col) = y;
-            } else {
-                const size_t at = (size_t)slot_part * RT + row_in;
-                *reinterpret_cast<f32x4 *>(a.part + at * HD + col) = v;
-                if (col == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(m, l);
-            }
-        };
+        if (g.t0 == t1) lds_barrier();  // (no tile's barrier made bad_seg known)
+        if (odd) {  // every wave has seen every V
+            one_by_one<KVT, HD, RT>(a, g, group, KT, T::UP);
+            continue;
+        }
+        const bool bad = g.lost || bad_seg == seg;
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
-            lsum[i] += __shfl_xor(lsum[i], 16);
-            lsum[i] += __shfl_xor(lsum[i], 32);
-        }
-        if constexpr (SPLIT) {
-            if (lg == 0)
+            l[i] = group_sum(l[i]);
+            if (w_row + i * 16 + li >= g.nrows) continue;
 #pragma unroll
-                for (int i = 0; i < QT; ++i) {
-                    w_ml[wave][i * 16 + li][0] = mrow[i];
-                    w_ml[wave][i * 16 + li][1] = lsum[i];
-                }
-            lds_barrier();  // and every wave is done with its tiles
-            f32x4 *const ow = reinterpret_cast<f32x4 *>(lds);
-#pragma unroll
-            for (int i = 0; i < QT; ++i) {
-                const int row = i * 16 + li;
-                float M = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) M = fmaxf(M, w_ml[w][row][0]);
-                const float f = __builtin_amdgcn_exp2f(mrow[i] - (M == -INFINITY ? 0.0f : M));
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    f32x4 v = o[i][d];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] *= f;
-                    ow[(wave * RT + row) * (HD / 4) + ((4 * d + lg) ^ (row & (HD / 4 < 16 ? HD / 4 - 1 : 15)))] = v;
-                }
-            }
-            lds_barrier();
-            const bool bad = bad_seg == seg;
-            for (int x = tid; x < RT * (HD / 4); x += 256) {
-                const int row = x / (HD / 4), c4 = x % (HD / 4), rr = rb * RT + row;
-                if (rr >= nrows) continue;
-                float M = -INFINITY, l = 0.0f;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) M = fmaxf(M, w_ml[w][row][0]);
-                const float ref = M == -INFINITY ? 0.0f : M;
-                f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    l += w_ml[w][row][1] * __builtin_amdgcn_exp2f(w_ml[w][row][0] - ref);
-                    v += ow[(w * RT + row) * (HD / 4) + (c4 ^ (row & (HD / 4 < 16 ? HD / 4 - 1 : 15)))];
-                }
-                put(row, rr / group, h * group + rr % group, 4 * c4, v, M, bad ? NAN : l);
-            }
-        } else {
-            const bool bad = bad_seg == seg;  // (set before the last tile's barrier)
-#pragma unroll
-            for (int i = 0; i < QT; ++i) {
-                if (w_row + i * 16 + li >= nrows) continue;
-                const int row = (SPLIT ? 0 : wave * 16 * QT) + i * 16 + li;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    put(row, node[i], head[i], 16 * d + 4 * lg, o[i][d], mrow[i], bad ? NAN : lsum[i]);
-            }
+            for (int n = 0; n < DT; ++n)
+                put<HD, RT>(a, g, group, wave * 16 * QT + i * 16 + li, o_col<T>(n, lg),
+                            o_quad<T>(o[i], n), m[i], bad ? NAN : l[i]);
         }
     }
 }
 
-// Joins the partials of every row whose units went to more than one workgroup:
-// one workgroup a row, a thread four elements of a head.
+// Joins the partials of the rows whose units went to more than one workgroup,
+// in the order of the positions: a wave a (row, head), the lanes four elements
+// of every 256 / HD-th partial.
 template <int HD>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int rt) {
+    constexpr int CL = HD / 4, SL = 64 / CL;
     const int r = blockIdx.x, lane = threadIdx.x & 63;
+    const int head = uniform((int)(blockIdx.y * 4 + (threadIdx.x >> 6)));
+    if (head >= a.n_heads) return;
     const int group = a.n_heads / a.n_kv;
     long long total = 0, base = -1;
     SeqRows mine{0, 0, 0};
@@ -704,52 +986,90 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int
         const unsigned long long hit = __ballot(r >= s.r0 && r < s.r0 + s.n);
         if (hit && base < 0) {
             const int at = __ffsll((long long)hit) - 1;
-            base = total + __shfl(inc - v, at);
+            base = uniform(total + __shfl(inc - v, at));
             mine = SeqRows{__shfl(s.r0, at), __shfl(s.n, at), __shfl(s.cached, at)};
         }
         total += __shfl(inc, 63);
     }
     if (base < 0) return;
+    mine = uniform(mine);
     const Work wk = work_of(mine, group, a.n_kv, kt, rt);
-    const Deal deal(total, a.wgs);
-    for (int x = threadIdx.x; x < a.n_heads * (HD / 4); x += 256) {
-        const int head = x / (HD / 4), col = x % (HD / 4) * 4;
-        const int h = head / group, rr = (r - mine.r0) * group + head % group;
-        const long long u0 = base + ((long long)h * wk.blocks + rr / rt) * wk.tiles;
-        const int w0 = deal.owner(u0), w1 = deal.owner(u0 + wk.tiles - 1);
-        if (w0 == w1) continue;  // one workgroup had them all, and wrote the output
-        auto at = [&](int w) { return (size_t)(w * 2 + (w == w0 ? 1 : 0)) * rt + rr % rt; };
-        float M = -INFINITY, L = 0.0f;
-        for (int w = w0; w <= w1; ++w) M = fmaxf(M, a.ml[at(w) * 2]);
-        const float ref = M == -INFINITY ? 0.0f : M;
-        f32x4 y = {0.f, 0.f, 0.f, 0.f};
-        for (int w = w0; w <= w1; ++w) {
-            const float2 ml = *reinterpret_cast<const float2 *>(a.ml + at(w) * 2);
-            const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-            L = __builtin_fmaf(f, ml.y, L);
-            const f32x4 v = *reinterpret_cast<const f32x4 *>(a.part + at(w) * HD + col);
+    const Deal deal(uniform(total), a.wgs);
+    const int h = head / group, rr = (r - mine.r0) * group + head - h * group;
+    const long long u0 = base + ((long long)h * wk.blocks + rr / rt) * wk.tiles;
+    const int w0 = uniform(deal.owner(u0)), w1 = uniform(deal.owner(u0 + wk.tiles - 1));
+    if (w0 == w1) return;  // one workgroup had them all, and wrote the output
+    auto at = [&](int w) { return (size_t)(w * 2 + (w == w0 ? 1 : 0)) * rt + rr % rt; };
+    const int col = lane % CL * 4, sl = lane / CL;
+    float M = -INFINITY, L = 0.0f;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    for (int c = w0; c <= w1; c += 64) {
+        const int n = min(64, w1 + 1 - c);
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (lane < n) ml = *reinterpret_cast<const float2 *>(a.ml + at(c + lane) * 2);
+        constexpr int D = 8;  // partials in flight
+        f32x4 v[D];
+        auto fetch = [&](int p0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(f, v[e], y[e]);
+            for (int d = 0; d < D; ++d)
+                v[d] = *reinterpret_cast<const f32x4 *>(a.part + at(c + min(p0 + d * SL + sl, n - 1)) * HD + col);
+        };
+        fetch(0);
+        float mx = ml.x;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+        const float Mn = fmaxf(M, mx), ref = Mn == -INFINITY ? 0.0f : Mn;
+        const float old = __builtin_amdgcn_exp2f(M - ref), f = __builtin_amdgcn_exp2f(ml.x - ref);
+        M = Mn;
+        float ls = lane < n ? f * ml.y : 0.0f;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) ls += __shfl_xor(ls, o);
+        L = L * old + ls;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= old;
+        for (int p0 = 0;;) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                const int p = p0 + d * SL + sl;
+                const float w = __shfl(f, p & 63);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    y[e] = p < n ? __builtin_fmaf(w, v[d][e], y[e]) : y[e];
+            }
+            p0 += D * SL;
+            if (p0 >= n) break;
+            fetch(p0);
         }
-        const float f = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = L == 0.0f ? 0.0f : y[e] * f;
-        *reinterpret_cast<f32x4 *>(a.out + (size_t)r * a.out_stride + (size_t)head * HD + col) = y;
     }
+#pragma unroll
+    for (int o = CL; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], o);
+    const float f = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = L == 0.0f ? 0.0f : y[e] * f;
+    if (sl == 0) *reinterpret_cast<f32x4 *>(a.out + (size_t)r * a.out_stride + (size_t)head * HD + col) = y;
 }
 
-template <typename KVT, int HD, int QT, bool SPLIT>
-int launch_tiles(cw_ctx *ctx, TreeArgs a) {
-    using C = TC<KVT, HD, QT, SPLIT>;
-    a.wgs = ctx->n_cu * (C::LDS <= 72 * 1024 ? 2 : 1);
+template <typename C>
+int launch_tiles(cw_ctx *ctx, TreeArgs a, void (*fn)(TreeArgs)) {
+    a.wgs = ctx->n_cu * C::PER_CU;
     const size_t rows = (size_t)a.wgs * 2 * C::RT;
     void *scratch = nullptr;
-    CW_TRY(ctx_scratch(ctx, rows * (HD + 2) * sizeof(float), &scratch));
+    CW_TRY(ctx_scratch(ctx, rows * (C::HD + 2) * sizeof(float), &scratch));
     a.part = static_cast<float *>(scratch);
-    a.ml = a.part + rows * HD;
-    CW_TRY(launch(ctx, "attention_tree", tree_kernel<KVT, HD, QT, SPLIT>, dim3(a.wgs), dim3(256), 0, a));
-    return launch(ctx, "attention_tree_merge", tree_merge_kernel<HD>, dim3(a.rows), dim3(256), 0, a,
-                  C::KT, C::RT);
+    a.ml = a.part + rows * C::HD;
+    CW_TRY(launch(ctx, "attention_tree", fn, dim3(a.wgs), dim3(256), 0, a));
+    return launch(ctx, "attention_tree_merge", tree_merge_kernel<C::HD>,
+                  dim3(a.rows, (a.n_heads + 3) / 4), dim3(256), 0, a, C::KT, C::RT);
+}
+template <typename KVT, int HD, int QT>
+int launch_split(cw_ctx *ctx, const TreeArgs &a) {
+    return launch_tiles<SplitCfg<KVT, HD, QT>>(ctx, a, tree_split_kernel<KVT, HD, QT>);
+}
+template <typename KVT, int HD, int QT>
+int launch_tile(cw_ctx *ctx, const TreeArgs &a) {
+    return launch_tiles<TileCfg<KVT, HD, QT>>(ctx, a, tree_tile_kernel<KVT, HD, QT>);
 }
 
 // By the rows of a (request, kv head) on average.
@@ -757,12 +1077,13 @@ template <typename KVT, int HD>
 int launch_by_rows(cw_ctx *ctx, const TreeArgs &a) {
     const long long rows = ((long long)a.rows + a.n_seq - 1) / a.n_seq * (a.n_heads / a.n_kv);
     if constexpr (HD * sizeof(KVT) <= 512) {
-        if (rows <= 16) return launch_tiles<KVT, HD, 1, true>(ctx, a);
-        if (rows <= 32) return launch_tiles<KVT, HD, 2, true>(ctx, a);
+        if (rows <= 16) return launch_split<KVT, HD, 1>(ctx, a);
+        if constexpr (HD <= 128)
+            if (rows <= 32) return launch_split<KVT, HD, 2>(ctx, a);
     }
     if constexpr (HD <= 128 && sizeof(KVT) == 2)
-        if (rows > 64) return launch_tiles<KVT, HD, 2, false>(ctx, a);
-    return launch_tiles<KVT, HD, 1, false>(ctx, a);
+        if (rows > 64) return launch_tile<KVT, HD, 2>(ctx, a);
+    return launch_tile<KVT, HD, 1>(ctx, a);
 }
 
 template <typename KVT>
