@@ -42,27 +42,25 @@ __device__ __forceinline__ bool sees(const TreeArgs &a, int row, int i, int j) {
            (a.mask[(size_t)row * a.mask_words + (j >> 5)] >> (j & 31) & 1);
 }
 
-// The lowest n of 32 bits (none below 0, all from 32 on)
-__device__ __forceinline__ uint32_t low_bits(int n) {
-    return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
-}
-
-// Bit r: node i of a request of n nodes sees node j + r, r < 4; nodes below 0
-// (cached positions) are seen.  Without branches for the lanes.
-__device__ __forceinline__ uint32_t sees4(const TreeArgs &a, int row, int i, int n, int j) {
-    uint32_t m;
+// Bit k: node i of a request of n nodes sees node j + k; nodes below 0 (cached
+// positions) are seen.  j is the same for all lanes.  Three words of the mask,
+// requested together.
+__device__ __forceinline__ uint64_t sees64(const TreeArgs &a, int row, int i, int n, int j) {
+    auto low = [](int k) { return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1; };
+    uint64_t m;
     if (a.mask) {
         const uint32_t *words = a.mask + (size_t)row * a.mask_words;
-        const int w = j >> 5;
-        uint32_t lo = words[min(max(w, 0), a.mask_words - 1)];
-        uint32_t hi = words[min(max(w + 1, 0), a.mask_words - 1)];
-        lo = w < 0 ? ~0u : w < a.mask_words ? lo : 0u;
-        hi = w + 1 < 0 ? ~0u : w + 1 < a.mask_words ? hi : 0u;
-        m = (uint32_t)(((uint64_t)hi << 32 | lo) >> (j & 31));
+        const int w = j >> 5, s = j & 31;
+        uint32_t x[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) x[k] = words[min(max(w + k, 0), a.mask_words - 1)];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) x[k] = w + k < 0 ? ~0u : w + k < a.mask_words ? x[k] : 0u;
+        m = ((uint64_t)x[1] << 32 | x[0]) >> s | ((uint64_t)x[2] << 32) << (32 - s);
     } else {
-        m = low_bits(i - j + 1);
+        m = low(i - j + 1);
     }
-    return m & low_bits(n - j);
+    return m & low(n - j);
 }
 
 // One (row, head) a workgroup: wave w takes positions w, w + 4, ..., a lane
@@ -200,12 +198,20 @@ __device__ __forceinline__ void split_f16(float v, _Float16 &hi, _Float16 &lo) {
     lo = (_Float16)(v - (float)hi);
 }
 
-// ---- who does what.  A unit is one tile of kt positions for one block of rt
-// rows (a row: a node and one of its query heads) of one kv head; the units of
-// a request are ordered (kv head, row block, tile), all of them dealt to the
-// workgroups in runs of q or q + 1, so that requests of any lengths share the
-// chip evenly.  A run's piece of a (kv head, row block) is a segment; what no
-// workgroup has whole is joined by tree_merge_kernel.
+// ---- who does what.  A tile is kt positions for one block of rt rows (a row: a
+// node and one of its query heads) of one kv head; the tiles of a request are
+// ordered (kv head, row block, position).  A row block costs kOpen units to
+// begin (its queries, the first tile's way from memory) and one for each tile;
+// all units are dealt to the workgroups in runs of q or q + 1, so that requests
+// of any lengths share the chip evenly.  A run's piece of a row block is a
+// segment; what no workgroup has whole is joined by tree_merge_kernel.
+// (kOpen 0, 2, 4 and 8: 48 single rows at 100 .. 8,000 positions 88, 74, 74 and
+// 77 us.  Workgroups of one CU and the XCDs are served unevenly, equal runs end
+// up to 1.5 times apart; short runs fetched by whoever is free gain nothing,
+// as the rest of the chip then has the memory to itself: 164 us either way for
+// 64 requests of 4,000 positions.)
+
+constexpr int kOpen = 3;
 
 struct Work {
     int tiles, blocks;
@@ -214,7 +220,7 @@ struct Work {
 __device__ __forceinline__ Work work_of(const SeqRows &s, int group, int n_kv, int kt, int rt) {
     if (!s.n) return Work{0, 0, 0};
     const int t = (s.cached + s.n + kt - 1) / kt, rb = (int)(((long long)s.n * group + rt - 1) / rt);
-    return Work{t, rb, (long long)n_kv * rb * t};
+    return Work{t, rb, (long long)n_kv * rb * (kOpen + t)};
 }
 
 __device__ __forceinline__ long long wave_scan(long long v, int lane) {
@@ -245,6 +251,7 @@ struct Seg {
     SeqRows s;
     int b, h, rb, t0, t1, nrows, last, part;  // part: its place among the partials
     bool whole, lost;                         // lost: positions that no table entry covers
+    bool once;                                // the request's only row block
 };
 struct Cursor {
     long long u, end, base;  // next unit, end of the run, first unit of request b
@@ -294,19 +301,23 @@ __device__ __forceinline__ bool next_segment(const TreeArgs &a, int group, Curso
             continue;
         }
         const long long local = cur.u - cur.base;
-        const int hr = uniform((int)(local / wk.tiles));
+        const int each = kOpen + wk.tiles, hr = uniform((int)(local / each));
+        const int from = uniform((int)(local - (long long)hr * each));
+        const int to = uniform((int)min((long long)each, from + (cur.end - cur.u)));
+        cur.u += to - from;
+        if (to <= kOpen) continue;  // the run ends before the row block's first tile
         g.b = cur.b;
-        g.t0 = uniform((int)(local - (long long)hr * wk.tiles));
-        g.t1 = uniform((int)min((long long)wk.tiles, g.t0 + (cur.end - cur.u)));
+        g.t0 = max(from - kOpen, 0);
+        g.t1 = to - kOpen;
         g.h = uniform(hr / wk.blocks);
         g.rb = uniform(hr - g.h * wk.blocks);
         g.nrows = g.s.n * group;
         g.last = g.s.cached + g.s.n - 1;
+        g.once = wk.blocks == 1;
         g.whole = g.t0 == 0 && g.t1 == wk.tiles;
         g.part = blockIdx.x * 2 + (g.t0 > 0 ? 0 : 1);
         g.lost = a.map.tables ? (g.last >> a.map.shift) >= a.map.max_blocks
                               : g.b >= a.map.n_blocks || g.last >= a.map.page;
-        cur.u += g.t1 - g.t0;
         return true;
     }
     return false;
@@ -410,6 +421,15 @@ struct Tile {
     typedef typename std::conditional<F16, f16x8, f32x4>::type frag;
 };
 
+// dma16 of lines that nobody reads again (non-temporal: 64 single rows at 4,000
+// positions 182 -> 165 us; where a second row block reads them it costs a tenth)
+__device__ __forceinline__ void dma16_once(const void *base, uint32_t off, unsigned char *lds_dst) {
+    asm volatile("global_load_lds_dwordx4 %0, %1 nt"
+                 :
+                 : "v"(off), "s"(base), "{m0}"(lds_off(lds_dst))
+                 : "memory");
+}
+
 // 16 positions of a kv head from slot `slot` on into LDS, 1 KB a DMA; rows
 // behind `rows` repeat it.  off: this lane's offsets where all 16 are there.
 template <typename T>
@@ -422,8 +442,12 @@ __device__ __forceinline__ void dma_offsets(uint32_t (&off)[T::NU], uint32_t row
 }
 template <typename T>
 __device__ __forceinline__ void dma_group(const char *src, unsigned char *dst, int rows,
-                                          const uint32_t (&off)[T::NU], uint32_t row_b, int lane) {
-    if (rows >= 15) {
+                                          const uint32_t (&off)[T::NU], uint32_t row_b, int lane,
+                                          bool once) {
+    if (rows >= 15 && once) {
+#pragma unroll
+        for (int n = 0; n < T::NU; ++n) dma16_once(src, off[n], dst + n * 1024);
+    } else if (rows >= 15) {
 #pragma unroll
         for (int n = 0; n < T::NU; ++n) dma16(src, off[n], dst + n * 1024);
     } else {
@@ -601,8 +625,8 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
             const size_t at = (size_t)(uint32_t)__builtin_amdgcn_readlane(slots, t - tb) * row_b;
             const int rows = g.last - (min(t * 4 + wave, g.last >> 4) << 4);
             unsigned char *const dst = mine + (t & 1) * C::STAGE;
-            dma_group<T>(kc + at, dst, rows, off, row_b, lane);
-            dma_group<T>(vc + at, dst + T::GROUPB, rows, off, row_b, lane);
+            dma_group<T>(kc + at, dst, rows, off, row_b, lane, g.once);
+            dma_group<T>(vc + at, dst + T::GROUPB, rows, off, row_b, lane, g.once);
         };
         const int t1 = g.lost ? g.t0 : g.t1;
         if (g.t0 < t1) {
@@ -665,7 +689,7 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
             if (k0 + 16 > g.s.cached) {  // nodes: by the mask
 #pragma unroll
                 for (int i = 0; i < QT; ++i) {
-                    const uint32_t vis = sees4(a, g.s.r0 + q.node[i], q.node[i], g.s.n, k0 + 4 * lg - g.s.cached);
+                    const uint64_t vis = sees64(a, g.s.r0 + q.node[i], q.node[i], g.s.n, k0 - g.s.cached) >> 4 * lg;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[i][0][r] = vis >> r & 1 ? s[i][0][r] : -INFINITY;
                 }
@@ -823,8 +847,8 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
             const size_t at = (size_t)(uint32_t)__builtin_amdgcn_readlane(slots, t - tb) * row_b;
             const int rows = g.last - (min(t * (KT / 16) + my_group, g.last >> 4) << 4);
             unsigned char *const dst = lds + (t & 1) * 2 * C::TILE + my_group * T::GROUPB;
-            if (C::GPW == 2 || wave < 2) dma_group<T>(kc + at, dst, rows, off, row_b, lane);
-            if (C::GPW == 2 || wave >= 2) dma_group<T>(vc + at, dst + C::TILE, rows, off, row_b, lane);
+            if (C::GPW == 2 || wave < 2) dma_group<T>(kc + at, dst, rows, off, row_b, lane, g.once);
+            if (C::GPW == 2 || wave >= 2) dma_group<T>(vc + at, dst + C::TILE, rows, off, row_b, lane, g.once);
         };
         const int t1 = g.lost ? g.t0 : g.t1;
         if (g.t0 < t1) {
@@ -868,6 +892,12 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
                 odd |= __any(x);
             }
             if (w_row >= g.nrows) continue;
+            uint64_t vis[QT];
+            if (tail) {
+#pragma unroll
+                for (int i = 0; i < QT; ++i)
+                    vis[i] = sees64(a, g.s.r0 + q.node[i], q.node[i], g.s.n, k0 - g.s.cached) >> 4 * lg;
+            }
             f32x4 s[QT][ST];
 #pragma unroll
             for (int n = 0; n < ST; ++n) {
@@ -881,12 +911,10 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
 #pragma unroll
                 for (int i = 0; i < QT; ++i)
 #pragma unroll
-                    for (int n = 0; n < ST; ++n) {
-                        const uint32_t vis = sees4(a, g.s.r0 + q.node[i], q.node[i], g.s.n,
-                                                   k0 + n * 16 + 4 * lg - g.s.cached);
+                    for (int n = 0; n < ST; ++n)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[i][n][r] = vis >> r & 1 ? s[i][n][r] : -INFINITY;
-                    }
+                        for (int r = 0; r < 4; ++r)
+                            s[i][n][r] = vis[i] >> (n * 16 + r) & 1 ? s[i][n][r] : -INFINITY;
             }
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
@@ -996,7 +1024,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int
     const Work wk = work_of(mine, group, a.n_kv, kt, rt);
     const Deal deal(uniform(total), a.wgs);
     const int h = head / group, rr = (r - mine.r0) * group + head - h * group;
-    const long long u0 = base + ((long long)h * wk.blocks + rr / rt) * wk.tiles;
+    const long long u0 = base + ((long long)h * wk.blocks + rr / rt) * (kOpen + wk.tiles) + kOpen;
     const int w0 = uniform(deal.owner(u0)), w1 = uniform(deal.owner(u0 + wk.tiles - 1));
     if (w0 == w1) return;  // one workgroup had them all, and wrote the output
     auto at = [&](int w) { return (size_t)(w * 2 + (w == w0 ? 1 : 0)) * rt + rr % rt; };
