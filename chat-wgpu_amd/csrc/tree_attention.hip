@@ -395,6 +395,9 @@ __device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, f
     }
 }
 
+// Instructions other than vector and scalar arithmetic stay on their side
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x6); }
+
 // whether one of the register's f16 pair, or its f32, is no finite number
 template <bool F16>
 __device__ __forceinline__ int not_finite(uint32_t w) {
@@ -898,14 +901,35 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
                 for (int i = 0; i < QT; ++i)
                     vis[i] = sees64(a, g.s.r0 + q.node[i], q.node[i], g.s.n, k0 - g.s.cached) >> 4 * lg;
             }
+            // fragments are requested AHEAD products' steps before they are used
             f32x4 s[QT][ST];
+            constexpr int KA = T::KS < 4 ? T::KS : 4, KN = ST * T::KS;
+            typename T::frag kf[KA + 1];
+            auto k_at = [&](int e) { return k_frag<T>(Ks + e / T::KS * T::GROUPB, e % T::KS, li, lg); };
 #pragma unroll
-            for (int n = 0; n < ST; ++n) {
-                typename T::frag kf[T::KS];
+            for (int e = 0; e < KA; ++e) kf[e] = k_at(e);
 #pragma unroll
-                for (int x = 0; x < T::KS; ++x) kf[x] = k_frag<T>(Ks + n * T::GROUPB, x, li, lg);
+            for (int e = 0; e < KN; ++e) {
+                if (e + KA < KN) kf[(e + KA) % (KA + 1)] = k_at(e + KA);
+                keep_order();
+                const typename T::frag k = kf[e % (KA + 1)];
+                const int n = e / T::KS, x = e % T::KS;
 #pragma unroll
-                for (int i = 0; i < QT; ++i) s[i][n] = scores<T, QT>(kf, q, i);
+                for (int i = 0; i < QT; ++i) {
+                    if (x == 0) s[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if constexpr (T::F16) {
+                        s[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.hi[i][x], s[i][n], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            s[i][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[r], q.f[i][x][r], s[i][n], 0, 0, 0);
+                    }
+                }
+                if constexpr (T::F16)
+#pragma unroll
+                    for (int i = 0; i < QT; ++i)
+                        s[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.lo[i][x], s[i][n], 0, 0, 0);
+                keep_order();
             }
             if (tail) {  // nodes: by the mask
 #pragma unroll
@@ -928,34 +952,45 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
                 }
             }
             if constexpr (T::F16) {
-                const int row = 4 * lg + (li >> 2), c = (li & 3) >> 1;
+                f16x8 ph[ST / 2][QT], pl[ST / 2][QT];
 #pragma unroll
-                for (int kk = 0; kk < ST / 2; ++kk) {
-                    f16x8 ph[QT], pl[QT];
+                for (int kk = 0; kk < ST / 2; ++kk)
 #pragma unroll
                     for (int i = 0; i < QT; ++i)
 #pragma unroll
                         for (int r = 0; r < 8; ++r) {
                             _Float16 h, w;
                             split_f16(s[i][2 * kk + r / 4][r % 4], h, w);
-                            ph[i][r] = h;
-                            pl[i][r] = w;
+                            ph[kk][i][r] = h;
+                            pl[kk][i][r] = w;
                         }
+                const int row = 4 * lg + (li >> 2), c = (li & 3) >> 1;
+                auto v_at = [&](int e) {
+                    // the k order of the fragments: rows 4 lg + j of both groups of 16
+                    const int d = e % DT;
+                    const unsigned char *p = Vs + e / DT * 2 * T::GROUPB + row * T::ROWB +
+                                             (((2 * d + c) ^ (row & T::SWZ)) << 4) + (li & 1) * 8;
+                    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
+                    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + T::GROUPB)));
+                    return __builtin_bit_cast(f16x8, make_uint4(x.x, x.y, y.x, y.y));
+                };
+                constexpr int VA = 3, VN = DT * (ST / 2);
+                f16x8 vf[VA + 1];
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        // the k order of the fragments: rows 4 lg + j of both groups
-                        const unsigned char *p = Vs + kk * 2 * T::GROUPB + row * T::ROWB +
-                                                 (((2 * d + c) ^ (row & T::SWZ)) << 4) + (li & 1) * 8;
-                        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
-                        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + T::GROUPB)));
-                        const f16x8 vf = __builtin_bit_cast(f16x8, make_uint4(x.x, x.y, y.x, y.y));
+                for (int e = 0; e < VA; ++e) vf[e] = v_at(e);
 #pragma unroll
-                        for (int i = 0; i < QT; ++i)
-                            o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[i], o[i][d], 0, 0, 0);
+                for (int e = 0; e < VN; ++e) {
+                    if (e + VA < VN) vf[(e + VA) % (VA + 1)] = v_at(e + VA);
+                    keep_order();
+                    const f16x8 v = vf[e % (VA + 1)];
+                    const int kk = e / DT, d = e % DT;
 #pragma unroll
-                        for (int i = 0; i < QT; ++i)
-                            o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[i], o[i][d], 0, 0, 0);
-                    }
+                    for (int i = 0; i < QT; ++i)
+                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[kk][i], o[i][d], 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < QT; ++i)
+                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[kk][i], o[i][d], 0, 0, 0);
+                    keep_order();
                 }
             } else {
 #pragma unroll
