@@ -141,9 +141,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ long long uniform(long long v) {
-    return (long long)(uint32_t)uniform((int)v) | (long long)uniform((int)(v >> 32)) << 32;
-}
 __device__ __forceinline__ SeqRows uniform(SeqRows s) {
     return SeqRows{uniform(s.r0), uniform(s.n), uniform(s.cached)};
 }
@@ -192,10 +189,24 @@ __device__ __forceinline__ float group_sum(float v) {
     return over_groups(v, [](float x, float y) { return x + y; });
 }
 
-// v = hi + lo in f16 (22 bits)
-__device__ __forceinline__ void split_f16(float v, _Float16 &hi, _Float16 &lo) {
-    hi = (_Float16)v;
-    lo = (_Float16)(v - (float)hi);
+// v = hi + lo, N values in f16 (22 bits), rounded to nearest even: two values
+// take two conversions and two mixed subtractions
+template <int N, typename H>
+__device__ __forceinline__ void split_f16(const float (&v)[N], H &hi, H &lo) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    uint32_t h[N / 2], l[N / 2];
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+        h[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2 * j], v[2 * j + 1]}), f16x2));
+        float a, b;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(h[j]), "v"(v[2 * j]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+            : "=v"(b) : "v"(h[j]), "v"(v[2 * j + 1]));
+        l[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+    }
+    __builtin_memcpy(&hi, h, sizeof(hi));
+    __builtin_memcpy(&lo, l, sizeof(lo));
 }
 
 // ---- who does what.  A tile is kt positions for one block of rt rows (a row: a
@@ -223,7 +234,21 @@ __device__ __forceinline__ Work work_of(const SeqRows &s, int group, int n_kv, i
     return Work{t, rb, (long long)n_kv * rb * (kOpen + t)};
 }
 
+// Sums over the lanes up to this one.  Requests of under 2^24 units each (all
+// that a device works off within hours) are added as 32 bits along the lanes.
 __device__ __forceinline__ long long wave_scan(long long v, int lane) {
+    if (!__any(v >> 24 != 0)) {
+        int x = (int)v;
+#define CW_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, true)
+        CW_SCAN_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8
+        CW_SCAN_STEP(0x112, 0xf);
+        CW_SCAN_STEP(0x114, 0xf);
+        CW_SCAN_STEP(0x118, 0xf);
+        CW_SCAN_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+        CW_SCAN_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef CW_SCAN_STEP
+        return x;
+    }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const long long o = __shfl_up(v, d);
@@ -232,17 +257,28 @@ __device__ __forceinline__ long long wave_scan(long long v, int lane) {
     return v;
 }
 
+__device__ __forceinline__ long long from_lane(long long v, int l) {
+    return (long long)(uint32_t)__builtin_amdgcn_readlane((int)v, l) |
+           (long long)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32;
+}
+
+// n / d of no negative numbers, in 32 bits where they fit
+__device__ __forceinline__ long long divide(long long n, long long d) {
+    if ((n | d) >> 31 == 0) return (long long)((uint32_t)n / (uint32_t)d);
+    return n / d;
+}
+
 struct Deal {
     long long q;
     int rem;
     __device__ Deal(long long units, int wgs) {
-        q = units / wgs;
+        q = divide(units, wgs);
         rem = (int)(units - q * wgs);
     }
     __device__ long long start(int w) const { return q * w + min(w, rem); }
     __device__ int owner(long long u) const {
         const long long big = (q + 1) * rem;
-        return u < big ? (int)(u / (q + 1)) : rem + (int)((u - big) / q);
+        return u < big ? (int)divide(u, q + 1) : rem + (int)divide(u - big, q);
     }
 };
 
@@ -258,17 +294,29 @@ struct Cursor {
     int b;
 };
 
+// The requests' rows: a lane each of the first 64, the others from memory
+struct Requests {
+    SeqRows s;
+    __device__ __forceinline__ SeqRows at(const TreeArgs &a, int b) const {
+        if (b < 64)
+            return SeqRows{__builtin_amdgcn_readlane(s.r0, b), __builtin_amdgcn_readlane(s.n, b),
+                           __builtin_amdgcn_readlane(s.cached, b)};
+        return uniform(seq_rows(a.first_row, a.cached, a.rows, b));
+    }
+};
+
 // The workgroup's run
 template <int KT, int RT>
-__device__ __forceinline__ Cursor first_unit(const TreeArgs &a, int group, int lane) {
-    auto units = [&](int b) {
-        return b < a.n_seq ? work_of(seq_rows(a.first_row, a.cached, a.rows, b), group, a.n_kv, KT,
-                                     RT).units : 0;
+__device__ __forceinline__ Cursor first_unit(const TreeArgs &a, int group, int lane, Requests &req) {
+    auto rows = [&](int b) {
+        return b < a.n_seq ? seq_rows(a.first_row, a.cached, a.rows, b) : SeqRows{0, 0, 0};
     };
-    const long long v0 = units(lane), inc0 = wave_scan(v0, lane);
-    long long total = __shfl(inc0, 63);
-    for (int c = 64; c < a.n_seq; c += 64) total += __shfl(wave_scan(units(c + lane), lane), 63);
-    const Deal deal(uniform(total), a.wgs);
+    auto units = [&](const SeqRows &s) { return work_of(s, group, a.n_kv, KT, RT).units; };
+    req.s = rows(lane);
+    const long long v0 = units(req.s), inc0 = wave_scan(v0, lane);
+    long long total = from_lane(inc0, 63);
+    for (int c = 64; c < a.n_seq; c += 64) total += from_lane(wave_scan(units(rows(c + lane)), lane), 63);
+    const Deal deal(total, a.wgs);
     Cursor cur{deal.start(blockIdx.x), deal.start(blockIdx.x + 1), 0, 0};
     if (cur.u >= cur.end) return cur;
     long long v = v0, inc = inc0;
@@ -277,13 +325,13 @@ __device__ __forceinline__ Cursor first_unit(const TreeArgs &a, int group, int l
         if (hit) {
             const int at = __ffsll((long long)hit) - 1;
             cur.b = c + at;
-            cur.base = uniform(__shfl(inc - v, at));
+            cur.base = from_lane(inc - v, at);
             return cur;
         }
-        const long long before = __shfl(inc, 63);
+        const long long before = from_lane(inc, 63);
         c += 64;
         if (c >= a.n_seq) break;
-        v = units(c + lane);
+        v = units(rows(c + lane));
         inc = wave_scan(v, lane) + before;
     }
     cur.end = cur.u;  // (not reached: u is below the total)
@@ -291,9 +339,10 @@ __device__ __forceinline__ Cursor first_unit(const TreeArgs &a, int group, int l
 }
 
 template <int KT, int RT>
-__device__ __forceinline__ bool next_segment(const TreeArgs &a, int group, Cursor &cur, Seg &g) {
+__device__ __forceinline__ bool next_segment(const TreeArgs &a, int group, const Requests &req,
+                                             Cursor &cur, Seg &g) {
     while (cur.u < cur.end && cur.b < a.n_seq) {
-        g.s = uniform(seq_rows(a.first_row, a.cached, a.rows, cur.b));
+        g.s = req.at(a, cur.b);
         const Work wk = work_of(g.s, group, a.n_kv, KT, RT);
         if (cur.u >= cur.base + wk.units) {
             cur.base += wk.units;
@@ -301,7 +350,7 @@ __device__ __forceinline__ bool next_segment(const TreeArgs &a, int group, Curso
             continue;
         }
         const long long local = cur.u - cur.base;
-        const int each = kOpen + wk.tiles, hr = uniform((int)(local / each));
+        const int each = kOpen + wk.tiles, hr = uniform((int)divide(local, each));
         const int from = uniform((int)(local - (long long)hr * each));
         const int to = uniform((int)min((long long)each, from + (cur.end - cur.u)));
         cur.u += to - from;
@@ -471,44 +520,48 @@ struct Query {
     float qs[QT];
     int node[QT];
 
-    __device__ void load(const TreeArgs &a, const Seg &g, int group, int w_row, int li, int lg) {
+    f32x4 raw[T::F16 ? QT : 1][T::F16 ? T::HD / 16 : 1];
+
+    // requests the rows; convert() once other requests are out
+    __device__ __forceinline__ void load(const TreeArgs &a, const Seg &g, int group, int w_row,
+                                         int li, int lg) {
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
             const int rr = min(w_row + i * 16 + li, g.nrows - 1);
             node[i] = rr / group;
             const float *qr = a.q + (size_t)(g.s.r0 + node[i]) * a.q_stride +
                               (size_t)(g.h * group + rr - node[i] * group) * T::HD;
-            qs[i] = a.scale;
+#pragma unroll
+            for (int x = 0; x < T::HD / 16; ++x) {
+                if constexpr (T::F16)
+                    raw[i][x] = *reinterpret_cast<const f32x4 *>(qr + 32 * (x / 2) + 8 * lg + 4 * (x % 2));
+                else
+                    f[i][x] = *reinterpret_cast<const f32x4 *>(qr + 16 * x + 4 * lg);
+            }
+        }
+    }
+    __device__ __forceinline__ void convert(float scale) {
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+            qs[i] = scale;
             if constexpr (T::F16) {
-                f32x4 v[T::HD / 32][2];
                 float mx = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < T::HD / 32; ++ks)
+                for (int x = 0; x < T::HD / 16; ++x)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        v[ks][x] = *reinterpret_cast<const f32x4 *>(qr + 32 * ks + 8 * lg + 4 * x);
-#pragma unroll
-                for (int ks = 0; ks < T::HD / 32; ++ks)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(v[ks][j / 4][j % 4]));
+                    for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fabsf(raw[i][x][j]));
                 mx = group_max(mx);
                 const int e = max(__builtin_amdgcn_frexp_expf(mx), -110);  // mx in [2^(e-1), 2^e)
                 const bool fin = mx > 0.0f && mx < INFINITY;
                 const float up = fin ? ldexpf(1.0f, 15 - e) : 1.0f;
-                qs[i] = fin ? ldexpf(a.scale, e - 15) : a.scale;
+                qs[i] = fin ? ldexpf(scale, e - 15) : scale;
 #pragma unroll
-                for (int ks = 0; ks < T::HD / 32; ++ks)
+                for (int ks = 0; ks < T::HD / 32; ++ks) {
+                    float w[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        _Float16 h, l;
-                        split_f16(v[ks][j / 4][j % 4] * up, h, l);
-                        hi[i][ks][j] = h;
-                        lo[i][ks][j] = l;
-                    }
-            } else {
-#pragma unroll
-                for (int x = 0; x < T::HD / 16; ++x)
-                    f[i][x] = *reinterpret_cast<const f32x4 *>(qr + 16 * x + 4 * lg);
+                    for (int j = 0; j < 8; ++j) w[j] = raw[i][2 * ks + j / 4][j % 4] * up;
+                    split_f16(w, hi[i][ks], lo[i][ks]);
+                }
             }
         }
     }
@@ -611,9 +664,10 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
     unsigned char *const mine = lds + wave * 2 * C::STAGE;
     uint32_t off[T::NU];
     dma_offsets<T>(off, row_b, lane);
-    Cursor cur = first_unit<KT, RT>(a, group, lane);
+    Requests req;
+    Cursor cur = first_unit<KT, RT>(a, group, lane, req);
     Seg g;
-    while (next_segment<KT, RT>(a, group, cur, g)) {
+    while (next_segment<KT, RT>(a, group, req, cur, g)) {
         lds_barrier();  // the last segment's reads of LDS are done
         const char *const kc = static_cast<const char *>(a.kc) + (size_t)g.h * T::ROWB;
         const char *const vc = static_cast<const char *>(a.vc) + (size_t)g.h * T::ROWB;
@@ -632,12 +686,13 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
             dma_group<T>(vc + at, dst + T::GROUPB, rows, off, row_b, lane, g.once);
         };
         const int t1 = g.lost ? g.t0 : g.t1;
+        Query<T, QT> q;
+        q.load(a, g, group, g.rb * RT, li, lg);
         if (g.t0 < t1) {
             look_up();
             load(g.t0);
         }
-        Query<T, QT> q;
-        q.load(a, g, group, g.rb * RT, li, lg);
+        q.convert(a.scale);
         f32x4 o[QT][DT];
         float m[QT], l[QT];
 #pragma unroll
@@ -727,14 +782,9 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
                         for (int r = 0; r < 4; ++r) o[i][d][r] *= alpha;
                 }
                 if constexpr (T::F16) {
+                    const float w[4] = {s[i][0][0], s[i][0][1], s[i][0][2], s[i][0][3]};
                     f16x4 ph, pl;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        _Float16 h, w;
-                        split_f16(s[i][0][r], h, w);
-                        ph[r] = h;
-                        pl[r] = w;
-                    }
+                    split_f16(w, ph, pl);
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
                         o[i][d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vh[d], ph, o[i][d], 0, 0, 0);
@@ -831,11 +881,12 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
     const int my_group = C::GPW == 2 ? wave : wave & 1;
     uint32_t off[T::NU];
     dma_offsets<T>(off, row_b, lane);
-    Cursor cur = first_unit<KT, RT>(a, group, lane);
+    Requests req;
+    Cursor cur = first_unit<KT, RT>(a, group, lane, req);
     if (tid == 0) bad_seg = 0;
     int seg = 0;
     Seg g;
-    while (next_segment<KT, RT>(a, group, cur, g)) {
+    while (next_segment<KT, RT>(a, group, req, cur, g)) {
         ++seg;
         lds_barrier();  // the last segment's reads of LDS are done, bad_seg is set up
         const char *const kc = static_cast<const char *>(a.kc) + (size_t)g.h * T::ROWB;
@@ -854,13 +905,14 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
             if (C::GPW == 2 || wave >= 2) dma_group<T>(vc + at, dst + C::TILE, rows, off, row_b, lane, g.once);
         };
         const int t1 = g.lost ? g.t0 : g.t1;
+        const int w_row = g.rb * RT + wave * 16 * QT;
+        Query<T, QT> q;
+        q.load(a, g, group, w_row, li, lg);
         if (g.t0 < t1) {
             look_up();
             load(g.t0);
         }
-        const int w_row = g.rb * RT + wave * 16 * QT;
-        Query<T, QT> q;
-        q.load(a, g, group, w_row, li, lg);
+        q.convert(a.scale);
         f32x4 o[QT][DT];
         float m[QT], l[QT];
         bool odd = false;
@@ -956,14 +1008,12 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
 #pragma unroll
                 for (int kk = 0; kk < ST / 2; ++kk)
 #pragma unroll
-                    for (int i = 0; i < QT; ++i)
+                    for (int i = 0; i < QT; ++i) {
+                        float w[8];
 #pragma unroll
-                        for (int r = 0; r < 8; ++r) {
-                            _Float16 h, w;
-                            split_f16(s[i][2 * kk + r / 4][r % 4], h, w);
-                            ph[kk][i][r] = h;
-                            pl[kk][i][r] = w;
-                        }
+                        for (int r = 0; r < 8; ++r) w[r] = s[i][2 * kk + r / 4][r % 4];
+                        split_f16(w, ph[kk][i], pl[kk][i]);
+                    }
                 const int row = 4 * lg + (li >> 2), c = (li & 3) >> 1;
                 auto v_at = [&](int e) {
                     // the k order of the fragments: rows 4 lg + j of both groups of 16
@@ -1049,15 +1099,14 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int
         const unsigned long long hit = __ballot(r >= s.r0 && r < s.r0 + s.n);
         if (hit && base < 0) {
             const int at = __ffsll((long long)hit) - 1;
-            base = uniform(total + __shfl(inc - v, at));
-            mine = SeqRows{__shfl(s.r0, at), __shfl(s.n, at), __shfl(s.cached, at)};
+            base = total + from_lane(inc - v, at);
+            mine = Requests{s}.at(a, at);
         }
-        total += __shfl(inc, 63);
+        total += from_lane(inc, 63);
     }
     if (base < 0) return;
-    mine = uniform(mine);
     const Work wk = work_of(mine, group, a.n_kv, kt, rt);
-    const Deal deal(uniform(total), a.wgs);
+    const Deal deal(total, a.wgs);
     const int h = head / group, rr = (r - mine.r0) * group + head - h * group;
     const long long u0 = base + ((long long)h * wk.blocks + rr / rt) * (kOpen + wk.tiles) + kOpen;
     const int w0 = uniform(deal.owner(u0)), w1 = uniform(deal.owner(u0 + wk.tiles - 1));
@@ -1145,7 +1194,7 @@ int launch_by_rows(cw_ctx *ctx, const TreeArgs &a) {
             if (rows <= 32) return launch_split<KVT, HD, 2>(ctx, a);
     }
     if constexpr (HD <= 128 && sizeof(KVT) == 2)
-        if (rows > 64) return launch_tile<KVT, HD, 2>(ctx, a);
+        if (rows > 256) return launch_tile<KVT, HD, 2>(ctx, a);
     return launch_tile<KVT, HD, 1>(ctx, a);
 }
 
