@@ -871,7 +871,7 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
     using T = Tile<KVT, HD>;
     constexpr int KT = C::KT, RT = C::RT, DT = T::DT, ST = C::ST;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
-    __shared__ int bad_seg;
+    __shared__ int bad_seg, odd_seg;  // the last segment without a block, with a V that is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
     const int group = a.n_heads / a.n_kv;
@@ -883,7 +883,7 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
     dma_offsets<T>(off, row_b, lane);
     Requests req;
     Cursor cur = first_unit<KT, RT>(a, group, lane, req);
-    if (tid == 0) bad_seg = 0;
+    if (tid == 0) bad_seg = odd_seg = 0;
     int seg = 0;
     Seg g;
     while (next_segment<KT, RT>(a, group, req, cur, g)) {
@@ -915,7 +915,6 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
         q.convert(a.scale);
         f32x4 o[QT][DT];
         float m[QT], l[QT];
-        bool odd = false;
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
             m[i] = -INFINITY;
@@ -936,15 +935,15 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
             const int k0 = t * KT;
             const unsigned char *const Ks = lds + (t & 1) * 2 * C::TILE, *const Vs = Ks + C::TILE;
             const bool tail = k0 + KT > g.s.cached;
-            if (tail) {
+            if (tail && (C::GPW == 2 || wave >= 2)) {  // the V rows that this wave loaded
                 int x = 0;
 #pragma unroll
-                for (int n = 0; n < C::TILE / 1024; ++n) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(Vs + n * 1024 + lane * 16);
+                for (int n = 0; n < T::NU; ++n) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(Vs + my_group * T::GROUPB + n * 1024 + lane * 16);
                     x |= not_finite<T::F16>(w.x) | not_finite<T::F16>(w.y) | not_finite<T::F16>(w.z) |
                          not_finite<T::F16>(w.w);
                 }
-                odd |= __any(x);
+                if (__any(x)) odd_seg = seg;
             }
             if (w_row >= g.nrows) continue;
             uint64_t vis[QT];
@@ -953,34 +952,46 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
                 for (int i = 0; i < QT; ++i)
                     vis[i] = sees64(a, g.s.r0 + q.node[i], q.node[i], g.s.n, k0 - g.s.cached) >> 4 * lg;
             }
-            // fragments are requested AHEAD products' steps before they are used
+            // Fragments are requested some steps before their products.  A product
+            // waits for the one before it of the same sum, so steps are of two
+            // sums: two tiles of rows, or two fragments for one.
+            constexpr int P = QT == 1 && T::F16 ? 2 : 1;
             f32x4 s[QT][ST];
-            constexpr int KA = T::KS < 4 ? T::KS : 4, KN = ST * T::KS;
-            typename T::frag kf[KA + 1];
-            auto k_at = [&](int e) { return k_frag<T>(Ks + e / T::KS * T::GROUPB, e % T::KS, li, lg); };
+            constexpr int KN = ST * T::KS, KA = KN < 4 ? KN : 4;
+            typename T::frag kf[KA + P];
+            auto k_n = [](int e) { return e / (P * T::KS) * P + e % P; };  // 16 positions, and
+            auto k_x = [](int e) { return e / P % T::KS; };                // part of their rows
+            auto k_at = [&](int e) { return k_frag<T>(Ks + k_n(e) * T::GROUPB, k_x(e), li, lg); };
 #pragma unroll
             for (int e = 0; e < KA; ++e) kf[e] = k_at(e);
 #pragma unroll
-            for (int e = 0; e < KN; ++e) {
-                if (e + KA < KN) kf[(e + KA) % (KA + 1)] = k_at(e + KA);
-                keep_order();
-                const typename T::frag k = kf[e % (KA + 1)];
-                const int n = e / T::KS, x = e % T::KS;
+            for (int e0 = 0; e0 < KN; e0 += P) {
 #pragma unroll
-                for (int i = 0; i < QT; ++i) {
-                    if (x == 0) s[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    if constexpr (T::F16) {
-                        s[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.hi[i][x], s[i][n], 0, 0, 0);
-                    } else {
+                for (int e = e0; e < e0 + P; ++e)
+                    if (e + KA < KN) kf[(e + KA) % (KA + P)] = k_at(e + KA);
+                keep_order();
+                if constexpr (T::F16) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+#pragma unroll
+                        for (int e = e0; e < e0 + P; ++e)
+#pragma unroll
+                            for (int i = 0; i < QT; ++i) {
+                                f32x4 &d = s[i][k_n(e)];
+                                if (half == 0 && k_x(e) == 0) d = f32x4{0.f, 0.f, 0.f, 0.f};
+                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    kf[e % (KA + P)], half ? q.lo[i][k_x(e)] : q.hi[i][k_x(e)], d, 0, 0, 0);
+                            }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < QT; ++i) {
+                        f32x4 &d = s[i][k_n(e0)];
+                        if (k_x(e0) == 0) d = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            s[i][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[r], q.f[i][x][r], s[i][n], 0, 0, 0);
+                            d = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e0 % (KA + P)][r], q.f[i][k_x(e0)][r], d, 0, 0, 0);
                     }
                 }
-                if constexpr (T::F16)
-#pragma unroll
-                    for (int i = 0; i < QT; ++i)
-                        s[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.lo[i][x], s[i][n], 0, 0, 0);
                 keep_order();
             }
             if (tail) {  // nodes: by the mask
@@ -1024,22 +1035,24 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
                     const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + T::GROUPB)));
                     return __builtin_bit_cast(f16x8, make_uint4(x.x, x.y, y.x, y.y));
                 };
-                constexpr int VA = 3, VN = DT * (ST / 2);
-                f16x8 vf[VA + 1];
+                constexpr int VA = 4, VN = DT * (ST / 2);
+                f16x8 vf[VA + P];
 #pragma unroll
                 for (int e = 0; e < VA; ++e) vf[e] = v_at(e);
 #pragma unroll
-                for (int e = 0; e < VN; ++e) {
-                    if (e + VA < VN) vf[(e + VA) % (VA + 1)] = v_at(e + VA);
+                for (int e0 = 0; e0 < VN; e0 += P) {
+#pragma unroll
+                    for (int e = e0; e < e0 + P; ++e)
+                        if (e + VA < VN) vf[(e + VA) % (VA + P)] = v_at(e + VA);
                     keep_order();
-                    const f16x8 v = vf[e % (VA + 1)];
-                    const int kk = e / DT, d = e % DT;
 #pragma unroll
-                    for (int i = 0; i < QT; ++i)
-                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[kk][i], o[i][d], 0, 0, 0);
+                    for (int half = 0; half < 2; ++half)
 #pragma unroll
-                    for (int i = 0; i < QT; ++i)
-                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[kk][i], o[i][d], 0, 0, 0);
+                        for (int e = e0; e < e0 + P; ++e)
+#pragma unroll
+                            for (int i = 0; i < QT; ++i)
+                                o[i][e % DT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    vf[e % (VA + P)], half ? pl[e / DT][i] : ph[e / DT][i], o[i][e % DT], 0, 0, 0);
                     keep_order();
                 }
             } else {
@@ -1062,8 +1075,9 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
                     }
             }
         }
-        if (g.t0 == t1) lds_barrier();  // (no tile's barrier made bad_seg known)
-        if (odd) {  // every wave has seen every V
+        // the last tile's odd_seg, or (no tile) bad_seg, known to all
+        if (g.t0 == t1 || t1 * KT > g.s.cached) lds_barrier();
+        if (uniform(odd_seg) == seg) {
             one_by_one<KVT, HD, RT>(a, g, group, KT, T::UP);
             continue;
         }
