@@ -1094,6 +1094,283 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
     }
 }
 
+// ---- more rows over an f32 cache.  The f32 products of the matrix cores run
+// at a sixteenth of the f16 rate, so K and V are split as q and the weights are
+// (hi + lo in f16, 22 bits) and take three products instead of one: hi hi, hi lo
+// and lo hi.  A wave loads its share of a tile into registers, scales it by the
+// power of two that brings its largest value to 2^14 .. 2^15, and leaves hi and
+// lo in LDS with that exponent: K's is undone in the scores' factor, V's in the
+// weights, against the largest exponent so far (which o follows as it does the
+// running maximum).
+template <int HD_, int QT>
+struct WideCfg : Tile<_Float16, HD_> {
+    typedef Tile<_Float16, HD_> T;
+    static constexpr int KT = HD_ == 64 ? 64 : 32, RT = 64 * QT, ST = KT / 16;
+    static constexpr int PW = KT / 4;                // positions of a wave
+    static constexpr int LPR = HD_ / 4;              // lanes of a row
+    static constexpr int NL = PW * LPR / 64;         // loads of its K
+    static constexpr int HALF = KT * T::ROWB;        // hi or lo of a tile's K or V
+    static constexpr int LDS = 2 * 4 * HALF;
+    static constexpr int PER_CU = LDS <= 72 * 1024 ? 2 : 1;
+};
+
+template <int HD, int QT>
+__global__ __launch_bounds__(256, (WideCfg<HD, QT>::PER_CU)) void tree_wide_kernel(TreeArgs a) {
+    using C = WideCfg<HD, QT>;
+    using T = Tile<_Float16, HD>;
+    constexpr int KT = C::KT, RT = C::RT, DT = T::DT, ST = C::ST, PW = C::PW, NL = C::NL;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
+    __shared__ int w_exp[2][2][4];    // exponents of a tile's K and V, a wave each
+    __shared__ int bad_seg, odd_seg;  // the last segment without a block, with a value that is not finite
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int li = lane & 15, lg = lane >> 4;
+    const int group = a.n_heads / a.n_kv;
+    const size_t row_f = (size_t)a.n_kv * HD;
+    const int my_group = wave * PW / 16, my_row = wave * PW % 16 + lane / C::LPR;  // of 16 positions
+    Requests req;
+    Cursor cur = first_unit<KT, RT>(a, group, lane, req);
+    if (tid == 0) bad_seg = odd_seg = 0;
+    int seg = 0;
+    Seg g;
+    while (next_segment<KT, RT>(a, group, req, cur, g)) {
+        ++seg;
+        lds_barrier();  // the last segment's reads of LDS are done, bad_seg is set up
+        const float *const kc = static_cast<const float *>(a.kc) + (size_t)g.h * HD + lane % C::LPR * 4;
+        const float *const vc = static_cast<const float *>(a.vc) + (size_t)g.h * HD + lane % C::LPR * 4;
+        int slots = 0, tb = g.t0;
+        auto look_up = [&]() {
+            slots = slot16(a, g, (tb + lane) * ST + my_group);
+            if (__any(slots < 0 && tb + lane < g.t1)) bad_seg = seg;
+            slots = max(slots, 0);  // a block has 16 positions: in the cache, and the row is lost
+        };
+        f32x4 rk[NL], rv[NL];
+        auto load = [&](int t) {
+            if (t - tb == 64) {
+                tb += 64;
+                look_up();
+            }
+            const int slot = __builtin_amdgcn_readlane(slots, t - tb);
+            const int rows = g.last - (min(t * ST + my_group, g.last >> 4) << 4);
+#pragma unroll
+            for (int n = 0; n < NL; ++n) {
+                const size_t at = (size_t)(slot + min(my_row + n * (64 / C::LPR), rows)) * row_f;
+                rk[n] = *reinterpret_cast<const f32x4 *>(kc + at);
+                rv[n] = *reinterpret_cast<const f32x4 *>(vc + at);
+            }
+        };
+        // the loaded rows, scaled and split, into LDS
+        auto store = [&](int t) {
+            unsigned char *const buf = lds + (t & 1) * 4 * C::HALF;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                f32x4(&r)[NL] = x ? rv : rk;
+                uint32_t top = 0;  // of the magnitudes' bits: ordered as the values, then inf and NaN
+#pragma unroll
+                for (int n = 0; n < NL; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float w = r[n][e];
+                        top = max(top, __builtin_bit_cast(uint32_t, w) & 0x7fffffffu);
+                    }
+#define CW_MAX_STEP(ctrl, rows) top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, ctrl, rows, 0xf, true))
+                CW_MAX_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8
+                CW_MAX_STEP(0x112, 0xf);
+                CW_MAX_STEP(0x114, 0xf);
+                CW_MAX_STEP(0x118, 0xf);
+                CW_MAX_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+                CW_MAX_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef CW_MAX_STEP
+                top = (uint32_t)__builtin_amdgcn_readlane((int)top, 63);
+                if (top >= 0x7f800000u) odd_seg = seg;
+                const int e = max((int)(top >> 23) - 126, -100);  // all below 2^e
+                const float up = __builtin_bit_cast(float, (uint32_t)(15 - min(e, 128) + 127) << 23);
+                w_exp[t & 1][x][wave] = e;
+#pragma unroll
+                for (int n = 0; n < NL; ++n) {
+                    const float w[4] = {r[n][0] * up, r[n][1] * up, r[n][2] * up, r[n][3] * up};
+                    f16x4 hi, lo;
+                    split_f16(w, hi, lo);
+                    const int row = wave * PW + lane / C::LPR + n * (64 / C::LPR), c = lane % C::LPR;
+                    unsigned char *const p = buf + x * 2 * C::HALF + row * T::ROWB +
+                                             (((c >> 1) ^ (row & T::SWZ)) << 4) + (c & 1) * 8;
+                    *reinterpret_cast<f16x4 *>(p) = hi;
+                    *reinterpret_cast<f16x4 *>(p + C::HALF) = lo;
+                }
+            }
+        };
+        const int t1 = g.lost ? g.t0 : g.t1;
+        const int w_row = g.rb * RT + wave * 16 * QT;
+        Query<T, QT> q;
+        q.load(a, g, group, w_row, li, lg);
+        if (g.t0 < t1) {
+            look_up();
+            load(g.t0);
+        }
+        q.convert(a.scale);
+        if (g.t0 < t1) {
+            store(g.t0);
+            if (g.t0 + 1 < t1) load(g.t0 + 1);
+        }
+        f32x4 o[QT][DT];
+        float m[QT], l[QT];
+        int E = -10000;  // o counts 2^(E - 15)
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        for (int t = g.t0; t < t1; ++t) {
+            lds_barrier();  // tile t is there, the other buffer free
+            const int k0 = t * KT;
+            const unsigned char *const Ks = lds + (t & 1) * 4 * C::HALF, *const Vs = Ks + 2 * C::HALF;
+            if (w_row < g.nrows) {
+                uint64_t vis[QT];
+                const bool tail = k0 + KT > g.s.cached;
+                if (tail) {
+#pragma unroll
+                    for (int i = 0; i < QT; ++i)
+                        vis[i] = sees64(a, g.s.r0 + q.node[i], q.node[i], g.s.n, k0 - g.s.cached) >> 4 * lg;
+                }
+                constexpr int P = QT == 1 ? 2 : 1;  // sums in flight, as above
+                f32x4 s[QT][ST];
+                constexpr int KN = ST * T::KS, KA = 2;
+                typename T::frag kh[KA + P], kl[KA + P];
+                auto k_n = [](int e) { return e / (P * T::KS) * P + e % P; };
+                auto k_x = [](int e) { return e / P % T::KS; };
+                auto k_get = [&](int e) {
+                    kh[e % (KA + P)] = k_frag<T>(Ks + k_n(e) * T::GROUPB, k_x(e), li, lg);
+                    kl[e % (KA + P)] = k_frag<T>(Ks + C::HALF + k_n(e) * T::GROUPB, k_x(e), li, lg);
+                };
+#pragma unroll
+                for (int e = 0; e < KA; ++e) k_get(e);
+#pragma unroll
+                for (int e0 = 0; e0 < KN; e0 += P) {
+#pragma unroll
+                    for (int e = e0; e < e0 + P; ++e)
+                        if (e + KA < KN) k_get(e + KA);
+                    keep_order();
+#pragma unroll
+                    for (int part = 0; part < 3; ++part)
+#pragma unroll
+                        for (int e = e0; e < e0 + P; ++e)
+#pragma unroll
+                            for (int i = 0; i < QT; ++i) {
+                                f32x4 &d = s[i][k_n(e)];
+                                if (part == 0 && k_x(e) == 0) d = f32x4{0.f, 0.f, 0.f, 0.f};
+                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    part == 2 ? kl[e % (KA + P)] : kh[e % (KA + P)],
+                                    part == 1 ? q.lo[i][k_x(e)] : q.hi[i][k_x(e)], d, 0, 0, 0);
+                            }
+                    keep_order();
+                }
+                // the tile's exponents: K's of this lane's positions, V's against all so far
+                float kf[ST], vf_[ST];
+                int top = E;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) top = max(top, w_exp[t & 1][1][w]);
+#pragma unroll
+                for (int n = 0; n < ST; ++n) {
+                    const int w = (16 * n + 4 * lg) / PW;
+                    kf[n] = ldexpf(1.0f, w_exp[t & 1][0][w] - 15);
+                    vf_[n] = ldexpf(1.0f, w_exp[t & 1][1][w] - top);
+                }
+                const float down = ldexpf(1.0f, E - top);
+                const bool grown = uniform(top) > uniform(E);
+                E = top;
+#pragma unroll
+                for (int i = 0; i < QT; ++i)
+#pragma unroll
+                    for (int n = 0; n < ST; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            s[i][n][r] *= kf[n];
+                            if (tail) s[i][n][r] = vis[i] >> (n * 16 + r) & 1 ? s[i][n][r] : -INFINITY;
+                        }
+#pragma unroll
+                for (int i = 0; i < QT; ++i) {
+                    const float before = m[i];
+                    const float alpha = soften<ST>(s[i], q.qs[i], T::UP, m[i], l[i]) * down;
+                    if (grown || __any(m[i] > before)) {
+#pragma unroll
+                        for (int d = 0; d < DT; ++d)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) o[i][d][r] *= alpha;
+                    }
+                }
+                f16x8 ph[ST / 2][QT], pl[ST / 2][QT];
+#pragma unroll
+                for (int kk = 0; kk < ST / 2; ++kk)
+#pragma unroll
+                    for (int i = 0; i < QT; ++i) {
+                        float w[8];
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) w[r] = s[i][2 * kk + r / 4][r % 4] * vf_[2 * kk + r / 4];
+                        split_f16(w, ph[kk][i], pl[kk][i]);
+                    }
+                const int row = 4 * lg + (li >> 2), c = (li & 3) >> 1;
+                auto v_at = [&](const unsigned char *base, int e) {
+                    const unsigned char *p = base + e / DT * 2 * T::GROUPB + row * T::ROWB +
+                                             (((2 * (e % DT) + c) ^ (row & T::SWZ)) << 4) + (li & 1) * 8;
+                    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
+                    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + T::GROUPB)));
+                    return __builtin_bit_cast(f16x8, make_uint4(x.x, x.y, y.x, y.y));
+                };
+                constexpr int VA = 2, VN = DT * (ST / 2);
+                f16x8 vh[VA + P], vl[VA + P];
+                auto v_get = [&](int e) {
+                    vh[e % (VA + P)] = v_at(Vs, e);
+                    vl[e % (VA + P)] = v_at(Vs + C::HALF, e);
+                };
+#pragma unroll
+                for (int e = 0; e < VA; ++e) v_get(e);
+#pragma unroll
+                for (int e0 = 0; e0 < VN; e0 += P) {
+#pragma unroll
+                    for (int e = e0; e < e0 + P; ++e)
+                        if (e + VA < VN) v_get(e + VA);
+                    keep_order();
+#pragma unroll
+                    for (int part = 0; part < 3; ++part)
+#pragma unroll
+                        for (int e = e0; e < e0 + P; ++e)
+#pragma unroll
+                            for (int i = 0; i < QT; ++i)
+                                o[i][e % DT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    part == 2 ? vl[e % (VA + P)] : vh[e % (VA + P)],
+                                    part == 1 ? pl[e / DT][i] : ph[e / DT][i], o[i][e % DT], 0, 0, 0);
+                    keep_order();
+                }
+            }
+            if (t + 1 < t1) {
+                store(t + 1);
+                if (t + 2 < t1) load(t + 2);
+            }
+        }
+        lds_barrier();  // bad_seg and odd_seg are known to all
+        if (uniform(odd_seg) == seg) {
+            one_by_one<float, HD, RT>(a, g, group, KT, T::UP);
+            continue;
+        }
+        const bool bad = g.lost || bad_seg == seg;
+        const float unit = ldexpf(1.0f, max(E, -200) - 15);
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+            l[i] = group_sum(l[i]);
+            if (w_row + i * 16 + li >= g.nrows) continue;
+#pragma unroll
+            for (int n = 0; n < DT; ++n) {
+                f32x4 v = o_quad<T>(o[i], n);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] *= unit;
+                put<HD, RT>(a, g, group, wave * 16 * QT + i * 16 + li, o_col<T>(n, lg), v, m[i],
+                            bad ? NAN : l[i]);
+            }
+        }
+    }
+}
+
 // Joins the partials of the rows whose units went to more than one workgroup,
 // in the order of the positions: a wave a (row, head), the lanes four elements
 // of every 256 / HD-th partial.
@@ -1193,9 +1470,14 @@ template <typename KVT, int HD, int QT>
 int launch_split(cw_ctx *ctx, const TreeArgs &a) {
     return launch_tiles<SplitCfg<KVT, HD, QT>>(ctx, a, tree_split_kernel<KVT, HD, QT>);
 }
-template <typename KVT, int HD, int QT>
+template <int HD, int QT>
 int launch_tile(cw_ctx *ctx, const TreeArgs &a) {
-    return launch_tiles<TileCfg<KVT, HD, QT>>(ctx, a, tree_tile_kernel<KVT, HD, QT>);
+    return launch_tiles<TileCfg<_Float16, HD, QT>>(ctx, a, tree_tile_kernel<_Float16, HD, QT>);
+}
+
+template <int HD, int QT>
+int launch_wide(cw_ctx *ctx, const TreeArgs &a) {
+    return launch_tiles<WideCfg<HD, QT>>(ctx, a, tree_wide_kernel<HD, QT>);
 }
 
 // By the rows of a (request, kv head) on average.
@@ -1207,9 +1489,13 @@ int launch_by_rows(cw_ctx *ctx, const TreeArgs &a) {
         if constexpr (HD <= 128)
             if (rows <= 32) return launch_split<KVT, HD, 2>(ctx, a);
     }
-    if constexpr (HD <= 128 && sizeof(KVT) == 2)
-        if (rows > 256) return launch_tile<KVT, HD, 2>(ctx, a);
-    return launch_tile<KVT, HD, 1>(ctx, a);
+    if constexpr (sizeof(KVT) == 4) {
+        return launch_wide<HD, 1>(ctx, a);
+    } else {
+        if constexpr (HD <= 128)
+            if (rows > 256) return launch_tile<HD, 2>(ctx, a);
+        return launch_tile<HD, 1>(ctx, a);
+    }
 }
 
 template <typename KVT>
