@@ -56,12 +56,32 @@ template <typename T, int N>
 struct alignas(sizeof(T) * N) Vec {
     T v[N];
 };
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// A unit that is read once (non-temporal: 4,100 rows with the cache write 36.7
+// -> 32.4 us)
+template <int V>
+__device__ __forceinline__ void read_once(float *to, const float *from) {
+    if constexpr (V == 4)
+        *reinterpret_cast<f32x4 *>(to) = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(from));
+    else
+        *to = *from;
+}
+template <int V, bool STREAM>
+__device__ __forceinline__ void put_unit(float *to, const float *from) {
+    if constexpr (STREAM)
+        __builtin_nontemporal_store(*reinterpret_cast<const f32x4 *>(from), reinterpret_cast<f32x4 *>(to));
+    else
+        *reinterpret_cast<Vec<float, V> *>(to) = *reinterpret_cast<const Vec<float, V> *>(from);
+}
 
 // Workgroup (row, part of the heads).  A unit is V pairs (a thread reads V
 // elements from either half, or 2 V in a row) or V copied elements; U units make
 // a head, `par` heads a round, and a thread keeps its unit's cosines for every
-// head it takes.  V = 4 where rows are 16-byte aligned, 1 where not.
-template <typename KVT, int V, bool PAIRS, bool CACHE>
+// head it takes.  V = 4 where rows are 16-byte aligned, 1 where not.  STREAM: y
+// is written past the caches.
+template <typename KVT, int V, bool PAIRS, bool CACHE, bool STREAM = false>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a, int U, int par) {
     const int r = blockIdx.x, pos = a.positions[r];
     if (pos < 0) return;
@@ -81,15 +101,14 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a, int U, 
     const bool write = CACHE && (unsigned)slot < (unsigned)a.n_slots;
     const int heads = write ? a.heads + 2 * a.kv_heads : a.heads;
     const float *row = a.x + (size_t)r * a.x_stride;
-    using F = Vec<float, V>;
     for (int h = blockIdx.y * par + tid / U; h < heads; h += gridDim.y * par) {
         const bool q = h < a.heads, k = h < a.heads + a.kv_heads;
         if (q && !rotates && !a.copy) continue;
         const float *src = row + (size_t)h * a.hd;
         Vec<float, 2 * V> x;
-        *reinterpret_cast<F *>(x.v) = *reinterpret_cast<const F *>(src + i0);
+        read_once<V>(x.v, src + i0);
         if (rotates) {
-            *reinterpret_cast<F *>(x.v + V) = *reinterpret_cast<const F *>(src + i1);
+            read_once<V>(x.v + V, src + i1);
             if (k) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
@@ -102,8 +121,8 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a, int U, 
         }
         if (q) {
             float *dst = a.y + (size_t)r * a.y_stride + (size_t)h * a.hd;
-            *reinterpret_cast<F *>(dst + i0) = *reinterpret_cast<F *>(x.v);
-            if (rotates) *reinterpret_cast<F *>(dst + i1) = *reinterpret_cast<F *>(x.v + V);
+            put_unit<V, STREAM>(dst + i0, x.v);
+            if (rotates) put_unit<V, STREAM>(dst + i1, x.v + V);
         } else if constexpr (CACHE) {
             const int g = h - a.heads - (k ? 0 : a.kv_heads);
             KVT *dst = static_cast<KVT *>(k ? a.kc : a.vc) +
@@ -119,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a, int U, 
 }
 
 template <typename KVT, bool CACHE>
-int launch_rope(cw_ctx *ctx, const char *label, const RopeArgs &a, bool wide) {
+int launch_rope(cw_ctx *ctx, const char *label, const RopeArgs &a, bool wide, bool stream = false) {
     const int V = wide ? 4 : 1;
     const bool tail = a.copy || (CACHE && a.hd > a.rot);
     const int U = a.rot / (2 * V) + (tail ? (a.hd - a.rot) / V : 0);
@@ -130,12 +149,17 @@ int launch_rope(cw_ctx *ctx, const char *label, const RopeArgs &a, bool wide) {
                               : rope_rows_kernel<KVT, 4, false, CACHE>)
                    : (a.pairs ? rope_rows_kernel<KVT, 1, true, CACHE>
                               : rope_rows_kernel<KVT, 1, false, CACHE>);
+    if constexpr (!CACHE)
+        if (wide && stream)
+            fn = a.pairs ? rope_rows_kernel<KVT, 4, true, false, true>
+                         : rope_rows_kernel<KVT, 4, false, false, true>;
     return launch(ctx, label, fn, grid, dim3(kThreads), 0, a, U, par);
 }
 
 // ---------------------------------------------------------------- block tables
 
-constexpr int kScan = 1024;  // threads of the one workgroup that sums lengths
+constexpr int kScan = 1024;     // threads of the one workgroup that sums lengths
+constexpr int kLdsSeqs = 4095;  // requests whose offsets are searched in LDS
 
 // Where each request's rows, new blocks and returned blocks begin; [n_seq + 1] each.
 struct Offsets {
@@ -151,32 +175,35 @@ struct TableArgs {
     Offsets off;
 };
 
+// The last b with first[b] <= i
+__device__ __forceinline__ int owner(const int *first, int n, int i) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (first[m] <= i) lo = m;
+        else hi = m;
+    }
+    return lo;
+}
+
 // Positions and slots of rows item, item + step, ...; table entries of new
 // blocks likewise.  top: free blocks once the returned ones are back.
-__device__ void fill_tables(const TableArgs &a, int item, int step, int live, int top) {
-    const int n = a.n_seq, R = a.off.first[n], D = a.off.need[n];
-    auto owner = [n](const int *first, int i) {  // the last b with first[b] <= i
-        int lo = 0, hi = n;
-        while (hi - lo > 1) {
-            const int m = (lo + hi) >> 1;
-            if (first[m] <= i) lo = m;
-            else hi = m;
-        }
-        return lo;
-    };
+__device__ void fill_tables(const TableArgs &a, const int *first, const int *need, int item, int step,
+                            int live, int top) {
+    const int n = a.n_seq, R = first[n], D = need[n];
     for (int i = item; live && i < D; i += step) {
-        const int b = owner(a.off.need, i), k = i - a.off.need[b];
-        const int had = a.held_out[b] - (a.off.need[b + 1] - a.off.need[b]);
+        const int b = owner(need, n, i), k = i - need[b];
+        const int had = a.held_out[b] - (need[b + 1] - need[b]);
         a.tables[(size_t)b * a.max_blocks + had + k] = a.free_list[top - 1 - i];
     }
     for (int r = item; r < a.rows; r += step) {
         int pos = -1, slot = -1;
         if (live && r < R) {
-            const int b = owner(a.off.first, r), i = r - a.off.first[b], c = a.cached[b];
+            const int b = owner(first, n, r), i = r - first[b], c = a.cached[b];
             const int e = (c + i) >> a.shift;
-            const int had = a.held_out[b] - (a.off.need[b + 1] - a.off.need[b]);
+            const int had = a.held_out[b] - (need[b + 1] - need[b]);
             const int id = e < had ? a.tables[(size_t)b * a.max_blocks + e]
-                                   : a.free_list[top - 1 - (a.off.need[b] + e - had)];
+                                   : a.free_list[top - 1 - (need[b] + e - had)];
             if ((unsigned)id < (unsigned)a.n_blocks)
                 slot = (id << a.shift) + ((c + i) & (a.page - 1));
             int depth = i;
@@ -195,48 +222,52 @@ __device__ void fill_tables(const TableArgs &a, int item, int step, int live, in
 
 // One workgroup: thread t sums the lengths of a run of requests, a scan over
 // the threads gives each its offsets, and a second walk writes them; then the
-// returned blocks.  FILL: the rows and tables too (few of either).
+// returned blocks.  FILL: the rows and tables too, offsets in LDS (few of
+// either; at most kLdsSeqs requests).  Bound by its chain of loads: lengths,
+// then table and free list.
 template <bool FILL>
 __global__ __launch_bounds__(kScan) void block_scan_kernel(TableArgs a) {
     __shared__ long long part[3][kScan / 64];
     __shared__ int flags, bad;
+    __shared__ int s_first[FILL ? kLdsSeqs + 1 : 1], s_need[FILL ? kLdsSeqs + 1 : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n_seq;
+    int *const first = FILL ? s_first : a.off.first, *const need_at = FILL ? s_need : a.off.need;
     if (tid == 0) flags = bad = 0;
-    __syncthreads();
     const int per = (n + kScan - 1) / kScan, b0 = min(n, tid * per), b1 = min(n, b0 + per);
     const int n_free = *a.n_free;
-    auto lengths = [&](int b, int &rows, int &need, int &give, int &held) {
-        const int c = a.cached[b], f = a.fresh[b];
-        held = a.held[b];
-        const long long len = f < 0 ? 0 : (long long)c + f;
-        const bool ok = c >= 0 && held >= 0 && held <= a.max_blocks && len <= 0x7fffffff;
-        const long long blocks = (len + a.page - 1) >> a.shift;  // at most 2^28 each
-        rows = max(f, 0);
-        give = f < 0 ? held : 0;
-        need = f < 0 || blocks < held ? 0 : (int)(blocks - held);
-        return ok;
-    };
-    long long sum[3] = {0, 0, 0};
-    for (int b = b0; b < b1; ++b) {
+    struct Lengths {
         int rows, need, give, held;
-        if (!lengths(b, rows, need, give, held)) {
-            bad = 1;  // (every writer writes the same)
+        bool ok;
+    };
+    auto lengths = [&](int b) {
+        const int c = a.cached[b], f = a.fresh[b], held = a.held[b];
+        const long long len = f < 0 ? 0 : (long long)c + f;
+        const long long blocks = (len + a.page - 1) >> a.shift;  // at most 2^28 each
+        return Lengths{max(f, 0), f < 0 || blocks < held ? 0 : (int)(blocks - held), f < 0 ? held : 0,
+                       held, c >= 0 && held >= 0 && held <= a.max_blocks && len <= 0x7fffffff};
+    };
+    Lengths mine{};  // of the first request, kept for the second walk
+    long long sum[3] = {0, 0, 0};
+    int over = 0, wrong = 0;
+    for (int b = b0; b < b1; ++b) {
+        const Lengths x = lengths(b);
+        if (b == b0) mine = x;
+        if (!x.ok) {
+            wrong = 1;
             continue;
         }
-        if (held + need > a.max_blocks) atomicOr(&flags, CW_BLOCKS_TABLE);
-        sum[0] += rows;
-        sum[1] += need;
-        sum[2] += give;
+        over |= x.held + x.need > a.max_blocks;
+        sum[0] += x.rows;
+        sum[1] += x.need;
+        sum[2] += x.give;
     }
+    __syncthreads();
+    if (over) flags = CW_BLOCKS_TABLE;  // (every writer writes the same)
+    if (wrong) bad = 1;
     long long inc[3];
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-        inc[k] = sum[k];
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const long long o = __shfl_up(inc[k], d);
-            if (lane >= d) inc[k] += o;
-        }
+        inc[k] = wave_scan(sum[k], lane);
         if (lane == 63) part[k][wave] = inc[k];
     }
     __syncthreads();
@@ -254,72 +285,102 @@ __global__ __launch_bounds__(kScan) void block_scan_kernel(TableArgs a) {
     }
     const long long back = n_free + total[2];
     int st = flags;
-    if (bad || n_free < 0 || back > a.n_blocks) st = CW_BLOCKS_BAD;
-    else {
+    if (bad || n_free < 0 || back > a.n_blocks) {
+        st = CW_BLOCKS_BAD;
+    } else {
         if (total[0] > a.rows) st |= CW_BLOCKS_ROWS;
         if (total[1] > back) st |= CW_BLOCKS_FREE;
     }
     const int live = st == 0, top = (int)back;
+    const bool gives = live && total[2] > 0;
     for (int b = b0; b < b1; ++b) {
-        int rows, need, give, held;
-        lengths(b, rows, need, give, held);
-        a.off.first[b] = live ? (int)inc[0] : 0;
-        a.off.need[b] = live ? (int)inc[1] : 0;
-        a.off.give[b] = live ? (int)inc[2] : 0;
-        a.first_row[b] = live ? (int)inc[0] : 0;
-        a.held_out[b] = live ? held + need - give : held;
-        inc[0] += rows;
-        inc[1] += need;
-        inc[2] += give;
+        const Lengths x = b == b0 ? mine : lengths(b);
+        first[b] = a.first_row[b] = live ? (int)inc[0] : 0;
+        need_at[b] = live ? (int)inc[1] : 0;
+        if (gives) a.off.give[b] = (int)inc[2];
+        a.held_out[b] = live ? x.held + x.need - x.give : x.held;
+        inc[0] += x.rows;
+        inc[1] += x.need;
+        inc[2] += x.give;
     }
     if (tid == 0) {
-        a.off.first[n] = a.first_row[n] = live ? (int)total[0] : 0;
-        a.off.need[n] = live ? (int)total[1] : 0;
-        a.off.give[n] = live ? (int)total[2] : 0;
+        first[n] = a.first_row[n] = live ? (int)total[0] : 0;
+        need_at[n] = live ? (int)total[1] : 0;
+        if (gives) a.off.give[n] = (int)total[2];
         a.n_free_out[0] = live ? top - (int)total[1] : n_free;
         a.status[0] = st;
     }
     __syncthreads();
-    if (live) {  // returned blocks, one request a wave
-        for (int b = wave; b < n; b += kScan / 64) {
-            const int g0 = a.off.give[b], g = a.off.give[b + 1] - g0;
-            for (int j = lane; j < g; j += 64)
-                a.free_list[n_free + g0 + j] = a.tables[(size_t)b * a.max_blocks + j];
+    if (gives) {  // returned blocks
+        for (int j = tid; j < (int)total[2]; j += kScan) {
+            const int b = owner(a.off.give, n, j);
+            a.free_list[n_free + j] = a.tables[(size_t)b * a.max_blocks + j - a.off.give[b]];
         }
         __syncthreads();
     }
-    if (FILL) fill_tables(a, tid, kScan, live, top);
+    if (FILL) fill_tables(a, first, need_at, tid, kScan, live, top);
 }
 
 // Rows and table entries, over the chip, behind block_scan_kernel<false>.
 __global__ __launch_bounds__(kThreads) void block_fill_kernel(TableArgs a) {
-    const int live = a.status[0] == 0;
-    const int top = a.n_free_out[0] + a.off.need[a.n_seq];
-    fill_tables(a, blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads, live, top);
+    __shared__ int s_first[kLdsSeqs + 1], s_need[kLdsSeqs + 1];
+    const int n = a.n_seq, live = a.status[0] == 0;
+    const int top = a.n_free_out[0] + a.off.need[n];
+    const int *first = a.off.first, *need = a.off.need;
+    if (n <= kLdsSeqs) {
+        for (int b = threadIdx.x; b <= n; b += kThreads) {
+            s_first[b] = first[b];
+            s_need[b] = need[b];
+        }
+        __syncthreads();
+        first = s_first;
+        need = s_need;
+    }
+    fill_tables(a, first, need, blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads, live, top);
 }
 
 // ---------------------------------------------------------------- accepted rows
 //
 // Row cached + i takes row cached + path[i], path increasing, so path[i] >= i
 // and no row is read after an earlier move wrote it: a thread that moves its 16
-// bytes of a row in order of i needs no copy of the rows, and may have several
-// loads in flight (a load's row is never among the rows stored before it).
-__global__ __launch_bounds__(kThreads) void accept_kernel(PageMap m, uint4 *k, uint4 *v,
+// bytes of a row in order of i needs no copy of the rows, and has the loads of
+// eight moves in flight (a load's row is never among the rows stored before it).
+// Lane i of each wave looks up move i.
+__global__ __launch_bounds__(kThreads) void accept_kernel(PageMap m, u32x4 *k, u32x4 *v,
                                                           int row_u4, const int *cached,
                                                           const int *path, int max_path,
                                                           const int *path_len, int *cached_out) {
-    const int b = blockIdx.y, c = cached[b];
+    constexpr int D = 8;
+    const int b = blockIdx.y, lane = threadIdx.x & 63, c = cached[b];
     const int n = min(max(path_len[b], 0), max_path);
     const int u = blockIdx.x * kThreads + threadIdx.x;
     if (u == 0 && cached_out) cached_out[b] = c + n;
-    if (u >= 2 * row_u4 || c < 0) return;
-    uint4 *const base = u < row_u4 ? k + u : v + (u - row_u4);
-    for (int i = 0; i < n; ++i) {
-        const int node = path[(size_t)b * max_path + i];
-        if (node < 0 || node > (1 << 30) || c > (1 << 30) || node == i) continue;
-        const int src = slot_of(m, b, c + node), dst = slot_of(m, b, c + i);
-        if (src < 0 || dst < 0) continue;
-        base[(size_t)dst * row_u4] = base[(size_t)src * row_u4];
+    if (c < 0 || c > 1 << 30) return;
+    const bool on = u < 2 * row_u4;
+    u32x4 *const base = u < row_u4 ? k + u : v + (on ? u - row_u4 : 0);
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        int src = -1, dst = -1;
+        if (i0 + lane < n) {
+            const int node = path[(size_t)b * max_path + i0 + lane];
+            if (node >= 0 && node <= 1 << 30 && node != i0 + lane) {
+                src = slot_of(m, b, c + node);
+                dst = slot_of(m, b, c + i0 + lane);
+            }
+            if (src < 0 || dst < 0) src = dst = -1;
+        }
+        for (int i = 0; i < min(n - i0, 64); i += D) {
+            u32x4 w[D];
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                // (without a move: slot 0, not stored)
+                w[d] = base[(size_t)max(__builtin_amdgcn_readlane(src, i + d), 0) * row_u4];
+            }
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                const int t = __builtin_amdgcn_readlane(dst, i + d);
+                if (on && t >= 0) base[(size_t)t * row_u4] = w[d];
+            }
+        }
     }
 }
 
@@ -525,7 +586,12 @@ int cw_rope_rows(cw_ctx *ctx, const cw_rope_spec *spec, const float *x, size_t x
     a.copy = !in_place && head_dim > spec->rot_dim;
     const bool wide = aligned16(x) && aligned16(y) && x_stride % 4 == 0 && y_stride % 4 == 0 &&
                       head_dim % 4 == 0 && a.rot % 8 == 0;
-    return launch_rope<float, false>(ctx, "rope_rows", a, wide);
+    // Past 32 MB (the eight L2s) whoever reads y next finds it in none of them;
+    // written past them 6,000 rows of 40 heads take 43.2 us, else 49.2.  With the
+    // cache write below, whose rows end in two places, it gains nothing (32.4
+    // against 35.2 us for 4,100 rows).
+    const bool stream = (size_t)rows * width * sizeof(float) > (size_t)32 << 20;
+    return launch_rope<float, false>(ctx, "rope_rows", a, wide, stream);
 }
 
 int cw_rope_kv_rows(cw_ctx *ctx, const cw_rope_spec *spec, const cw_kv_pages *kv,
@@ -595,7 +661,7 @@ int cw_block_tables(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const
                 kv->n_blocks, b->max_blocks, b->mask, b->mask_words, b->tables, held_out,
                 free_list, n_free_out, b->first_row, positions, slots, status,
                 Offsets{s, s + n, s + 2 * n}};
-    if (b->rows <= 2 * kScan)
+    if (b->rows <= 2 * kScan && b->n_seq <= kLdsSeqs)
         return launch(ctx, "block_tables", block_scan_kernel<true>, dim3(1), dim3(kScan), 0, a);
     CW_TRY(launch(ctx, "block_tables", block_scan_kernel<false>, dim3(1), dim3(kScan), 0, a));
     const int blocks = std::min((b->rows + kThreads - 1) / kThreads, 4 * ctx->n_cu);
@@ -613,7 +679,7 @@ int cw_kv_accept(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const in
     const int row_u4 = kv->n_kv_heads * kv->head_dim * (kv->kv_dtype == CW_F16 ? 2 : 4) / 16;
     const dim3 grid((2 * row_u4 + kThreads - 1) / kThreads, b->n_seq);
     return launch(ctx, "kv_accept", accept_kernel, grid, dim3(kThreads), 0, map,
-                  static_cast<uint4 *>(kv->k), static_cast<uint4 *>(kv->v), row_u4, b->cached, path,
+                  static_cast<u32x4 *>(kv->k), static_cast<u32x4 *>(kv->v), row_u4, b->cached, path,
                   max_path, path_len, cached_out);
 }
 

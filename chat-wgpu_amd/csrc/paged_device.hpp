@@ -29,6 +29,29 @@ constexpr int kMaxRows = 1 << 23;  // of a call: a launch takes under 2^32 threa
 int check_pages(const char *what, const cw_kv_pages *kv, const cw_batch *b, bool need_kv,
                 PageMap *map);
 
+// Sums over the lanes up to this one, of no negative values; those under 2^24
+// are added in 32 bits along the lanes.
+__device__ __forceinline__ long long wave_scan(long long v, int lane) {
+    if (!__any(v >> 24 != 0)) {
+        int x = (int)v;
+#define CW_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, true)
+        CW_SCAN_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8
+        CW_SCAN_STEP(0x112, 0xf);
+        CW_SCAN_STEP(0x114, 0xf);
+        CW_SCAN_STEP(0x118, 0xf);
+        CW_SCAN_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+        CW_SCAN_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef CW_SCAN_STEP
+        return x;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
 // Whether `rows` rows of wa floats, sa apart from a on, and of wb floats, sb
 // apart from b on, share no float.  Rows of different strides that lie within
 // each other's range count as sharing one.

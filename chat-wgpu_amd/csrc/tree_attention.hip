@@ -234,29 +234,6 @@ __device__ __forceinline__ Work work_of(const SeqRows &s, int group, int n_kv, i
     return Work{t, rb, (long long)n_kv * rb * (kOpen + t)};
 }
 
-// Sums over the lanes up to this one.  Requests of under 2^24 units each (all
-// that a device works off within hours) are added as 32 bits along the lanes.
-__device__ __forceinline__ long long wave_scan(long long v, int lane) {
-    if (!__any(v >> 24 != 0)) {
-        int x = (int)v;
-#define CW_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, true)
-        CW_SCAN_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8
-        CW_SCAN_STEP(0x112, 0xf);
-        CW_SCAN_STEP(0x114, 0xf);
-        CW_SCAN_STEP(0x118, 0xf);
-        CW_SCAN_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
-        CW_SCAN_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
-#undef CW_SCAN_STEP
-        return x;
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-
 __device__ __forceinline__ long long from_lane(long long v, int l) {
     return (long long)(uint32_t)__builtin_amdgcn_readlane((int)v, l) |
            (long long)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32;
@@ -595,16 +572,16 @@ __device__ __forceinline__ f32x4 scores(const typename T::frag (&kf)[T::KS], con
     return s + t;
 }
 
-// Running softmax of one row (this lane's: li) over N tiles of 16 scores, which
-// become the weights; returns the factor of what was summed before.
+// Running softmax of one row (this lane's: li) over N tiles of 16 scores, each
+// with a (positive) factor, which become the weights; returns the factor of
+// what was summed before.
 template <int N>
-__device__ __forceinline__ float soften(f32x4 (&s)[N], float qs, float up, float &m, float &l) {
-    float mx = s[0][0];
+__device__ __forceinline__ float soften(f32x4 (&s)[N], const float (&f)[N], float up, float &m, float &l) {
+    float mx = -INFINITY;
 #pragma unroll
     for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[n][r]);
-    const float mnew = fmaxf(m, group_max(mx) * qs);
+        mx = fmaxf(mx, fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])) * f[n]);
+    const float mnew = fmaxf(m, group_max(mx));
     // a row that has seen nothing keeps -inf: its weights are 2^-inf = 0
     const float ref = mnew == -INFINITY ? 0.0f : mnew;
     const float alpha = __builtin_amdgcn_exp2f(m - ref);
@@ -614,7 +591,7 @@ __device__ __forceinline__ float soften(f32x4 (&s)[N], float qs, float up, float
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], qs, up - ref));
+            s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], f[n], up - ref));
             ls += s[n][r];
         }
     l = l * alpha + ls;
@@ -774,7 +751,8 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
                 const float before = m[i];
-                const float alpha = soften<1>(s[i], q.qs[i], T::UP, m[i], l[i]);
+                const float f[1] = {q.qs[i]};
+                const float alpha = soften<1>(s[i], f, T::UP, m[i], l[i]);
                 if (__any(m[i] > before)) {
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
@@ -1006,7 +984,10 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
 #pragma unroll
             for (int i = 0; i < QT; ++i) {
                 const float before = m[i];
-                const float alpha = soften<ST>(s[i], q.qs[i], T::UP, m[i], l[i]);
+                float f[ST];
+#pragma unroll
+                for (int n = 0; n < ST; ++n) f[n] = q.qs[i];
+                const float alpha = soften<ST>(s[i], f, T::UP, m[i], l[i]);
                 if (__any(m[i] > before)) {
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
@@ -1164,14 +1145,19 @@ __global__ __launch_bounds__(256, (WideCfg<HD, QT>::PER_CU)) void tree_wide_kern
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 f32x4(&r)[NL] = x ? rv : rk;
-                uint32_t top = 0;  // of the magnitudes' bits: ordered as the values, then inf and NaN
+                // the largest magnitude's bits (ordered as the values, then inf and
+                // NaN): as signed bits of the positive, as unsigned of the negative
+                uint32_t un = 0;
+                int sn = 0;
 #pragma unroll
                 for (int n = 0; n < NL; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float w = r[n][e];
-                        top = max(top, __builtin_bit_cast(uint32_t, w) & 0x7fffffffu);
+                        un = max(un, __builtin_bit_cast(uint32_t, w));
+                        sn = max(sn, __builtin_bit_cast(int, w));
                     }
+                uint32_t top = max((uint32_t)sn, un >> 31 ? un & 0x7fffffffu : 0u);
 #define CW_MAX_STEP(ctrl, rows) top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, ctrl, rows, 0xf, true))
                 CW_MAX_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8
                 CW_MAX_STEP(0x112, 0xf);
@@ -1280,18 +1266,19 @@ __global__ __launch_bounds__(256, (WideCfg<HD, QT>::PER_CU)) void tree_wide_kern
                 const bool grown = uniform(top) > uniform(E);
                 E = top;
 #pragma unroll
-                for (int i = 0; i < QT; ++i)
-#pragma unroll
-                    for (int n = 0; n < ST; ++n)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            s[i][n][r] *= kf[n];
-                            if (tail) s[i][n][r] = vis[i] >> (n * 16 + r) & 1 ? s[i][n][r] : -INFINITY;
-                        }
-#pragma unroll
                 for (int i = 0; i < QT; ++i) {
+                    if (tail) {
+#pragma unroll
+                        for (int n = 0; n < ST; ++n)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                s[i][n][r] = vis[i] >> (n * 16 + r) & 1 ? s[i][n][r] : -INFINITY;
+                    }
+                    float f[ST];
+#pragma unroll
+                    for (int n = 0; n < ST; ++n) f[n] = q.qs[i] * kf[n];
                     const float before = m[i];
-                    const float alpha = soften<ST>(s[i], q.qs[i], T::UP, m[i], l[i]) * down;
+                    const float alpha = soften<ST>(s[i], f, T::UP, m[i], l[i]) * down;
                     if (grown || __any(m[i] > before)) {
 #pragma unroll
                         for (int d = 0; d < DT; ++d)

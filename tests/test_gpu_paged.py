@@ -47,6 +47,8 @@ ROPE = [
     (3, 4, 80, 20, "halves", "bands", 3.0, 3, 0, 70000),    # odd strides: element by element
     (9, 2, 64, 32, "pairs", "linear", 4.0, 0, 1, 70000),    # an unaligned start
     (700, 40, 128, 128, "halves", "yarn", 4.0, 1024, 0, 131072),
+    (2100, 32, 128, 96, "halves", "linear", 2.0, 0, 0, 9000),  # past 32 MB of rows
+    (1100, 64, 128, 128, "pairs", "plain", 1.0, 4, 0, 9000),
 ]
 
 
