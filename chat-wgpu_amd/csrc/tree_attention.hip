@@ -551,22 +551,22 @@ __device__ __forceinline__ typename T::frag k_frag(const unsigned char *Ks, int 
 }
 
 // s^T = K q^T of 16 positions, K's fragments in registers
-template <typename T, int QT>
-__device__ __forceinline__ f32x4 scores(const typename T::frag (&kf)[T::KS], const Query<T, QT> &q, int i) {
+template <typename T>
+__device__ __forceinline__ f32x4 scores(const typename T::frag (&kf)[T::KS], const Query<T, 1> &q) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f}, t = s;  // two chains
     if constexpr (T::F16) {
 #pragma unroll
         for (int x = 0; x < T::KS; ++x) {
-            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x], q.hi[i][x], s, 0, 0, 0);
-            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x], q.lo[i][x], t, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x], q.hi[0][x], s, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x], q.lo[0][x], t, 0, 0, 0);
         }
     } else {
 #pragma unroll
         for (int x = 0; x < T::KS; ++x) {
-            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][0], q.f[i][x][0], s, 0, 0, 0);
-            t = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][1], q.f[i][x][1], t, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][2], q.f[i][x][2], s, 0, 0, 0);
-            t = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][3], q.f[i][x][3], t, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][0], q.f[0][x][0], s, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][1], q.f[0][x][1], t, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][2], q.f[0][x][2], s, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][3], q.f[0][x][3], t, 0, 0, 0);
         }
     }
     return s + t;
@@ -612,13 +612,13 @@ __device__ __forceinline__ int o_col(int n, int lg) {
     return T::F16 ? 16 * n + 4 * lg : n / 4 * 64 + 16 * lg + n % 4 * 4;
 }
 
-// ---- few rows of a kv head (at most 32): a workgroup's four waves share them
+// ---- few rows of a kv head (at most 16): a workgroup's four waves share them
 // and take 16 of a tile's 64 positions each, through LDS of their own, so
 // nothing waits for another wave before the end of a segment.
-template <typename KVT, int HD, int QT>
+template <typename KVT, int HD>
 struct SplitCfg : Tile<KVT, HD> {
     typedef Tile<KVT, HD> T;
-    static constexpr int KT = 64, RT = 16 * QT;
+    static constexpr int KT = 64, RT = 16;
     static constexpr int STAGE = 2 * T::GROUPB;  // K and V of a wave's 16 positions
     static constexpr int LDS = 4 * 2 * STAGE;
     static constexpr int PER_CU = LDS <= 72 * 1024 ? 2 : 1;
@@ -626,9 +626,9 @@ struct SplitCfg : Tile<KVT, HD> {
     static_assert(LDS + 4096 <= 160 * 1024, "stages must fit a CU");
 };
 
-template <typename KVT, int HD, int QT>
-__global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_split_kernel(TreeArgs a) {
-    using C = SplitCfg<KVT, HD, QT>;
+template <typename KVT, int HD>
+__global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_kernel(TreeArgs a) {
+    using C = SplitCfg<KVT, HD>;
     using T = Tile<KVT, HD>;
     constexpr int KT = C::KT, RT = C::RT, DT = T::DT;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
@@ -663,22 +663,17 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
             dma_group<T>(vc + at, dst + T::GROUPB, rows, off, row_b, lane, g.once);
         };
         const int t1 = g.lost ? g.t0 : g.t1;
-        Query<T, QT> q;
+        Query<T, 1> q;
         q.load(a, g, group, g.rb * RT, li, lg);
         if (g.t0 < t1) {
             look_up();
             load(g.t0);
         }
         q.convert(a.scale);
-        f32x4 o[QT][DT];
-        float m[QT], l[QT];
+        f32x4 o[DT];
+        float m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < QT; ++i) {
-            m[i] = -INFINITY;
-            l[i] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int t = g.t0; t < t1; ++t) {
             if (t + 1 < t1) {
                 if (t + 1 - tb == 64) {
@@ -717,17 +712,12 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
-            f32x4 s[QT][1];
-#pragma unroll
-            for (int i = 0; i < QT; ++i) s[i][0] = scores<T, QT>(kf, q, i);
+            f32x4 s[1] = {scores<T>(kf, q)};
             const int k0 = t * KT + wave * 16;
             if (k0 + 16 > g.s.cached) {  // nodes: by the mask
+                const uint64_t vis = sees64(a, g.s.r0 + q.node[0], q.node[0], g.s.n, k0 - g.s.cached) >> 4 * lg;
 #pragma unroll
-                for (int i = 0; i < QT; ++i) {
-                    const uint64_t vis = sees64(a, g.s.r0 + q.node[i], q.node[i], g.s.n, k0 - g.s.cached) >> 4 * lg;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[i][0][r] = vis >> r & 1 ? s[i][0][r] : -INFINITY;
-                }
+                for (int r = 0; r < 4; ++r) s[0][r] = vis >> r & 1 ? s[0][r] : -INFINITY;
                 int x = 0;
                 if constexpr (T::F16) {
 #pragma unroll
@@ -748,44 +738,37 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
                 }
                 odd |= __any(x);
             }
+            const float before = m, f[1] = {q.qs[0]};
+            const float alpha = soften<1>(s, f, T::UP, m, l);
+            if (__any(m > before)) {
 #pragma unroll
-            for (int i = 0; i < QT; ++i) {
-                const float before = m[i];
-                const float f[1] = {q.qs[i]};
-                const float alpha = soften<1>(s[i], f, T::UP, m[i], l[i]);
-                if (__any(m[i] > before)) {
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
+            }
+            if constexpr (T::F16) {
+                const float w[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+                f16x4 ph, pl;
+                split_f16(w, ph, pl);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vh[d], ph, o[d], 0, 0, 0);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vh[d], pl, o[d], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[i][d][r] *= alpha;
-                }
-                if constexpr (T::F16) {
-                    const float w[4] = {s[i][0][0], s[i][0][1], s[i][0][2], s[i][0][3]};
-                    f16x4 ph, pl;
-                    split_f16(w, ph, pl);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vh[d], ph, o[i][d], 0, 0, 0);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-                        o[i][d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vh[d], pl, o[i][d], 0, 0, 0);
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int d = 0; d < DT; ++d)
-                            o[i][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[r][d / 4][d % 4], s[i][0][r], o[i][d], 0, 0, 0);
-                }
+                        o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[r][d / 4][d % 4], s[0][r], o[d], 0, 0, 0);
             }
         }
         // join the waves
-#pragma unroll
-        for (int i = 0; i < QT; ++i) {
-            l[i] = group_sum(l[i]);
-            if (lg == 0) {
-                w_ml[wave][i * 16 + li][0] = m[i];
-                w_ml[wave][i * 16 + li][1] = bad ? NAN : l[i];
-            }
+        l = group_sum(l);
+        if (lg == 0) {
+            w_ml[wave][li][0] = m;
+            w_ml[wave][li][1] = bad ? NAN : l;
         }
         if (lane == 0) w_odd[wave] = odd;
         lds_barrier();  // and every wave is done with its stages
@@ -795,20 +778,16 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
         }
         constexpr int OS = HD / 4 < 16 ? HD / 4 - 1 : 15;
         f32x4 *const ow = reinterpret_cast<f32x4 *>(lds);
+        float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < QT; ++i) {
-            const int row = i * 16 + li;
-            float M = -INFINITY;
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, w_ml[w][li][0]);
+        const float down = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
 #pragma unroll
-            for (int w = 0; w < 4; ++w) M = fmaxf(M, w_ml[w][row][0]);
-            const float f = __builtin_amdgcn_exp2f(m[i] - (M == -INFINITY ? 0.0f : M));
+        for (int n = 0; n < DT; ++n) {
+            f32x4 v = o_quad<T>(o, n);
 #pragma unroll
-            for (int n = 0; n < DT; ++n) {
-                f32x4 v = o_quad<T>(o[i], n);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= f;
-                ow[(wave * RT + row) * (HD / 4) + ((o_col<T>(n, lg) / 4) ^ (row & OS))] = v;
-            }
+            for (int e = 0; e < 4; ++e) v[e] *= down;
+            ow[(wave * RT + li) * (HD / 4) + ((o_col<T>(n, lg) / 4) ^ (li & OS))] = v;
         }
         lds_barrier();
         for (int x = tid; x < RT * (HD / 4); x += 256) {
@@ -829,11 +808,14 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD, QT>::PER_CU)) void tree_spl
     }
 }
 
-// ---- more rows: the four waves take 16 QT rows each, and share the tile's
-// positions in LDS.
-template <typename KVT, int HD, int QT>
-struct TileCfg : Tile<KVT, HD> {
-    typedef Tile<KVT, HD> T;
+// ---- more rows over an f16 cache: the four waves take 16 QT rows each, and share
+// the tile's positions in LDS.  (Tiles of 32 positions, two workgroups a CU with
+// three tiles on their way each: 25.7 us for 61 nodes at 4,100 positions, against
+// 21.6; one workgroup of eight waves, with tiles of 64 positions: 44 us for twelve
+// requests of 4 to 16 nodes, against 36.)
+template <int HD_, int QT>
+struct TileCfg : Tile<_Float16, HD_> {
+    typedef Tile<_Float16, HD_> T;
     static constexpr int KT = T::ROWB <= 256 ? 64 : 32, RT = 64 * QT;
     static constexpr int ST = KT / 16;
     static constexpr int TILE = KT * T::ROWB;
@@ -843,10 +825,10 @@ struct TileCfg : Tile<KVT, HD> {
     static_assert(LDS + 4096 <= 160 * 1024, "tiles must fit a CU");
 };
 
-template <typename KVT, int HD, int QT>
-__global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile_kernel(TreeArgs a) {
-    using C = TileCfg<KVT, HD, QT>;
-    using T = Tile<KVT, HD>;
+template <int HD, int QT>
+__global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kernel(TreeArgs a) {
+    using C = TileCfg<HD, QT>;
+    using T = Tile<_Float16, HD>;
     constexpr int KT = C::KT, RT = C::RT, DT = T::DT, ST = C::ST;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
     __shared__ int bad_seg, odd_seg;  // the last segment without a block, with a V that is not finite
@@ -918,8 +900,8 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
 #pragma unroll
                 for (int n = 0; n < T::NU; ++n) {
                     const uint4 w = *reinterpret_cast<const uint4 *>(Vs + my_group * T::GROUPB + n * 1024 + lane * 16);
-                    x |= not_finite<T::F16>(w.x) | not_finite<T::F16>(w.y) | not_finite<T::F16>(w.z) |
-                         not_finite<T::F16>(w.w);
+                    x |= not_finite<true>(w.x) | not_finite<true>(w.y) | not_finite<true>(w.z) |
+                         not_finite<true>(w.w);
                 }
                 if (__any(x)) odd_seg = seg;
             }
@@ -933,10 +915,10 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
             // Fragments are requested some steps before their products.  A product
             // waits for the one before it of the same sum, so steps are of two
             // sums: two tiles of rows, or two fragments for one.
-            constexpr int P = QT == 1 && T::F16 ? 2 : 1;
+            constexpr int P = QT == 1 ? 2 : 1;
             f32x4 s[QT][ST];
             constexpr int KN = ST * T::KS, KA = KN < 4 ? KN : 4;
-            typename T::frag kf[KA + P];
+            f16x8 kf[KA + P];
             auto k_n = [](int e) { return e / (P * T::KS) * P + e % P; };  // 16 positions, and
             auto k_x = [](int e) { return e / P % T::KS; };                // part of their rows
             auto k_at = [&](int e) { return k_frag<T>(Ks + k_n(e) * T::GROUPB, k_x(e), li, lg); };
@@ -948,28 +930,17 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
                 for (int e = e0; e < e0 + P; ++e)
                     if (e + KA < KN) kf[(e + KA) % (KA + P)] = k_at(e + KA);
                 keep_order();
-                if constexpr (T::F16) {
 #pragma unroll
-                    for (int half = 0; half < 2; ++half)
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-                        for (int e = e0; e < e0 + P; ++e)
+                    for (int e = e0; e < e0 + P; ++e)
 #pragma unroll
-                            for (int i = 0; i < QT; ++i) {
-                                f32x4 &d = s[i][k_n(e)];
-                                if (half == 0 && k_x(e) == 0) d = f32x4{0.f, 0.f, 0.f, 0.f};
-                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    kf[e % (KA + P)], half ? q.lo[i][k_x(e)] : q.hi[i][k_x(e)], d, 0, 0, 0);
-                            }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < QT; ++i) {
-                        f32x4 &d = s[i][k_n(e0)];
-                        if (k_x(e0) == 0) d = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            d = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e0 % (KA + P)][r], q.f[i][k_x(e0)][r], d, 0, 0, 0);
-                    }
-                }
+                        for (int i = 0; i < QT; ++i) {
+                            f32x4 &d = s[i][k_n(e)];
+                            if (half == 0 && k_x(e) == 0) d = f32x4{0.f, 0.f, 0.f, 0.f};
+                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                kf[e % (KA + P)], half ? q.lo[i][k_x(e)] : q.hi[i][k_x(e)], d, 0, 0, 0);
+                        }
                 keep_order();
             }
             if (tail) {  // nodes: by the mask
@@ -995,71 +966,51 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
                         for (int r = 0; r < 4; ++r) o[i][d][r] *= alpha;
                 }
             }
-            if constexpr (T::F16) {
-                f16x8 ph[ST / 2][QT], pl[ST / 2][QT];
+            f16x8 ph[ST / 2][QT], pl[ST / 2][QT];
 #pragma unroll
-                for (int kk = 0; kk < ST / 2; ++kk)
+            for (int kk = 0; kk < ST / 2; ++kk)
 #pragma unroll
-                    for (int i = 0; i < QT; ++i) {
-                        float w[8];
+                for (int i = 0; i < QT; ++i) {
+                    float w[8];
 #pragma unroll
-                        for (int r = 0; r < 8; ++r) w[r] = s[i][2 * kk + r / 4][r % 4];
-                        split_f16(w, ph[kk][i], pl[kk][i]);
-                    }
-                const int row = 4 * lg + (li >> 2), c = (li & 3) >> 1;
-                auto v_at = [&](int e) {
-                    // the k order of the fragments: rows 4 lg + j of both groups of 16
-                    const int d = e % DT;
-                    const unsigned char *p = Vs + e / DT * 2 * T::GROUPB + row * T::ROWB +
-                                             (((2 * d + c) ^ (row & T::SWZ)) << 4) + (li & 1) * 8;
-                    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
-                    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + T::GROUPB)));
-                    return __builtin_bit_cast(f16x8, make_uint4(x.x, x.y, y.x, y.y));
-                };
-                constexpr int VA = 4, VN = DT * (ST / 2);
-                f16x8 vf[VA + P];
+                    for (int r = 0; r < 8; ++r) w[r] = s[i][2 * kk + r / 4][r % 4];
+                    split_f16(w, ph[kk][i], pl[kk][i]);
+                }
+            const int row = 4 * lg + (li >> 2), c = (li & 3) >> 1;
+            auto v_at = [&](int e) {
+                // the k order of the fragments: rows 4 lg + j of both groups of 16
+                const int d = e % DT;
+                const unsigned char *p = Vs + e / DT * 2 * T::GROUPB + row * T::ROWB +
+                                         (((2 * d + c) ^ (row & T::SWZ)) << 4) + (li & 1) * 8;
+                const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p));
+                const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + T::GROUPB)));
+                return __builtin_bit_cast(f16x8, make_uint4(x.x, x.y, y.x, y.y));
+            };
+            constexpr int VA = 4, VN = DT * (ST / 2);
+            f16x8 vf[VA + P];
 #pragma unroll
-                for (int e = 0; e < VA; ++e) vf[e] = v_at(e);
+            for (int e = 0; e < VA; ++e) vf[e] = v_at(e);
 #pragma unroll
-                for (int e0 = 0; e0 < VN; e0 += P) {
+            for (int e0 = 0; e0 < VN; e0 += P) {
+#pragma unroll
+                for (int e = e0; e < e0 + P; ++e)
+                    if (e + VA < VN) vf[(e + VA) % (VA + P)] = v_at(e + VA);
+                keep_order();
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
                     for (int e = e0; e < e0 + P; ++e)
-                        if (e + VA < VN) vf[(e + VA) % (VA + P)] = v_at(e + VA);
-                    keep_order();
 #pragma unroll
-                    for (int half = 0; half < 2; ++half)
-#pragma unroll
-                        for (int e = e0; e < e0 + P; ++e)
-#pragma unroll
-                            for (int i = 0; i < QT; ++i)
-                                o[i][e % DT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    vf[e % (VA + P)], half ? pl[e / DT][i] : ph[e / DT][i], o[i][e % DT], 0, 0, 0);
-                    keep_order();
-                }
-            } else {
-#pragma unroll
-                for (int n = 0; n < ST; ++n)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int row = 4 * lg + r;
-#pragma unroll
-                        for (int c = 0; c < HD / 64; ++c) {
-                            const f32x4 vf = *reinterpret_cast<const f32x4 *>(
-                                Vs + n * T::GROUPB + row * T::ROWB + (((16 * c + li) ^ (row & T::SWZ)) << 4));
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                                for (int i = 0; i < QT; ++i)
-                                    o[i][4 * c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                        vf[e], s[i][n][r], o[i][4 * c + e], 0, 0, 0);
-                        }
-                    }
+                        for (int i = 0; i < QT; ++i)
+                            o[i][e % DT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                vf[e % (VA + P)], half ? pl[e / DT][i] : ph[e / DT][i], o[i][e % DT], 0, 0, 0);
+                keep_order();
             }
         }
         // the last tile's odd_seg, or (no tile) bad_seg, known to all
         if (g.t0 == t1 || t1 * KT > g.s.cached) lds_barrier();
         if (uniform(odd_seg) == seg) {
-            one_by_one<KVT, HD, RT>(a, g, group, KT, T::UP);
+            one_by_one<_Float16, HD, RT>(a, g, group, KT, T::UP);
             continue;
         }
         const bool bad = g.lost || bad_seg == seg;
@@ -1083,10 +1034,10 @@ __global__ __launch_bounds__(256, (TileCfg<KVT, HD, QT>::PER_CU)) void tree_tile
 // lo in LDS with that exponent: K's is undone in the scores' factor, V's in the
 // weights, against the largest exponent so far (which o follows as it does the
 // running maximum).
-template <int HD_, int QT>
+template <int HD_>
 struct WideCfg : Tile<_Float16, HD_> {
     typedef Tile<_Float16, HD_> T;
-    static constexpr int KT = HD_ == 64 ? 64 : 32, RT = 64 * QT, ST = KT / 16;
+    static constexpr int KT = HD_ == 64 ? 64 : 32, RT = 64, ST = KT / 16;
     static constexpr int PW = KT / 4;                // positions of a wave
     static constexpr int LPR = HD_ / 4;              // lanes of a row
     static constexpr int NL = PW * LPR / 64;         // loads of its K
@@ -1095,11 +1046,12 @@ struct WideCfg : Tile<_Float16, HD_> {
     static constexpr int PER_CU = LDS <= 72 * 1024 ? 2 : 1;
 };
 
-template <int HD, int QT>
-__global__ __launch_bounds__(256, (WideCfg<HD, QT>::PER_CU)) void tree_wide_kernel(TreeArgs a) {
-    using C = WideCfg<HD, QT>;
+template <int HD>
+__global__ __launch_bounds__(256, (WideCfg<HD>::PER_CU)) void tree_wide_kernel(TreeArgs a) {
+    using C = WideCfg<HD>;
     using T = Tile<_Float16, HD>;
     constexpr int KT = C::KT, RT = C::RT, DT = T::DT, ST = C::ST, PW = C::PW, NL = C::NL;
+    constexpr int QT = 1;  // tiles of 16 rows a wave: a second one does not fit the registers
     __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
     __shared__ int w_exp[2][2][4];    // exponents of a tile's K and V, a wave each
     __shared__ int bad_seg, odd_seg;  // the last segment without a block, with a value that is not finite
@@ -1219,7 +1171,7 @@ __global__ __launch_bounds__(256, (WideCfg<HD, QT>::PER_CU)) void tree_wide_kern
                     for (int i = 0; i < QT; ++i)
                         vis[i] = sees64(a, g.s.r0 + q.node[i], q.node[i], g.s.n, k0 - g.s.cached) >> 4 * lg;
                 }
-                constexpr int P = QT == 1 ? 2 : 1;  // sums in flight, as above
+                constexpr int P = 2;  // sums in flight, as above
                 f32x4 s[QT][ST];
                 constexpr int KN = ST * T::KS, KA = 2;
                 typename T::frag kh[KA + P], kl[KA + P];
@@ -1359,14 +1311,12 @@ __global__ __launch_bounds__(256, (WideCfg<HD, QT>::PER_CU)) void tree_wide_kern
 }
 
 // Joins the partials of the rows whose units went to more than one workgroup,
-// in the order of the positions: a wave a (row, head), the lanes four elements
-// of every 256 / HD-th partial.
+// in the order of the positions: a wave every so many heads of a row, the lanes
+// four elements of every 256 / HD-th partial.
 template <int HD>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int rt) {
     constexpr int CL = HD / 4, SL = 64 / CL;
     const int r = blockIdx.x, lane = threadIdx.x & 63;
-    const int head = uniform((int)(blockIdx.y * 4 + (threadIdx.x >> 6)));
-    if (head >= a.n_heads) return;
     const int group = a.n_heads / a.n_kv;
     long long total = 0, base = -1;
     SeqRows mine{0, 0, 0};
@@ -1385,60 +1335,62 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int
     if (base < 0) return;
     const Work wk = work_of(mine, group, a.n_kv, kt, rt);
     const Deal deal(total, a.wgs);
-    const int h = head / group, rr = (r - mine.r0) * group + head - h * group;
-    const long long u0 = base + ((long long)h * wk.blocks + rr / rt) * (kOpen + wk.tiles) + kOpen;
-    const int w0 = uniform(deal.owner(u0)), w1 = uniform(deal.owner(u0 + wk.tiles - 1));
-    if (w0 == w1) return;  // one workgroup had them all, and wrote the output
-    auto at = [&](int w) { return (size_t)(w * 2 + (w == w0 ? 1 : 0)) * rt + rr % rt; };
     const int col = lane % CL * 4, sl = lane / CL;
-    float M = -INFINITY, L = 0.0f;
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    for (int c = w0; c <= w1; c += 64) {
-        const int n = min(64, w1 + 1 - c);
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        if (lane < n) ml = *reinterpret_cast<const float2 *>(a.ml + at(c + lane) * 2);
-        constexpr int D = 8;  // partials in flight
-        f32x4 v[D];
-        auto fetch = [&](int p0) {
+    for (int head = uniform((int)(blockIdx.y * 4 + (threadIdx.x >> 6))); head < a.n_heads; head += gridDim.y * 4) {
+        const int h = head / group, rr = (r - mine.r0) * group + head - h * group;
+        const long long u0 = base + ((long long)h * wk.blocks + rr / rt) * (kOpen + wk.tiles) + kOpen;
+        const int w0 = uniform(deal.owner(u0)), w1 = uniform(deal.owner(u0 + wk.tiles - 1));
+        if (w0 == w1) continue;  // one workgroup had them all, and wrote the output
+        auto at = [&](int w) { return (size_t)(w * 2 + (w == w0 ? 1 : 0)) * rt + rr % rt; };
+        float M = -INFINITY, L = 0.0f;
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+        for (int c = w0; c <= w1; c += 64) {
+            const int n = min(64, w1 + 1 - c);
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (lane < n) ml = *reinterpret_cast<const float2 *>(a.ml + at(c + lane) * 2);
+            constexpr int D = 8;  // partials in flight
+            f32x4 v[D];
+            auto fetch = [&](int p0) {
 #pragma unroll
-            for (int d = 0; d < D; ++d)
-                v[d] = *reinterpret_cast<const f32x4 *>(a.part + at(c + min(p0 + d * SL + sl, n - 1)) * HD + col);
-        };
-        fetch(0);
-        float mx = ml.x;
+                for (int d = 0; d < D; ++d)
+                    v[d] = *reinterpret_cast<const f32x4 *>(a.part + at(c + min(p0 + d * SL + sl, n - 1)) * HD + col);
+            };
+            fetch(0);
+            float mx = ml.x;
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        const float Mn = fmaxf(M, mx), ref = Mn == -INFINITY ? 0.0f : Mn;
-        const float old = __builtin_amdgcn_exp2f(M - ref), f = __builtin_amdgcn_exp2f(ml.x - ref);
-        M = Mn;
-        float ls = lane < n ? f * ml.y : 0.0f;
+            for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+            const float Mn = fmaxf(M, mx), ref = Mn == -INFINITY ? 0.0f : Mn;
+            const float old = __builtin_amdgcn_exp2f(M - ref), f = __builtin_amdgcn_exp2f(ml.x - ref);
+            M = Mn;
+            float ls = lane < n ? f * ml.y : 0.0f;
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) ls += __shfl_xor(ls, o);
-        L = L * old + ls;
+            for (int o = 32; o >= 1; o >>= 1) ls += __shfl_xor(ls, o);
+            L = L * old + ls;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] *= old;
-        for (int p0 = 0;;) {
+            for (int e = 0; e < 4; ++e) y[e] *= old;
+            for (int p0 = 0;;) {
 #pragma unroll
-            for (int d = 0; d < D; ++d) {
-                const int p = p0 + d * SL + sl;
-                const float w = __shfl(f, p & 63);
+                for (int d = 0; d < D; ++d) {
+                    const int p = p0 + d * SL + sl;
+                    const float w = __shfl(f, p & 63);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    y[e] = p < n ? __builtin_fmaf(w, v[d][e], y[e]) : y[e];
+                    for (int e = 0; e < 4; ++e)
+                        y[e] = p < n ? __builtin_fmaf(w, v[d][e], y[e]) : y[e];
+                }
+                p0 += D * SL;
+                if (p0 >= n) break;
+                fetch(p0);
             }
-            p0 += D * SL;
-            if (p0 >= n) break;
-            fetch(p0);
         }
+#pragma unroll
+        for (int o = CL; o < 64; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], o);
+        const float f = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = L == 0.0f ? 0.0f : y[e] * f;
+        if (sl == 0) *reinterpret_cast<f32x4 *>(a.out + (size_t)r * a.out_stride + (size_t)head * HD + col) = y;
     }
-#pragma unroll
-    for (int o = CL; o < 64; o <<= 1)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], o);
-    const float f = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = L == 0.0f ? 0.0f : y[e] * f;
-    if (sl == 0) *reinterpret_cast<f32x4 *>(a.out + (size_t)r * a.out_stride + (size_t)head * HD + col) = y;
 }
 
 template <typename C>
@@ -1450,34 +1402,42 @@ int launch_tiles(cw_ctx *ctx, TreeArgs a, void (*fn)(TreeArgs)) {
     a.part = static_cast<float *>(scratch);
     a.ml = a.part + rows * C::HD;
     CW_TRY(launch(ctx, "attention_tree", fn, dim3(a.wgs), dim3(256), 0, a));
+    // four heads a workgroup while that is about what the chip holds at once, more
+    // for more rows (which also share the look at the lengths): 8 requests of 128
+    // nodes 32 us with four each
+    const int by_chip = (8 * ctx->n_cu + a.rows - 1) / a.rows;
     return launch(ctx, "attention_tree_merge", tree_merge_kernel<C::HD>,
-                  dim3(a.rows, (a.n_heads + 3) / 4), dim3(256), 0, a, C::KT, C::RT);
+                  dim3(a.rows, std::min((a.n_heads + 3) / 4, by_chip)), dim3(256), 0, a, C::KT, C::RT);
 }
-template <typename KVT, int HD, int QT>
+template <typename KVT, int HD>
 int launch_split(cw_ctx *ctx, const TreeArgs &a) {
-    return launch_tiles<SplitCfg<KVT, HD, QT>>(ctx, a, tree_split_kernel<KVT, HD, QT>);
+    return launch_tiles<SplitCfg<KVT, HD>>(ctx, a, tree_split_kernel<KVT, HD>);
 }
 template <int HD, int QT>
 int launch_tile(cw_ctx *ctx, const TreeArgs &a) {
-    return launch_tiles<TileCfg<_Float16, HD, QT>>(ctx, a, tree_tile_kernel<_Float16, HD, QT>);
+    return launch_tiles<TileCfg<HD, QT>>(ctx, a, tree_tile_kernel<HD, QT>);
 }
-
-template <int HD, int QT>
+template <int HD>
 int launch_wide(cw_ctx *ctx, const TreeArgs &a) {
-    return launch_tiles<WideCfg<HD, QT>>(ctx, a, tree_wide_kernel<HD, QT>);
+    return launch_tiles<WideCfg<HD>>(ctx, a, tree_wide_kernel<HD>);
 }
 
-// By the rows of a (request, kv head) on average.
+// By the rows of a (request, kv head) on average; us at head_dim 128, 8 requests
+// of 4,000 positions unless said otherwise:
+//   f16, 4 / 16 / 32 rows: split 26.4 / 28.5 / 34.2 (of two tiles of rows), tiles
+//   27.1 / 27.4 / 30.3; one request of 4 rows: 8.7 and 10.3; tiles of 64 and of
+//   128 rows: 54 and 51 for 128 rows with joins of 10 and 12, 159 and 153 for 512,
+//   28.6 and 34 for 244 of a single request;
+//   f32, 8 / 16 / 32 rows: split 46 / 48 / 71, wide 54 / 55 / 58.
+// head_dim 256: the split kernel's registers leave a CU one workgroup, 27.9 us for
+// 4 rows over f16; tiles 27.3.
 template <typename KVT, int HD>
 int launch_by_rows(cw_ctx *ctx, const TreeArgs &a) {
     const long long rows = ((long long)a.rows + a.n_seq - 1) / a.n_seq * (a.n_heads / a.n_kv);
-    if constexpr (HD * sizeof(KVT) <= 512) {
-        if (rows <= 16) return launch_split<KVT, HD, 1>(ctx, a);
-        if constexpr (HD <= 128)
-            if (rows <= 32) return launch_split<KVT, HD, 2>(ctx, a);
-    }
+    if constexpr (HD <= 128)
+        if (rows <= (sizeof(KVT) == 2 ? 8 : 16)) return launch_split<KVT, HD>(ctx, a);
     if constexpr (sizeof(KVT) == 4) {
-        return launch_wide<HD, 1>(ctx, a);
+        return launch_wide<HD>(ctx, a);
     } else {
         if constexpr (HD <= 128)
             if (rows > 256) return launch_tile<HD, 2>(ctx, a);
