@@ -1033,7 +1033,10 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
 // power of two that brings its largest value to 2^14 .. 2^15, and leaves hi and
 // lo in LDS with that exponent: K's is undone in the scores' factor, V's in the
 // weights, against the largest exponent so far (which o follows as it does the
-// running maximum).
+// running maximum).  A position is so kept to 22 bits down to 2^-17 of its
+// neighbours' largest, and to 2^-40 of that below: of the same order as the
+// weights.  Nodes that a row does not see must not cost its others their bits,
+// so where a node is further from its neighbours the segment is taken one by one.
 template <int HD_>
 struct WideCfg : Tile<_Float16, HD_> {
     typedef Tile<_Float16, HD_> T;
@@ -1052,6 +1055,8 @@ __global__ __launch_bounds__(256, (WideCfg<HD>::PER_CU)) void tree_wide_kernel(T
     using T = Tile<_Float16, HD>;
     constexpr int KT = C::KT, RT = C::RT, DT = T::DT, ST = C::ST, PW = C::PW, NL = C::NL;
     constexpr int QT = 1;  // tiles of 16 rows a wave: a second one does not fit the registers
+    constexpr int kNone = -10000;  // exponent of nothing but zeros
+    constexpr int kFar = 16;       // exponents so far apart cost bits
     __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
     __shared__ int w_exp[2][2][4];    // exponents of a tile's K and V, a wave each
     __shared__ int bad_seg, odd_seg;  // the last segment without a block, with a value that is not finite
@@ -1122,7 +1127,27 @@ __global__ __launch_bounds__(256, (WideCfg<HD>::PER_CU)) void tree_wide_kernel(T
                 if (top >= 0x7f800000u) odd_seg = seg;
                 const int e = max((int)(top >> 23) - 126, -100);  // all below 2^e
                 const float up = __builtin_bit_cast(float, (uint32_t)(15 - min(e, 128) + 127) << 23);
-                w_exp[t & 1][x][wave] = e;
+                w_exp[t & 1][x][wave] = x && !top ? kNone : e;
+                if (t * KT + KT > g.s.cached) {  // some nodes' values: are they far apart?
+                    const float near = ldexpf(1.0f, e - 14);
+                    float mx[NL];
+                    bool far = false;
+#pragma unroll
+                    for (int n = 0; n < NL; ++n) {
+                        mx[n] = fmaxf(fmaxf(fabsf(r[n][0]), fabsf(r[n][1])), fmaxf(fabsf(r[n][2]), fabsf(r[n][3])));
+                        far |= mx[n] < near;
+                    }
+                    if (__any(far)) {
+                        far = false;
+#pragma unroll
+                        for (int n = 0; n < NL; ++n) {
+#pragma unroll
+                            for (int off = 1; off < C::LPR; off <<= 1) mx[n] = fmaxf(mx[n], __shfl_xor(mx[n], off));
+                            far |= mx[n] > 0.0f && mx[n] < near;
+                        }
+                        if (__any(far)) odd_seg = seg;
+                    }
+                }
 #pragma unroll
                 for (int n = 0; n < NL; ++n) {
                     const float w[4] = {r[n][0] * up, r[n][1] * up, r[n][2] * up, r[n][3] * up};
@@ -1151,7 +1176,7 @@ __global__ __launch_bounds__(256, (WideCfg<HD>::PER_CU)) void tree_wide_kernel(T
         }
         f32x4 o[QT][DT];
         float m[QT], l[QT];
-        int E = -10000;  // o counts 2^(E - 15)
+        int E = kNone;  // o counts 2^(E - 15)
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
             m[i] = -INFINITY;
@@ -1205,9 +1230,14 @@ __global__ __launch_bounds__(256, (WideCfg<HD>::PER_CU)) void tree_wide_kernel(T
                 }
                 // the tile's exponents: K's of this lane's positions, V's against all so far
                 float kf[ST], vf_[ST];
-                int top = E;
+                int top = E, least = 1000;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) top = max(top, w_exp[t & 1][1][w]);
+                for (int w = 0; w < 4; ++w) {
+                    const int e = w_exp[t & 1][1][w];
+                    top = max(top, e);
+                    least = e == kNone ? least : min(least, e);
+                }
+                if (tail && (least < top - kFar || (E != kNone && E < top - kFar))) odd_seg = seg;
 #pragma unroll
                 for (int n = 0; n < ST; ++n) {
                     const int w = (16 * n + 4 * lg) / PW;
@@ -1228,7 +1258,7 @@ __global__ __launch_bounds__(256, (WideCfg<HD>::PER_CU)) void tree_wide_kernel(T
                     }
                     float f[ST];
 #pragma unroll
-                    for (int n = 0; n < ST; ++n) f[n] = q.qs[i] * kf[n];
+                    for (int n = 0; n < ST; ++n) f[n] = fmaxf(q.qs[i] * kf[n], 1e-37f);  // (-inf keeps its sign)
                     const float before = m[i];
                     const float alpha = soften<ST>(s[i], f, T::UP, m[i], l[i]) * down;
                     if (grown || __any(m[i] > before)) {

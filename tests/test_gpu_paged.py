@@ -434,6 +434,35 @@ def test_attention_masked_values_stay_out(ctx, rng, hd, kv):
 
 
 @pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("nodes", [[7, 20], range(24, 40), [39]])
+@pytest.mark.parametrize("what", ["k", "v", "both"])
+def test_attention_large_values_stay_out(ctx, rng, what, nodes, hd, kv):
+    """Nodes of huge K or V cost the rows that do not see them no bits."""
+    n = 40
+    mask = np.concatenate([po.tree(rng, n, 2), po.tree(rng, n, 2)])
+    bits = np.zeros(2, np.uint32)
+    for i in nodes:
+        bits[i // 32] |= np.uint32(1 << i % 32)
+    mask &= ~bits
+    mask[[30, n + 30]] |= bits
+    b = Batch(ctx, rng, [0, 45], [n, n], 4, 2, hd, kv, 16, mask=mask)
+    huge = {"f16": 3e4, "f32": 3e37}[kv]
+    k, v = b.k.copy(), b.v.copy()
+    for s in range(2):
+        for i in nodes:
+            at_ = po.slot_of(b.tables, 16, s, int(b.cached[s]) + i)
+            if what != "v":
+                b.k[at_] = (huge * rng.uniform(-1, 1, b.k[at_].shape)).astype(b.k.dtype)
+            if what != "k":
+                b.v[at_] = huge
+    got = b.run()
+    keep = np.setdiff1d(np.arange(2 * n), [30, n + 30])
+    ref, bound = po.attention(b.q, k, v, b.tables, 16, b.cached, b.first, mask)
+    assert np.all(np.abs(got - ref)[keep] <= bound[keep])
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
 def test_attention_infinite_values_of_seen_nodes(ctx, rng, kv):
     """A seen V of +inf gives +inf in its element, and nothing else changes."""
     b = Batch(ctx, rng, [20], [9], 2, 1, 128, kv, 16)
@@ -453,6 +482,16 @@ def test_attention_magnitudes(ctx, rng, q_scale, v_scale, kv):
     """Queries far from one: scores of any size, a softmax down to one key."""
     b = Batch(ctx, rng, [150, 4], [12, 3], 4, 2, 128, kv, 16, tree=True, q_scale=q_scale,
               v_scale=v_scale)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("q_scale,k_scale,v_scale", [(1e-30, 1e-30, 1.0), (1.0, 0.0, 0.0), (1e18, 1e-19, 1e30),
+                                                     (1e-12, 1e12, 1e-30)])
+def test_attention_magnitudes_of_many_rows(ctx, rng, q_scale, k_scale, v_scale, hd):
+    """Queries and an f32 cache far from one, more rows than 16."""
+    b = Batch(ctx, rng, [150, 0], [40, 33], 4, 2, hd, "f32", 16, tree=True, q_scale=q_scale)
+    b.k, b.v = b.k * np.float32(k_scale), b.v * np.float32(v_scale)
     b.check(b.run())
 
 
