@@ -1499,6 +1499,9 @@ extern "C" int cw_attention_tree(cw_ctx *ctx, const cw_kv_pages *kv, const cw_ba
     CW_CHECK_ARG(n_heads > 0 && n_heads <= 4096 && n_heads % kv->n_kv_heads == 0,
                  "cw_attention_tree: n_heads=%d must be a multiple of n_kv_heads=%d (at most 4096)",
                  n_heads, kv->n_kv_heads);
+    CW_CHECK_ARG((long long)b->rows * (n_heads / kv->n_kv_heads) <= 1 << 30,
+                 "cw_attention_tree: %d rows of %d query heads a kv head are more than 2^30", b->rows,
+                 n_heads / kv->n_kv_heads);
     const size_t width = (size_t)n_heads * kv->head_dim;
     CW_CHECK_ARG(q_stride >= width && out_stride >= width && q_stride < (1u << 31) &&
                      out_stride < (1u << 31) && q_stride % 4 == 0 && out_stride % 4 == 0,

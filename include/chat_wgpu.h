@@ -183,7 +183,10 @@ int cw_q4_gemm(cw_ctx *ctx, const float *x, int m, const uint16_t *scales, const
 /* change.  Device values are checked on the device: a row, slot, block */
 /* or request out of its range is left out, never read or written       */
 /* (which result says so is stated below).  The calls leave the context's */
-/* device current, as cw_ctx_create does.                               */
+/* device current, as cw_ctx_create does.  cw_block_tables and             */
+/* cw_attention_tree use the context's scratch, the rotations a table of   */
+/* 4 rot_dim bytes for each specification, which the context keeps: the   */
+/* first call of a kind comes before cw_graph_begin (else CW_ERR_STATE).  */
 /* ---------------------------------------------------------------- */
 
 /* which elements of a head form a rotated pair */
@@ -285,9 +288,10 @@ int cw_block_tables(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const
  * sqrt(head_dim)) v_p, kv head h / (n_heads / n_kv_heads), rows of q and out
  * q_stride and out_stride floats apart (multiples of 4, 16-byte aligned).
  * K and V of positions that a row does not see do not reach it, whatever they
- * hold.  A row that sees nothing (or only scores of -inf) gives zeros; the
+ * hold; K that it sees, and V of cached positions, have to be finite, or that
+ * row's own result may be NaN.  A row that sees nothing (or only scores of -inf) gives zeros; the
  * rows of a request with positions whose block is not in the cache give NaN.
- * cached[b] + rows of b is at most 2^30.  out must not overlap q.  Covers a
+ * cached[b] + rows of b is at most 2^30, b->rows * n_heads / n_kv_heads too.  out must not overlap q.  Covers a
  * decode step (one row each, mask NULL), pieces of prompts (mask NULL) and
  * trees of drafted tokens. */
 int cw_attention_tree(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const float *q,

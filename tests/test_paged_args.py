@@ -135,6 +135,12 @@ def test_attention_tree():
     refused(call(out=4096 + 1024), "overlap")
 
 
+def test_attention_tree_rows_of_many_heads():
+    """Rows are counted per kv head in 32 bits."""
+    refused(cw.lib().cw_attention_tree(CTX, pages(n_kv_heads=1), batch(rows=1 << 23), P, 1 << 20, 4096,
+                                       1 << 50, 1 << 20), "2^30")
+
+
 def test_kv_accept():
     lib = cw.lib()
     refused(lib.cw_kv_accept(CTX, pages(), batch(), None, 4, P, None), "null")
