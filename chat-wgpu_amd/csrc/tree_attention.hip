@@ -385,7 +385,7 @@ __device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, f
     constexpr int E = HD / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const KVT *kc = static_cast<const KVT *>(a.kc), *vc = static_cast<const KVT *>(a.vc);
-    for (int row = wave; row < RT && g.rb * RT + row < g.nrows; row += 4) {
+    for (int row = wave; row < RT && g.rb * RT + row < g.nrows; row += blockDim.x >> 6) {
         const int rr = g.rb * RT + row, node = rr / group;
         const size_t head = (size_t)(g.h * group + rr - node * group) * HD + lane * E;
         float q[E], o[E] = {}, m = -INFINITY, l = 0.0f;
@@ -618,7 +618,7 @@ __device__ __forceinline__ int o_col(int n, int lg) {
 template <typename KVT, int HD>
 struct SplitCfg : Tile<KVT, HD> {
     typedef Tile<KVT, HD> T;
-    static constexpr int KT = 64, RT = 16;
+    static constexpr int NW = 4, KT = 64, RT = 16;
     static constexpr int STAGE = 2 * T::GROUPB;  // K and V of a wave's 16 positions
     static constexpr int LDS = 4 * 2 * STAGE;
     static constexpr int PER_CU = LDS <= 72 * 1024 ? 2 : 1;
@@ -816,7 +816,7 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
 template <int HD_, int QT>
 struct TileCfg : Tile<_Float16, HD_> {
     typedef Tile<_Float16, HD_> T;
-    static constexpr int KT = T::ROWB <= 256 ? 64 : 32, RT = 64 * QT;
+    static constexpr int NW = 4, KT = T::ROWB <= 256 ? 64 : 32, RT = 64 * QT;
     static constexpr int ST = KT / 16;
     static constexpr int TILE = KT * T::ROWB;
     static constexpr int LDS = 4 * TILE;  // two buffers of K and V
@@ -1033,32 +1033,36 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
 // power of two that brings its largest value to 2^14 .. 2^15, and leaves hi and
 // lo in LDS with that exponent: K's is undone in the scores' factor, V's in the
 // weights, against the largest exponent so far (which o follows as it does the
-// running maximum).  A position is so kept to 22 bits down to 2^-17 of its
+// running maximum).  Every wave of a workgroup has 16 rows and a share of each
+// tile; with eight waves the same conversions serve twice the rows (one workgroup
+// a CU, tiles of 64 positions): 256 rows of each of 8 requests at 4,000 positions
+// 154 us instead of 215, 64 rows 62 either way.  A position is so kept to 22 bits down to 2^-17 of its
 // neighbours' largest, and to 2^-40 of that below: of the same order as the
 // weights.  Nodes that a row does not see must not cost its others their bits,
 // so where a node is further from its neighbours the segment is taken one by one.
-template <int HD_>
+template <int HD_, int NW_>
 struct WideCfg : Tile<_Float16, HD_> {
     typedef Tile<_Float16, HD_> T;
-    static constexpr int KT = HD_ == 64 ? 64 : 32, RT = 64, ST = KT / 16;
-    static constexpr int PW = KT / 4;                // positions of a wave
+    static constexpr int NW = NW_;
+    static constexpr int KT = NW == 4 ? (HD_ == 64 ? 64 : 32) : (HD_ == 256 ? 32 : 64), RT = 16 * NW, ST = KT / 16;
+    static constexpr int PW = KT / NW;               // positions of a wave
     static constexpr int LPR = HD_ / 4;              // lanes of a row
     static constexpr int NL = PW * LPR / 64;         // loads of its K
     static constexpr int HALF = KT * T::ROWB;        // hi or lo of a tile's K or V
     static constexpr int LDS = 2 * 4 * HALF;
-    static constexpr int PER_CU = LDS <= 72 * 1024 ? 2 : 1;
+    static constexpr int PER_CU = NW == 4 && LDS <= 72 * 1024 ? 2 : 1;
 };
 
-template <int HD>
-__global__ __launch_bounds__(256, (WideCfg<HD>::PER_CU)) void tree_wide_kernel(TreeArgs a) {
-    using C = WideCfg<HD>;
+template <int HD, int NW>
+__global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void tree_wide_kernel(TreeArgs a) {
+    using C = WideCfg<HD, NW>;
     using T = Tile<_Float16, HD>;
     constexpr int KT = C::KT, RT = C::RT, DT = T::DT, ST = C::ST, PW = C::PW, NL = C::NL;
     constexpr int QT = 1;  // tiles of 16 rows a wave: a second one does not fit the registers
     constexpr int kNone = -10000;  // exponent of nothing but zeros
     constexpr int kFar = 16;       // exponents so far apart cost bits
     __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
-    __shared__ int w_exp[2][2][4];    // exponents of a tile's K and V, a wave each
+    __shared__ int w_exp[2][2][NW];   // exponents of a tile's K and V, a wave each
     __shared__ int bad_seg, odd_seg;  // the last segment without a block, with a value that is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
@@ -1188,6 +1192,18 @@ __global__ __launch_bounds__(256, (WideCfg<HD>::PER_CU)) void tree_wide_kernel(T
             lds_barrier();  // tile t is there, the other buffer free
             const int k0 = t * KT;
             const unsigned char *const Ks = lds + (t & 1) * 4 * C::HALF, *const Vs = Ks + 2 * C::HALF;
+            // Of a SIMD's two waves one prepares the next tile before its products
+            // and one behind them, so that conversions run beside products (128
+            // rows of eight requests 162 -> 155 us; at head_dim 256, where it
+            // costs registers, 183 -> 192)
+            constexpr bool EARLY = NW == 8 && HD <= 128;
+            auto next = [&]() {
+                if (t + 1 < t1) {
+                    store(t + 1);
+                    if (t + 2 < t1) load(t + 2);
+                }
+            };
+            if (EARLY && wave >= 4) next();
             if (w_row < g.nrows) {
                 uint64_t vis[QT];
                 const bool tail = k0 + KT > g.s.cached;
@@ -1232,7 +1248,7 @@ __global__ __launch_bounds__(256, (WideCfg<HD>::PER_CU)) void tree_wide_kernel(T
                 float kf[ST], vf_[ST];
                 int top = E, least = 1000;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
+                for (int w = 0; w < NW; ++w) {
                     const int e = w_exp[t & 1][1][w];
                     top = max(top, e);
                     least = e == kNone ? least : min(least, e);
@@ -1312,10 +1328,7 @@ __global__ __launch_bounds__(256, (WideCfg<HD>::PER_CU)) void tree_wide_kernel(T
                     keep_order();
                 }
             }
-            if (t + 1 < t1) {
-                store(t + 1);
-                if (t + 2 < t1) load(t + 2);
-            }
+            if (!EARLY || wave < 4) next();
         }
         lds_barrier();  // bad_seg and odd_seg are known to all
         if (uniform(odd_seg) == seg) {
@@ -1431,7 +1444,7 @@ int launch_tiles(cw_ctx *ctx, TreeArgs a, void (*fn)(TreeArgs)) {
     CW_TRY(ctx_scratch(ctx, rows * (C::HD + 2) * sizeof(float), &scratch));
     a.part = static_cast<float *>(scratch);
     a.ml = a.part + rows * C::HD;
-    CW_TRY(launch(ctx, "attention_tree", fn, dim3(a.wgs), dim3(256), 0, a));
+    CW_TRY(launch(ctx, "attention_tree", fn, dim3(a.wgs), dim3(C::NW * 64), 0, a));
     // four heads a workgroup while that is about what the chip holds at once, more
     // for more rows (which also share the look at the lengths): 8 requests of 128
     // nodes 32 us with four each
@@ -1447,9 +1460,9 @@ template <int HD, int QT>
 int launch_tile(cw_ctx *ctx, const TreeArgs &a) {
     return launch_tiles<TileCfg<HD, QT>>(ctx, a, tree_tile_kernel<HD, QT>);
 }
-template <int HD>
+template <int HD, int NW>
 int launch_wide(cw_ctx *ctx, const TreeArgs &a) {
-    return launch_tiles<WideCfg<HD>>(ctx, a, tree_wide_kernel<HD>);
+    return launch_tiles<WideCfg<HD, NW>>(ctx, a, tree_wide_kernel<HD, NW>);
 }
 
 // By the rows of a (request, kv head) on average; us at head_dim 128, 8 requests
@@ -1459,6 +1472,9 @@ int launch_wide(cw_ctx *ctx, const TreeArgs &a) {
 //   128 rows: 54 and 51 for 128 rows with joins of 10 and 12, 159 and 153 for 512,
 //   28.6 and 34 for 244 of a single request;
 //   f32, 8 / 16 / 32 rows: split 46 / 48 / 71, wide 54 / 55 / 58.
+// Over f32 eight waves: 64 and 256 rows 35 / 39 and 113 / 93 (four / eight waves)
+// at head_dim 64, 2,000 positions at head_dim 256 49 / 56 for 64 and 265 / 183
+// for 512; at head_dim 128 they are no slower from 32 rows on.
 // head_dim 256: the split kernel's registers leave a CU one workgroup, 27.9 us for
 // 4 rows over f16; tiles 27.3.
 template <typename KVT, int HD>
@@ -1467,7 +1483,9 @@ int launch_by_rows(cw_ctx *ctx, const TreeArgs &a) {
     if constexpr (HD <= 128)
         if (rows <= (sizeof(KVT) == 2 ? 8 : 16)) return launch_split<KVT, HD>(ctx, a);
     if constexpr (sizeof(KVT) == 4) {
-        return launch_wide<HD>(ctx, a);
+        if constexpr (HD != 128)
+            if (rows <= 64) return launch_wide<HD, 4>(ctx, a);
+        return launch_wide<HD, 8>(ctx, a);
     } else {
         if constexpr (HD <= 128)
             if (rows > 256) return launch_tile<HD, 2>(ctx, a);
