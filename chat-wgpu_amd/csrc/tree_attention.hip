@@ -1058,7 +1058,6 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
     using C = WideCfg<HD, NW>;
     using T = Tile<_Float16, HD>;
     constexpr int KT = C::KT, RT = C::RT, DT = T::DT, ST = C::ST, PW = C::PW, NL = C::NL;
-    constexpr int QT = 1;  // tiles of 16 rows a wave: a second one does not fit the registers
     constexpr int kNone = -10000;  // exponent of nothing but zeros
     constexpr int kFar = 16;       // exponents so far apart cost bits
     __shared__ __attribute__((aligned(1024))) unsigned char lds[C::LDS];
@@ -1166,8 +1165,8 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
             }
         };
         const int t1 = g.lost ? g.t0 : g.t1;
-        const int w_row = g.rb * RT + wave * 16 * QT;
-        Query<T, QT> q;
+        const int w_row = g.rb * RT + wave * 16;
+        Query<T, 1> q;
         q.load(a, g, group, w_row, li, lg);
         if (g.t0 < t1) {
             look_up();
@@ -1178,16 +1177,11 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
             store(g.t0);
             if (g.t0 + 1 < t1) load(g.t0 + 1);
         }
-        f32x4 o[QT][DT];
-        float m[QT], l[QT];
+        f32x4 o[DT];
+        float m = -INFINITY, l = 0.0f;
         int E = kNone;  // o counts 2^(E - 15)
 #pragma unroll
-        for (int i = 0; i < QT; ++i) {
-            m[i] = -INFINITY;
-            l[i] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[i][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int t = g.t0; t < t1; ++t) {
             lds_barrier();  // tile t is there, the other buffer free
             const int k0 = t * KT;
@@ -1205,15 +1199,11 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
             };
             if (EARLY && wave >= 4) next();
             if (w_row < g.nrows) {
-                uint64_t vis[QT];
+                uint64_t vis = 0;
                 const bool tail = k0 + KT > g.s.cached;
-                if (tail) {
-#pragma unroll
-                    for (int i = 0; i < QT; ++i)
-                        vis[i] = sees64(a, g.s.r0 + q.node[i], q.node[i], g.s.n, k0 - g.s.cached) >> 4 * lg;
-                }
+                if (tail) vis = sees64(a, g.s.r0 + q.node[0], q.node[0], g.s.n, k0 - g.s.cached) >> 4 * lg;
                 constexpr int P = 2;  // sums in flight, as above
-                f32x4 s[QT][ST];
+                f32x4 s[ST];
                 constexpr int KN = ST * T::KS, KA = 2;
                 typename T::frag kh[KA + P], kl[KA + P];
                 auto k_n = [](int e) { return e / (P * T::KS) * P + e % P; };
@@ -1233,15 +1223,13 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
 #pragma unroll
                     for (int part = 0; part < 3; ++part)
 #pragma unroll
-                        for (int e = e0; e < e0 + P; ++e)
-#pragma unroll
-                            for (int i = 0; i < QT; ++i) {
-                                f32x4 &d = s[i][k_n(e)];
-                                if (part == 0 && k_x(e) == 0) d = f32x4{0.f, 0.f, 0.f, 0.f};
-                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    part == 2 ? kl[e % (KA + P)] : kh[e % (KA + P)],
-                                    part == 1 ? q.lo[i][k_x(e)] : q.hi[i][k_x(e)], d, 0, 0, 0);
-                            }
+                        for (int e = e0; e < e0 + P; ++e) {
+                            f32x4 &d = s[k_n(e)];
+                            if (part == 0 && k_x(e) == 0) d = f32x4{0.f, 0.f, 0.f, 0.f};
+                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                part == 2 ? kl[e % (KA + P)] : kh[e % (KA + P)],
+                                part == 1 ? q.lo[0][k_x(e)] : q.hi[0][k_x(e)], d, 0, 0, 0);
+                        }
                     keep_order();
                 }
                 // the tile's exponents: K's of this lane's positions, V's against all so far
@@ -1263,37 +1251,32 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
                 const float down = ldexpf(1.0f, E - top);
                 const bool grown = uniform(top) > uniform(E);
                 E = top;
+                if (tail) {
 #pragma unroll
-                for (int i = 0; i < QT; ++i) {
-                    if (tail) {
+                    for (int n = 0; n < ST; ++n)
 #pragma unroll
-                        for (int n = 0; n < ST; ++n)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                s[i][n][r] = vis[i] >> (n * 16 + r) & 1 ? s[i][n][r] : -INFINITY;
-                    }
-                    float f[ST];
-#pragma unroll
-                    for (int n = 0; n < ST; ++n) f[n] = fmaxf(q.qs[i] * kf[n], 1e-37f);  // (-inf keeps its sign)
-                    const float before = m[i];
-                    const float alpha = soften<ST>(s[i], f, T::UP, m[i], l[i]) * down;
-                    if (grown || __any(m[i] > before)) {
-#pragma unroll
-                        for (int d = 0; d < DT; ++d)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) o[i][d][r] *= alpha;
-                    }
+                        for (int r = 0; r < 4; ++r)
+                            s[n][r] = vis >> (n * 16 + r) & 1 ? s[n][r] : -INFINITY;
                 }
-                f16x8 ph[ST / 2][QT], pl[ST / 2][QT];
+                float f[ST];
 #pragma unroll
-                for (int kk = 0; kk < ST / 2; ++kk)
+                for (int n = 0; n < ST; ++n) f[n] = fmaxf(q.qs[0] * kf[n], 1e-37f);  // (-inf keeps its sign)
+                const float before = m;
+                const float alpha = soften<ST>(s, f, T::UP, m, l) * down;
+                if (grown || __any(m > before)) {
 #pragma unroll
-                    for (int i = 0; i < QT; ++i) {
-                        float w[8];
+                    for (int d = 0; d < DT; ++d)
 #pragma unroll
-                        for (int r = 0; r < 8; ++r) w[r] = s[i][2 * kk + r / 4][r % 4] * vf_[2 * kk + r / 4];
-                        split_f16(w, ph[kk][i], pl[kk][i]);
-                    }
+                        for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
+                }
+                f16x8 ph[ST / 2], pl[ST / 2];
+#pragma unroll
+                for (int kk = 0; kk < ST / 2; ++kk) {
+                    float w[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) w[r] = s[2 * kk + r / 4][r % 4] * vf_[2 * kk + r / 4];
+                    split_f16(w, ph[kk], pl[kk]);
+                }
                 const int row = 4 * lg + (li >> 2), c = (li & 3) >> 1;
                 auto v_at = [&](const unsigned char *base, int e) {
                     const unsigned char *p = base + e / DT * 2 * T::GROUPB + row * T::ROWB +
@@ -1320,11 +1303,9 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
                     for (int part = 0; part < 3; ++part)
 #pragma unroll
                         for (int e = e0; e < e0 + P; ++e)
-#pragma unroll
-                            for (int i = 0; i < QT; ++i)
-                                o[i][e % DT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    part == 2 ? vl[e % (VA + P)] : vh[e % (VA + P)],
-                                    part == 1 ? pl[e / DT][i] : ph[e / DT][i], o[i][e % DT], 0, 0, 0);
+                            o[e % DT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                part == 2 ? vl[e % (VA + P)] : vh[e % (VA + P)],
+                                part == 1 ? pl[e / DT] : ph[e / DT], o[e % DT], 0, 0, 0);
                     keep_order();
                 }
             }
@@ -1337,17 +1318,14 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
         }
         const bool bad = g.lost || bad_seg == seg;
         const float unit = ldexpf(1.0f, max(E, -200) - 15);
-#pragma unroll
-        for (int i = 0; i < QT; ++i) {
-            l[i] = group_sum(l[i]);
-            if (w_row + i * 16 + li >= g.nrows) continue;
+        l = group_sum(l);
+        if (w_row + li < g.nrows) {
 #pragma unroll
             for (int n = 0; n < DT; ++n) {
-                f32x4 v = o_quad<T>(o[i], n);
+                f32x4 v = o_quad<T>(o, n);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] *= unit;
-                put<HD, RT>(a, g, group, wave * 16 * QT + i * 16 + li, o_col<T>(n, lg), v, m[i],
-                            bad ? NAN : l[i]);
+                put<HD, RT>(a, g, group, wave * 16 + li, o_col<T>(n, lg), v, m, bad ? NAN : l);
             }
         }
     }
