@@ -31,7 +31,7 @@ struct TreeArgs {
     int n_heads, n_kv;
     float scale;  // log2(e) / sqrt(hd)
     int wgs;      // workgroups that share the units (tree_kernel)
-    float *part;  // [wgs][2][row block][hd] partial o, then
+    float *part;  // [wgs][2][row block][hd] partial o (part_at), then
     float *ml;    // [wgs][2][row block][2] their (max log2 e, sum)
 };
 
@@ -358,23 +358,39 @@ __device__ __forceinline__ int slot16(const TreeArgs &a, const Seg &g, int gi) {
     return (unsigned)id < (unsigned)a.map.n_blocks ? (id << a.map.shift) + (p0 & (a.map.page - 1)) : -1;
 }
 
-// Four elements of a row's result: the output where the segment has every
-// tile, else a partial
+// Where elements col .. col + 3 (col % 4 = 0) of a row of a partial o lie: as the
+// products leave 16 rows in a wave's lanes, so that it stores, and the join loads,
+// 1 KB in a piece; for few rows (the split kernel's) one after the other
 template <int HD, int RT>
-__device__ __forceinline__ void put(const TreeArgs &a, const Seg &g, int group, int row, int col,
-                                    f32x4 v, float m, float l) {
-    if (g.whole) {
-        const int rr = g.rb * RT + row, node = rr / group;
+__device__ __forceinline__ size_t part_at(size_t row, int col) {
+    if (RT == 16) return row * HD + col;
+    return (row / 16 * (HD / 16) + col / 16) * 256 + (size_t)((col / 4 % 4) * 16 + (int)(row % 16)) * 4;
+}
+
+// Where a row's elements 16 n + 4 c4 .. + 3 go: the output where the segment has
+// every tile (over the row's sum l), else a partial
+struct Dest {
+    float *p;
+    int step;  // from one n to the next
+    float l;   // what they are divided by; 1 for a partial
+    __device__ __forceinline__ void put(int n, f32x4 v) const {
         const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = l == 0.0f ? 0.0f : v[e] * f;
-        *reinterpret_cast<f32x4 *>(a.out + (size_t)(g.s.r0 + node) * a.out_stride +
-                                   (size_t)(g.h * group + rr - node * group) * HD + col) = v;
-    } else {
-        const size_t at = (size_t)g.part * RT + row;
-        *reinterpret_cast<f32x4 *>(a.part + at * HD + col) = v;
-        if (col == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(m, l);
+        *reinterpret_cast<f32x4 *>(p + n * step) = v;
     }
+};
+template <int HD, int RT>
+__device__ __forceinline__ Dest dest(const TreeArgs &a, const Seg &g, int group, int row, int c4,
+                                     float m, float l) {
+    if (g.whole) {
+        const int rr = g.rb * RT + row, node = rr / group;
+        return Dest{a.out + (size_t)(g.s.r0 + node) * a.out_stride +
+                        (size_t)(g.h * group + rr - node * group) * HD + c4 * 4, 16, l};
+    }
+    const size_t at = (size_t)g.part * RT + row;
+    if (c4 == 0) *reinterpret_cast<float2 *>(a.ml + at * 2) = make_float2(m, l);
+    return Dest{a.part + part_at<HD, RT>(at, c4 * 4), 256, 1.0f};
 }
 
 // A segment whose nodes have a V that is no finite number: as 0 * V it would
@@ -415,7 +431,7 @@ __device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, f
             if (g.whole)
                 a.out[(size_t)(g.s.r0 + node) * a.out_stride + head + e] = l == 0.0f ? 0.0f : o[e] / l;
             else
-                a.part[part * HD + lane * E + e] = o[e];
+                a.part[part_at<HD, RT>(part, lane * E & ~3) + (lane * E + e) % 4] = o[e];
         }
         if (!g.whole && lane == 0) *reinterpret_cast<float2 *>(a.ml + part * 2) = make_float2(m, l);
     }
@@ -803,7 +819,7 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
                 L += w_ml[w][row][1] * __builtin_amdgcn_exp2f(w_ml[w][row][0] - ref);
                 v += ow[(w * RT + row) * (HD / 4) + (c4 ^ (row & OS))];
             }
-            put<HD, RT>(a, g, group, row, 4 * c4, v, M, L);
+            dest<HD, RT>(a, g, group, row, c4, M, L).put(0, v);
         }
     }
 }
@@ -1017,11 +1033,13 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
             l[i] = group_sum(l[i]);
-            if (w_row + i * 16 + li >= g.nrows) continue;
+            int at = lane;
+            asm volatile("" : "+v"(at));  // (addresses of its own, not kept through the tiles)
+            const int row = wave * 16 * QT + i * 16 + (at & 15);
+            if (g.rb * RT + row >= g.nrows) continue;
+            const Dest to = dest<HD, RT>(a, g, group, row, at >> 4, m[i], bad ? NAN : l[i]);
 #pragma unroll
-            for (int n = 0; n < DT; ++n)
-                put<HD, RT>(a, g, group, wave * 16 * QT + i * 16 + li, o_col<T>(n, lg),
-                            o_quad<T>(o[i], n), m[i], bad ? NAN : l[i]);
+            for (int n = 0; n < DT; ++n) to.put(n, o[i][n]);
         }
     }
 }
@@ -1319,23 +1337,131 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
         const bool bad = g.lost || bad_seg == seg;
         const float unit = ldexpf(1.0f, max(E, -200) - 15);
         l = group_sum(l);
-        if (w_row + li < g.nrows) {
+        int at = lane;
+        asm volatile("" : "+v"(at));  // (addresses of its own, not kept through the tiles)
+        const int row = wave * 16 + (at & 15);
+        if (g.rb * RT + row < g.nrows) {
+            const Dest to = dest<HD, RT>(a, g, group, row, at >> 4, m, bad ? NAN : l);
 #pragma unroll
             for (int n = 0; n < DT; ++n) {
-                f32x4 v = o_quad<T>(o, n);
+                f32x4 v = o[n];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] *= unit;
-                put<HD, RT>(a, g, group, wave * 16 + li, o_col<T>(n, lg), v, m, bad ? NAN : l);
+                to.put(n, v);
             }
         }
     }
 }
 
-// Joins the partials of the rows whose units went to more than one workgroup,
-// in the order of the positions: a wave every so many heads of a row, the lanes
-// four elements of every 256 / HD-th partial.
-template <int HD>
+// Joins the partials of the rows whose units were dealt to several workgroups,
+// in the order of the positions.  16 rows of a request and kv head, 16 elements of
+// them, are one wave's registers as the products left them; a lane has its row's
+// maximum and sum beside them.  A workgroup has four such pieces of 16 elements,
+// or (SPLIT) one, whose partials its waves share: four times the workgroups, for
+// few rows of many partials, which wait for what a CU can have on its way (up to
+// 46 rows at 9,390 positions at head_dim 256, 85 partials each: 13 us, 35 without;
+// twelve requests of 4 to 16 rows, with more workgroups than CUs: 9.0, 6.7
+// without).  A wave a row and head instead took 26 us for 1,024 rows of 32 heads,
+// this 16: lengths and owners are looked up once for 16 rows.
+template <int HD, bool SPLIT>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int rt) {
+    constexpr int D = 4;  // partials in flight
+    __shared__ float s_m[SPLIT ? 4 : 1][16], s_l[SPLIT ? 4 : 1][16];
+    __shared__ f32x4 s_y[SPLIT ? 4 : 1][SPLIT ? 64 : 1];
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4, wave = uniform((int)(threadIdx.x >> 6));
+    const int h = blockIdx.y, n = SPLIT ? blockIdx.z : blockIdx.z * 4 + wave;
+    const int group = a.n_heads / a.n_kv;
+    long long total = 0, base = -1, tiles = 0;
+    int tile = 0;
+    SeqRows mine{0, 0, 0};
+    for (int c = 0; c < a.n_seq; c += 64) {
+        SeqRows s{0, 0, 0};
+        if (c + lane < a.n_seq) s = seq_rows(a.first_row, a.cached, a.rows, c + lane);
+        const long long v = work_of(s, group, a.n_kv, kt, rt).units, inc = wave_scan(v, lane);
+        const long long t = ((long long)s.n * group + 15) / 16, upto = wave_scan(t, lane) + tiles;
+        const unsigned long long hit = __ballot(upto > blockIdx.x);
+        if (hit && base < 0) {
+            const int at = __ffsll((long long)hit) - 1;
+            base = total + from_lane(inc - v, at);
+            tile = (int)(blockIdx.x - from_lane(upto - t, at));
+            mine = Requests{s}.at(a, at);
+        }
+        total += from_lane(inc, 63);
+        tiles = from_lane(upto, 63);
+    }
+    if (base < 0) return;
+    const Work wk = work_of(mine, group, a.n_kv, kt, rt);
+    const Deal deal(total, a.wgs);
+    const int rb = tile * 16 / rt, row = tile * 16 - rb * rt;  // of the row block
+    const long long u0 = base + ((long long)h * wk.blocks + rb) * (kOpen + wk.tiles) + kOpen;
+    const int first = uniform(deal.owner(u0)), last = uniform(deal.owner(u0 + wk.tiles - 1));
+    if (first == last) return;  // one workgroup had them all, and wrote the output
+    const int lr = min(li, mine.n * group - 1 - tile * 16);  // (rows behind the last: not loaded)
+    const int each = SPLIT ? (last - first + 4) / 4 : last - first + 1;
+    const int w0 = SPLIT ? first + wave * each : first, w1 = min(w0 + each, last + 1);
+    float M = -INFINITY, L = 0.0f;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    for (int c = w0; c < w1; c += D) {
+        float2 ml[D];
+        f32x4 v[D];
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int w = min(c + d, w1 - 1);
+            const size_t at = (size_t)(w * 2 + (w == first ? 1 : 0)) * rt + row;
+            ml[d] = *reinterpret_cast<const float2 *>(a.ml + (at + lr) * 2);
+            v[d] = *reinterpret_cast<const f32x4 *>(a.part + at * HD + n * 256 + lg * 64 + lr * 4);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // all of them requested
+        float Mn = M;
+#pragma unroll
+        for (int d = 0; d < D; ++d) Mn = fmaxf(Mn, ml[d].x);
+        const float ref = Mn == -INFINITY ? 0.0f : Mn, old = __builtin_amdgcn_exp2f(M - ref);
+        M = Mn;
+        L *= old;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= old;
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const bool has = c + d < w1;  // (else the last one again)
+            const float f = __builtin_amdgcn_exp2f(ml[d].x - ref);
+            L = has ? __builtin_fmaf(f, ml[d].y, L) : L;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = has ? __builtin_fmaf(f, v[d][e], y[e]) : y[e];
+        }
+    }
+    if constexpr (SPLIT) {
+        if (lg == 0) {
+            s_m[wave][li] = M;
+            s_l[wave][li] = L;
+        }
+        s_y[wave][lane] = y;
+        __syncthreads();
+        if (wave > 0) return;
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w][li]);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        L = 0.0f;
+        y = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(s_m[w][li] - ref);
+            L = __builtin_fmaf(f, s_l[w][li], L);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(f, s_y[w][lane][e], y[e]);
+        }
+    }
+    const int rr = tile * 16 + li, node = rr / group;
+    if (node >= mine.n) return;
+    const float f = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = L == 0.0f ? 0.0f : y[e] * f;
+    *reinterpret_cast<f32x4 *>(a.out + (size_t)(mine.r0 + node) * a.out_stride +
+                               (size_t)(h * group + rr - node * group) * HD + n * 16 + lg * 4) = y;
+}
+
+// The same for few rows a request (the split kernel's): a wave every so many
+// heads of a row, the lanes four elements of every 256 / HD-th partial.  (48
+// single rows of 4 query heads a kv head 4.5 us; in tiles of 16 rows 6.9.)
+template <int HD>
+__global__ __launch_bounds__(256) void tree_merge_rows_kernel(TreeArgs a, int kt, int rt) {
     constexpr int CL = HD / 4, SL = 64 / CL;
     const int r = blockIdx.x, lane = threadIdx.x & 63;
     const int group = a.n_heads / a.n_kv;
@@ -1423,12 +1549,20 @@ int launch_tiles(cw_ctx *ctx, TreeArgs a, void (*fn)(TreeArgs)) {
     a.part = static_cast<float *>(scratch);
     a.ml = a.part + rows * C::HD;
     CW_TRY(launch(ctx, "attention_tree", fn, dim3(a.wgs), dim3(C::NW * 64), 0, a));
-    // four heads a workgroup while that is about what the chip holds at once, more
-    // for more rows (which also share the look at the lengths): 8 requests of 128
-    // nodes 32 us with four each
-    const int by_chip = (8 * ctx->n_cu + a.rows - 1) / a.rows;
-    return launch(ctx, "attention_tree_merge", tree_merge_kernel<C::HD>,
-                  dim3(a.rows, std::min((a.n_heads + 3) / 4, by_chip)), dim3(256), 0, a, C::KT, C::RT);
+    if (C::RT == 16) {
+        // four heads a workgroup while that is about what the chip holds at once, more
+        // for more rows, which also share the look at the lengths
+        const int by_chip = (8 * ctx->n_cu + a.rows - 1) / a.rows;
+        return launch(ctx, "attention_tree_merge", tree_merge_rows_kernel<C::HD>,
+                      dim3(a.rows, std::min((a.n_heads + 3) / 4, by_chip)), dim3(256), 0, a, C::KT, C::RT);
+    }
+    // tiles of 16 rows that the requests have at most
+    const unsigned tiles = (unsigned)((long long)a.rows * (a.n_heads / a.n_kv) / 16) + a.n_seq;
+    if ((long long)tiles * a.n_kv * (C::HD / 64) <= ctx->n_cu)
+        return launch(ctx, "attention_tree_merge", tree_merge_kernel<C::HD, true>,
+                      dim3(tiles, a.n_kv, C::HD / 16), dim3(256), 0, a, C::KT, C::RT);
+    return launch(ctx, "attention_tree_merge", tree_merge_kernel<C::HD, false>,
+                  dim3(tiles, a.n_kv, C::HD / 64), dim3(256), 0, a, C::KT, C::RT);
 }
 template <typename KVT, int HD>
 int launch_split(cw_ctx *ctx, const TreeArgs &a) {
@@ -1495,8 +1629,8 @@ extern "C" int cw_attention_tree(cw_ctx *ctx, const cw_kv_pages *kv, const cw_ba
     CW_CHECK_ARG(n_heads > 0 && n_heads <= 4096 && n_heads % kv->n_kv_heads == 0,
                  "cw_attention_tree: n_heads=%d must be a multiple of n_kv_heads=%d (at most 4096)",
                  n_heads, kv->n_kv_heads);
-    CW_CHECK_ARG((long long)b->rows * (n_heads / kv->n_kv_heads) <= 1 << 30,
-                 "cw_attention_tree: %d rows of %d query heads a kv head are more than 2^30", b->rows,
+    CW_CHECK_ARG((long long)b->rows * (n_heads / kv->n_kv_heads) <= 1 << 27,
+                 "cw_attention_tree: %d rows of %d query heads a kv head are more than 2^27", b->rows,
                  n_heads / kv->n_kv_heads);
     const size_t width = (size_t)n_heads * kv->head_dim;
     CW_CHECK_ARG(q_stride >= width && out_stride >= width && q_stride < (1u << 31) &&

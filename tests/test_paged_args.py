@@ -136,9 +136,9 @@ def test_attention_tree():
 
 
 def test_attention_tree_rows_of_many_heads():
-    """Rows are counted per kv head in 32 bits."""
+    """Rows are counted per kv head, 16 to a workgroup of the join."""
     refused(cw.lib().cw_attention_tree(CTX, pages(n_kv_heads=1), batch(rows=1 << 23), P, 1 << 20, 4096,
-                                       1 << 50, 1 << 20), "2^30")
+                                       1 << 50, 1 << 20), "2^27")
 
 
 def test_kv_accept():
