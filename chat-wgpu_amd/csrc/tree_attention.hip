@@ -349,12 +349,15 @@ __device__ __forceinline__ bool next_segment(const TreeArgs &a, int group, const
     return false;
 }
 
-// The first slot of the 16 positions of group gi of the request (a block holds
-// all 16); -1 where the table names no block
-__device__ __forceinline__ int slot16(const TreeArgs &a, const Seg &g, int gi) {
+// The block of the 16 positions of group gi of the request (a block holds all 16),
+// and their first slot; -1 where the table names no block
+__device__ __forceinline__ int block16(const TreeArgs &a, const Seg &g, int gi) {
+    const int p0 = min(gi, g.last >> 4) << 4;
+    return a.map.tables ? a.map.tables[(size_t)g.b * a.map.max_blocks + (p0 >> a.map.shift)] : 0;
+}
+__device__ __forceinline__ int slot16(const TreeArgs &a, const Seg &g, int gi, int id) {
     const int p0 = min(gi, g.last >> 4) << 4;
     if (!a.map.tables) return g.b * a.map.page + p0;
-    const int id = a.map.tables[(size_t)g.b * a.map.max_blocks + (p0 >> a.map.shift)];
     return (unsigned)id < (unsigned)a.map.n_blocks ? (id << a.map.shift) + (p0 & (a.map.page - 1)) : -1;
 }
 
@@ -666,8 +669,9 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
         const char *const vc = static_cast<const char *>(a.vc) + (size_t)g.h * T::ROWB;
         bool bad = g.lost, odd = false;
         int slots = 0, tb = g.t0;  // of this wave's positions of tile tb + lane
-        auto look_up = [&]() {
-            slots = slot16(a, g, (tb + lane) * 4 + wave);
+        auto ids = [&]() { return block16(a, g, (tb + lane) * 4 + wave); };
+        auto look_up = [&](int id) {
+            slots = slot16(a, g, (tb + lane) * 4 + wave, id);
             bad |= __any(slots < 0 && tb + lane < g.t1);
             slots = max(slots, 0);  // a block has 16 positions: in the cache, and the row is lost
         };
@@ -679,10 +683,11 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
             dma_group<T>(vc + at, dst + T::GROUPB, rows, off, row_b, lane, g.once);
         };
         const int t1 = g.lost ? g.t0 : g.t1;
+        const int first_ids = g.t0 < t1 ? ids() : 0;  // requested before the queries
         Query<T, 1> q;
         q.load(a, g, group, g.rb * RT, li, lg);
         if (g.t0 < t1) {
-            look_up();
+            look_up(first_ids);
             load(g.t0);
         }
         q.convert(a.scale);
@@ -694,7 +699,7 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
             if (t + 1 < t1) {
                 if (t + 1 - tb == 64) {
                     tb += 64;
-                    look_up();
+                    look_up(ids());
                 }
                 wait_lds();  // reads of the tile before, whose place this takes
                 load(t + 1);
@@ -868,8 +873,9 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
         const char *const kc = static_cast<const char *>(a.kc) + (size_t)g.h * T::ROWB;
         const char *const vc = static_cast<const char *>(a.vc) + (size_t)g.h * T::ROWB;
         int slots = 0, tb = g.t0;
-        auto look_up = [&]() {
-            slots = slot16(a, g, (tb + lane) * (KT / 16) + my_group);
+        auto ids = [&]() { return block16(a, g, (tb + lane) * (KT / 16) + my_group); };
+        auto look_up = [&](int id) {
+            slots = slot16(a, g, (tb + lane) * (KT / 16) + my_group, id);
             if (__any(slots < 0 && tb + lane < g.t1)) bad_seg = seg;
             slots = max(slots, 0);  // a block has 16 positions: in the cache, and the row is lost
         };
@@ -882,10 +888,11 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
         };
         const int t1 = g.lost ? g.t0 : g.t1;
         const int w_row = g.rb * RT + wave * 16 * QT;
+        const int first_ids = g.t0 < t1 ? ids() : 0;  // requested before the queries
         Query<T, QT> q;
         q.load(a, g, group, w_row, li, lg);
         if (g.t0 < t1) {
-            look_up();
+            look_up(first_ids);
             load(g.t0);
         }
         q.convert(a.scale);
@@ -904,7 +911,7 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
             if (t + 1 < t1) {
                 if (t + 1 - tb == 64) {
                     tb += 64;
-                    look_up();
+                    look_up(ids());
                 }
                 load(t + 1);
             }
@@ -1097,8 +1104,9 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
         const float *const kc = static_cast<const float *>(a.kc) + (size_t)g.h * HD + lane % C::LPR * 4;
         const float *const vc = static_cast<const float *>(a.vc) + (size_t)g.h * HD + lane % C::LPR * 4;
         int slots = 0, tb = g.t0;
-        auto look_up = [&]() {
-            slots = slot16(a, g, (tb + lane) * ST + my_group);
+        auto ids = [&]() { return block16(a, g, (tb + lane) * ST + my_group); };
+        auto look_up = [&](int id) {
+            slots = slot16(a, g, (tb + lane) * ST + my_group, id);
             if (__any(slots < 0 && tb + lane < g.t1)) bad_seg = seg;
             slots = max(slots, 0);  // a block has 16 positions: in the cache, and the row is lost
         };
@@ -1106,7 +1114,7 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
         auto load = [&](int t) {
             if (t - tb == 64) {
                 tb += 64;
-                look_up();
+                look_up(ids());
             }
             const int slot = __builtin_amdgcn_readlane(slots, t - tb);
             const int rows = g.last - (min(t * ST + my_group, g.last >> 4) << 4);
@@ -1184,10 +1192,11 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
         };
         const int t1 = g.lost ? g.t0 : g.t1;
         const int w_row = g.rb * RT + wave * 16;
+        const int first_ids = g.t0 < t1 ? ids() : 0;  // requested before the queries
         Query<T, 1> q;
         q.load(a, g, group, w_row, li, lg);
         if (g.t0 < t1) {
-            look_up();
+            look_up(first_ids);
             load(g.t0);
         }
         q.convert(a.scale);

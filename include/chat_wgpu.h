@@ -289,11 +289,12 @@ int cw_block_tables(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const
  * q_stride and out_stride floats apart (multiples of 4, 16-byte aligned).
  * K and V of positions that a row does not see do not reach it, whatever they
  * hold; K that it sees, and V of cached positions, have to be finite, or that
- * row's own result may be NaN.  A row that sees nothing (or only scores of -inf) gives zeros; the
- * rows of a request with positions whose block is not in the cache give NaN.
- * cached[b] + rows of b is at most 2^30, b->rows * n_heads / n_kv_heads 2^27.  out must not overlap q.  Covers a
- * decode step (one row each, mask NULL), pieces of prompts (mask NULL) and
- * trees of drafted tokens. */
+ * row's own result may be NaN.  A row that sees nothing (or only scores of
+ * -inf) gives zeros; the rows of a request with positions whose block is not
+ * in the cache give NaN.  cached[b] + rows of b is at most 2^30, b->rows *
+ * n_heads / n_kv_heads at most 2^27.  out must not overlap q.  Covers a decode
+ * step (one row each, mask NULL), pieces of prompts (mask NULL) and trees of
+ * drafted tokens. */
 int cw_attention_tree(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const float *q,
                       size_t q_stride, int n_heads, float *out, size_t out_stride);
 /* Keeps the accepted nodes of each request: for i < path_len[b] the K and V of
