@@ -211,11 +211,15 @@ __device__ __forceinline__ void split_f16(const float (&v)[N], H &hi, H &lo) {
 
 // ---- who does what.  A tile is kt positions for one block of rt rows (a row: a
 // node and one of its query heads) of one kv head; the tiles of a request are
-// ordered (kv head, row block, position).  A row block costs kOpen units to
-// begin (its queries, the first tile's way from memory) and one for each tile;
-// all units are dealt to the workgroups in runs of q or q + 1, so that requests
-// of any lengths share the chip evenly.  A run's piece of a row block is a
-// segment; what no workgroup has whole is joined by tree_merge_kernel.
+// ordered (kv head, row block, position).  A row block costs kOpen tiles to begin
+// (its queries, the first tile's way from memory) and the positions that its rows
+// can see, of which without a mask later blocks have more; all of it is dealt to
+// the workgroups in equal runs, so that requests of any lengths share the chip
+// evenly, and a tile belongs to the run that its first position is in.  A run's
+// piece of a row block is a segment; what no workgroup has whole is joined by
+// tree_merge_kernel.  (Where every block of a prompt counts and takes the tiles of
+// the last, 2,000 rows of 16 heads take 85 us instead of 58, eight prompts of 345
+// over f32 55 instead of 44.)
 // (kOpen 0, 2, 4 and 8: 48 single rows at 100 .. 8,000 positions 88, 74, 74 and
 // 77 us.  Workgroups of one CU and the XCDs are served unevenly, equal runs end
 // up to 1.5 times apart; short runs fetched by whoever is free gain nothing,
@@ -225,13 +229,40 @@ __device__ __forceinline__ void split_f16(const float (&v)[N], H &hi, H &lo) {
 constexpr int kOpen = 3;
 
 struct Work {
-    int tiles, blocks;
-    long long units;
+    int blocks;     // of rows
+    int len, grow;
+    int c, n, group, kt, rt;
+    bool causal;
+    // units before block i of a kv head; begin(blocks): of all (under 2^61 for all
+    // heads and requests: at most 2^33 rows of query heads in a call)
+    __device__ __forceinline__ long long begin(int i) const {
+        return (long long)((uint64_t)(uint32_t)i * (2u * len + (uint32_t)(i + 1) * grow) >> 1);
+    }
+    __device__ __forceinline__ int size(int i) const { return len + (i + 1) * grow; }
+    __device__ __forceinline__ long long first_tile(int i) const { return begin(i) + kOpen * kt; }
+    __device__ __forceinline__ int tiles(int i) const {
+        const int seen = causal ? min(n, ((i + 1) * rt - 1) / group + 1) : n;
+        return (c + seen + kt - 1) / kt;
+    }
+    // the block that unit x of a kv head is in
+    __device__ __forceinline__ int block(long long x) const {
+        int lo = 0, hi = blocks;
+        while (hi - lo > 1) {
+            const int m = (lo + hi) >> 1;
+            if (begin(m) <= x) lo = m;
+            else hi = m;
+        }
+        return lo;
+    }
 };
-__device__ __forceinline__ Work work_of(const SeqRows &s, int group, int n_kv, int kt, int rt) {
-    if (!s.n) return Work{0, 0, 0};
-    const int t = (s.cached + s.n + kt - 1) / kt, rb = (int)(((long long)s.n * group + rt - 1) / rt);
-    return Work{t, rb, (long long)n_kv * rb * (kOpen + t)};
+__device__ __forceinline__ Work work_of(const TreeArgs &a, const SeqRows &s, int group, int kt, int rt) {
+    // without a mask block i sees at most 1 + (i + 1) rt / group nodes; a tile that is
+    // begun counts whole
+    const int blocks = (int)(((long long)s.n * group + rt - 1) / rt);
+    const bool causal = !a.mask && blocks > 1;
+    const int see = causal ? s.cached + kt : (s.cached + s.n + kt - 1) / kt * kt;
+    return Work{blocks, kOpen * kt + see,
+                causal ? (rt + group - 1) / group : 0, s.cached, s.n, group, kt, rt, causal};
 }
 
 __device__ __forceinline__ long long from_lane(long long v, int l) {
@@ -245,17 +276,23 @@ __device__ __forceinline__ long long divide(long long n, long long d) {
     return n / d;
 }
 
+// Runs of q or q + 1 tiles' units, none shorter than a tile: so a run inside a row
+// block has a tile's first
 struct Deal {
-    long long q;
-    int rem;
-    __device__ Deal(long long units, int wgs) {
-        q = divide(units, wgs);
-        rem = (int)(units - q * wgs);
+    long long q, units;
+    int rem, kt;
+    __device__ Deal(long long u, int wgs, int kt) : units(u), kt(kt) {
+        const long long t = (u + kt - 1) / kt;
+        q = divide(t, wgs);
+        rem = (int)(t - q * wgs);
     }
-    __device__ long long start(int w) const { return q * w + min(w, rem); }
+    __device__ long long start(int w) const {
+        const long long u = (q * w + min(w, rem)) * kt;
+        return u < units ? u : units;
+    }
     __device__ int owner(long long u) const {
-        const long long big = (q + 1) * rem;
-        return u < big ? (int)divide(u, q + 1) : rem + (int)divide(u - big, q);
+        const long long t = u / kt, big = (q + 1) * rem;
+        return t < big ? (int)divide(t, q + 1) : rem + (int)divide(t - big, q);
     }
 };
 
@@ -265,6 +302,7 @@ struct Seg {
     int b, h, rb, t0, t1, nrows, last, part;  // part: its place among the partials
     bool whole, lost;                         // lost: positions that no table entry covers
     bool once;                                // the request's only row block
+    bool rest;                                // its last tile is the row block's, and positions follow
 };
 struct Cursor {
     long long u, end, base;  // next unit, end of the run, first unit of request b
@@ -288,12 +326,15 @@ __device__ __forceinline__ Cursor first_unit(const TreeArgs &a, int group, int l
     auto rows = [&](int b) {
         return b < a.n_seq ? seq_rows(a.first_row, a.cached, a.rows, b) : SeqRows{0, 0, 0};
     };
-    auto units = [&](const SeqRows &s) { return work_of(s, group, a.n_kv, KT, RT).units; };
+    auto units = [&](const SeqRows &s) {
+        const Work w = work_of(a, s, group, KT, RT);
+        return a.n_kv * w.begin(w.blocks);
+    };
     req.s = rows(lane);
     const long long v0 = units(req.s), inc0 = wave_scan(v0, lane);
     long long total = from_lane(inc0, 63);
     for (int c = 64; c < a.n_seq; c += 64) total += from_lane(wave_scan(units(rows(c + lane)), lane), 63);
-    const Deal deal(total, a.wgs);
+    const Deal deal(total, a.wgs, KT);
     Cursor cur{deal.start(blockIdx.x), deal.start(blockIdx.x + 1), 0, 0};
     if (cur.u >= cur.end) return cur;
     long long v = v0, inc = inc0;
@@ -320,27 +361,31 @@ __device__ __forceinline__ bool next_segment(const TreeArgs &a, int group, const
                                              Cursor &cur, Seg &g) {
     while (cur.u < cur.end && cur.b < a.n_seq) {
         g.s = req.at(a, cur.b);
-        const Work wk = work_of(g.s, group, a.n_kv, KT, RT);
-        if (cur.u >= cur.base + wk.units) {
-            cur.base += wk.units;
+        const Work wk = work_of(a, g.s, group, KT, RT);
+        const long long per = wk.begin(wk.blocks);  // of a kv head
+        if (cur.u >= cur.base + a.n_kv * per) {
+            cur.base += a.n_kv * per;
             ++cur.b;
             continue;
         }
         const long long local = cur.u - cur.base;
-        const int each = kOpen + wk.tiles, hr = uniform((int)divide(local, each));
-        const int from = uniform((int)(local - (long long)hr * each));
-        const int to = uniform((int)min((long long)each, from + (cur.end - cur.u)));
-        cur.u += to - from;
-        if (to <= kOpen) continue;  // the run ends before the row block's first tile
+        g.h = uniform((int)divide(local, per));
+        const long long x = local - g.h * per;
+        g.rb = uniform(wk.block(x));
+        // of the block's units, less than 2^31: the run's
+        const int from = uniform((int)(x - wk.begin(g.rb))), left = wk.size(g.rb) - from;
+        const int take = cur.end - cur.u < left ? (int)(cur.end - cur.u) : left;
+        cur.u += take;
+        const int tiles = wk.tiles(g.rb), open = kOpen * KT;
+        g.t0 = uniform((unsigned)max(from - open + KT - 1, 0) / KT);
+        g.t1 = uniform(min(tiles, (int)((unsigned)max(from + take - open + KT - 1, 0) / KT)));
+        if (g.t0 >= g.t1) continue;  // no tile begins in it
         g.b = cur.b;
-        g.t0 = max(from - kOpen, 0);
-        g.t1 = to - kOpen;
-        g.h = uniform(hr / wk.blocks);
-        g.rb = uniform(hr - g.h * wk.blocks);
         g.nrows = g.s.n * group;
         g.last = g.s.cached + g.s.n - 1;
         g.once = wk.blocks == 1;
-        g.whole = g.t0 == 0 && g.t1 == wk.tiles;
+        g.whole = g.t0 == 0 && g.t1 == tiles;
+        g.rest = g.t1 == tiles && tiles * KT <= g.last;
         g.part = blockIdx.x * 2 + (g.t0 > 0 ? 0 : 1);
         g.lost = a.map.tables ? (g.last >> a.map.shift) >= a.map.max_blocks
                               : g.b >= a.map.n_blocks || g.last >= a.map.page;
@@ -359,6 +404,16 @@ __device__ __forceinline__ int slot16(const TreeArgs &a, const Seg &g, int gi, i
     const int p0 = min(gi, g.last >> 4) << 4;
     if (!a.map.tables) return g.b * a.map.page + p0;
     return (unsigned)id < (unsigned)a.map.n_blocks ? (id << a.map.shift) + (p0 & (a.map.page - 1)) : -1;
+}
+
+// Whether the table names no block for one of the positions behind the row block's
+// last tile (which no row of it sees)
+template <int KT>
+__device__ __forceinline__ bool rest_lost(const TreeArgs &a, const Seg &g, int lane) {
+    if (!g.rest || g.lost) return false;
+    int bad = 0;
+    for (int gi = g.t1 * (KT / 16) + lane; gi <= g.last >> 4; gi += 64) bad |= slot16(a, g, gi, block16(a, g, gi)) < 0;
+    return __any(bad);
 }
 
 // Where elements col .. col + 3 (col % 4 = 0) of a row of a partial o lie: as the
@@ -786,6 +841,7 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
             }
         }
         // join the waves
+        bad |= rest_lost<KT>(a, g, lane);
         l = group_sum(l);
         if (lg == 0) {
             w_ml[wave][li][0] = m;
@@ -1036,7 +1092,7 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
             one_by_one<_Float16, HD, RT>(a, g, group, KT, T::UP);
             continue;
         }
-        const bool bad = g.lost || bad_seg == seg;
+        const bool bad = g.lost || bad_seg == seg || rest_lost<KT>(a, g, lane);
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
             l[i] = group_sum(l[i]);
@@ -1343,7 +1399,7 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
             one_by_one<float, HD, RT>(a, g, group, KT, T::UP);
             continue;
         }
-        const bool bad = g.lost || bad_seg == seg;
+        const bool bad = g.lost || bad_seg == seg || rest_lost<KT>(a, g, lane);
         const float unit = ldexpf(1.0f, max(E, -200) - 15);
         l = group_sum(l);
         int at = lane;
@@ -1372,9 +1428,10 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
 // twelve requests of 4 to 16 rows, with more workgroups than CUs: 9.0, 6.7
 // without).  A wave a row and head instead took 26 us for 1,024 rows of 32 heads,
 // this 16: lengths and owners are looked up once for 16 rows.
-template <int HD, bool SPLIT>
-__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int rt) {
-    constexpr int D = 4;  // partials in flight
+template <typename C, bool SPLIT>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
+    constexpr int HD = C::HD, kt = C::KT, rt = C::RT;
+    constexpr int D = SPLIT ? 8 : 4;  // partials in flight
     __shared__ float s_m[SPLIT ? 4 : 1][16], s_l[SPLIT ? 4 : 1][16];
     __shared__ f32x4 s_y[SPLIT ? 4 : 1][SPLIT ? 64 : 1];
     const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4, wave = uniform((int)(threadIdx.x >> 6));
@@ -1386,7 +1443,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int
     for (int c = 0; c < a.n_seq; c += 64) {
         SeqRows s{0, 0, 0};
         if (c + lane < a.n_seq) s = seq_rows(a.first_row, a.cached, a.rows, c + lane);
-        const long long v = work_of(s, group, a.n_kv, kt, rt).units, inc = wave_scan(v, lane);
+        const Work w = work_of(a, s, group, kt, rt);
+        const long long v = a.n_kv * w.begin(w.blocks), inc = wave_scan(v, lane);
         const long long t = ((long long)s.n * group + 15) / 16, upto = wave_scan(t, lane) + tiles;
         const unsigned long long hit = __ballot(upto > blockIdx.x);
         if (hit && base < 0) {
@@ -1399,11 +1457,11 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int
         tiles = from_lane(upto, 63);
     }
     if (base < 0) return;
-    const Work wk = work_of(mine, group, a.n_kv, kt, rt);
-    const Deal deal(total, a.wgs);
+    const Work wk = work_of(a, mine, group, kt, rt);
+    const Deal deal(total, a.wgs, kt);
     const int rb = tile * 16 / rt, row = tile * 16 - rb * rt;  // of the row block
-    const long long u0 = base + ((long long)h * wk.blocks + rb) * (kOpen + wk.tiles) + kOpen;
-    const int first = uniform(deal.owner(u0)), last = uniform(deal.owner(u0 + wk.tiles - 1));
+    const long long u0 = base + h * wk.begin(wk.blocks) + wk.first_tile(rb);
+    const int first = uniform(deal.owner(u0)), last = uniform(deal.owner(u0 + (long long)(wk.tiles(rb) - 1) * kt));
     if (first == last) return;  // one workgroup had them all, and wrote the output
     const int lr = min(li, mine.n * group - 1 - tile * 16);  // (rows behind the last: not loaded)
     const int each = SPLIT ? (last - first + 4) / 4 : last - first + 1;
@@ -1469,8 +1527,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int kt, int
 // The same for few rows a request (the split kernel's): a wave every so many
 // heads of a row, the lanes four elements of every 256 / HD-th partial.  (48
 // single rows of 4 query heads a kv head 4.5 us; in tiles of 16 rows 6.9.)
-template <int HD>
-__global__ __launch_bounds__(256) void tree_merge_rows_kernel(TreeArgs a, int kt, int rt) {
+template <typename C>
+__global__ __launch_bounds__(256) void tree_merge_rows_kernel(TreeArgs a) {
+    constexpr int HD = C::HD, kt = C::KT, rt = C::RT;
     constexpr int CL = HD / 4, SL = 64 / CL;
     const int r = blockIdx.x, lane = threadIdx.x & 63;
     const int group = a.n_heads / a.n_kv;
@@ -1479,7 +1538,8 @@ __global__ __launch_bounds__(256) void tree_merge_rows_kernel(TreeArgs a, int kt
     for (int c = 0; c < a.n_seq; c += 64) {
         SeqRows s{0, 0, 0};
         if (c + lane < a.n_seq) s = seq_rows(a.first_row, a.cached, a.rows, c + lane);
-        const long long v = work_of(s, group, a.n_kv, kt, rt).units, inc = wave_scan(v, lane);
+        const Work w = work_of(a, s, group, kt, rt);
+        const long long v = a.n_kv * w.begin(w.blocks), inc = wave_scan(v, lane);
         const unsigned long long hit = __ballot(r >= s.r0 && r < s.r0 + s.n);
         if (hit && base < 0) {
             const int at = __ffsll((long long)hit) - 1;
@@ -1489,13 +1549,14 @@ __global__ __launch_bounds__(256) void tree_merge_rows_kernel(TreeArgs a, int kt
         total += from_lane(inc, 63);
     }
     if (base < 0) return;
-    const Work wk = work_of(mine, group, a.n_kv, kt, rt);
-    const Deal deal(total, a.wgs);
+    const Work wk = work_of(a, mine, group, kt, rt);
+    const Deal deal(total, a.wgs, kt);
     const int col = lane % CL * 4, sl = lane / CL;
     for (int head = uniform((int)(blockIdx.y * 4 + (threadIdx.x >> 6))); head < a.n_heads; head += gridDim.y * 4) {
         const int h = head / group, rr = (r - mine.r0) * group + head - h * group;
-        const long long u0 = base + ((long long)h * wk.blocks + rr / rt) * (kOpen + wk.tiles) + kOpen;
-        const int w0 = uniform(deal.owner(u0)), w1 = uniform(deal.owner(u0 + wk.tiles - 1));
+        const int rb = rr / rt;
+        const long long u0 = base + h * wk.begin(wk.blocks) + wk.first_tile(rb);
+        const int w0 = uniform(deal.owner(u0)), w1 = uniform(deal.owner(u0 + (long long)(wk.tiles(rb) - 1) * kt));
         if (w0 == w1) continue;  // one workgroup had them all, and wrote the output
         auto at = [&](int w) { return (size_t)(w * 2 + (w == w0 ? 1 : 0)) * rt + rr % rt; };
         float M = -INFINITY, L = 0.0f;
@@ -1558,20 +1619,21 @@ int launch_tiles(cw_ctx *ctx, TreeArgs a, void (*fn)(TreeArgs)) {
     a.part = static_cast<float *>(scratch);
     a.ml = a.part + rows * C::HD;
     CW_TRY(launch(ctx, "attention_tree", fn, dim3(a.wgs), dim3(C::NW * 64), 0, a));
-    if (C::RT == 16) {
+    if constexpr (C::RT == 16) {
         // four heads a workgroup while that is about what the chip holds at once, more
         // for more rows, which also share the look at the lengths
         const int by_chip = (8 * ctx->n_cu + a.rows - 1) / a.rows;
-        return launch(ctx, "attention_tree_merge", tree_merge_rows_kernel<C::HD>,
-                      dim3(a.rows, std::min((a.n_heads + 3) / 4, by_chip)), dim3(256), 0, a, C::KT, C::RT);
+        return launch(ctx, "attention_tree_merge", tree_merge_rows_kernel<C>,
+                      dim3(a.rows, std::min((a.n_heads + 3) / 4, by_chip)), dim3(256), 0, a);
+    } else {
+        // tiles of 16 rows that the requests have at most
+        const unsigned tiles = (unsigned)((long long)a.rows * (a.n_heads / a.n_kv) / 16) + a.n_seq;
+        if ((long long)tiles * a.n_kv * (C::HD / 64) <= ctx->n_cu)
+            return launch(ctx, "attention_tree_merge", tree_merge_kernel<C, true>,
+                          dim3(tiles, a.n_kv, C::HD / 16), dim3(256), 0, a);
+        return launch(ctx, "attention_tree_merge", tree_merge_kernel<C, false>,
+                      dim3(tiles, a.n_kv, C::HD / 64), dim3(256), 0, a);
     }
-    // tiles of 16 rows that the requests have at most
-    const unsigned tiles = (unsigned)((long long)a.rows * (a.n_heads / a.n_kv) / 16) + a.n_seq;
-    if ((long long)tiles * a.n_kv * (C::HD / 64) <= ctx->n_cu)
-        return launch(ctx, "attention_tree_merge", tree_merge_kernel<C::HD, true>,
-                      dim3(tiles, a.n_kv, C::HD / 16), dim3(256), 0, a, C::KT, C::RT);
-    return launch(ctx, "attention_tree_merge", tree_merge_kernel<C::HD, false>,
-                  dim3(tiles, a.n_kv, C::HD / 64), dim3(256), 0, a, C::KT, C::RT);
 }
 template <typename KVT, int HD>
 int launch_split(cw_ctx *ctx, const TreeArgs &a) {
@@ -1641,6 +1703,8 @@ extern "C" int cw_attention_tree(cw_ctx *ctx, const cw_kv_pages *kv, const cw_ba
     CW_CHECK_ARG((long long)b->rows * (n_heads / kv->n_kv_heads) <= 1 << 27,
                  "cw_attention_tree: %d rows of %d query heads a kv head are more than 2^27", b->rows,
                  n_heads / kv->n_kv_heads);
+    CW_CHECK_ARG((long long)b->rows * n_heads <= 1LL << 33,
+                 "cw_attention_tree: %d rows of %d query heads are more than 2^33", b->rows, n_heads);
     const size_t width = (size_t)n_heads * kv->head_dim;
     CW_CHECK_ARG(q_stride >= width && out_stride >= width && q_stride < (1u << 31) &&
                      out_stride < (1u << 31) && q_stride % 4 == 0 && out_stride % 4 == 0,

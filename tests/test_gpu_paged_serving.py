@@ -26,6 +26,28 @@ def test_attention_of_many_requests(ctx, rng, hd, contig, most, kv):
     b.check(b.run())
 
 
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kvh,hd", [(4, 2, 128), (7, 1, 128), (16, 1, 64), (7, 1, 256), (66, 1, 64), (3, 3, 32)])
+def test_attention_of_prompts(ctx, rng, heads, kvh, hd, kv):
+    """Prompts with little or nothing cached: later rows see more than earlier
+    ones, and a block of rows only the positions up to its last."""
+    b = Batch(ctx, rng, [0, 0, 5, 40, 0], [330, 64, 65, 129, 1], heads, kvh, hd, kv, 16, spare_rows=2)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("heads,hd", [(1, 128), (8, 128), (8, 64), (8, 256), (2, 32)])
+def test_a_lost_block_behind_the_first_rows(ctx, rng, heads, hd, kv):
+    """Every row of a request with a block that is not there is NaN, the rows
+    too that come before it."""
+    b = Batch(ctx, rng, [0, 30], [300, 9], heads, 1, hd, kv, 16)
+    good = b.run()
+    b.check(good)
+    b.tables[0, 18] = -1  # positions 288 .. 299
+    got = b.run()
+    assert np.all(np.isnan(got[:300])) and np.array_equal(got[300:], good[300:])
+
+
 @pytest.mark.parametrize("rows_cap", [300, 9000])
 def test_tables_of_many_requests(ctx, rng, rows_cap):
     """More requests than the offsets in LDS hold."""

@@ -139,6 +139,8 @@ def test_attention_tree_rows_of_many_heads():
     """Rows are counted per kv head, 16 to a workgroup of the join."""
     refused(cw.lib().cw_attention_tree(CTX, pages(n_kv_heads=1), batch(rows=1 << 23), P, 1 << 20, 4096,
                                        1 << 50, 1 << 20), "2^27")
+    refused(cw.lib().cw_attention_tree(CTX, pages(n_kv_heads=1024), batch(rows=1 << 23), P, 1 << 20, 4096,
+                                       1 << 50, 1 << 20), "2^33")
 
 
 def test_kv_accept():
