@@ -35,6 +35,12 @@ struct TreeArgs {
     float *ml;    // [wgs][2][row block][2] their (max log2 e, sum)
 };
 
+// Whether positions of the request lie behind its table, or its slots
+__device__ __forceinline__ bool lost_length(const TreeArgs &a, const SeqRows &s) {
+    const int last = s.cached + s.n - 1;
+    return a.map.tables ? (last >> a.map.shift) >= a.map.max_blocks : last >= a.map.page;
+}
+
 // Whether node i of a request sees its node j (row: the node's row of the mask)
 __device__ __forceinline__ bool sees(const TreeArgs &a, int row, int i, int j) {
     if (!a.mask) return j <= i;
@@ -89,9 +95,10 @@ __global__ __launch_bounds__(kThreads) void tree_row_kernel(TreeArgs a) {
     for (int e = 0; e < E; ++e)
         q[e] = on ? a.q[(size_t)r * a.q_stride + (size_t)h * HD + e0 + e] : 0.0f;
     float m = -INFINITY, l = 0.0f;
-    bool lost = false;  // a position without a block
+    bool lost = lost_length(a, s);  // or a position without a block
+    const int end = lost ? 0 : s.cached + s.n;
     const KVT *kc = static_cast<const KVT *>(a.kc), *vc = static_cast<const KVT *>(a.vc);
-    for (int p = wave; p < s.cached + s.n; p += W) {
+    for (int p = wave; p < end; p += W) {
         const int slot = slot_of(a.map, lo, p);
         lost |= slot < 0;
         if (slot < 0 || (p >= s.cached && !sees(a, r, i, p - s.cached))) continue;
@@ -230,11 +237,10 @@ constexpr int kOpen = 3;
 
 struct Work {
     int blocks;     // of rows
-    int len, grow;
+    int len, grow;  // block i: len + (i + 1) grow units
     int c, n, group, kt, rt;
     bool causal;
-    // units before block i of a kv head; begin(blocks): of all (under 2^61 for all
-    // heads and requests: at most 2^33 rows of query heads in a call)
+    // units before block i of a kv head; begin(blocks): of all
     __device__ __forceinline__ long long begin(int i) const {
         return (long long)((uint64_t)(uint32_t)i * (2u * len + (uint32_t)(i + 1) * grow) >> 1);
     }
@@ -257,12 +263,17 @@ struct Work {
 };
 __device__ __forceinline__ Work work_of(const TreeArgs &a, const SeqRows &s, int group, int kt, int rt) {
     // without a mask block i sees at most 1 + (i + 1) rt / group nodes; a tile that is
-    // begun counts whole
-    const int blocks = (int)(((long long)s.n * group + rt - 1) / rt);
-    const bool causal = !a.mask && blocks > 1;
-    const int see = causal ? s.cached + kt : (s.cached + s.n + kt - 1) / kt * kt;
-    return Work{blocks, kOpen * kt + see,
-                causal ? (rt + group - 1) / group : 0, s.cached, s.n, group, kt, rt, causal};
+    // begun counts whole; of a request that is lost nothing is read
+    const bool lost = lost_length(a, s);
+    const int blocks = (int)(((long long)s.n * group + rt - 1) / rt), c = lost ? 0 : s.cached;
+    const int n = lost ? 1 : s.n;
+    const bool causal = !a.mask && blocks > 1 && !lost;
+    const int see = causal ? c + kt : (c + n + kt - 1) / kt * kt;
+    Work w{blocks, kOpen * kt + see, causal ? (rt + group - 1) / group : 0, c, n, group, kt, rt, causal};
+    // sums over 2^16 requests and 2^10 heads stay below 2^62, whatever the device
+    // arrays hold
+    if (w.begin(blocks) >> 36) w.blocks = 0;
+    return w;
 }
 
 __device__ __forceinline__ long long from_lane(long long v, int l) {
@@ -387,8 +398,7 @@ __device__ __forceinline__ bool next_segment(const TreeArgs &a, int group, const
         g.whole = g.t0 == 0 && g.t1 == tiles;
         g.rest = g.t1 == tiles && tiles * KT <= g.last;
         g.part = blockIdx.x * 2 + (g.t0 > 0 ? 0 : 1);
-        g.lost = a.map.tables ? (g.last >> a.map.shift) >= a.map.max_blocks
-                              : g.b >= a.map.n_blocks || g.last >= a.map.page;
+        g.lost = lost_length(a, g.s);
         return true;
     }
     return false;
@@ -1458,6 +1468,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
     }
     if (base < 0) return;
     const Work wk = work_of(a, mine, group, kt, rt);
+    if (!wk.blocks) return;
     const Deal deal(total, a.wgs, kt);
     const int rb = tile * 16 / rt, row = tile * 16 - rb * rt;  // of the row block
     const long long u0 = base + h * wk.begin(wk.blocks) + wk.first_tile(rb);
@@ -1550,6 +1561,7 @@ __global__ __launch_bounds__(256) void tree_merge_rows_kernel(TreeArgs a) {
     }
     if (base < 0) return;
     const Work wk = work_of(a, mine, group, kt, rt);
+    if (!wk.blocks) return;
     const Deal deal(total, a.wgs, kt);
     const int col = lane % CL * 4, sl = lane / CL;
     for (int head = uniform((int)(blockIdx.y * 4 + (threadIdx.x >> 6))); head < a.n_heads; head += gridDim.y * 4) {

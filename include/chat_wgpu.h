@@ -292,7 +292,9 @@ int cw_block_tables(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const
  * row's own result may be NaN.  A row that sees nothing (or only scores of
  * -inf) gives zeros; the rows of a request with positions whose block is not
  * in the cache give NaN.  cached[b] + rows of b is at most 2^30, b->rows *
- * n_heads at most 2^33 and 2^27 of them a kv head.  out must not overlap q.
+ * n_heads at most 2^33 and 2^27 of them a kv head (and the product of the two
+ * for a request and kv head at most 2^39: one beyond has no rows).  out must
+ * not overlap q.
  * Covers a decode step (one row each, mask NULL), pieces of prompts (mask
  * NULL) and trees of drafted tokens. */
 int cw_attention_tree(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const float *q,

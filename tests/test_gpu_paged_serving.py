@@ -48,6 +48,19 @@ def test_a_lost_block_behind_the_first_rows(ctx, rng, heads, hd, kv):
     assert np.all(np.isnan(got[:300])) and np.array_equal(got[300:], good[300:])
 
 
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("heads,hd,contig", [(1, 128, False), (8, 128, True), (8, 64, False), (8, 256, False),
+                                             (2, 32, True)])
+def test_a_length_behind_the_cache(ctx, rng, heads, hd, contig, kv):
+    """A length of a billion positions that the cache does not have: NaN for that
+    request's rows, the others as they were."""
+    b = Batch(ctx, rng, [0, 30], [300, 9], heads, 1, hd, kv, 16, contig=contig)
+    ref, bound = po.attention(b.q, b.k, b.v, b.tables, b.page, b.cached, b.first)
+    b.cached[0] = (1 << 30) - 300
+    got = b.run()
+    assert np.all(np.isnan(got[:300])) and np.all(np.abs(got - ref)[300:] <= bound[300:])
+
+
 @pytest.mark.parametrize("rows_cap", [300, 9000])
 def test_tables_of_many_requests(ctx, rng, rows_cap):
     """More requests than the offsets in LDS hold."""
