@@ -15,8 +15,6 @@ namespace {
 
 using namespace cwi;
 
-constexpr int kThreads = 256;
-
 struct TreeArgs {
     const float *q;
     size_t q_stride;
@@ -69,15 +67,16 @@ __device__ __forceinline__ uint64_t sees64(const TreeArgs &a, int row, int i, in
     return m & low(n - j);
 }
 
-// One (row, head) a workgroup: wave w takes positions w, w + 4, ..., a lane
-// HD / 64 elements of each (or one, of HD lanes); the waves' (max, sum, o) meet
-// in LDS.
-template <typename KVT, int HD>
-__global__ __launch_bounds__(kThreads) void tree_row_kernel(TreeArgs a) {
-    constexpr int E = HD > 64 ? HD / 64 : 1, W = kThreads / 64;
-    __shared__ float so[W][HD], sm[W], sl[W];
+// head_dim 16, which the products below have no form for: one (row, head) a
+// workgroup, 16 lanes a position, four positions at once; the groups' (max, sum, o)
+// meet in LDS.  Bound by the loads' latency and the caches, which have K and V for
+// every head of a row again.
+template <typename KVT, int THREADS>
+__global__ __launch_bounds__(THREADS) void tree_row_kernel(TreeArgs a) {
+    constexpr int HD = 16, G = THREADS / HD, U = 4;
+    __shared__ float so[G][HD], sm[G], sl[G];
     const int r = blockIdx.x, h = blockIdx.y, g = h / (a.n_heads / a.n_kv);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int e = threadIdx.x % HD, mine = threadIdx.x / HD;
     // the request whose rows hold r
     int lo = 0, hi = a.n_seq;
     while (hi - lo > 1) {
@@ -88,53 +87,55 @@ __global__ __launch_bounds__(kThreads) void tree_row_kernel(TreeArgs a) {
     const SeqRows s = seq_rows(a.first_row, a.cached, a.rows, lo);
     const int i = r - s.r0;
     if (i < 0 || i >= s.n) return;
-    const int e0 = lane * E;
-    const bool on = e0 < HD;
-    float q[E], o[E] = {};
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        q[e] = on ? a.q[(size_t)r * a.q_stride + (size_t)h * HD + e0 + e] : 0.0f;
-    float m = -INFINITY, l = 0.0f;
+    const float q = a.q[(size_t)r * a.q_stride + (size_t)h * HD + e];
+    float m = -INFINITY, l = 0.0f, o = 0.0f;
     bool lost = lost_length(a, s);  // or a position without a block
     const int end = lost ? 0 : s.cached + s.n;
     const KVT *kc = static_cast<const KVT *>(a.kc), *vc = static_cast<const KVT *>(a.vc);
-    for (int p = wave; p < end; p += W) {
-        const int slot = slot_of(a.map, lo, p);
-        lost |= slot < 0;
-        if (slot < 0 || (p >= s.cached && !sees(a, r, i, p - s.cached))) continue;
-        const size_t at = ((size_t)slot * a.n_kv + g) * HD + e0;
-        float d = 0.0f;
+    for (int p0 = mine; p0 < end; p0 += G * U) {
+        float k[U], v[U], d[U];
+        bool on[U];
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (on) d = __builtin_fmaf(q[e], (float)kc[at + e], d);
+        for (int u = 0; u < U; ++u) {
+            const int p = p0 + u * G, slot = p < end ? slot_of(a.map, lo, p) : 0;
+            lost |= slot < 0;
+            on[u] = p < end && slot >= 0 && (p < s.cached || sees(a, r, i, p - s.cached));
+            const size_t at = ((size_t)max(slot, 0) * a.n_kv + g) * HD + e;
+            k[u] = on[u] ? (float)kc[at] : 0.0f;
+            v[u] = on[u] ? (float)vc[at] : 0.0f;
+        }
 #pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) d += __shfl_xor(d, off);
-        d *= a.scale;
-        const float mn = fmaxf(m, d), ref = mn == -INFINITY ? 0.0f : mn;
-        const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(d - ref);
-        m = mn;
-        l = __builtin_fmaf(l, f, w);
+        for (int u = 0; u < U; ++u) {
+            d[u] = q * k[u];
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (on) o[e] = __builtin_fmaf(o[e], f, w * (float)vc[at + e]);
+            for (int off = HD / 2; off >= 1; off >>= 1) d[u] += __shfl_xor(d[u], off);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (!on[u]) continue;
+            const float x = d[u] * a.scale;
+            const float mn = fmaxf(m, x), ref = mn == -INFINITY ? 0.0f : mn;
+            const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(x - ref);
+            m = mn;
+            l = __builtin_fmaf(l, f, w);
+            o = __builtin_fmaf(o, f, w * v[u]);
+        }
     }
-    if (on)
-#pragma unroll
-        for (int e = 0; e < E; ++e) so[wave][e0 + e] = o[e];
-    if (lane == 0) sm[wave] = m, sl[wave] = lost ? NAN : l;
+    so[mine][e] = o;
+    if (e == 0) sm[mine] = m, sl[mine] = lost ? NAN : l;
     __syncthreads();
-    float M = -INFINITY, L = 0.0f;
+    if (mine > 0) return;
+    float M = -INFINITY, L = 0.0f, y = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w]);
+    for (int w = 0; w < G; ++w) M = fmaxf(M, sm[w]);
     const float ref = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-    for (int w = 0; w < W; ++w) L += sl[w] * __builtin_amdgcn_exp2f(sm[w] - ref);
-    for (int e = threadIdx.x; e < HD; e += kThreads) {
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) v += so[w][e] * __builtin_amdgcn_exp2f(sm[w] - ref);
-        a.out[(size_t)r * a.out_stride + (size_t)h * HD + e] = L == 0.0f ? 0.0f : v / L;
+    for (int w = 0; w < G; ++w) {
+        const float f = __builtin_amdgcn_exp2f(sm[w] - ref);
+        L += sl[w] * f;
+        y += so[w][e] * f;
     }
+    a.out[(size_t)r * a.out_stride + (size_t)h * HD + e] = L == 0.0f ? 0.0f : y / L;
 }
 
 // ---------------------------------------------------------------- tiles on the matrix cores
@@ -466,20 +467,21 @@ __device__ __forceinline__ Dest dest(const TreeArgs &a, const Seg &g, int group,
 // row, a lane HD / 64 elements.  (up: the tiles' weights carry 2^up.)
 template <typename KVT, int HD, int RT>
 __device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, float up) {
-    constexpr int E = HD / 64;
+    constexpr int E = HD < 64 ? 1 : HD / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool on = lane * E < HD;  // (all, from head_dim 64 on)
     const KVT *kc = static_cast<const KVT *>(a.kc), *vc = static_cast<const KVT *>(a.vc);
     for (int row = wave; row < RT && g.rb * RT + row < g.nrows; row += blockDim.x >> 6) {
         const int rr = g.rb * RT + row, node = rr / group;
         const size_t head = (size_t)(g.h * group + rr - node * group) * HD + lane * E;
         float q[E], o[E] = {}, m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) q[e] = a.q[(size_t)(g.s.r0 + node) * a.q_stride + head + e];
+        for (int e = 0; e < E; ++e) q[e] = on ? a.q[(size_t)(g.s.r0 + node) * a.q_stride + head + e] : 0.0f;
         for (int p = g.t0 * kt; p < min(g.t1 * kt, g.last + 1); ++p) {
             const int slot = slot_of(a.map, g.b, p);
             const int j = p - g.s.cached;
             if (slot < 0 || (j >= 0 && !sees(a, g.s.r0 + node, node, j))) continue;
-            const size_t at = ((size_t)slot * a.n_kv + g.h) * HD + lane * E;
+            const size_t at = ((size_t)slot * a.n_kv + g.h) * HD + (on ? lane * E : 0);
             float d = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; ++e) d = __builtin_fmaf(q[e], (float)kc[at + e], d);
@@ -495,7 +497,7 @@ __device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, f
         }
         const size_t part = (size_t)g.part * RT + row;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
+        for (int e = 0; e < E && on; ++e) {
             if (g.whole)
                 a.out[(size_t)(g.s.r0 + node) * a.out_stride + head + e] = l == 0.0f ? 0.0f : o[e] / l;
             else
@@ -1127,15 +1129,16 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
 // running maximum).  Every wave of a workgroup has 16 rows and a share of each
 // tile; with eight waves the same conversions serve twice the rows (one workgroup
 // a CU, tiles of 64 positions): 256 rows of each of 8 requests at 4,000 positions
-// 154 us instead of 215, 64 rows 62 either way.  A position is so kept to 22 bits down to 2^-17 of its
-// neighbours' largest, and to 2^-40 of that below: of the same order as the
-// weights.  Nodes that a row does not see must not cost its others their bits,
-// so where a node is further from its neighbours the segment is taken one by one.
+// 154 us instead of 215, 64 rows 62 either way.  A position is so kept to 22 bits
+// down to 2^-17 of its neighbours' largest, and to 2^-40 of that below: of the same
+// order as the weights.  Nodes that a row does not see must not cost its others
+// their bits, so where a node is further from its neighbours the segment is taken
+// one by one.
 template <int HD_, int NW_>
 struct WideCfg : Tile<_Float16, HD_> {
     typedef Tile<_Float16, HD_> T;
     static constexpr int NW = NW_;
-    static constexpr int KT = NW == 4 ? (HD_ == 64 ? 64 : 32) : (HD_ == 256 ? 32 : 64), RT = 16 * NW, ST = KT / 16;
+    static constexpr int KT = NW == 4 ? (HD_ <= 64 ? 64 : 32) : (HD_ == 256 ? 32 : 64), RT = 16 * NW, ST = KT / 16;
     static constexpr int PW = KT / NW;               // positions of a wave
     static constexpr int LPR = HD_ / 4;              // lanes of a row
     static constexpr int NL = PW * LPR / 64;         // loads of its K
@@ -1474,6 +1477,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
     const long long u0 = base + h * wk.begin(wk.blocks) + wk.first_tile(rb);
     const int first = uniform(deal.owner(u0)), last = uniform(deal.owner(u0 + (long long)(wk.tiles(rb) - 1) * kt));
     if (first == last) return;  // one workgroup had them all, and wrote the output
+    if (!SPLIT && n * 16 >= HD) return;
     const int lr = min(li, mine.n * group - 1 - tile * 16);  // (rows behind the last: not loaded)
     const int each = SPLIT ? (last - first + 4) / 4 : last - first + 1;
     const int w0 = SPLIT ? first + wave * each : first, w1 = min(w0 + each, last + 1);
@@ -1640,11 +1644,11 @@ int launch_tiles(cw_ctx *ctx, TreeArgs a, void (*fn)(TreeArgs)) {
     } else {
         // tiles of 16 rows that the requests have at most
         const unsigned tiles = (unsigned)((long long)a.rows * (a.n_heads / a.n_kv) / 16) + a.n_seq;
-        if ((long long)tiles * a.n_kv * (C::HD / 64) <= ctx->n_cu)
+        if ((long long)tiles * a.n_kv * ((C::HD + 63) / 64) <= ctx->n_cu)
             return launch(ctx, "attention_tree_merge", tree_merge_kernel<C, true>,
                           dim3(tiles, a.n_kv, C::HD / 16), dim3(256), 0, a);
         return launch(ctx, "attention_tree_merge", tree_merge_kernel<C, false>,
-                      dim3(tiles, a.n_kv, C::HD / 64), dim3(256), 0, a);
+                      dim3(tiles, a.n_kv, (C::HD + 63) / 64), dim3(256), 0, a);
     }
 }
 template <typename KVT, int HD>
@@ -1675,7 +1679,7 @@ int launch_wide(cw_ctx *ctx, const TreeArgs &a) {
 template <typename KVT, int HD>
 int launch_by_rows(cw_ctx *ctx, const TreeArgs &a) {
     const long long rows = ((long long)a.rows + a.n_seq - 1) / a.n_seq * (a.n_heads / a.n_kv);
-    if constexpr (HD <= 128)
+    if constexpr (HD <= 128 && (HD > 32 || sizeof(KVT) == 2))  // (its V reads of f32 are 64 elements wide)
         if (rows <= (sizeof(KVT) == 2 ? 8 : 16)) return launch_split<KVT, HD>(ctx, a);
     if constexpr (sizeof(KVT) == 4) {
         if constexpr (HD != 128)
@@ -1690,11 +1694,16 @@ int launch_by_rows(cw_ctx *ctx, const TreeArgs &a) {
 
 template <typename KVT>
 int launch_by_size(cw_ctx *ctx, const TreeArgs &a, int hd) {
+    if (hd == 32) return launch_by_rows<KVT, 32>(ctx, a);
     if (hd == 64) return launch_by_rows<KVT, 64>(ctx, a);
     if (hd == 128) return launch_by_rows<KVT, 128>(ctx, a);
     if (hd == 256) return launch_by_rows<KVT, 256>(ctx, a);
-    auto fn = hd == 16 ? tree_row_kernel<KVT, 16> : tree_row_kernel<KVT, 32>;
-    return launch(ctx, "attention_tree", fn, dim3(a.rows, a.n_heads), dim3(kThreads), 0, a);
+    // 1,024 threads for what would leave a CU two workgroups (4,000 positions: 8 and
+    // 512 (row, head)s 34 and 89 us, with 256 threads 124 and 212), else 256 (4,096
+    // of them over f32: 362 us, 610 with 1,024)
+    const bool few = (long long)a.rows * a.n_heads <= 2 * ctx->n_cu;
+    return few ? launch(ctx, "attention_tree", tree_row_kernel<KVT, 1024>, dim3(a.rows, a.n_heads), dim3(1024), 0, a)
+               : launch(ctx, "attention_tree", tree_row_kernel<KVT, 256>, dim3(a.rows, a.n_heads), dim3(256), 0, a);
 }
 
 }  // namespace
