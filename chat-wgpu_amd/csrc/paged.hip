@@ -21,25 +21,31 @@ constexpr int kThreads = 256;
 // the product's distance to the next whole quarter turn is exact to 2^-53 of
 // the turns (4e-8 of a turn at 2^31 turns, 4e-14 at a million positions), so
 // far positions cost no accuracy; in f32 a position of a million would leave
-// 0.06 of a radian.  The rest, at most pi / 4, is rounded to f32 once.
+// 0.06 of a radian.  The rest, at most pi / 4, is x + lo in f32.
 
 // cos and sin of 2 pi t by their Taylor series at the nearest quarter turn
-// (|x| <= pi / 4: the first term left out is 2e-9)
-__device__ __forceinline__ float2 turn(double t, float gain) {
+// (|x| <= pi / 4: the first term left out is 2e-9), lo by the first two terms of
+// the angles' sum: half a step and a little in all, as a rounding of the exact ones;
+// times a gain of 48 bits
+__device__ __forceinline__ float2 turn(double t, float gain, float gain_lo) {
     t -= rint(t);
     const double q = rint(4.0 * t);
-    const float x = (float)((t - 0.25 * q) * 6.283185307179586);
+    const double rest = (t - 0.25 * q) * 6.283185307179586;
+    const float x = (float)rest, lo = (float)(rest - x);
     const float z = x * x;
-    const float s = x * (1.0f + z * (-1.0f / 6 + z * (1.0f / 120 + z * (-1.0f / 5040 + z * (1.0f / 362880)))));
-    const float c = 1.0f + z * (-0.5f + z * (1.0f / 24 + z * (-1.0f / 720 + z * (1.0f / 40320 - z * (1.0f / 3628800)))));
+    const float s = x + (x * z * (-1.0f / 6 + z * (1.0f / 120 + z * (-1.0f / 5040 + z * (1.0f / 362880)))) +
+                         (lo - 0.5f * z * lo));
+    const float c = 1.0f + (z * (-0.5f + z * (1.0f / 24 + z * (-1.0f / 720 + z * (1.0f / 40320 - z * (1.0f / 3628800))))) -
+                            x * lo);
     const int k = (int)q & 3;
     const float cc = k & 1 ? s : c, ss = k & 1 ? c : s;
-    return make_float2((k == 1 || k == 2 ? -cc : cc) * gain, (k >= 2 ? -ss : ss) * gain);
+    const float gc = __builtin_fmaf(cc, gain, cc * gain_lo), gs = __builtin_fmaf(ss, gain, ss * gain_lo);
+    return make_float2(k == 1 || k == 2 ? -gc : gc, k >= 2 ? -gs : gs);
 }
 
 struct RopeArgs {
     const double *turns;  // [rot / 2]
-    float gain;
+    float gain, gain_lo;
     int rot, pairs;       // rotated elements of a head; CW_ROPE_PAIRS
     const float *x;
     size_t x_stride;
@@ -95,7 +101,7 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a, int U, 
     float2 cs[V];
     if (rotates) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) cs[j] = turn((double)pos * a.turns[V * u + j], a.gain);
+        for (int j = 0; j < V; ++j) cs[j] = turn((double)pos * a.turns[V * u + j], a.gain, a.gain_lo);
     }
     const int slot = CACHE ? a.slots[r] : -1;
     const bool write = CACHE && (unsigned)slot < (unsigned)a.n_slots;
@@ -485,9 +491,10 @@ int ctx_rope_turns(cw_ctx *ctx, const char *what, cw_rope_spec s, const double *
     return CW_OK;
 }
 
-float spec_gain(const cw_rope_spec &s) {
-    if (s.scaling != CW_ROPE_YARN) return 1.0f;
-    return (float)(s.gain > 0.0 ? s.gain : 0.1 * std::log(s.factor) + 1.0);
+void spec_gain(const cw_rope_spec &s, RopeArgs *a) {
+    const double g = s.scaling != CW_ROPE_YARN ? 1.0 : s.gain > 0.0 ? s.gain : 0.1 * std::log(s.factor) + 1.0;
+    a->gain = (float)g;
+    a->gain_lo = (float)(g - a->gain);
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -572,7 +579,7 @@ int cw_rope_rows(cw_ctx *ctx, const cw_rope_spec *spec, const float *x, size_t x
     CW_HIP(hipSetDevice(ctx->device));
     RopeArgs a{};
     CW_TRY(ctx_rope_turns(ctx, "cw_rope_rows", *spec, &a.turns));
-    a.gain = spec_gain(*spec);
+    spec_gain(*spec, &a);
     a.rot = spec->rot_dim;
     a.pairs = spec->layout == CW_ROPE_PAIRS;
     a.x = x;
@@ -618,7 +625,7 @@ int cw_rope_kv_rows(cw_ctx *ctx, const cw_rope_spec *spec, const cw_kv_pages *kv
     CW_HIP(hipSetDevice(ctx->device));
     RopeArgs a{};
     CW_TRY(ctx_rope_turns(ctx, "cw_rope_kv_rows", *spec, &a.turns));
-    a.gain = spec_gain(*spec);
+    spec_gain(*spec, &a);
     a.rot = spec->rot_dim;
     a.pairs = spec->layout == CW_ROPE_PAIRS;
     a.x = qkv;
