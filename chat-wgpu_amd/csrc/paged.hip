@@ -86,7 +86,8 @@ __device__ __forceinline__ void put_unit(float *to, const float *from) {
 // elements from either half, or 2 V in a row) or V copied elements; U units make
 // a head, `par` heads a round, and a thread keeps its unit's cosines for every
 // head it takes.  V = 4 where rows are 16-byte aligned, 1 where not.  STREAM: y
-// is written past the caches.
+// is written past the caches.  Bound by memory: 6,000 rows of 40 heads 43 us,
+// 5.6 TB/s read and written; few rows by the launch, 4 us.
 template <typename KVT, int V, bool PAIRS, bool CACHE, bool STREAM = false>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a, int U, int par) {
     const int r = blockIdx.x, pos = a.positions[r];
@@ -230,7 +231,7 @@ __device__ void fill_tables(const TableArgs &a, const int *first, const int *nee
 // the threads gives each its offsets, and a second walk writes them; then the
 // returned blocks.  FILL: the rows and tables too, offsets in LDS (few of
 // either; at most kLdsSeqs requests).  Bound by its chain of loads: lengths,
-// then table and free list.
+// then table and free list: 48 requests of a row each 5.0 us.
 template <bool FILL>
 __global__ __launch_bounds__(kScan) void block_scan_kernel(TableArgs a) {
     __shared__ long long part[3][kScan / 64];
@@ -327,7 +328,8 @@ __global__ __launch_bounds__(kScan) void block_scan_kernel(TableArgs a) {
     if (FILL) fill_tables(a, first, need_at, tid, kScan, live, top);
 }
 
-// Rows and table entries, over the chip, behind block_scan_kernel<false>.
+// Rows and table entries, over the chip, behind block_scan_kernel<false> (600
+// requests of up to 400 rows: 5 us each).
 __global__ __launch_bounds__(kThreads) void block_fill_kernel(TableArgs a) {
     __shared__ int s_first[kLdsSeqs + 1], s_need[kLdsSeqs + 1];
     const int n = a.n_seq, live = a.status[0] == 0;
@@ -351,7 +353,8 @@ __global__ __launch_bounds__(kThreads) void block_fill_kernel(TableArgs a) {
 // and no row is read after an earlier move wrote it: a thread that moves its 16
 // bytes of a row in order of i needs no copy of the rows, and has the loads of
 // eight moves in flight (a load's row is never among the rows stored before it).
-// Lane i of each wave looks up move i.
+// Lane i of each wave looks up move i.  A launch and three dependent loads: 3.4 us
+// for 48 requests of six moves.
 __global__ __launch_bounds__(kThreads) void accept_kernel(PageMap m, u32x4 *k, u32x4 *v,
                                                           int row_u4, const int *cached,
                                                           const int *path, int max_path,

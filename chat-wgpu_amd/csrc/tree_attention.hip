@@ -700,7 +700,8 @@ __device__ __forceinline__ int o_col(int n, int lg) {
 
 // ---- few rows of a kv head (at most 16): a workgroup's four waves share them
 // and take 16 of a tile's 64 positions each, through LDS of their own, so
-// nothing waits for another wave before the end of a segment.
+// nothing waits for another wave before the end of a segment.  Bound by memory: 48
+// single rows at 100 .. 8,000 positions (366 MB) 64.5 us, 5.7 TB/s.
 template <typename KVT, int HD>
 struct SplitCfg : Tile<KVT, HD> {
     typedef Tile<KVT, HD> T;
@@ -898,7 +899,10 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
 }
 
 // ---- more rows over an f16 cache: the four waves take 16 QT rows each, and share
-// the tile's positions in LDS.  (Tiles of 32 positions, two workgroups a CU with
+// the tile's positions in LDS.  Of many rows the products bound it: 128 nodes of
+// each of 8 requests at 4,000 positions, 32 heads, 147 us, 910 TFLOP/s of them; of
+// few the chain of lengths, block ids, first tile and four tiles a workgroup: 61
+// nodes at 4,100 positions 22 us.  (Tiles of 32 positions, two workgroups a CU with
 // three tiles on their way each: 25.7 us for 61 nodes at 4,100 positions, against
 // 21.6; one workgroup of eight waves, with tiles of 64 positions: 44 us for twelve
 // requests of 4 to 16 nodes, against 36.)
