@@ -464,7 +464,8 @@ __device__ __forceinline__ Dest dest(const TreeArgs &a, const Seg &g, int group,
 
 // A segment whose nodes have a V that is no finite number: as 0 * V it would
 // reach rows that do not see it, so the products are taken one by one, a wave a
-// row, a lane HD / 64 elements.  (up: the tiles' weights carry 2^up.)
+// row, a lane HD / 64 elements.  Every block of the segment is in the cache.  (up:
+// the tiles' weights carry 2^up.)
 template <typename KVT, int HD, int RT>
 __device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, float up) {
     constexpr int E = HD < 64 ? 1 : HD / 64;
@@ -480,8 +481,8 @@ __device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, f
         for (int p = g.t0 * kt; p < min(g.t1 * kt, g.last + 1); ++p) {
             const int slot = slot_of(a.map, g.b, p);
             const int j = p - g.s.cached;
-            if (slot < 0 || (j >= 0 && !sees(a, g.s.r0 + node, node, j))) continue;
-            const size_t at = ((size_t)slot * a.n_kv + g.h) * HD + (on ? lane * E : 0);
+            if (j >= 0 && !sees(a, g.s.r0 + node, node, j)) continue;
+            const size_t at = ((size_t)max(slot, 0) * a.n_kv + g.h) * HD + (on ? lane * E : 0);
             float d = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; ++e) d = __builtin_fmaf(q[e], (float)kc[at + e], d);
@@ -860,9 +861,11 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
             w_ml[wave][li][0] = m;
             w_ml[wave][li][1] = bad ? NAN : l;
         }
-        if (lane == 0) w_odd[wave] = odd;
+        if (lane == 0) w_odd[wave] = (int)odd | (int)bad << 1;
         lds_barrier();  // and every wave is done with its stages
-        if (uniform(w_odd[0] | w_odd[1] | w_odd[2] | w_odd[3])) {
+        // (a request that has lost a block gets NaN below: its tiles may hold
+        // anything, and nothing of them is an answer)
+        if (uniform(w_odd[0] | w_odd[1] | w_odd[2] | w_odd[3]) == 1) {
             one_by_one<KVT, HD, RT>(a, g, group, KT, T::UP);
             continue;
         }
@@ -1104,11 +1107,11 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
         }
         // the last tile's odd_seg, or (no tile) bad_seg, known to all
         if (g.t0 == t1 || t1 * KT > g.s.cached) lds_barrier();
-        if (uniform(odd_seg) == seg) {
+        const bool bad = g.lost || uniform(bad_seg) == seg || rest_lost<KT>(a, g, lane);
+        if (!bad && uniform(odd_seg) == seg) {
             one_by_one<_Float16, HD, RT>(a, g, group, KT, T::UP);
             continue;
         }
-        const bool bad = g.lost || bad_seg == seg || rest_lost<KT>(a, g, lane);
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
             l[i] = group_sum(l[i]);
@@ -1412,11 +1415,11 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
             if (!EARLY || wave < 4) next();
         }
         lds_barrier();  // bad_seg and odd_seg are known to all
-        if (uniform(odd_seg) == seg) {
+        const bool bad = g.lost || uniform(bad_seg) == seg || rest_lost<KT>(a, g, lane);
+        if (!bad && uniform(odd_seg) == seg) {
             one_by_one<float, HD, RT>(a, g, group, KT, T::UP);
             continue;
         }
-        const bool bad = g.lost || bad_seg == seg || rest_lost<KT>(a, g, lane);
         const float unit = ldexpf(1.0f, max(E, -200) - 15);
         l = group_sum(l);
         int at = lane;

@@ -1,0 +1,63 @@
+"""Values, masks and lengths at the edges of what the paged operators accept,
+on the MI355X: each against its definition in 64 bits, with the bounds of
+test_gpu_paged."""
+import numpy as np
+import pytest
+
+import paged_oracle as po
+from test_gpu_paged import Batch
+
+pytestmark = pytest.mark.gpu
+
+# kv, heads, kv heads, hd, new rows of the first of two requests (the second
+# has two): few and many rows of a kv head, every head size
+KERNELS = [
+    ("f16", 2, 1, 64, 3), ("f16", 2, 1, 128, 3), ("f16", 8, 1, 128, 12), ("f16", 8, 1, 128, 90),
+    ("f16", 2, 1, 256, 3), ("f16", 8, 1, 256, 90), ("f16", 2, 1, 32, 3), ("f16", 8, 1, 32, 90),
+    ("f32", 2, 1, 64, 3), ("f32", 2, 1, 128, 3), ("f32", 8, 1, 64, 12), ("f32", 8, 1, 64, 90),
+    ("f32", 8, 1, 128, 12), ("f32", 8, 1, 128, 90), ("f32", 2, 1, 32, 3), ("f32", 8, 1, 32, 90),
+    ("f32", 2, 1, 256, 3), ("f32", 8, 1, 256, 90), ("f16", 2, 1, 16, 3), ("f16", 8, 1, 16, 90),
+    ("f32", 2, 1, 16, 3), ("f32", 8, 1, 16, 90),
+]
+
+
+def free_block_0(b):
+    """Block 0 is nobody's and holds NaN: its owner takes an unused one."""
+    spare = int(np.setdiff1d(np.arange(b.blocks), b.tables)[-1])
+    if spare == 0:
+        return
+    b.tables[b.tables == 0] = spare
+    for a in (b.k, b.v):
+        a[spare * b.page:(spare + 1) * b.page] = a[:b.page]
+        a[:b.page] = np.nan
+
+
+# ------------------------------------------------------- blocks that are missing
+
+# (behind_inf: few rows are one row block, behind whose last tile nothing lies)
+@pytest.mark.parametrize("case,what", [
+    (c, w) for c in KERNELS for w in ("node", "cached", "cached_inf", "cached_far", "tile_inf",
+                                      "behind_inf")[:None if c[4] == 90 else -1]])
+def test_a_lost_block_is_nan_whatever_the_values(ctx, rng, case, what):
+    """NaN for every row of a request with a block that is not there: also
+    where block 0 holds NaN, a node's V is infinite (far from the block, in
+    its tile, or before it), or a node is far from its neighbours."""
+    kv, heads, kvh, hd, new = case
+    cached = 100 if what == "tile_inf" else 70
+    b = Batch(ctx, rng, [cached, 40], [new, 2], heads, kvh, hd, kv, 16)
+    free_block_0(b)
+    if what == "tile_inf":
+        b.k[:16] = b.v[:16] = 1
+    good = b.run()
+    b.check(good)
+    node = po.slot_of(b.tables, 16, 0, cached + 1)
+    if what.endswith("inf"):
+        b.v[node] = np.inf
+    if what.endswith("far"):
+        b.k[node], b.v[node] = b.k[node] * b.k.dtype.type(1e-4), 0
+        b.v[node, 0, 3] = 1e-7
+    entry = {"n": 4, "c": 1, "b": 9, "t": 4}[what[0]]  # positions 64 .., 16 .., 144 ..
+    b.tables[0, entry] = -1 if hd != 64 else b.blocks
+    got = b.run()
+    assert np.all(np.isnan(got[:new])), np.argwhere(~np.isnan(got[:new]))[:3]
+    assert np.array_equal(got[new:], good[new:])
