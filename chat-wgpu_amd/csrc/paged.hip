@@ -214,10 +214,13 @@ __device__ void fill_tables(const TableArgs &a, const int *first, const int *nee
             if ((unsigned)id < (unsigned)a.n_blocks)
                 slot = (id << a.shift) + ((c + i) & (a.page - 1));
             int depth = i;
-            if (a.mask) {
+            if (a.mask) {  // the bits of the request's own nodes
+                const int nodes = first[b + 1] - first[b];
                 depth = -1;
-                for (int w = 0; w < a.mask_words; ++w)
-                    depth += __popc(a.mask[(size_t)r * a.mask_words + w]);
+                for (int w = 0; w < a.mask_words && 32 * w < nodes; ++w) {
+                    const uint32_t own = nodes - 32 * w >= 32 ? ~0u : (1u << (nodes - 32 * w)) - 1;
+                    depth += __popc(a.mask[(size_t)r * a.mask_words + w] & own);
+                }
                 depth = max(depth, 0);
             }
             pos = c + depth;

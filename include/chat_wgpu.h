@@ -237,8 +237,9 @@ typedef struct cw_batch {
     int *tables;           /* [n_seq][max_blocks]: block of positions j*page .. or NULL */
     int max_blocks;
     const uint32_t *mask;  /* [rows][mask_words]: bit j of a row: it sees its request's node j.
-                              Nodes behind the last bit are not seen.  NULL: every node sees
-                              itself and the nodes before it */
+                              Nodes behind the last bit are not seen, bits behind the last node
+                              count for nothing.  NULL: every node sees itself and the nodes
+                              before it */
     int mask_words;
 } cw_batch;
 

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import paged_oracle as po
-from test_gpu_paged import Batch
+from test_gpu_paged import Batch, i32, run_tables, same_step, tables_state
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,43 @@ def test_a_lost_block_is_nan_whatever_the_values(ctx, rng, case, what):
     got = b.run()
     assert np.all(np.isnan(got[:new])), np.argwhere(~np.isnan(got[:new]))[:3]
     assert np.array_equal(got[new:], good[new:])
+
+
+# ------------------------------------------------------------------------ masks
+
+@pytest.mark.parametrize("rows_cap", [0, 4000])  # one launch, and two
+def test_block_tables_masks_of_more_bits_than_nodes(ctx, rng, rows_cap):
+    """A row's position counts the nodes it sees of its request; bits behind
+    the request's last node are no nodes."""
+    fresh = np.array([5, 33, 1, 64, 0, -1, 31, 32, 70, 2])
+    cached = rng.integers(0, 90, len(fresh))
+    words = 3
+    mask = np.concatenate([po.tree(rng, max(0, int(f)), words) for f in fresh])
+    mask[4] = 0  # a row that sees nothing keeps the first new position
+    wide, r = mask.copy(), 0
+    for f in np.maximum(fresh, 0):
+        for w in range(words):
+            wide[r:r + f, w] |= np.uint32(0xffffffff << min(max(f - 32 * w, 0), 32) & 0xffffffff)
+        r += f
+    rows = max(r, rows_cap)
+    mask, wide = (np.pad(m, ((0, rows - r), (0, 0))) for m in (mask, wide))
+    width = int((-(-(cached + np.maximum(fresh, 0)) // 16)).max()) + 1
+    tables, held, free, n_free, blocks = tables_state(rng, cached, fresh, 16, width, 3)
+    args = (i32(cached), i32(fresh), held, tables, free, n_free, 16, blocks, rows)
+    want = po.block_tables(*args, mask)
+    assert want[0] == 0
+    same_step(run_tables(ctx, *args, wide), want)
+
+
+@pytest.mark.parametrize("case", KERNELS)
+def test_attention_masks_of_more_bits_than_nodes(ctx, rng, case):
+    """Bits behind a request's last node show nothing."""
+    kv, heads, kvh, hd, new = case
+    b = Batch(ctx, rng, [70, 40], [new, 2], heads, kvh, hd, kv, 16, tree=True)
+    first = b.run()
+    b.check(first)
+    for r in range(new + 2):
+        n = new if r < new else 2
+        for w in range(b.mask.shape[1]):
+            b.mask[r, w] |= np.uint32(0xffffffff << min(max(n - 32 * w, 0), 32) & 0xffffffff)
+    assert np.array_equal(b.run(), first)
