@@ -67,6 +67,15 @@ __device__ __forceinline__ uint64_t sees64(const TreeArgs &a, int row, int i, in
     return m & low(n - j);
 }
 
+// Over f32 the weights carry 2^-bits, the bits of the request's length: the sum of
+// all its weights times V is then no larger than the largest V, so any V that f32
+// holds has its mean.  (Sums of f16 V cannot get past f32.)  The factor is the same
+// for every segment of a request and cancels in o / sum.
+template <typename KVT>
+__device__ __forceinline__ float unit_of(const SeqRows &s) {
+    return sizeof(KVT) == 4 ? ldexpf(1.0f, __builtin_clz((unsigned)(s.cached + s.n)) - 32) : 1.0f;
+}
+
 // head_dim 16, which the products below have no form for: one (row, head) a
 // workgroup, 16 lanes a position, four positions at once; the groups' (max, sum, o)
 // meet in LDS.  Bound by the loads' latency and the caches, which have K and V for
@@ -87,7 +96,7 @@ __global__ __launch_bounds__(THREADS) void tree_row_kernel(TreeArgs a) {
     const SeqRows s = seq_rows(a.first_row, a.cached, a.rows, lo);
     const int i = r - s.r0;
     if (i < 0 || i >= s.n) return;
-    const float q = a.q[(size_t)r * a.q_stride + (size_t)h * HD + e];
+    const float q = a.q[(size_t)r * a.q_stride + (size_t)h * HD + e], unit = unit_of<KVT>(s);
     float m = -INFINITY, l = 0.0f, o = 0.0f;
     bool lost = lost_length(a, s);  // or a position without a block
     const int end = lost ? 0 : s.cached + s.n;
@@ -115,7 +124,7 @@ __global__ __launch_bounds__(THREADS) void tree_row_kernel(TreeArgs a) {
             if (!on[u]) continue;
             const float x = d[u] * a.scale;
             const float mn = fmaxf(m, x), ref = mn == -INFINITY ? 0.0f : mn;
-            const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(x - ref);
+            const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(x - ref) * unit;
             m = mn;
             l = __builtin_fmaf(l, f, w);
             o = __builtin_fmaf(o, f, w * v[u]);
@@ -464,10 +473,10 @@ __device__ __forceinline__ Dest dest(const TreeArgs &a, const Seg &g, int group,
 
 // A segment whose nodes have a V that is no finite number: as 0 * V it would
 // reach rows that do not see it, so the products are taken one by one, a wave a
-// row, a lane HD / 64 elements.  Every block of the segment is in the cache.  (up:
-// the tiles' weights carry 2^up.)
+// row, a lane HD / 64 elements.  Every block of the segment is in the cache.  (The
+// weights carry 2^up, where the tiles' do, and `unit`.)
 template <typename KVT, int HD, int RT>
-__device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, float up) {
+__device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, float up, float unit) {
     constexpr int E = HD < 64 ? 1 : HD / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool on = lane * E < HD;  // (all, from head_dim 64 on)
@@ -490,7 +499,7 @@ __device__ void one_by_one(const TreeArgs &a, const Seg &g, int group, int kt, f
             for (int off = 32; off >= 1; off >>= 1) d += __shfl_xor(d, off);
             d *= a.scale;
             const float mn = fmaxf(m, d), ref = mn == -INFINITY ? 0.0f : mn;
-            const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(d - ref + up);
+            const float f = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(d - ref + up) * unit;
             m = mn;
             l = __builtin_fmaf(l, f, w);
 #pragma unroll
@@ -660,10 +669,10 @@ __device__ __forceinline__ f32x4 scores(const typename T::frag (&kf)[T::KS], con
 }
 
 // Running softmax of one row (this lane's: li) over N tiles of 16 scores, each
-// with a (positive) factor, which become the weights; returns the factor of
-// what was summed before.
+// with a (positive) factor, which become the weights (times 2^up and `unit`);
+// returns the factor of what was summed before.
 template <int N>
-__device__ __forceinline__ float soften(f32x4 (&s)[N], const float (&f)[N], float up, float &m, float &l) {
+__device__ __forceinline__ float soften(f32x4 (&s)[N], const float (&f)[N], float up, float unit, float &m, float &l) {
     float mx = -INFINITY;
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -678,7 +687,7 @@ __device__ __forceinline__ float soften(f32x4 (&s)[N], const float (&f)[N], floa
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], f[n], up - ref));
+            s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], f[n], up - ref)) * unit;
             ls += s[n][r];
         }
     l = l * alpha + ls;
@@ -760,6 +769,7 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
             load(g.t0);
         }
         q.convert(a.scale);
+        const float unit = unit_of<KVT>(g.s);
         f32x4 o[DT];
         float m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -829,7 +839,7 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
                 odd |= __any(x);
             }
             const float before = m, f[1] = {q.qs[0]};
-            const float alpha = soften<1>(s, f, T::UP, m, l);
+            const float alpha = soften<1>(s, f, T::UP, unit, m, l);
             if (__any(m > before)) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
@@ -866,7 +876,7 @@ __global__ __launch_bounds__(256, (SplitCfg<KVT, HD>::PER_CU)) void tree_split_k
         // (a request that has lost a block gets NaN below: its tiles may hold
         // anything, and nothing of them is an answer)
         if (uniform(w_odd[0] | w_odd[1] | w_odd[2] | w_odd[3]) == 1) {
-            one_by_one<KVT, HD, RT>(a, g, group, KT, T::UP);
+            one_by_one<KVT, HD, RT>(a, g, group, KT, T::UP, unit);
             continue;
         }
         constexpr int OS = HD / 4 < 16 ? HD / 4 - 1 : 15;
@@ -1056,7 +1066,7 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
                 float f[ST];
 #pragma unroll
                 for (int n = 0; n < ST; ++n) f[n] = q.qs[i];
-                const float alpha = soften<ST>(s[i], f, T::UP, m[i], l[i]);
+                const float alpha = soften<ST>(s[i], f, T::UP, 1.0f, m[i], l[i]);
                 if (__any(m[i] > before)) {
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
@@ -1109,7 +1119,7 @@ __global__ __launch_bounds__(256, (TileCfg<HD, QT>::PER_CU)) void tree_tile_kern
         if (g.t0 == t1 || t1 * KT > g.s.cached) lds_barrier();
         const bool bad = g.lost || uniform(bad_seg) == seg || rest_lost<KT>(a, g, lane);
         if (!bad && uniform(odd_seg) == seg) {
-            one_by_one<_Float16, HD, RT>(a, g, group, KT, T::UP);
+            one_by_one<_Float16, HD, RT>(a, g, group, KT, T::UP, 1.0f);
             continue;
         }
 #pragma unroll
@@ -1282,7 +1292,7 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
         }
         f32x4 o[DT];
         float m = -INFINITY, l = 0.0f;
-        int E = kNone;  // o counts 2^(E - 15)
+        int E = kNone;  // V counts 2^(E - 15) in o
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int t = g.t0; t < t1; ++t) {
@@ -1365,7 +1375,7 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
 #pragma unroll
                 for (int n = 0; n < ST; ++n) f[n] = fmaxf(q.qs[0] * kf[n], 1e-37f);  // (-inf keeps its sign)
                 const float before = m;
-                const float alpha = soften<ST>(s, f, T::UP, m, l) * down;
+                const float alpha = soften<ST>(s, f, T::UP, 1.0f, m, l) * down;
                 if (grown || __any(m > before)) {
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
@@ -1416,12 +1426,13 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
         }
         lds_barrier();  // bad_seg and odd_seg are known to all
         const bool bad = g.lost || uniform(bad_seg) == seg || rest_lost<KT>(a, g, lane);
+        // o counts 2^(E - 30), the weights 2^-15, until here: no sum of them gets far
+        const float unit = unit_of<float>(g.s), per_l = ldexpf(unit, -15), per_o = ldexpf(1.0f, max(E, -200) - 30);
         if (!bad && uniform(odd_seg) == seg) {
-            one_by_one<float, HD, RT>(a, g, group, KT, T::UP);
+            one_by_one<float, HD, RT>(a, g, group, KT, T::UP, per_l);
             continue;
         }
-        const float unit = ldexpf(1.0f, max(E, -200) - 15);
-        l = group_sum(l);
+        l = group_sum(l) * per_l;
         int at = lane;
         asm volatile("" : "+v"(at));  // (addresses of its own, not kept through the tiles)
         const int row = wave * 16 + (at & 15);
@@ -1431,7 +1442,7 @@ __global__ __launch_bounds__(64 * NW, (WideCfg<HD, NW>::PER_CU * NW / 4)) void t
             for (int n = 0; n < DT; ++n) {
                 f32x4 v = o[n];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] *= unit;
+                for (int r = 0; r < 4; ++r) v[r] = v[r] * unit * per_o;
                 to.put(n, v);
             }
         }

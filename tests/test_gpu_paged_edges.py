@@ -101,3 +101,24 @@ def test_attention_masks_of_more_bits_than_nodes(ctx, rng, case):
         for w in range(b.mask.shape[1]):
             b.mask[r, w] |= np.uint32(0xffffffff << min(max(n - 32 * w, 0), 32) & 0xffffffff)
     assert np.array_equal(b.run(), first)
+
+
+# ------------------------------------------------------------- the largest values
+
+@pytest.mark.parametrize("hidden", [False, True])
+@pytest.mark.parametrize("cached", [[150, 0], [0, 3100], [2047, 2046]])
+@pytest.mark.parametrize("case", KERNELS)
+def test_attention_of_the_largest_values(ctx, rng, case, cached, hidden):
+    """V up to the type's largest: sums of many such values are past it, their
+    mean is not.  hidden: beside a node of NaN that no row sees."""
+    kv, heads, kvh, hd, new = case
+    b = Batch(ctx, rng, cached, [new, 2], heads, kvh, hd, kv, 16, tree=hidden, q_scale=0.1)
+    most = float(np.finfo(b.v.dtype).max) * 0.98
+    held = ~np.isnan(b.v[:, 0, 0].astype(np.float32))
+    b.v[held] = (most * rng.uniform(0.5, 1.0, b.v[held].shape)).astype(b.v.dtype)
+    b.v[held, :, 1::2] *= -1
+    if hidden:
+        b.mask[:new, 0] &= ~np.uint32(1 << 1)
+        at_ = po.slot_of(b.tables, 16, 0, int(b.cached[0]) + 1)
+        b.k[at_] = b.v[at_] = np.nan
+    b.check(b.run())
