@@ -93,9 +93,19 @@ __global__ __launch_bounds__(THREADS) void tree_row_kernel(TreeArgs a) {
         if (a.first_row[m] <= r) lo = m;
         else hi = m;
     }
-    const SeqRows s = seq_rows(a.first_row, a.cached, a.rows, lo);
+    SeqRows s = seq_rows(a.first_row, a.cached, a.rows, lo);
+    auto has = [&](const SeqRows &t) { return r >= t.r0 && r < t.r0 + t.n; };
+    // a row range that is out of order leads the search astray: look at all
+    for (int c = 0; !has(s) && c < a.n_seq; c += 64) {
+        const int b = min(c + (int)(threadIdx.x & 63), a.n_seq - 1);
+        const unsigned long long hit = __ballot(has(seq_rows(a.first_row, a.cached, a.rows, b)));
+        if (hit) {
+            lo = c + __ffsll((long long)hit) - 1;
+            s = seq_rows(a.first_row, a.cached, a.rows, lo);
+        }
+    }
+    if (!has(s)) return;
     const int i = r - s.r0;
-    if (i < 0 || i >= s.n) return;
     const float q = a.q[(size_t)r * a.q_stride + (size_t)h * HD + e], unit = unit_of<KVT>(s);
     float m = -INFINITY, l = 0.0f, o = 0.0f;
     bool lost = lost_length(a, s);  // or a position without a block

@@ -4,6 +4,7 @@ test_gpu_paged."""
 import numpy as np
 import pytest
 
+import cw
 import paged_oracle as po
 from test_gpu_paged import Batch, i32, run_tables, same_step, tables_state
 
@@ -122,3 +123,25 @@ def test_attention_of_the_largest_values(ctx, rng, case, cached, hidden):
         at_ = po.slot_of(b.tables, 16, 0, int(b.cached[0]) + 1)
         b.k[at_] = b.v[at_] = np.nan
     b.check(b.run())
+
+
+# -------------------------------------------------------------------- row ranges
+
+@pytest.mark.parametrize("case", KERNELS)
+def test_a_bad_row_range_among_good_ones(ctx, rng, case):
+    """A request whose rows lie behind the last has none, and neither has the
+    one that would begin there; the others, before and behind, are right."""
+    kv, heads, kvh, hd, new = case
+    b = Batch(ctx, rng, [70, 40, 9, 33, 20], [new, 2, 4, 1, 5], heads, kvh, hd, kv, 16)
+    good = b.run()
+    b.check(good)
+    first, heads = b.first.copy(), b.dims[0]
+    first[2] = b.rows + 9
+    b.dev = cw.batch(ctx.storage(b.cached), 5, b.rows, ctx.storage(first), ctx.storage(b.tables),
+                     b.tables.shape[1])
+    out = ctx.storage(np.full((b.rows, heads * hd), 7.5, np.float32))
+    ctx.attention_tree(b.pages, b.dev, b.qd, heads, out=out)
+    got = out.download().reshape(good.shape)
+    assert np.all(got[new:new + 6] == 7.5)
+    got[new:new + 6] = good[new:new + 6]
+    b.check(got)
