@@ -367,14 +367,15 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(PageMap m, u32x4 *k, u
     const int n = min(max(path_len[b], 0), max_path);
     const int u = blockIdx.x * kThreads + threadIdx.x;
     if (u == 0 && cached_out) cached_out[b] = c + n;
-    if (c < 0 || c > 1 << 30) return;
+    if (c < 0) return;
     const bool on = u < 2 * row_u4;
     u32x4 *const base = u < row_u4 ? k + u : v + (on ? u - row_u4 : 0);
     for (int i0 = 0; i0 < n; i0 += 64) {
         int src = -1, dst = -1;
         if (i0 + lane < n) {
             const int node = path[(size_t)b * max_path + i0 + lane];
-            if (node >= 0 && node <= 1 << 30 && node != i0 + lane) {
+            // (no position is past 2^31 - 1)
+            if (node >= 0 && node != i0 + lane && max(node, i0 + lane) <= 0x7fffffff - c) {
                 src = slot_of(m, b, c + node);
                 dst = slot_of(m, b, c + i0 + lane);
             }

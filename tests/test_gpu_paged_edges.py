@@ -145,3 +145,26 @@ def test_a_bad_row_range_among_good_ones(ctx, rng, case):
     assert np.all(got[new:new + 6] == 7.5)
     got[new:new + 6] = good[new:new + 6]
     b.check(got)
+
+
+# ------------------------------------------------------------------ long requests
+
+def test_kv_accept_past_a_billion_positions(rng):
+    """Moves at positions past 2^30, which a request without tables can have."""
+    page, hd = (1 << 30) + 4096, 16
+    with cw.Context(0) as c:
+        kd, vd = (c.empty((page, hd), np.float16) for _ in range(2))
+        pages = cw.kv_pages(kd, vd, cw.CW_F16, 1, hd, page, 1)
+        cached = (1 << 30) + 1000
+        new = rng.standard_normal((2, 40, hd)).astype(np.float16)
+        views = [cw.DeviceArray(c, (40, hd), np.float16, d.ptr + cached * hd * 2) for d in (kd, vd)]
+        for d, a in zip(views, new):
+            d.upload(a)
+        path, out = [0, 3, 4, 17, 39], c.empty(1, np.int32)
+        batch = cw.batch(c.storage(i32([cached])), 1, 1, None, None, 0)
+        c.kv_accept(pages, batch, c.storage(i32([path])), 5, c.storage(i32([5])), out)
+        for d, a in zip(views, new):
+            want = a.copy()
+            want[:5] = a[path]
+            assert d.download().tobytes() == want.tobytes()
+        assert out.download()[0] == cached + 5
