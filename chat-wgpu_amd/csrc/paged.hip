@@ -685,7 +685,8 @@ int cw_block_tables(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const
 int cw_kv_accept(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const int *path,
                  int max_path, const int *path_len, int *cached_out) {
     CW_CHECK_ARG(ctx && kv && b && path && path_len, "cw_kv_accept: null argument");
-    CW_CHECK_ARG(max_path > 0, "cw_kv_accept: max_path=%d must be positive", max_path);
+    CW_CHECK_ARG(max_path > 0 && max_path <= 1 << 30,
+                 "cw_kv_accept: max_path=%d must be positive and at most 2^30", max_path);
     PageMap map;
     CW_TRY(check_pages("cw_kv_accept", kv, b, true, &map));
     CW_CHECK_ARG(cached_out != b->cached, "cw_kv_accept: cached_out is cached");

@@ -303,9 +303,9 @@ int cw_attention_tree(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, con
 /* Keeps the accepted nodes of each request: for i < path_len[b] the K and V of
  * node path[b*max_path + i] (increasing in i) move to position cached[b] + i,
  * and cached_out[b] = cached[b] + path_len[b] (NULL: not wanted; it must not
- * be b->cached).  Of b only cached, n_seq, tables and max_blocks are used.  A
- * path_len outside 0 .. max_path counts as the nearer of the two; a move from
- * or to a position that has no block is left out. */
+ * be b->cached).  Of b only cached, n_seq, tables and max_blocks are used.
+ * max_path is at most 2^30; a path_len outside 0 .. max_path counts as the nearer
+ * of the two; a move from or to a position that has no block is left out. */
 int cw_kv_accept(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const int *path,
                  int max_path, const int *path_len, int *cached_out);
 
