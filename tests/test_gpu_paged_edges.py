@@ -6,6 +6,8 @@ import pytest
 
 import cw
 import paged_oracle as po
+import test_gpu_paged as tp
+import test_gpu_paged_serving as ts
 from test_gpu_paged import Batch, i32, run_tables, same_step, tables_state
 
 pytestmark = pytest.mark.gpu
@@ -168,3 +170,32 @@ def test_kv_accept_past_a_billion_positions(rng):
             want[:5] = a[path]
             assert d.download().tobytes() == want.tobytes()
         assert out.download()[0] == cached + 5
+
+
+# ------------------------------------------------------------------- head_dim 16
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("check", [
+    lambda *a: tp.test_attention_masked_values_stay_out(*a[:2], 16, a[2]),
+    lambda *a: tp.test_attention_bad_requests(*a[:2], 16, a[2]),
+    lambda *a: ts.test_attention_of_many_requests(*a[:2], 16, False, 4, a[2]),
+    lambda *a: ts.test_attention_of_many_requests(*a[:2], 16, True, 4, a[2]),
+    lambda *a: ts.test_attention_of_prompts(*a[:2], 7, 1, 16, a[2]),
+    lambda *a: ts.test_a_lost_block_behind_the_first_rows(*a[:2], 1, 16, a[2]),
+    lambda *a: ts.test_a_lost_block_behind_the_first_rows(*a[:2], 8, 16, a[2]),
+    lambda *a: ts.test_a_length_behind_the_cache(*a[:2], 1, 16, False, a[2]),
+    lambda *a: ts.test_a_length_behind_the_cache(*a[:2], 8, 16, True, a[2]),
+], ids=["masked", "bad_requests", "many", "many_contig", "prompts", "lost_few", "lost_many",
+        "length_few", "length_many"])
+def test_head_dim_16(ctx, rng, check, kv):
+    """What the other head sizes are held to, over few (row, head)s and many."""
+    check(ctx, rng, kv)
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kvh,cached,new,tree", [
+    (8, 2, [300, 0, 17, 1000], [40, 30, 1, 9], True), (5, 5, [0, 63, 64], [1, 200, 0], False),
+    (16, 1, [2500, 5], [33, 2], True)])
+def test_head_dim_16_of_many_rows(ctx, rng, heads, kvh, cached, new, tree, kv):
+    b = Batch(ctx, rng, cached, new, heads, kvh, 16, kv, 16, tree=tree, spare_rows=4)
+    b.check(b.run(q_pad=4, out_pad=8))
