@@ -100,7 +100,7 @@ float f16_bits_to_f32(uint16_t h) {
 
 // What would allocate or synchronise cannot run while a graph is being
 // recorded: the first use at a size must come before cw_graph_begin.
-static int refuse_while_capturing(const cw_ctx *ctx, const char *what) {
+int refuse_while_capturing(const cw_ctx *ctx, const char *what) {
     if (!ctx->capturing) return CW_OK;
     set_error("%s while a graph is being recorded: run the sequence once before cw_graph_begin",
               what);

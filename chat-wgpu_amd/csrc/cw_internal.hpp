@@ -119,10 +119,12 @@ struct cw_ctx {
     // RoPE tables; a deque, so a table's address stays valid as others are added
     std::deque<cw_rope_tab> ropes;
 
-    // frequencies of cw_rope_spec's, one device table each (paged.hip)
+    // frequencies of cw_rope_spec's, one device table each, the oldest first; of
+    // those that no recording names at most kRopeTurns are kept (paged.hip)
     struct RopeTurns {
         cw_rope_spec spec;
         double *turns;
+        bool recorded;
     };
     std::deque<RopeTurns> rope_turns;
 
@@ -138,6 +140,8 @@ struct cw_ctx {
 
 namespace cwi {
 
+// CW_ERR_STATE while a recording is open: `what` would allocate or synchronise.
+int refuse_while_capturing(const cw_ctx *ctx, const char *what);
 // Scratch of at least `bytes` for the standalone kernels (synchronises the
 // stream before it replaces a smaller buffer).
 int ctx_scratch(cw_ctx *ctx, size_t bytes, void **out);

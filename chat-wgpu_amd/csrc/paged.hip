@@ -2,6 +2,7 @@
 // cache write, block tables from request lengths, the move of accepted rows.
 // The attention over that cache is tree_attention.hip's.
 
+#include <algorithm>
 #include <cmath>
 #include <new>
 #include <vector>
@@ -459,6 +460,11 @@ void rope_turns_host(const cw_rope_spec &s, double *turns) {
     }
 }
 
+// Tables of specs that no recording names: a base or factor that follows the
+// context's length makes a new one every step, so the oldest one's memory is taken
+// for the next.  (A recorded kernel may read its table until the context ends.)
+constexpr int kRopeTurns = 64;
+
 // The device table of a spec's turns: made on first use, kept by the context.
 int ctx_rope_turns(cw_ctx *ctx, const char *what, cw_rope_spec s, const double **out) {
     s.layout = 0;
@@ -467,28 +473,42 @@ int ctx_rope_turns(cw_ctx *ctx, const char *what, cw_rope_spec s, const double *
     if (s.scaling != CW_ROPE_YARN) s.beta_fast = s.beta_slow = 0.0;
     if (s.scaling != CW_ROPE_BANDS) s.low_turns = s.high_turns = 0.0;
     if (s.scaling == CW_ROPE_PLAIN || s.scaling == CW_ROPE_LINEAR) s.trained = 0;
-    for (const auto &t : ctx->rope_turns)
+    for (auto &t : ctx->rope_turns)
         if (same_spec(t.spec, s)) {
+            t.recorded |= ctx->capturing;
             *out = t.turns;
             return CW_OK;
         }
-    if (ctx->capturing) {
-        set_error("%s: a table of frequencies must be built while a graph is being recorded: run "
-                  "the sequence once before cw_graph_begin", what);
-        return CW_ERR_STATE;
-    }
-    double host[128];
+    CW_TRY(refuse_while_capturing(ctx, "a table of frequencies must be built"));
+    constexpr int kMost = 128;  // pairs of a head
+    double host[kMost];
     rope_turns_host(s, host);
     const size_t bytes = (size_t)(s.rot_dim / 2) * sizeof(double);
+    int kept = 0;
+    for (const auto &t : ctx->rope_turns) kept += !t.recorded;
     void *p = nullptr;
-    CW_HIP(hipMalloc(&p, bytes));
+    if (kept >= kRopeTurns) {
+        const auto old = std::find_if(ctx->rope_turns.begin(), ctx->rope_turns.end(),
+                                      [](const auto &t) { return !t.recorded; });
+        p = old->turns;
+        // (out of the list first: after an error below nothing names a half table)
+        ctx->rope_turns.erase(old);
+        // launches that read it are done
+        hipError_t e = hipStreamSynchronize(ctx->stream);
+        if (e != hipSuccess) {
+            (void)hipFree(p);
+            return hip_fail(e, "ctx_rope_turns: reusing a table of frequencies", __FILE__, __LINE__);
+        }
+    } else {
+        CW_HIP(hipMalloc(&p, kMost * sizeof(double)));
+    }
     hipError_t e = hipMemcpy(p, host, bytes, hipMemcpyHostToDevice);
     if (e != hipSuccess) {
         (void)hipFree(p);
         return hip_fail(e, "the copy of a table of frequencies", __FILE__, __LINE__);
     }
     try {
-        ctx->rope_turns.push_back({s, static_cast<double *>(p)});
+        ctx->rope_turns.push_back({s, static_cast<double *>(p), false});
     } catch (const std::bad_alloc &) {
         (void)hipFree(p);
         set_error("%s: out of host memory", what);

@@ -185,8 +185,9 @@ int cw_q4_gemm(cw_ctx *ctx, const float *x, int m, const uint16_t *scales, const
 /* (which result says so is stated below).  The calls leave the context's */
 /* device current, as cw_ctx_create does.  cw_block_tables and             */
 /* cw_attention_tree use the context's scratch, the rotations a table of   */
-/* 4 rot_dim bytes for each specification, which the context keeps: the   */
-/* first call of a kind comes before cw_graph_begin (else CW_ERR_STATE).  */
+/* 1 KB for each specification, of which the context keeps those that a   */
+/* recording uses and 64 others: the first call of a kind comes before    */
+/* cw_graph_begin (else CW_ERR_STATE).                                    */
 /* ---------------------------------------------------------------- */
 
 /* which elements of a head form a rotated pair */

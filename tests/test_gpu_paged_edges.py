@@ -1,6 +1,8 @@
 """Values, masks and lengths at the edges of what the paged operators accept,
 on the MI355X: each against its definition in 64 bits, with the bounds of
 test_gpu_paged."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -199,3 +201,53 @@ def test_head_dim_16(ctx, rng, check, kv):
 def test_head_dim_16_of_many_rows(ctx, rng, heads, kvh, cached, new, tree, kv):
     b = Batch(ctx, rng, cached, new, heads, kvh, 16, kv, 16, tree=tree, spare_rows=4)
     b.check(b.run(q_pad=4, out_pad=8))
+
+
+# ----------------------------------------------------------- many specifications
+
+def test_frequencies_of_many_specifications(ctx, rng):
+    """A base that changes every step: each call is rotated by its own, a
+    recording keeps its table, and the device's memory does not fill up."""
+    rows, heads, hd = 5, 3, 64
+    x = rng.standard_normal((rows, heads * hd)).astype(np.float32)
+    pos = i32([0, 7, 900, 40000, 131071])
+    xd, pd, y = ctx.storage(x), ctx.storage(pos), ctx.empty((rows, heads * hd))
+    x3 = x.reshape(rows, heads, hd)
+    pair = np.abs(x3) + np.abs(np.roll(x3, hd // 2, -1))
+    tol = pair * (7 * tp.H + pos[:, None, None] * 1e-15)
+
+    def check(theta):
+        ref = po.rotate(x3, pos, po.rope_freqs(hd, theta, "plain"), hd, False, 1.0)
+        assert np.all(np.abs(y.download().reshape(ref.shape) - ref) <= tol), theta
+
+    def rotate(theta):
+        ctx.rope_rows(cw.rope_spec(hd, theta), xd, pd, rows, heads, hd, y=y)
+
+    rotate(3e5)
+    ctx.graph_begin()
+    rotate(3e5)
+    g = ctx.graph_end()
+    for i in range(150):
+        rotate(1e4 + i)
+        if i % 3 == 0:  # (else several are queued behind one another)
+            check(1e4 + i)
+        if i % 50 == 0:
+            g.launch()
+            check(3e5)
+    rotate(1e4)
+    check(1e4)
+
+    def free():
+        n = (C.c_size_t * 2)()
+        assert cw.lib().hipMemGetInfo(C.byref(n, 0), C.byref(n, C.sizeof(C.c_size_t))) == 0
+        return n[0]
+
+    ctx.flush()
+    before = free()
+    for i in range(8000):
+        rotate(2e4 + i)
+    check(2e4 + 7999)
+    g.launch()
+    check(3e5)
+    g.close()
+    assert before - free() <= 4 << 20
