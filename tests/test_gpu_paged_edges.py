@@ -129,6 +129,24 @@ def test_attention_of_the_largest_values(ctx, rng, case, cached, hidden):
     b.check(b.run())
 
 
+@pytest.mark.parametrize("what", ["k", "v", "both"])
+@pytest.mark.parametrize("case", [c for c in KERNELS if c[0] == "f32"])
+def test_attention_of_cached_values_far_apart(ctx, rng, case, what):
+    """Cached positions far below the ones beside them, which every row sees:
+    the error counts from the largest."""
+    kv, heads, kvh, hd, new = case
+    b = Batch(ctx, rng, [333, 40], [new, 2], heads, kvh, hd, kv, 16, tree=True)
+    for s in range(2):
+        for p in range(int(b.cached[s])):
+            f = np.float32(2.0 ** -int(rng.integers(0, 45)))
+            at_ = po.slot_of(b.tables, 16, s, p)
+            if what != "v":
+                b.k[at_] *= f
+            if what != "k":
+                b.v[at_] *= f
+    b.check(b.run())
+
+
 # -------------------------------------------------------------------- row ranges
 
 @pytest.mark.parametrize("case", KERNELS)
