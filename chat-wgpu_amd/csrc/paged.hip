@@ -19,10 +19,10 @@ constexpr int kThreads = 256;
 //
 // y_a = g (x_a cos - x_b sin), y_b = g (x_b cos + x_a sin) for each pair (a, b),
 // at the angle pos * f.  The table holds f / 2 pi in f64 (turns per position):
-// the product's distance to the next whole quarter turn is exact to 2^-53 of
-// the turns (4e-8 of a turn at 2^31 turns, 4e-14 at a million positions), so
-// far positions cost no accuracy; in f32 a position of a million would leave
-// 0.06 of a radian.  The rest, at most pi / 4, is x + lo in f32.
+// its rounding and the product's are 2^-53 of the turns each, of which a position
+// has 0.16 at most: 3.6e-11 of a turn in all at a million positions, 7.6e-8 at
+// 2^31, so far positions cost next to no accuracy; in f32 a position of a million
+// would leave 0.06 of a radian.  The rest, at most pi / 4, is x + lo in f32.
 
 // cos and sin of 2 pi t by their Taylor series at the nearest quarter turn
 // (|x| <= pi / 4: the first term left out is 2e-9), lo by the first two terms of

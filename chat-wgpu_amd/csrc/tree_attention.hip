@@ -76,8 +76,8 @@ __device__ __forceinline__ float unit_of(const SeqRows &s) {
     return sizeof(KVT) == 4 ? ldexpf(1.0f, __builtin_clz((unsigned)(s.cached + s.n)) - 32) : 1.0f;
 }
 
-// head_dim 16, which the products below have no form for: one (row, head) a
-// workgroup, 16 lanes a position, four positions at once; the groups' (max, sum, o)
+// head_dim 16, for which the tiles below (K fragments and o of 32 elements and
+// more) are not laid out: one (row, head) a workgroup, 16 lanes a position, four positions at once; the groups' (max, sum, o)
 // meet in LDS.  Bound by the loads' latency and the caches, which have K and V for
 // every head of a row again.
 template <typename KVT, int THREADS>
@@ -247,8 +247,9 @@ __device__ __forceinline__ void split_f16(const float (&v)[N], H &hi, H &lo) {
 // tree_merge_kernel.  (Where every block of a prompt counts and takes the tiles of
 // the last, 2,000 rows of 16 heads take 85 us instead of 58, eight prompts of 345
 // over f32 55 instead of 44.)
-// (kOpen 0, 2, 4 and 8: 48 single rows at 100 .. 8,000 positions 88, 74, 74 and
-// 77 us.  Workgroups of one CU and the XCDs are served unevenly, equal runs end
+// (kOpen 0, 2, 3, 4 and 8, us with the join: 48 single rows at 100 .. 8,000 positions
+// 83, 71.2, 70.9, 71.0 and 73; 61 nodes at 4,100 30.8, 28.5, 28.1, 27.9 and 28.1;
+// four pieces of 80 to 300 rows over f32 97, 91.3, 91.5, 92.1 and 96.5.  Workgroups of one CU and the XCDs are served unevenly, equal runs end
 // up to 1.5 times apart; short runs fetched by whoever is free gain nothing,
 // as the rest of the chip then has the memory to itself: 164 us either way for
 // 64 requests of 4,000 positions.)

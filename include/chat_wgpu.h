@@ -297,6 +297,13 @@ int cw_block_tables(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const
  * n_heads at most 2^33 and 2^27 of them a kv head (and the product of the two
  * for a request and kv head at most 2^39: one beyond has no rows).  out must
  * not overlap q.
+ * Precision: scores, softmax and sums are f32.  For the matrix cores q (under a
+ * power of two a row and head) and the softmax's weights are held to 22 bits, and
+ * over CW_F32 so are K and V: a K more than 2^17 below the largest of the 4 to 16
+ * positions beside it, and a V that far below the largest of its request, to 2^-40
+ * of that (of what the row sees).  Nothing is held to fewer than 24 bits at
+ * head_dim 16, and over CW_F32 at head_dim 64 and 128 where b->rows / b->n_seq
+ * (rounded up) times n_heads / n_kv_heads is at most 16.
  * Covers a decode step (one row each, mask NULL), pieces of prompts (mask
  * NULL) and trees of drafted tokens. */
 int cw_attention_tree(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const float *q,
