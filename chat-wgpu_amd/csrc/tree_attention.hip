@@ -70,7 +70,9 @@ __device__ __forceinline__ uint64_t sees64(const TreeArgs &a, int row, int i, in
 // Over f32 the weights carry 2^-bits, the bits of the request's length: the sum of
 // all its weights times V is then no larger than the largest V, so any V that f32
 // holds has its mean.  (Sums of f16 V cannot get past f32.)  The factor is the same
-// for every segment of a request and cancels in o / sum.
+// for every segment of a request and cancels in o / sum.  It costs V below 2^bits
+// times f32's smallest normal value the bits that subnormal sums lack: at 3,000
+// positions none of 1e-35, 5e-6 of 1e-37.
 template <typename KVT>
 __device__ __forceinline__ float unit_of(const SeqRows &s) {
     return sizeof(KVT) == 4 ? ldexpf(1.0f, __builtin_clz((unsigned)(s.cached + s.n)) - 32) : 1.0f;
