@@ -1,0 +1,287 @@
+// Rows of logits under a server's rules: penalties for repeated tokens, biases,
+// grammar masks; the likeliest token and its log softmax.
+//
+// With c_v the times that token v was generated and seen_v whether it occurs at
+// all (tokens of the request, nodes that the row sees):
+//   l_v = x_v; seen_v: l_v > 0 ? l_v / repeat : l_v * repeat;
+//   l_v -= frequency c_v + presence [c_v > 0]; l_v += bias_v; not allowed: -inf.
+// The token is t = argmax l, its log softmax -log(1 + s), s = sum of exp(l_v -
+// l_t) over v != t.  s is kept without the token's own 1, which for a likely
+// token would take all of s's digits.
+//
+// One pass over the logits.  A workgroup has a slice of a row's vocabulary and
+// counts the slice's tokens in LDS: it reads the request's whole history and
+// keeps what falls into its slice, so no count goes through memory.  Counts are
+// whole numbers and a bias is chosen by its place in the list, so the order of the
+// LDS atomics does not show.  (max, s, index) of the slices are joined by a second
+// launch in a fixed order.
+
+#include "paged_device.hpp"
+
+namespace {
+
+using namespace cwi;
+
+constexpr int kThreads = 256;
+constexpr uint32_t kPrompt = 0x80000000u;  // a token's count: seen, though not generated
+
+struct LogitArgs {
+    cw_logit_rules r;
+    const int *first_row;
+    int n_seq, batch_rows;
+    const uint32_t *mask;
+    int mask_words;
+    const int *at;
+    const float *x;
+    size_t stride;
+    int vocab;
+    float *out;
+    size_t out_stride;
+    int slice, parts;  // tokens a workgroup takes (a multiple of 32), workgroups a row
+    struct Top *part;  // [rows][parts]; null: no token is wanted
+    uint32_t *token;
+    float *logprob;
+};
+
+constexpr int kNone = -1, kPadding = -2;
+
+// The largest of some logits, its index (kNone: all are -inf or NaN), and the sum
+// of exp(l - m) over the others.
+struct Top {
+    float m, s;
+    int i;
+};
+
+__device__ __forceinline__ Top join(Top a, Top b) {
+    if (b.i >= 0 && (a.i < 0 || b.m > a.m || (b.m == a.m && b.i < a.i))) {
+        const Top t = a;
+        a = b;
+        b = t;
+    }
+    if (b.i >= 0) a.s += (1.0f + b.s) * expf(b.m - a.m);
+    else a.s += b.s;  // 0 or NaN
+    return a;
+}
+
+__device__ __forceinline__ Top wave_join(Top a) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const Top o{__shfl_xor(a.m, d), __shfl_xor(a.s, d), __shfl_xor(a.i, d)};
+        // (both lanes join in the lower one's order: the same bits)
+        a = threadIdx.x & d ? join(o, a) : join(a, o);
+    }
+    return a;
+}
+
+template <typename V>
+__device__ __forceinline__ V rule(const V *p, int b, V none) {
+    return p ? p[b] : none;
+}
+
+// V logits at a time: 4 where rows are 16-byte aligned and whole fours, else 1.
+template <int V>
+__global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
+    extern __shared__ uint32_t lds[];
+    __shared__ int owner;
+    __shared__ Top tops[kThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const size_t row = blockIdx.y;
+    const int lo = blockIdx.x * a.slice, n = min(a.slice, a.vocab - lo);
+    const bool counts = a.r.tokens || a.r.node_token, biased = a.r.bias;
+    uint32_t *const count = lds, *const last = lds + (counts ? a.slice : 0);
+
+    // the request whose rows the batch row is among
+    const int br = a.at ? a.at[row] : (int)row;
+    if (tid == 0) owner = a.n_seq;
+    for (int v = tid; v < (counts + biased) * a.slice; v += kThreads) lds[v] = 0;
+    __syncthreads();
+    for (int b = tid; b < a.n_seq; b += kThreads) {
+        const int r0 = a.first_row[b], r1 = a.first_row[b + 1];
+        if (r0 >= 0 && r0 <= br && br < r1 && r1 <= a.batch_rows) atomicMin(&owner, b);
+    }
+    __syncthreads();
+    const int b = owner;
+    if (b == a.n_seq) {
+        if (a.part && tid == 0) a.part[row * a.parts + blockIdx.x].i = kPadding;
+        return;
+    }
+    auto add = [&](int v, bool made) {
+        if ((unsigned)(v - lo) < (unsigned)n) {
+            if (made) atomicAdd(&count[v - lo], 1u);
+            else atomicOr(&count[v - lo], kPrompt);
+        }
+    };
+    if (a.r.tokens) {
+        const int len = min(max(a.r.length[b], 0), a.r.max_len), made = rule(a.r.prompt, b, 0);
+        const int *t = a.r.tokens + (size_t)b * a.r.max_len;
+        for (int i = tid; i < len; i += kThreads) add(t[i], i >= made);
+    }
+    if (a.r.node_token) {
+        const int r0 = a.first_row[b], nodes = a.first_row[b + 1] - r0, self = br - r0;
+        for (int j = tid; j < nodes; j += kThreads) {
+            const bool sees = !a.mask ? j <= self
+                                      : j < 32 * a.mask_words &&
+                                            (a.mask[(size_t)br * a.mask_words + (j >> 5)] >> (j & 31) & 1);
+            if (sees) add(a.r.node_token[r0 + j], true);
+        }
+    }
+    if (biased) {
+        const int e0 = a.r.bias_first[b], e1 = a.r.bias_first[b + 1];
+        if (e0 >= 0 && e1 <= a.r.n_bias)
+            for (int e = e0 + tid; e < e1; e += kThreads) {
+                const int v = a.r.bias_token[e];
+                if ((unsigned)(v - lo) < (unsigned)n) atomicMax(&last[v - lo], (uint32_t)e + 1);
+            }
+    }
+    const float repeat = rule(a.r.repeat, b, 1.0f), presence = rule(a.r.presence, b, 0.0f);
+    const float frequency = rule(a.r.frequency, b, 0.0f);
+    const uint32_t *allowed = nullptr;
+    if (a.r.allowed) {
+        const int k = a.r.allowed_row ? a.r.allowed_row[row] : (int)row;
+        if ((unsigned)k < (unsigned)a.r.n_allowed) allowed = a.r.allowed + (size_t)k * a.r.allowed_words;
+    }
+    __syncthreads();
+
+    const float *x = a.x + row * a.stride;
+    Top top{-INFINITY, 0.0f, kNone};
+    for (int v0 = lo + tid * V; v0 < lo + n; v0 += kThreads * V) {
+        float l[V];
+        if constexpr (V == 4) {
+            const float4 q = *reinterpret_cast<const float4 *>(x + v0);
+            l[0] = q.x;
+            l[1] = q.y;
+            l[2] = q.z;
+            l[3] = q.w;
+        } else {
+            l[0] = x[v0];
+        }
+        const uint32_t bits = allowed ? allowed[v0 >> 5] >> (v0 & 31) : ~0u;
+        float best = top.m;
+        int at = -1;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (counts) {
+                const uint32_t c = count[v0 - lo + j];
+                if (c) {
+                    l[j] = l[j] > 0.0f ? l[j] / repeat : l[j] * repeat;
+                    const uint32_t made = c & ~kPrompt;
+                    if (made) l[j] = __builtin_fmaf(-frequency, (float)made, l[j]) - presence;
+                }
+            }
+            if (biased) {
+                const uint32_t e = last[v0 - lo + j];
+                if (e) l[j] += a.r.bias[e - 1];
+            }
+            if (!(bits >> j & 1)) l[j] = -INFINITY;
+            if (l[j] > best) {
+                best = l[j];
+                at = j;
+            }
+        }
+        if (a.out) {
+            float *o = a.out + row * a.out_stride + v0;
+            if constexpr (V == 4) *reinterpret_cast<float4 *>(o) = make_float4(l[0], l[1], l[2], l[3]);
+            else o[0] = l[0];
+        }
+        if (a.part) {
+            if (at >= 0) {
+                // (1 + s: the former largest is now one of the others)
+                if (top.i >= 0) top.s = (1.0f + top.s) * expf(top.m - best);
+                top.m = best;
+                top.i = v0 + at;
+            }
+            const float m = top.i >= 0 ? top.m : 0.0f;  // (-inf - -inf)
+#pragma unroll
+            for (int j = 0; j < V; ++j) top.s += j == at ? 0.0f : expf(l[j] - m);
+        }
+    }
+    if (!a.part) return;
+    top = wave_join(top);
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kThreads / 64; ++w) top = join(top, tops[w]);
+        a.part[row * a.parts + blockIdx.x] = top;
+    }
+}
+
+__global__ __launch_bounds__(64) void logits_join_kernel(LogitArgs a) {
+    const size_t row = blockIdx.x;
+    const Top *p = a.part + row * a.parts;
+    if (p[0].i == kPadding) return;
+    Top top{-INFINITY, 0.0f, kNone};
+    for (int i = threadIdx.x; i < a.parts; i += 64) top = join(top, p[i]);
+    top = wave_join(top);
+    if (threadIdx.x == 0) {
+        if (a.token) a.token[row] = top.i >= 0 ? (uint32_t)top.i : CW_NO_TOKEN;
+        if (a.logprob) a.logprob[row] = top.i >= 0 ? -log1pf(top.s) : -INFINITY;
+    }
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+
+using namespace cwi;
+
+extern "C" int cw_logits_rows(cw_ctx *ctx, const cw_logit_rules *rules, const cw_batch *b,
+                              const int *at, const float *logits, size_t stride, int rows,
+                              int vocab, float *out, size_t out_stride, uint32_t *token,
+                              float *logprob) {
+    CW_CHECK_ARG(ctx && rules && b && logits, "cw_logits_rows: null argument");
+    CW_CHECK_ARG(out || token || logprob, "cw_logits_rows: no output");
+    CW_CHECK_ARG(rows > 0 && rows <= 65535 && vocab > 0 && vocab <= 1 << 24,
+                 "cw_logits_rows: rows=%d (at most 65535) vocab=%d (2^24)", rows, vocab);
+    CW_CHECK_ARG(b->first_row && b->n_seq > 0 && b->n_seq <= 65535 && b->rows > 0 &&
+                     b->rows <= kMaxRows,
+                 "cw_logits_rows: a batch of n_seq=%d (1 .. 65535) and rows=%d (1 .. 2^23) with first_row",
+                 b->n_seq, b->rows);
+    CW_CHECK_ARG(!b->mask || b->mask_words > 0, "cw_logits_rows: mask_words=%d", b->mask_words);
+    CW_CHECK_ARG(stride >= (size_t)vocab && stride < (1u << 31),
+                 "cw_logits_rows: stride %zu of rows of %d logits", stride, vocab);
+    if (out) {
+        CW_CHECK_ARG(out_stride >= (size_t)vocab && out_stride < (1u << 31),
+                     "cw_logits_rows: out_stride %zu of rows of %d logits", out_stride, vocab);
+        CW_CHECK_ARG((out == logits && out_stride == stride) ||
+                         rows_apart(rows, logits, stride, vocab, out, out_stride, vocab),
+                     "cw_logits_rows: rows of logits and out overlap");
+    }
+    const cw_logit_rules &r = *rules;
+    CW_CHECK_ARG(!r.tokens || (r.length && r.max_len > 0),
+                 "cw_logits_rows: tokens need their length and max_len=%d", r.max_len);
+    CW_CHECK_ARG(!r.bias || (r.bias_first && r.bias_token && r.n_bias > 0),
+                 "cw_logits_rows: biases need bias_first, bias_token and n_bias=%d", r.n_bias);
+    CW_CHECK_ARG(!r.allowed || (r.n_allowed > 0 && r.allowed_words >= (vocab + 31) / 32),
+                 "cw_logits_rows: n_allowed=%d masks of allowed_words=%d for %d tokens",
+                 r.n_allowed, r.allowed_words, vocab);
+    CW_HIP(hipSetDevice(ctx->device));
+    LogitArgs a{};
+    a.r = r;
+    a.first_row = b->first_row;
+    a.n_seq = b->n_seq;
+    a.batch_rows = b->rows;
+    a.mask = b->mask;
+    a.mask_words = b->mask_words;
+    a.at = at;
+    a.x = logits;
+    a.stride = stride;
+    a.vocab = vocab;
+    a.out = out;
+    a.out_stride = out_stride;
+    a.token = token;
+    a.logprob = logprob;
+    a.slice = 4096;
+    a.parts = (vocab + a.slice - 1) / a.slice;
+    if (token || logprob) {
+        void *scratch = nullptr;
+        CW_TRY(ctx_scratch(ctx, (size_t)rows * a.parts * sizeof(Top), &scratch));
+        a.part = static_cast<Top *>(scratch);
+    }
+    const int tables = (r.tokens || r.node_token ? 1 : 0) + (r.bias ? 1 : 0);
+    const bool wide = aligned16(logits) && stride % 4 == 0 && vocab % 4 == 0 &&
+                      (!out || (aligned16(out) && out_stride % 4 == 0));
+    CW_TRY(launch(ctx, "logits_rows", wide ? logits_kernel<4> : logits_kernel<1>,
+                  dim3(a.parts, rows), dim3(kThreads), tables * a.slice * 4, a));
+    if (!a.part) return CW_OK;
+    return launch(ctx, "logits_join", logits_join_kernel, dim3(rows), dim3(64), 0, a);
+}

@@ -1,5 +1,5 @@
-// Several requests in one paged KV cache: rotary rows with and without the
-// cache write, block tables from request lengths, the move of accepted rows.
+// Several requests in one paged KV cache: rotary rows with and without the norm
+// of each head and the cache write, block tables from request lengths, the move of accepted rows.
 // The attention over that cache is tree_attention.hip's.
 
 #include <algorithm>
@@ -162,6 +162,170 @@ int launch_rope(cw_ctx *ctx, const char *label, const RopeArgs &a, bool wide, bo
             fn = a.pairs ? rope_rows_kernel<KVT, 4, true, false, true>
                          : rope_rows_kernel<KVT, 4, false, false, true>;
     return launch(ctx, label, fn, grid, dim3(kThreads), 0, a, U, par);
+}
+
+// ---------------------------------------------------------------- normalised heads
+//
+// y = rotation of x / sqrt(sum(x^2) / hd + eps) * gain for each head: the norm's
+// factor is the head's, so a head's G lanes (a power of two, one for every eight
+// elements) hold it whole, add its squares up among themselves and rotate what
+// they hold.  A lane has four pairs (4 elements of either half, or 8 in a row), or
+// 8 elements behind rot, and keeps its angles for the heads it takes.
+
+struct NormArgs {
+    const float *q_gain, *k_gain;  // [hd]
+    float eps;
+    int q_heads;  // heads under q_gain; those behind them are keys
+};
+
+// y and the cache rows of head h: 8 elements, 4 from i0 on and 4 from i1
+template <typename KVT, bool CACHE, bool WIDE, bool STREAM>
+__device__ __forceinline__ void put_head(const RopeArgs &a, int r, int slot, int h, int i0, int i1,
+                                         const float *x) {
+    if (h < a.heads) {
+        float *dst = a.y + (size_t)r * a.y_stride + (size_t)h * a.hd;
+        if constexpr (WIDE) {
+            put_unit<4, STREAM>(dst + i0, x);
+            put_unit<4, STREAM>(dst + i1, x + 4);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                dst[i0 + j] = x[j];
+                dst[i1 + j] = x[4 + j];
+            }
+        }
+    } else if constexpr (CACHE) {
+        const bool k = h < a.heads + a.kv_heads;
+        const int g = h - a.heads - (k ? 0 : a.kv_heads);
+        KVT *dst = static_cast<KVT *>(k ? a.kc : a.vc) + ((size_t)slot * a.kv_heads + g) * a.hd;
+        Vec<KVT, 8> o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o.v[j] = (KVT)x[j];  // f16: to nearest even
+        using O = Vec<KVT, 4>;
+        *reinterpret_cast<O *>(dst + i0) = *reinterpret_cast<O *>(o.v);
+        *reinterpret_cast<O *>(dst + i1) = *reinterpret_cast<O *>(o.v + 4);
+    }
+}
+
+// Workgroup (row, part of the heads).  WIDE: rows and gains are 16-byte aligned;
+// STREAM as above.
+template <typename KVT, bool PAIRS, bool CACHE, bool WIDE, bool STREAM = false>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeArgs a, NormArgs n, int G) {
+    const int r = blockIdx.x, pos = a.positions[r];
+    if (pos < 0) return;
+    const int tid = threadIdx.x, par = kThreads / G;
+    const int u = tid & (G - 1), rot_units = a.rot / 8;
+    const bool on = u < a.hd / 8, rotates = u < rot_units;
+    const int i0 = !on ? 0 : !rotates || PAIRS ? 8 * u : 4 * u;
+    const int i1 = rotates && !PAIRS ? i0 + a.rot / 2 : i0 + 4;
+    float2 cs[4];
+    if (rotates) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) cs[j] = turn((double)pos * a.turns[4 * u + j], a.gain, a.gain_lo);
+    }
+    const int slot = CACHE ? a.slots[r] : -1;
+    const bool write = CACHE && (unsigned)slot < (unsigned)a.n_slots;
+    const int heads = write ? a.heads + 2 * a.kv_heads : a.heads;
+    const float *row = a.x + (size_t)r * a.x_stride;
+    for (int h = blockIdx.y * par + tid / G; h < heads; h += gridDim.y * par) {
+        const float *src = row + (size_t)h * a.hd;
+        Vec<float, 8> x;
+        if constexpr (WIDE) {
+            read_once<4>(x.v, src + i0);
+            read_once<4>(x.v + 4, src + i1);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x.v[j] = src[i0 + j];
+                x.v[4 + j] = src[i1 + j];
+            }
+        }
+        if (h < a.heads + (CACHE ? a.kv_heads : 0)) {  // (values stay as they are)
+            const float *gain = h < n.q_heads ? n.q_gain : n.k_gain;
+            float ss = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(x.v[j], x.v[j], ss);
+            if (!on) ss = 0.0f;
+            for (int d = 1; d < G; d <<= 1) ss += __shfl_xor(ss, d);
+            const float inv = 1.0f / sqrtf(ss / (float)a.hd + n.eps);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x.v[j] = x.v[j] * inv * gain[i0 + j];
+                x.v[4 + j] = x.v[4 + j] * inv * gain[i1 + j];
+            }
+            if (rotates) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float &xa = x.v[PAIRS ? 2 * j : j], &xb = x.v[PAIRS ? 2 * j + 1 : 4 + j];
+                    const float ya = __builtin_fmaf(xa, cs[j].x, -(xb * cs[j].y));
+                    xb = __builtin_fmaf(xb, cs[j].x, xa * cs[j].y);
+                    xa = ya;
+                }
+            }
+        }
+        if (on) put_head<KVT, CACHE, WIDE, STREAM>(a, r, slot, h, i0, i1, x.v);
+    }
+}
+
+// Heads or rotated parts that are no whole eighths: a wave a head, an element or a
+// pair a lane.
+template <typename KVT, bool CACHE>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_any_kernel(RopeArgs a, NormArgs n) {
+    const int r = blockIdx.x, pos = a.positions[r], lane = threadIdx.x & 63;
+    if (pos < 0) return;
+    const int slot = CACHE ? a.slots[r] : -1;
+    const bool write = CACHE && (unsigned)slot < (unsigned)a.n_slots;
+    const int h = blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6);
+    if (h >= (write ? a.heads + 2 * a.kv_heads : a.heads)) return;
+    const float *src = a.x + (size_t)r * a.x_stride + (size_t)h * a.hd;
+    const bool normed = h < a.heads + (CACHE ? a.kv_heads : 0);
+    const float *gain = h < n.q_heads ? n.q_gain : n.k_gain;
+    float ss = 0.0f;
+    for (int i = lane; i < a.hd; i += 64) ss = __builtin_fmaf(src[i], src[i], ss);
+    for (int d = 1; d < 64; d <<= 1) ss += __shfl_xor(ss, d);
+    const float inv = 1.0f / sqrtf(ss / (float)a.hd + n.eps);
+    auto get = [&](int i) { return normed ? src[i] * inv * gain[i] : src[i]; };
+    auto put = [&](int i, float v) {
+        if (h < a.heads) {
+            a.y[(size_t)r * a.y_stride + (size_t)h * a.hd + i] = v;
+        } else if constexpr (CACHE) {
+            const bool k = h < a.heads + a.kv_heads;
+            const int g = h - a.heads - (k ? 0 : a.kv_heads);
+            static_cast<KVT *>(k ? a.kc : a.vc)[((size_t)slot * a.kv_heads + g) * a.hd + i] = (KVT)v;
+        }
+    };
+    const int rot = normed ? a.rot : 0;
+    for (int p = lane; p < rot / 2; p += 64) {
+        const float2 cs = turn((double)pos * a.turns[p], a.gain, a.gain_lo);
+        const int ia = a.pairs ? 2 * p : p, ib = a.pairs ? ia + 1 : p + rot / 2;
+        const float xa = get(ia), xb = get(ib);
+        put(ia, __builtin_fmaf(xa, cs.x, -(xb * cs.y)));
+        put(ib, __builtin_fmaf(xb, cs.x, xa * cs.y));
+    }
+    for (int i = rot + lane; i < a.hd; i += 64) put(i, get(i));
+}
+
+template <typename KVT, bool CACHE>
+int launch_qk_norm(cw_ctx *ctx, const char *label, const RopeArgs &a, const NormArgs &n, bool wide,
+                   bool stream = false) {
+    const int heads = a.heads + (CACHE ? 2 * a.kv_heads : 0);
+    if (a.hd % 8 || a.rot % 8) {
+        constexpr int kHeads = kThreads / 64;
+        return launch(ctx, label, qk_norm_rope_any_kernel<KVT, CACHE>,
+                      dim3(a.rows, (heads + kHeads - 1) / kHeads), dim3(kThreads), 0, a, n);
+    }
+    int G = 1;
+    while (G < a.hd / 8) G <<= 1;
+    const int par = kThreads / G;
+    auto fn = wide ? (a.pairs ? qk_norm_rope_kernel<KVT, true, CACHE, true>
+                              : qk_norm_rope_kernel<KVT, false, CACHE, true>)
+                   : (a.pairs ? qk_norm_rope_kernel<KVT, true, CACHE, false>
+                              : qk_norm_rope_kernel<KVT, false, CACHE, false>);
+    if constexpr (!CACHE)
+        if (wide && stream)
+            fn = a.pairs ? qk_norm_rope_kernel<KVT, true, false, true, true>
+                         : qk_norm_rope_kernel<KVT, false, false, true, true>;
+    return launch(ctx, label, fn, dim3(a.rows, (heads + par - 1) / par), dim3(kThreads), 0, a, n, G);
 }
 
 // ---------------------------------------------------------------- block tables
@@ -526,6 +690,58 @@ void spec_gain(const cw_rope_spec &s, RopeArgs *a) {
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
+int check_norm(const char *what, const float *q_gain, int n_heads, const float *k_gain,
+               int n_kv_heads, float eps) {
+    CW_CHECK_ARG((q_gain || n_heads == 0) && (k_gain || n_kv_heads == 0),
+                 "%s: null gain of %d query and %d key heads", what, n_heads, n_kv_heads);
+    CW_CHECK_ARG(std::isfinite(eps) && eps >= 0.0f, "%s: eps=%g", what, (double)eps);
+    return CW_OK;
+}
+
+// Checks of rows of [q | k | v] that go to q_out and the cache; *a but for the
+// frequencies, and whether q's rows are 16-byte aligned.
+int check_kv_rows(const char *what, const cw_rope_spec *spec, const cw_kv_pages *kv,
+                  const float *qkv, size_t stride, const int *positions, const int *slots, int rows,
+                  int n_heads, float *q_out, size_t q_stride, RopeArgs *a, bool *wide) {
+    CW_CHECK_ARG(rows > 0 && rows <= kMaxRows && n_heads >= 0 && n_heads <= 4096,
+                 "%s: rows=%d (at most 2^23) n_heads=%d (4096)", what, rows, n_heads);
+    CW_CHECK_ARG((n_heads > 0) == (q_out != nullptr), "%s: q_out goes with n_heads=%d", what,
+                 n_heads);
+    PageMap map;
+    CW_TRY(check_pages(what, kv, nullptr, true, &map));
+    CW_TRY(check_spec(what, *spec, kv->head_dim));
+    const size_t q_width = (size_t)n_heads * kv->head_dim;
+    const size_t width = q_width + 2 * (size_t)kv->n_kv_heads * kv->head_dim;
+    CW_CHECK_ARG(stride >= width && stride < (1u << 31), "%s: stride %zu of rows of %zu floats",
+                 what, stride, width);
+    CW_CHECK_ARG(!n_heads || (q_stride >= q_width && q_stride < (1u << 31)),
+                 "%s: q_stride %zu of rows of %zu floats", what, q_stride, q_width);
+    const bool in_place = n_heads && q_out == qkv && q_stride == stride;
+    CW_CHECK_ARG(!n_heads || in_place ||
+                     rows_apart(rows, qkv, stride, width, q_out, q_stride, q_width),
+                 "%s: rows of qkv and q_out overlap", what);
+    spec_gain(*spec, a);
+    a->rot = spec->rot_dim;
+    a->pairs = spec->layout == CW_ROPE_PAIRS;
+    a->x = qkv;
+    a->x_stride = stride;
+    a->positions = positions;
+    a->slots = slots;
+    a->rows = rows;
+    a->heads = n_heads;
+    a->kv_heads = kv->n_kv_heads;
+    a->hd = kv->head_dim;
+    a->y = q_out;
+    a->y_stride = q_stride;
+    a->copy = !in_place && kv->head_dim > spec->rot_dim;
+    a->kc = kv->k;
+    a->vc = kv->v;
+    a->n_slots = kv->page * kv->n_blocks;
+    *wide = aligned16(qkv) && stride % 4 == 0 &&
+            (!n_heads || (aligned16(q_out) && q_stride % 4 == 0));
+    return CW_OK;
+}
+
 }  // namespace
 
 namespace cwi {
@@ -632,47 +848,79 @@ int cw_rope_kv_rows(cw_ctx *ctx, const cw_rope_spec *spec, const cw_kv_pages *kv
                     const float *qkv, size_t stride, const int *positions, const int *slots,
                     int rows, int n_heads, float *q_out, size_t q_stride) {
     CW_CHECK_ARG(ctx && spec && kv && qkv && positions && slots, "cw_rope_kv_rows: null argument");
-    CW_CHECK_ARG(rows > 0 && rows <= kMaxRows && n_heads >= 0 && n_heads <= 4096,
-                 "cw_rope_kv_rows: rows=%d (at most 2^23) n_heads=%d (4096)", rows, n_heads);
-    CW_CHECK_ARG((n_heads > 0) == (q_out != nullptr),
-                 "cw_rope_kv_rows: q_out goes with n_heads=%d", n_heads);
-    PageMap map;
-    CW_TRY(check_pages("cw_rope_kv_rows", kv, nullptr, true, &map));
-    CW_TRY(check_spec("cw_rope_kv_rows", *spec, kv->head_dim));
-    const size_t q_width = (size_t)n_heads * kv->head_dim;
-    const size_t width = q_width + 2 * (size_t)kv->n_kv_heads * kv->head_dim;
-    CW_CHECK_ARG(stride >= width && stride < (1u << 31), "cw_rope_kv_rows: stride %zu of rows of %zu floats",
-                 stride, width);
-    CW_CHECK_ARG(!n_heads || (q_stride >= q_width && q_stride < (1u << 31)),
-                 "cw_rope_kv_rows: q_stride %zu of rows of %zu floats", q_stride, q_width);
-    const bool in_place = n_heads && q_out == qkv && q_stride == stride;
-    CW_CHECK_ARG(!n_heads || in_place ||
-                     rows_apart(rows, qkv, stride, width, q_out, q_stride, q_width),
-                 "cw_rope_kv_rows: rows of qkv and q_out overlap");
+    RopeArgs a{};
+    bool wide = false;
+    CW_TRY(check_kv_rows("cw_rope_kv_rows", spec, kv, qkv, stride, positions, slots, rows, n_heads,
+                         q_out, q_stride, &a, &wide));
+    CW_HIP(hipSetDevice(ctx->device));
+    CW_TRY(ctx_rope_turns(ctx, "cw_rope_kv_rows", *spec, &a.turns));
+    wide = wide && a.rot % 8 == 0;
+    if (kv->kv_dtype == CW_F16) return launch_rope<_Float16, true>(ctx, "rope_kv_rows", a, wide);
+    return launch_rope<float, true>(ctx, "rope_kv_rows", a, wide);
+}
+
+int cw_qk_norm_rope_rows(cw_ctx *ctx, const cw_rope_spec *spec, const float *x, size_t x_stride,
+                         const float *q_gain, const float *k_gain, float eps, const int *positions,
+                         int rows, int n_heads, int n_kv_heads, int head_dim, float *y,
+                         size_t y_stride) {
+    CW_CHECK_ARG(ctx && spec && x && positions && y, "cw_qk_norm_rope_rows: null argument");
+    CW_CHECK_ARG(rows > 0 && rows <= kMaxRows && n_heads >= 0 && n_heads <= 4096 &&
+                     n_kv_heads >= 0 && n_kv_heads <= 4096 && n_heads + n_kv_heads > 0 &&
+                     head_dim > 0 && head_dim <= 256,
+                 "cw_qk_norm_rope_rows: rows=%d (at most 2^23) n_heads=%d n_kv_heads=%d (4096) "
+                 "head_dim=%d (256)",
+                 rows, n_heads, n_kv_heads, head_dim);
+    CW_TRY(check_norm("cw_qk_norm_rope_rows", q_gain, n_heads, k_gain, n_kv_heads, eps));
+    CW_TRY(check_spec("cw_qk_norm_rope_rows", *spec, head_dim));
+    const size_t width = (size_t)(n_heads + n_kv_heads) * head_dim;
+    CW_CHECK_ARG(x_stride >= width && y_stride >= width && x_stride < (1u << 31) &&
+                     y_stride < (1u << 31),
+                 "cw_qk_norm_rope_rows: strides %zu and %zu of rows of %zu floats", x_stride,
+                 y_stride, width);
+    const bool in_place = x == y && x_stride == y_stride;
+    CW_CHECK_ARG(in_place || rows_apart(rows, x, x_stride, width, y, y_stride, width),
+                 "cw_qk_norm_rope_rows: rows of x and y overlap");
     CW_HIP(hipSetDevice(ctx->device));
     RopeArgs a{};
-    CW_TRY(ctx_rope_turns(ctx, "cw_rope_kv_rows", *spec, &a.turns));
+    CW_TRY(ctx_rope_turns(ctx, "cw_qk_norm_rope_rows", *spec, &a.turns));
     spec_gain(*spec, &a);
     a.rot = spec->rot_dim;
     a.pairs = spec->layout == CW_ROPE_PAIRS;
-    a.x = qkv;
-    a.x_stride = stride;
+    a.x = x;
+    a.x_stride = x_stride;
     a.positions = positions;
-    a.slots = slots;
     a.rows = rows;
-    a.heads = n_heads;
-    a.kv_heads = kv->n_kv_heads;
-    a.hd = kv->head_dim;
-    a.y = q_out;
-    a.y_stride = q_stride;
-    a.copy = !in_place && kv->head_dim > spec->rot_dim;
-    a.kc = kv->k;
-    a.vc = kv->v;
-    a.n_slots = kv->page * kv->n_blocks;
-    const bool wide = aligned16(qkv) && stride % 4 == 0 && a.rot % 8 == 0 &&
-                      (!n_heads || (aligned16(q_out) && q_stride % 4 == 0));
-    if (kv->kv_dtype == CW_F16) return launch_rope<_Float16, true>(ctx, "rope_kv_rows", a, wide);
-    return launch_rope<float, true>(ctx, "rope_kv_rows", a, wide);
+    a.heads = n_heads + n_kv_heads;
+    a.hd = head_dim;
+    a.y = y;
+    a.y_stride = y_stride;
+    const bool wide = aligned16(x) && aligned16(y) && x_stride % 4 == 0 && y_stride % 4 == 0 &&
+                      aligned16(q_gain) && aligned16(k_gain);
+    // as in cw_rope_rows
+    const bool stream = (size_t)rows * width * sizeof(float) > (size_t)32 << 20;
+    return launch_qk_norm<float, false>(ctx, "qk_norm_rope_rows", a,
+                                        NormArgs{q_gain, k_gain, eps, n_heads}, wide, stream);
+}
+
+int cw_qk_norm_rope_kv_rows(cw_ctx *ctx, const cw_rope_spec *spec, const cw_kv_pages *kv,
+                            const float *qkv, size_t stride, const float *q_gain,
+                            const float *k_gain, float eps, const int *positions,
+                            const int *slots, int rows, int n_heads, float *q_out,
+                            size_t q_stride) {
+    CW_CHECK_ARG(ctx && spec && kv && qkv && positions && slots,
+                 "cw_qk_norm_rope_kv_rows: null argument");
+    RopeArgs a{};
+    bool wide = false;
+    CW_TRY(check_kv_rows("cw_qk_norm_rope_kv_rows", spec, kv, qkv, stride, positions, slots, rows,
+                         n_heads, q_out, q_stride, &a, &wide));
+    CW_TRY(check_norm("cw_qk_norm_rope_kv_rows", q_gain, n_heads, k_gain, kv->n_kv_heads, eps));
+    CW_HIP(hipSetDevice(ctx->device));
+    CW_TRY(ctx_rope_turns(ctx, "cw_qk_norm_rope_kv_rows", *spec, &a.turns));
+    wide = wide && aligned16(q_gain) && aligned16(k_gain);
+    const NormArgs n{q_gain, k_gain, eps, n_heads};
+    if (kv->kv_dtype == CW_F16)
+        return launch_qk_norm<_Float16, true>(ctx, "qk_norm_rope_kv_rows", a, n, wide);
+    return launch_qk_norm<float, true>(ctx, "qk_norm_rope_kv_rows", a, n, wide);
 }
 
 int cw_block_tables(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const int *fresh,

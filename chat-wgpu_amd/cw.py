@@ -79,6 +79,22 @@ class Batch(C.Structure):
                 ("max_blocks", _I), ("mask", _P), ("mask_words", _I)]
 
 
+NO_TOKEN = 0xffffffff
+
+
+class Moe(C.Structure):
+    _fields_ = [("dim", _I), ("hidden", _I), ("n_experts", _I), ("top_k", _I), ("normalise", _I),
+                ("router", _P), ("gate_scales", _P), ("up_scales", _P), ("down_scales", _P),
+                ("gate_quants", _P), ("up_quants", _P), ("down_quants", _P)]
+
+
+class LogitRules(C.Structure):
+    _fields_ = [("tokens", _P), ("length", _P), ("prompt", _P), ("max_len", _I),
+                ("node_token", _P), ("repeat", _P), ("presence", _P), ("frequency", _P),
+                ("bias_first", _P), ("bias_token", _P), ("bias", _P), ("n_bias", _I),
+                ("allowed", _P), ("n_allowed", _I), ("allowed_words", _I), ("allowed_row", _P)]
+
+
 # name -> (restype, argtypes); every declaration of include/chat_wgpu.h
 _SIGS = {
     "cw_ctx_create": (_I, [_I, C.POINTER(_P)]),
@@ -119,6 +135,13 @@ _SIGS = {
                              _P, _P, _P]),
     "cw_attention_tree": (_I, [_P, C.POINTER(KvPages), C.POINTER(Batch), _P, _SZ, _I, _P, _SZ]),
     "cw_kv_accept": (_I, [_P, C.POINTER(KvPages), C.POINTER(Batch), _P, _I, _P, _P]),
+    "cw_qk_norm_rope_rows": (_I, [_P, C.POINTER(RopeSpec), _P, _SZ, _P, _P, _F, _P, _I, _I, _I,
+                                  _I, _P, _SZ]),
+    "cw_qk_norm_rope_kv_rows": (_I, [_P, C.POINTER(RopeSpec), C.POINTER(KvPages), _P, _SZ, _P, _P,
+                                     _F, _P, _P, _I, _I, _P, _SZ]),
+    "cw_moe_rows": (_I, [_P, C.POINTER(Moe), _P, _I, _P, _P, _P, _P, _P]),
+    "cw_logits_rows": (_I, [_P, C.POINTER(LogitRules), C.POINTER(Batch), _P, _P, _SZ, _I, _I, _P,
+                            _SZ, _P, _P]),
     "cw_q4_quantize": (_I, [_P, _SZ, _SZ, _P, _P]),
     "cw_q4_split_blocks": (_I, [_P, _SZ, _P, _P]),
     "cw_synth_key": (_U64, [_U64, C.c_char_p]),
@@ -220,6 +243,24 @@ def batch(cached, n_seq, rows, first_row, tables, max_blocks, mask=None, mask_wo
     [n_seq, max_blocks] or None, mask [rows, mask_words] or None)."""
     return Batch(_opt(cached), n_seq, rows, _opt(first_row), _opt(tables), max_blocks,
                  _opt(mask), mask_words)
+
+
+def moe(dim, hidden, n_experts, top_k, router, gate_s, gate_q, up_s, up_q, down_s, down_q,
+        normalise=True):
+    """A mixture-of-experts layer over split Q4_0 experts (device arrays; scales
+    [n_experts, out, in / 32], quants [n_experts, out, in / 32, 16])."""
+    return Moe(dim, hidden, n_experts, top_k, int(bool(normalise)), router.ptr, gate_s.ptr, up_s.ptr,
+               down_s.ptr, gate_q.ptr, up_q.ptr, down_q.ptr)
+
+
+def logit_rules(tokens=None, length=None, prompt=None, max_len=0, node_token=None, repeat=None,
+                presence=None, frequency=None, bias_first=None, bias_token=None, bias=None, n_bias=0,
+                allowed=None, n_allowed=0, allowed_words=0, allowed_row=None):
+    """What a step's logits are under (device arrays or None; cw_logit_rules)."""
+    return LogitRules(_opt(tokens), _opt(length), _opt(prompt), max_len, _opt(node_token),
+                      _opt(repeat), _opt(presence), _opt(frequency), _opt(bias_first),
+                      _opt(bias_token), _opt(bias), n_bias, _opt(allowed), n_allowed, allowed_words,
+                      _opt(allowed_row))
 
 
 # ---------------------------------------------------------------- host-side helpers
@@ -569,6 +610,43 @@ class Context:
     def kv_accept(self, kv, batch, path, max_path, path_len, cached_out=None):
         check(lib().cw_kv_accept(self.h, kv, batch, path.ptr, max_path, path_len.ptr,
                                  _opt(cached_out)))
+
+    def qk_norm_rope_rows(self, spec, x, q_gain, k_gain, positions, rows, n_heads, n_kv_heads,
+                          head_dim, eps=1e-6, x_stride=None, y=None, y_stride=None):
+        width = (n_heads + n_kv_heads) * head_dim
+        y = y if y is not None else self.empty((rows, width))
+        check(lib().cw_qk_norm_rope_rows(self.h, spec, x.ptr, x_stride or width, _opt(q_gain),
+                                         _opt(k_gain), eps, positions.ptr, rows, n_heads,
+                                         n_kv_heads, head_dim, y.ptr, y_stride or width))
+        return y
+
+    def qk_norm_rope_kv_rows(self, spec, kv, qkv, q_gain, k_gain, positions, slots, rows, n_heads,
+                             eps=1e-6, stride=None, q_out=None, q_stride=None):
+        width = n_heads * kv.head_dim
+        if q_out is None and n_heads:
+            q_out = self.empty((rows, width))
+        check(lib().cw_qk_norm_rope_kv_rows(self.h, spec, kv, qkv.ptr,
+                                            stride or width + 2 * kv.n_kv_heads * kv.head_dim,
+                                            _opt(q_gain), _opt(k_gain), eps, positions.ptr,
+                                            slots.ptr, rows, n_heads, _opt(q_out),
+                                            q_stride or width))
+        return q_out
+
+    def moe_rows(self, moe, x, rows, residual=None, positions=None, y=None, experts=None,
+                 weights=None):
+        """experts, weights [rows, top_k] (int32, float32) are filled where given."""
+        y = y if y is not None else self.empty((rows, moe.dim))
+        check(lib().cw_moe_rows(self.h, moe, x.ptr, rows, _opt(positions), _opt(residual), y.ptr,
+                                _opt(experts), _opt(weights)))
+        return y
+
+    def logits_rows(self, rules, batch, logits, rows, vocab, at=None, stride=None, out=None,
+                    out_stride=None, token=None, logprob=None):
+        """Fills those of out, token (uint32, NO_TOKEN where nothing may follow)
+        and logprob that are given."""
+        check(lib().cw_logits_rows(self.h, rules, batch, _opt(at), logits.ptr, stride or vocab,
+                                   rows, vocab, _opt(out), out_stride or vocab, _opt(token),
+                                   _opt(logprob)))
 
     def graph_begin(self):
         """Record the following launches (cw_graph_begin)."""

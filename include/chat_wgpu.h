@@ -318,6 +318,94 @@ int cw_kv_accept(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const in
                  int max_path, const int *path_len, int *cached_out);
 
 /* ---------------------------------------------------------------- */
+/* The rest of such a step, from the q | k | v rows to the next tokens: */
+/* norms of query and key heads with the rotation, a mixture-of-experts */
+/* layer, the rules that a row's logits are under.  Device values are   */
+/* checked on the device as above.                                      */
+/* ---------------------------------------------------------------- */
+
+/* cw_rope_rows of normalised heads (norm.wgsl:20-42 for each head, as the
+ * reference's QK-norm before its RoPE, qwen3.rs:160-165): every head of n_heads
+ * query and then n_kv_heads key heads of a row becomes x * inverseSqrt(sum(x^2) /
+ * head_dim + eps) * gain, gain [head_dim] q_gain or k_gain, and is rotated.  The
+ * sum of a head's squares is f32 (heads of values past 2^56 may give zeros).
+ * Padding rows, overlaps and in-place use as in cw_rope_rows; n_heads or
+ * n_kv_heads may be 0 (its gain NULL). */
+int cw_qk_norm_rope_rows(cw_ctx *ctx, const cw_rope_spec *spec, const float *x, size_t x_stride,
+                         const float *q_gain, const float *k_gain, float eps, const int *positions,
+                         int rows, int n_heads, int n_kv_heads, int head_dim, float *y,
+                         size_t y_stride);
+/* The same with the cache write of cw_rope_kv_rows: q normalised and rotated
+ * into q_out, k normalised and rotated and v as it is into the cache row slots[r]. */
+int cw_qk_norm_rope_kv_rows(cw_ctx *ctx, const cw_rope_spec *spec, const cw_kv_pages *kv,
+                            const float *qkv, size_t stride, const float *q_gain,
+                            const float *k_gain, float eps, const int *positions,
+                            const int *slots, int rows, int n_heads, float *q_out,
+                            size_t q_stride);
+
+/* A layer of n_experts SwiGLU feed-forward networks of split Q4_0 matrices
+ * (scales and quants of all experts one behind the other), of which every row
+ * passes through the top_k that its router prefers. */
+typedef struct cw_moe {
+    int dim, hidden;       /* multiples of 32, at most 32768 */
+    int n_experts, top_k;  /* at most 512; at most 32 and n_experts */
+    int normalise;         /* 1: the top_k weights are divided by their sum */
+    const float *router;   /* [n_experts][dim], 16-byte aligned */
+    const uint16_t *gate_scales, *up_scales, *down_scales; /* [n_experts][out][in/32] */
+    const uint8_t *gate_quants, *up_quants;  /* [n_experts][hidden][dim/32][16], 16-byte aligned */
+    const uint8_t *down_quants;              /* [n_experts][dim][hidden/32][16] */
+} cw_moe;
+/* y[r] = [residual[r] +] sum of p_e * Wdown_e (silu(Wgate_e x[r]) * (Wup_e x[r]))
+ * over the top_k experts e of the largest router scores router[e] . x[r] (the
+ * lower index among equal ones), p their softmax over all experts.  Scores are
+ * f64, so that the choice does not hang on rounding; products are f32, as in
+ * cw_q4_gemm (block scales finite; x 16-byte aligned).  experts and weights
+ * [rows][top_k] receive the choice in order of score, and p (NULL: not wanted).
+ * positions (NULL: none): a row of a negative position is padding, neither read
+ * nor written.  y may be residual; it must not overlap x.  A row whose x is not
+ * finite gives NaN, and experts in range; other rows are not touched by it.
+ * rows at most 65536. */
+int cw_moe_rows(cw_ctx *ctx, const cw_moe *moe, const float *x, int rows, const int *positions,
+                const float *residual, float *y, int *experts, float *weights);
+
+/* What the logits of a step's rows are under; every pointer but rows of arrays
+ * that belong together may be NULL (no such rule).  Request b has the tokens
+ * tokens[b*max_len + i], i < length[b], the first prompt[b] of them its prompt's;
+ * with node_token row i of the request follows also the tokens of the nodes that
+ * it sees (cw_batch's mask, itself among them), which count as generated.  A
+ * token outside the vocabulary counts for nothing, a length outside 0 ..
+ * max_len as the nearer of the two. */
+typedef struct cw_logit_rules {
+    const int *tokens, *length, *prompt; /* [n_seq][max_len], [n_seq], [n_seq] (NULL: no prompt) */
+    int max_len;
+    const int *node_token;   /* [rows of the batch] */
+    const float *repeat;     /* [n_seq], positive: l / repeat (l > 0) or l * repeat of any token seen */
+    const float *presence;   /* [n_seq]: off l of a generated token */
+    const float *frequency;  /* [n_seq]: off l for each time that it was generated */
+    const int *bias_first;   /* [n_seq+1]: request b's biases are entries bias_first[b] .. [b+1]-1 */
+    const int *bias_token;   /* [n_bias]; of a token listed twice the last entry counts */
+    const float *bias;       /* [n_bias]: added to l */
+    int n_bias;
+    const uint32_t *allowed; /* [n_allowed][allowed_words]: bit v: token v may follow */
+    int n_allowed, allowed_words;
+    const int *allowed_row;  /* [rows of logits]: the row's mask, outside 0 .. n_allowed-1 none
+                                (NULL: row i's is i) */
+} cw_logit_rules;
+#define CW_NO_TOKEN 0xffffffffu
+/* Applies the rules to rows of logits, row i at logits + i*stride: of batch row
+ * at[i] (NULL: i).  In this order: repeat, frequency, presence, bias, -inf where
+ * not allowed, each rounded to f32.  out (NULL: not wanted; it may be logits with
+ * the same stride) receives them, token[i] the index of the largest (the lowest
+ * among equal ones; NaN is never it), logprob[i] its log softmax; where all are
+ * -inf or NaN CW_NO_TOKEN and -inf (NULL: not wanted).  Logits that are not
+ * allowed do not reach the others.  A row of no request is padding: nothing of it
+ * is written.  Of the batch first_row, n_seq, rows and the mask are used.  vocab
+ * at most 2^24, rows at most 65535. */
+int cw_logits_rows(cw_ctx *ctx, const cw_logit_rules *rules, const cw_batch *b, const int *at,
+                   const float *logits, size_t stride, int rows, int vocab, float *out,
+                   size_t out_stride, uint32_t *token, float *logprob);
+
+/* ---------------------------------------------------------------- */
 /* Host-side Q4 helpers                                              */
 /* ---------------------------------------------------------------- */
 
