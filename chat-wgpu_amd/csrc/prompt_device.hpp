@@ -1,5 +1,5 @@
 // Device code shared by the batched prompt phase's kernels (q4_gemm.hip,
-// prefill.hip).
+// prefill.hip) and the products of experts (moe.hip).
 
 #pragma once
 
@@ -9,6 +9,8 @@ namespace cwi {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kT = 256;
 
@@ -39,6 +41,34 @@ __device__ __forceinline__ auto sum_parts(int S, At at) {
     }
     return s < S ? add(v, at(s)) : v;
 }
+
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+constexpr float kUnscale = 0.0625f;  // the factor 16 of products with nibbles()
+
+// 4 quant bytes -> the B fragment of their 8 weights
+__device__ __forceinline__ f16x8 nibbles(uint32_t w) {
+    const f16x2 o1 = {(_Float16)1032.0f, (_Float16)1032.0f};
+    const f16x2 o16 = {(_Float16)1152.0f, (_Float16)1152.0f};
+    // v_and_or_b32 takes no literal: the masks in scalar registers, the exponents in
+    // a vector register, which the compiler, knowing their values, would not do (it
+    // takes an and and an or).  No instruction is written out: the compiler would not
+    // see that one writes a register in which a matrix product is still under way.
+    uint32_t m1 = 0x000F000Fu, m16 = 0x00F000F0u, one = 0x64006400u;
+    asm("" : "+s"(m1));
+    asm("" : "+s"(m16));
+    asm("" : "+v"(one));
+    const uint32_t h = w >> 8;
+    auto sub = [&](uint32_t v, uint32_t mask, f16x2 o) {
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, (v & mask) | one) - o);
+    };
+    return __builtin_bit_cast(f16x8, (u32x4){sub(w, m1, o1), sub(w, m16, o16), sub(h, m1, o1),
+                                             sub(h, m16, o16)});
+}
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
 

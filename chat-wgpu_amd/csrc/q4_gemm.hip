@@ -39,10 +39,6 @@ namespace {
 
 using namespace cwi;
 
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-constexpr float kUnscale = 0.0625f;  // the products' factor 16
 constexpr int kChain = 16;           // blocks per chain of f32 sums (a multiple of every stage)
 
 // ---------------------------------------------------------------------------
@@ -92,8 +88,6 @@ __device__ __forceinline__ float4 sum4(const float *p, int S, size_t stride) {
         return *reinterpret_cast<const float4 *>(p + (size_t)s * stride);
     });
 }
-
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
 // Scales whose rows are not whole groups of eight blocks (or whose address is
 // not a multiple of 16), copied to rows that are: the GEMM loads them a group
@@ -403,26 +397,6 @@ __device__ __forceinline__ void tile_of(int w, int total, int NT, int MT, int *m
     const int r = t / NT;
     *mt = r % MT;
     *sp = r / MT;
-}
-
-__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-// 4 quant bytes -> the B fragment of their 8 weights
-__device__ __forceinline__ f16x8 nibbles(uint32_t w) {
-    const f16x2 o1 = {(_Float16)1032.0f, (_Float16)1032.0f};
-    const f16x2 o16 = {(_Float16)1152.0f, (_Float16)1152.0f};
-    const uint32_t h = w >> 8;
-    // one v_and_or_b32: the compiler, which would need two literals for it,
-    // takes an and and an or
-    auto sub = [](uint32_t v, uint32_t mask, f16x2 o) {
-        uint32_t r;
-        asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(v), "s"(mask), "v"(0x64006400u));
-        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, r) - o);
-    };
-    return __builtin_bit_cast(f16x8, (u32x4){sub(w, 0x000F000Fu, o1), sub(w, 0x00F000F0u, o16),
-                                             sub(h, 0x000F000Fu, o1), sub(h, 0x00F000F0u, o16)});
 }
 
 // The row of y's columns that W tile column c belongs to, from the tile's

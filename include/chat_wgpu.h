@@ -361,8 +361,8 @@ typedef struct cw_moe {
  * f64, so that the choice does not hang on rounding; products are f32, as in
  * cw_q4_gemm (block scales finite; x 16-byte aligned).  experts and weights
  * [rows][top_k] receive the choice in order of score, and p (NULL: not wanted).
- * positions (NULL: none): a row of a negative position is padding, neither read
- * nor written.  y may be residual; it must not overlap x.  A row whose x is not
+ * positions (NULL: none): a row of a negative position is padding: what it holds
+ * does not count, and nothing of it is written.  y may be residual; it must not overlap x.  A row whose x is not
  * finite gives NaN, and experts in range; other rows are not touched by it.
  * rows at most 65536. */
 int cw_moe_rows(cw_ctx *ctx, const cw_moe *moe, const float *x, int rows, const int *positions,
