@@ -23,9 +23,9 @@ using namespace cwi;
 
 constexpr int kMaxExperts = 512, kMaxTop = 32;
 constexpr int kTile = 8;       // rows of one MFMA
-constexpr int kFew = kTile;    // rows that need no lists: every expert has one tile at most
+constexpr int kMaxSplits = 8;  // workgroups that share a score's sum
 constexpr int kChunk = 1024;   // rows that go through the layer together, at most
-constexpr size_t kChunkBytes = (size_t)1 << 30;  // of workspace, unless kFew rows need more
+constexpr size_t kChunkBytes = (size_t)1 << 30;  // of workspace, unless kTile rows need more
 
 struct MoeArgs {
     cw_moe m;
@@ -35,17 +35,16 @@ struct MoeArgs {
     float *y;
     int *experts;     // the caller's, or null
     float *weights;
-    double *score;    // [rows][n_experts]
+    double *score;    // [splits][rows][n_experts]
+    int splits;
     int *ids;         // [rows][top_k]; -1: a padding row's
     float *p;         // [rows][top_k]
-    uint8_t *ximg, *himg;    // images of x and of h: [row][block][hi | lo][group] x 16 B
+    uint8_t *ximg, *himg;    // images of x and of h: [row][block][group][hi | lo] x 16 B
     float *xscale, *hscale;
     float *h;         // [rows][top_k][hidden]
     float *z;         // [rows][top_k][dim]
-    // more than kFew rows: (row, choice) pairs by expert, and tiles of them
-    int *list;        // [rows * top_k]
-    int4 *tiles;      // expert, first of the list, count
-    int *n_tiles;
+    int *count;       // [n_experts]: pairs (row, choice) of each, and
+    int *list;        // [n_experts][rows]: those pairs, row * top_k + choice
 };
 
 __device__ __forceinline__ bool live(const MoeArgs &a, int r) {
@@ -102,9 +101,9 @@ __device__ void split_row(const float *x, int K, uint8_t *img, float *scale) {
         u32x4 hi, lo;
         split8(*reinterpret_cast<const float4 *>(x + at(c)),
                *reinterpret_cast<const float4 *>(x + at(c) + 16), sc, &hi, &lo);
-        uint8_t *o = img + (size_t)(c >> 2) * 128 + (c & 3) * 16;
-        *reinterpret_cast<u32x4 *>(o) = hi;
-        *reinterpret_cast<u32x4 *>(o + 64) = lo;
+        u32x4 *o = reinterpret_cast<u32x4 *>(img + (size_t)c * 32);
+        o[0] = hi;
+        o[1] = lo;
     }
 }
 
@@ -118,256 +117,332 @@ __device__ __forceinline__ bool ahead(double a, int i, double b, int j) {
 // as -inf they are chosen last.
 __device__ __forceinline__ double ranked(double s) { return s >= -INFINITY ? s : -INFINITY; }
 
-// Scores of at most R rows, a workgroup an expert (f64 products of f32 values are
-// exact, their sums are off by 2^-53 of the terms); the workgroups behind the
-// experts make the rows' images.
-template <int R>
-__global__ __launch_bounds__(256) void moe_score_few_kernel(MoeArgs a) {
-    __shared__ double red[4][R];
-    const int tid = threadIdx.x, dim = a.m.dim, E = a.m.n_experts;
-    const int e = blockIdx.x;
-    if (e >= E) {
-        const int r = e - E;
+// The scores of one row, a workgroup an expert (f64 products of f32 values are
+// exact, their sums are off by 2^-53 of the terms); the last workgroup makes the
+// row's image.  128 scores of 2,048: 2.7 us, where the matrix cores' 8 workgroups
+// would wait for 128 KB each.
+__global__ __launch_bounds__(256) void moe_score_row_kernel(MoeArgs a) {
+    __shared__ double red[4];
+    const int tid = threadIdx.x, dim = a.m.dim, e = blockIdx.x;
+    if (e == a.m.n_experts) {
+        split_row<256>(a.x, dim, a.ximg, a.xscale);
+        return;
+    }
+    double s = 0.0;
+    const float *w = a.m.router + (size_t)e * dim;
+#pragma unroll 2
+    for (int i = tid * 4; i < dim; i += 1024) {
+        const float4 v = *reinterpret_cast<const float4 *>(w + i);
+        const float4 x = *reinterpret_cast<const float4 *>(a.x + i);
+        s = fma((double)x.x, (double)v.x, s);
+        s = fma((double)x.y, (double)v.y, s);
+        s = fma((double)x.z, (double)v.z, s);
+        s = fma((double)x.w, (double)v.w, s);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+    if ((tid & 63) == 0) red[tid >> 6] = s;
+    __syncthreads();
+    if (tid == 0) a.score[e] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// A part of the sum of the scores of 16 rows and 16 experts a workgroup, on the f64
+// matrix cores, the waves sharing it out; then the rows' images.  The first clears
+// the experts' counts.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+__global__ __launch_bounds__(256) void moe_score_kernel(MoeArgs a) {
+    __shared__ double red[4][256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int dim = a.m.dim, E = a.m.n_experts;
+    const int et = (E + 15) / 16, rt = (a.rows + 15) / 16, tiles = et * rt;
+    int b = blockIdx.x;
+    if (b == 0)
+        for (int e = tid; e < E; e += 256) a.count[e] = 0;
+    if (b >= tiles * a.splits) {
+        const int r = b - tiles * a.splits;
         split_row<256>(a.x + (size_t)r * dim, dim, a.ximg + (size_t)r * dim * 4, a.xscale + r);
         return;
     }
-    double s[R] = {};
-    const float *w = a.m.router + (size_t)e * dim;
-    for (int i = tid * 4; i < dim; i += 1024) {
-        const float4 v = *reinterpret_cast<const float4 *>(w + i);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const float4 x = *reinterpret_cast<const float4 *>(a.x + (size_t)min(r, a.rows - 1) * dim + i);
-            s[r] = fma((double)x.x, (double)v.x, s[r]);
-            s[r] = fma((double)x.y, (double)v.y, s[r]);
-            s[r] = fma((double)x.z, (double)v.z, s[r]);
-            s[r] = fma((double)x.w, (double)v.w, s[r]);
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) s[r] += __shfl_xor(s[r], d);
-        if ((tid & 63) == 0) red[tid >> 6][r] = s[r];
-    }
-    __syncthreads();
-    if (tid < a.rows)
-        a.score[(size_t)tid * E + e] = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
-}
-
-// Scores of 16 rows and 16 experts a workgroup, on the f64 matrix cores, whose 16
-// waves split the sum; then the rows' images.
-typedef double f64x4 __attribute__((ext_vector_type(4)));
-__global__ __launch_bounds__(1024) void moe_score_kernel(MoeArgs a) {
-    __shared__ double red[16][256];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int dim = a.m.dim, E = a.m.n_experts;
-    const int et = (E + 15) / 16, rt = (a.rows + 15) / 16;
-    if ((int)blockIdx.x >= et * rt) {
-        const int r = blockIdx.x - et * rt;
-        split_row<1024>(a.x + (size_t)r * dim, dim, a.ximg + (size_t)r * dim * 4, a.xscale + r);
-        return;
-    }
-    const int e0 = blockIdx.x % et * 16, r0 = blockIdx.x / et * 16;
+    const int part = b / tiles;
+    b %= tiles;
+    const int e0 = b % et * 16, r0 = b / et * 16;
     const int li = lane & 15, lg = lane >> 4;
     const float *x = a.x + (size_t)min(r0 + li, a.rows - 1) * dim + 4 * lg;
     const float *w = a.m.router + (size_t)min(e0 + li, E - 1) * dim + 4 * lg;
     f64x4 acc = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll 4
-    for (int i = wave * 16; i < dim; i += 256) {
-        const float4 u = *reinterpret_cast<const float4 *>(x + i);
-        const float4 v = *reinterpret_cast<const float4 *>(w + i);
-        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u.x, (double)v.x, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u.y, (double)v.y, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u.z, (double)v.z, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u.w, (double)v.w, acc, 0, 0, 0);
+    const int by = a.splits * 64;
+    for (int i0 = (part * 4 + wave) * 16; i0 < dim; i0 += 4 * by) {
+        float4 u[4], v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = i0 + k * by < dim ? i0 + k * by : i0;
+            u[k] = *reinterpret_cast<const float4 *>(x + i);
+            v[k] = *reinterpret_cast<const float4 *>(w + i);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i0 + k * by >= dim) break;
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[k].x, (double)v[k].x, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[k].y, (double)v[k].y, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[k].z, (double)v[k].z, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[k].w, (double)v[k].w, acc, 0, 0, 0);
+        }
     }
     // D[4 r + lane / 16][lane % 16] in element r
 #pragma unroll
     for (int r = 0; r < 4; ++r) red[wave][(4 * r + lg) * 16 + li] = acc[r];
     __syncthreads();
-    if (tid >= 256) return;
-    double s = 0.0;
-#pragma unroll
-    for (int w16 = 0; w16 < 16; ++w16) s += red[w16][tid];
     const int r = r0 + (tid >> 4), e = e0 + (tid & 15);
-    if (r < a.rows && e < E) a.score[(size_t)r * E + e] = s;
+    if (r < a.rows && e < E)
+        a.score[((size_t)part * a.rows + r) * E + e] =
+            (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
 }
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double dpp_max(double v) {
-    const int2 o = __builtin_bit_cast(int2, v);
-    const int2 s = {__builtin_amdgcn_update_dpp(o.x, o.x, CTRL, ROWS, 0xf, false),
-                    __builtin_amdgcn_update_dpp(o.y, o.y, CTRL, ROWS, 0xf, false)};
-    return fmax(v, __builtin_bit_cast(double, s));
+// score[e] = row r's scores, by a workgroup of NT threads (not yet synchronised).
+template <int NT>
+__device__ __forceinline__ void load_scores(const MoeArgs &a, int r, double *score) {
+    const int E = a.m.n_experts;
+    for (int e = threadIdx.x; e < E; e += NT) {
+        double s = a.score[(size_t)r * E + e];
+        for (int i = 1; i < a.splits; ++i) s += a.score[((size_t)i * a.rows + r) * E + e];
+        score[e] = ranked(s);
+    }
 }
 
-// The largest of the lanes' values, in every lane.
-__device__ __forceinline__ double wave_max(double v) {
-    v = dpp_max<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
-    v = dpp_max<0x112, 0xf>(v);
-    v = dpp_max<0x114, 0xf>(v);
-    v = dpp_max<0x118, 0xf>(v);
-    v = dpp_max<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
-    v = dpp_max<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-    const int2 o = __builtin_bit_cast(int2, v);
-    return __builtin_bit_cast(double, int2{__builtin_amdgcn_readlane(o.x, 63),
-                                           __builtin_amdgcn_readlane(o.y, 63)});
+// f(expert, rank) for every expert, by `per` lanes each that count those ahead of
+// it (8 rounds of finding the largest of 128 took 10 us a row, this 0.3).
+template <int NT, typename F>
+__device__ __forceinline__ void ranks(const double *score, int E, F f) {
+    int per = 1;
+    while (per < 64 && 2 * per * E <= NT) per *= 2;
+    const int part = threadIdx.x % per;
+    for (int e0 = 0; e0 < E; e0 += NT / per) {
+        const int e = e0 + threadIdx.x / per;
+        const double mine = score[min(e, E - 1)];
+        int n = 0;
+#pragma unroll 8
+        for (int i = part; i < E; i += per) n += ahead(score[i], i, mine, e);
+        for (int d = 1; d < per; d <<= 1) n += __shfl_xor(n, d);
+        if (part == 0 && e < E) f(e, n);
+    }
 }
 
-// The choice of row r by one wave: ids, p and the caller's copies.
+// The choice of row r by a workgroup of NT threads: ids, p, the caller's copies,
+// and (LISTS) the experts' lists, whose order hangs on the atomics: which of a
+// tile's rows a pair becomes does not show in its result.
+template <int NT, bool LISTS>
 __device__ void choose(const MoeArgs &a, int r) {
-    constexpr int N = kMaxExperts / 64;
-    const int lane = threadIdx.x & 63, E = a.m.n_experts, K = a.m.top_k;
+    __shared__ double score[kMaxExperts], term[kMaxTop], part[NT / 64];
+    __shared__ int id[kMaxTop];
+    const int tid = threadIdx.x, E = a.m.n_experts, K = a.m.top_k;
     if (!live(a, r)) {
-        if (lane < K) a.ids[r * K + lane] = -1;
+        if (tid < K) a.ids[r * K + tid] = -1;
         return;
     }
-    const int n = (E + 63) / 64;
-    double v[N], most = -INFINITY;
+    load_scores<NT>(a, r, score);
+    __syncthreads();
+    ranks<NT>(score, E, [&](int e, int n) {
+        if (n < K) id[n] = e;
+    });
+    __syncthreads();
+    const double most = score[id[0]];
+    if (tid < K) term[tid] = exp(score[id[tid]] - most);
+    if (!a.m.normalise) {
+        double s = 0.0;
+        for (int e = tid; e < E; e += NT) s += exp(score[e] - most);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const int e = lane + 64 * j;
-        v[j] = j < n && e < E ? a.score[(size_t)r * E + e] : 0.0;
-        if (j < n && e < E) most = fmax(most, v[j]);
+        for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+        if ((tid & 63) == 0) part[tid >> 6] = s;
     }
-    most = wave_max(most);
-    double all = 0.0, sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        if (j >= n) break;
-        if (lane + 64 * j < E) all += exp(v[j] - most);
-        v[j] = ranked(v[j]);
-    }
-    for (int d = 32; d >= 1; d >>= 1) all += __shfl_xor(all, d);
-    unsigned taken = 0;
-    double mine = 0.0;
-    int id = 0;
-    for (int k = 0; k < K; ++k) {
-        double best = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j < n && lane + 64 * j < E && !(taken >> j & 1)) best = fmax(best, v[j]);
-        best = wave_max(best);
-        int at = E;
-#pragma unroll
-        for (int j = N - 1; j >= 0; --j) {
-            if (j >= n) continue;
-            const uint64_t m = __ballot(lane + 64 * j < E && !(taken >> j & 1) && v[j] == best);
-            if (m) at = 64 * j + __builtin_ctzll(m);
-        }
-        if (lane == (at & 63)) taken |= 1u << (at >> 6);
-        if (lane == k) {
-            mine = exp(best - most);
-            id = at;
-        }
-    }
-    for (int k = 0; k < K; ++k) sum += __shfl(mine, k);
-    if (lane >= K) return;
-    const float p = (float)(mine / (a.m.normalise ? sum : all));
-    a.ids[r * K + lane] = id;
-    a.p[r * K + lane] = p;
-    if (a.experts) a.experts[r * K + lane] = id;
-    if (a.weights) a.weights[r * K + lane] = p;
+    __syncthreads();
+    if (tid >= K) return;
+    double sum = 0.0;
+    if (a.m.normalise)
+        for (int k = 0; k < K; ++k) sum += term[k];
+    else
+        for (int w = 0; w < NT / 64; ++w) sum += part[w];
+    const int i = r * K + tid, e = id[tid];
+    const float p = (float)(term[tid] / sum);
+    a.ids[i] = e;
+    a.p[i] = p;
+    if (a.experts) a.experts[i] = e;
+    if (a.weights) a.weights[i] = p;
+    if constexpr (LISTS) a.list[(size_t)e * a.rows + atomicAdd(&a.count[e], 1)] = i;
 }
 
-// The pairs (row * top_k + choice) by expert and their tiles of `tile` pairs, by
-// one workgroup.  Which row of its tile a pair gets hangs on the order of LDS
-// atomics; its result does not.
-__device__ void sort_pairs(const MoeArgs &a, int tile) {
-    __shared__ int count[kMaxExperts], first[kMaxExperts];
-    const int tid = threadIdx.x, E = a.m.n_experts, P = a.rows * a.m.top_k;
-    for (int e = tid; e < E; e += blockDim.x) count[e] = 0;
-    __syncthreads();
-    for (int i = tid; i < P; i += blockDim.x)
-        if (a.ids[i] >= 0) atomicAdd(&count[a.ids[i]], 1);
-    __syncthreads();
-    if (tid < 64) {
-        constexpr int N = kMaxExperts / 64;
-        int pairs = 0, tiles = 0;
-        for (int j = 0; j < N; ++j) {
-            const int e = tid * N + j, c = e < E ? count[e] : 0;
-            pairs += c;
-            tiles += (c + tile - 1) / tile;
-        }
-        int p = pairs, t = tiles;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int op = __shfl_up(p, d), ot = __shfl_up(t, d);
-            if (tid >= d) {
-                p += op;
-                t += ot;
-            }
-        }
-        if (tid == 63) a.n_tiles[0] = t;
-        p -= pairs;
-        t -= tiles;
-        for (int j = 0; j < N; ++j) {
-            const int e = tid * N + j, c = e < E ? count[e] : 0;
-            if (e < E) first[e] = p;
-            for (int i = 0; i < c; i += tile) a.tiles[t++] = make_int4(e, p + i, min(tile, c - i), 0);
-            p += c;
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < P; i += blockDim.x)
-        if (a.ids[i] >= 0) a.list[atomicAdd(&first[a.ids[i]], 1)] = i;
-}
-
-__global__ __launch_bounds__(1024) void moe_choose_kernel(MoeArgs a, int tile, int sort) {
-    for (int r = blockIdx.x * 16 + (threadIdx.x >> 6); r < a.rows; r += gridDim.x * 16) choose(a, r);
-    if (!sort) return;
-    __syncthreads();
-    sort_pairs(a, tile);
-}
-
-__global__ __launch_bounds__(1024) void moe_sort_kernel(MoeArgs a, int tile) { sort_pairs(a, tile); }
+__global__ __launch_bounds__(256) void moe_choose_kernel(MoeArgs a) { choose<256, true>(a, blockIdx.x); }
 
 // ---------------------------------------------------------------- products
+//
+// A stage is 16 W rows of J groups of four blocks, brought into LDS by the wave that
+// takes it and by no other, so nothing but a wave's own wait count orders it.  Loads
+// straight into registers ask for 16 bytes of another row with every lane, and the
+// L1s, which take 64 bytes of neighbouring lanes a cycle, then bound everything (48
+// rows of 128 experts: 30 million accesses, 49 of 70 us).  In LDS quants lie as
+// [row][slot] x 16 B, two groups (a line of a row of W) or four blocks at a time, with
+// block b in slot b ^ row / 2 & 7 or b ^ row / 4 & 3, so that the reads of a word, four
+// bytes of each row's block, touch every bank once; then scales [row][2 J words].
+template <int J>
+struct Stage {
+    static constexpr int Q = J * 1024, BYTES = Q + (J > 2 ? 512 : 256);
+    static constexpr int DMAS = J + (J > 2 ? 2 : 1);
+    static constexpr int LINE = J % 2 ? 4 : 8;  // blocks of a row that lie together
+};
 
-// What a wave holds of one step of four blocks: CT tiles of 16 W rows, MT tiles of
-// eight x rows.
-template <int MT, int CT>
+// A lane's offsets: its rows and blocks of the DMAs, its words of the scales', and of
+// LDS the words of the blocks that it multiplies.
+template <int J>
+struct StageLane {
+    uint32_t q[2], s[2], at[Stage<J>::LINE], scale;
+    int block[2], word[2];
+};
+template <int J>
+__device__ __forceinline__ StageLane<J> stage_lane(int lane, int nb) {
+    constexpr int L = Stage<J>::LINE;
+    StageLane<J> l;
+    const int li = lane & 15, lg = lane >> 4;
+    // L = 8: DMAs of rows 0 .. 7 and 8 .. 15; 4: of all 16 rows, the second two unused
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int row = L == 8 ? 8 * k + (lane >> 3) : lane >> 2;
+        l.q[k] = (uint32_t)row * nb * 16;
+        l.block[k] = L == 8 ? (lane ^ row >> 1) & 7 : (lane ^ row >> 2) & 3;
+        const int i = min(lane + 64 * k, 32 * J - 1);
+        l.word[k] = i % (2 * J);
+        l.s[k] = (uint32_t)(i / (2 * J)) * nb * 2;
+    }
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+        l.at[i] = li * (16 * L) + (L == 8 ? (i ^ li >> 1) & 7 : (i ^ li >> 2) & 3) * 16 + lg * 4;
+    l.scale = Stage<J>::Q + li * 8 * J;
+    return l;
+}
+
+// DMAs from a base that is the same in every lane, wherever the compiler has it: it
+// may come straight from a vector instruction, which the assembler's hazard rules
+// want five wait states after (and M0 one).
+template <typename T>
+__device__ __forceinline__ const T *uniform(const T *p) {
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+    return reinterpret_cast<const T *>((uintptr_t)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ void dma16u(const void *base, uint32_t off, unsigned char *lds_dst) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(off), "s"(uniform(static_cast<const char *>(base))), "{m0}"(lds_off(lds_dst))
+                 : "memory");
+}
+// 4 bytes a lane, at lds_dst + 4 i
+__device__ __forceinline__ void dma4u(const void *base, uint32_t off, unsigned char *lds_dst) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1"
+                 :
+                 : "v"(off), "s"(uniform(static_cast<const char *>(base))), "{m0}"(lds_off(lds_dst))
+                 : "memory");
+}
+
+// Asks for a stage: q and s point at the first row's first block, of which groups
+// [0, jn) exist (those behind re-read the last).
+template <int J>
+__device__ __forceinline__ void issue_stage(const StageLane<J> &l, const uint8_t *q, const uint16_t *s,
+                                            int jn, unsigned char *buf) {
+    constexpr int L = Stage<J>::LINE;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int k = L == 8 ? j & 1 : 0, first = L == 8 ? j / 2 * 8 : j * 4;  // the line's first block
+        // (min: whole lines but for the row's last stage)
+        dma16u(q + 16 * min(first, 4 * jn - 4), l.q[k] + 16 * min(l.block[k], max(4 * jn - first, 4) - 1),
+               buf + j * 1024);
+    }
+#pragma unroll
+    for (int t = 0; t < (J > 2 ? 2 : 1); ++t)
+        dma4u(s, l.s[t] + 4 * min(l.word[t], 2 * jn - 1), buf + Stage<J>::Q + 256 * t);
+}
+
+// acc[m] += the stage times the x fragments x(m, block), which are 0 for blocks that
+// do not exist.  A block's products are scaled and added while the next one's run and
+// its weights are decoded; a group's words are read a group ahead.
+template <int J, int MT, typename X>
+__device__ __forceinline__ void multiply_stage(const StageLane<J> &l, const unsigned char *buf, X x,
+                                               f32x4 (&acc)[MT]) {
+    constexpr int L = Stage<J>::LINE;
+    uint32_t w[2][4];
+    uint2 d4[2];
+    auto read = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[j & 1][i] = *reinterpret_cast<const uint32_t *>(
+                buf + (L == 8 ? l.at[4 * (j & 1) + i] + j / 2 * 2048 : l.at[i] + j * 1024));
+        d4[j & 1] = *reinterpret_cast<const uint2 *>(buf + l.scale + 8 * j);
+    };
+    f32x4 t[2][MT];
+    auto add = [&](int k) {
+        const uint2 s = d4[k / 4 & 1];
+        const f16x2 d2 = __builtin_bit_cast(f16x2, k & 2 ? s.y : s.x);
+        const float d = (float)d2[k & 1];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[m][r] = __builtin_fmaf(d, t[k & 1][m][r], acc[m][r]);
+    };
+    f16x8 b[2];
+    read(0);
+    b[0] = nibbles(w[0][0]);
+#pragma unroll
+    for (int k = 0; k < 4 * J; ++k) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) t[k & 1][m] = mfma16(x(m, k), b[k & 1], f32x4{0.f, 0.f, 0.f, 0.f});
+        if (k + 1 < 4 * J) b[k + 1 & 1] = nibbles(w[(k + 1) / 4 & 1][(k + 1) & 3]);
+        if (k > 0) add(k - 1);
+        // (behind the last use of the scales that it replaces)
+        if (k % 4 == 0 && k / 4 + 1 < J) read(k / 4 + 1);
+        // (else all products come first, each in registers of its own)
+        __builtin_amdgcn_sched_group_barrier(0x008, MT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 9 + 4 * MT, 0);
+    }
+    add(4 * J - 1);
+    // the sums are wanted here (the compiler would put them off to the next stage, and
+    // keep every product until then)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+        asm volatile("" : "+v"(acc[m][0]), "+v"(acc[m][1]), "+v"(acc[m][2]), "+v"(acc[m][3]));
+}
+
+// Rows that are no whole groups of four blocks, or whose scales are not 8-byte
+// aligned: a lane of the 16 x 4 (W row, k group) loads block 4 s + group of its row,
+// and the lane groups hand each other their words (two swaps of lane halves, two of
+// rows of 16).
+template <int MT>
 struct Step {
-    u32x4 q[CT], x[MT][4];
-    uint2 d[CT];
+    u32x4 q[4], x[MT][4];
+    uint2 d[4];
 };
-
-// A wave's operands: uniform bases and the lane's offsets into them.
-template <int MT, int CT>
 struct Operands {
-    const uint8_t *q[CT];   // the tile's first W row
-    const uint16_t *d[CT];
-    const uint8_t *x;
-    uint32_t row;           // the lane's W row of a tile
-    size_t xo[MT];
-    int nb, lg;
+    const uint8_t *q[4];   // the column tiles' first W rows
+    const uint16_t *d[4];
 };
 
-// WHOLE: rows are whole steps, and their scales 8-byte aligned.  Else blocks past
-// the row's end re-read its last under a scale of 0.
-template <int MT, int CT, bool WHOLE>
-__device__ __forceinline__ void load_step(const Operands<MT, CT> &o, int s, Step<MT, CT> &f) {
-    const int b = WHOLE ? 4 * s + o.lg : min(4 * s + o.lg, o.nb - 1);
+template <int MT>
+__device__ __forceinline__ void load_step(const Operands &o, const uint8_t *img, const size_t (&xo)[MT],
+                                          int nb, int s, Step<MT> &f) {
+    const int lane = threadIdx.x & 63, row = lane & 15, lg = lane >> 4;
+    const int b = min(4 * s + lg, nb - 1);
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        f.q[c] = __builtin_nontemporal_load(
-            reinterpret_cast<const u32x4 *>(o.q[c] + (o.row * o.nb + b) * 16u));
-        const uint16_t *d = o.d[c] + o.row * o.nb + 4 * s;
-        if constexpr (WHOLE) {
-            f.d[c] = *reinterpret_cast<const uint2 *>(d);
-        } else {
-            uint32_t v[4];
+    for (int c = 0; c < 4; ++c) {
+        f.q[c] = *reinterpret_cast<const u32x4 *>(o.q[c] + (uint32_t)(row * nb + b) * 16);
+        const uint16_t *d = o.d[c] + row * nb + 4 * s;
+        uint32_t v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = 4 * s + i < o.nb ? d[i] : 0;
-            f.d[c] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
-        }
+        for (int i = 0; i < 4; ++i) v[i] = 4 * s + i < nb ? d[i] : 0;
+        f.d[c] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            f.x[m][i] = *reinterpret_cast<const u32x4 *>(
-                o.x + o.xo[m] + (size_t)(WHOLE ? 4 * s + i : min(4 * s + i, o.nb - 1)) * 128);
+            f.x[m][i] = *reinterpret_cast<const u32x4 *>(img + xo[m] +
+                                                         (size_t)min(4 * s + i, nb - 1) * 128);
 }
 
 // Word w of the lane groups' blocks -> block i of word `group`.
@@ -379,10 +454,10 @@ __device__ __forceinline__ u32x4 exchange(u32x4 q) {
     return u32x4{c[0], d[0], c[1], d[1]};
 }
 
-template <int MT, int CT>
-__device__ __forceinline__ void multiply(const Step<MT, CT> &f, f32x4 (&acc)[MT][CT]) {
+template <int MT>
+__device__ __forceinline__ void multiply_step(const Step<MT> &f, f32x4 (&acc)[4][MT]) {
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
+    for (int c = 0; c < 4; ++c) {
         const u32x4 w = exchange(f.q[c]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -393,265 +468,258 @@ __device__ __forceinline__ void multiply(const Step<MT, CT> &f, f32x4 (&acc)[MT]
             for (int m = 0; m < MT; ++m) {
                 const f32x4 t = mfma16(__builtin_bit_cast(f16x8, f.x[m][i]), b, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[m][c][r] = __builtin_fmaf(d, t[r], acc[m][c][r]);
+                for (int r = 0; r < 4; ++r) acc[c][m][r] = __builtin_fmaf(d, t[r], acc[c][m][r]);
             }
         }
     }
 }
 
-// acc += the products of steps s, s + by, ... of the row's n: two steps' loads in
-// flight.
-template <int MT, int CT, bool WHOLE>
-__device__ __forceinline__ void products(const Operands<MT, CT> &o, int s, int by, int n,
-                                         f32x4 (&acc)[MT][CT]) {
+// acc += the products of steps s, s + by, ...: two steps' loads in flight.
+template <int MT>
+__device__ __forceinline__ void multiply_steps(const Operands &o, const uint8_t *img,
+                                               const size_t (&xo)[MT], int nb, int s, int by,
+                                               f32x4 (&acc)[4][MT]) {
+    const int n = (nb + 3) / 4;
     if (s >= n) return;
-    Step<MT, CT> f[2];
-    load_step<MT, CT, WHOLE>(o, s, f[0]);
+    Step<MT> f[2];
+    load_step<MT>(o, img, xo, nb, s, f[0]);
     for (;; s += 2 * by) {
-        load_step<MT, CT, WHOLE>(o, min(s + by, n - 1), f[1]);
-        multiply<MT, CT>(f[0], acc);
+        load_step<MT>(o, img, xo, nb, min(s + by, n - 1), f[1]);
+        multiply_step<MT>(f[0], acc);
         if (s + by >= n) break;
-        load_step<MT, CT, WHOLE>(o, min(s + 2 * by, n - 1), f[0]);
-        multiply<MT, CT>(f[1], acc);
+        load_step<MT>(o, img, xo, nb, min(s + 2 * by, n - 1), f[0]);
+        multiply_step<MT>(f[1], acc);
         if (s + 2 * by >= n) break;
     }
 }
 
-// ---------------------------------------------------------------- few rows
-//
-// Three launches and no lists.  A workgroup of the first product has one choice
-// (row, rank) and 16 columns of h; it finds the expert from the scores, and whether
-// another row chose it too: the first such row's workgroups compute all of them.
+// ---------------------------------------------------------------- tiles of pairs
 
-constexpr int kFewThreads = 512, kFewWaves = kFewThreads / 64;
+constexpr int kThreads = 256, kWaves = 4;
 
-template <bool WHOLE>
-__global__ __launch_bounds__(kFewThreads) void moe_up_few_kernel(MoeArgs a) {
-    extern __shared__ double score[];  // [rows][n_experts]
-    __shared__ f32x4 red[kFewWaves][2][64];
-    __shared__ int chosen, rank_of[kFew];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int E = a.m.n_experts, K = a.m.top_k, hidden = a.m.hidden;
-    if ((int)blockIdx.x < a.rows) {
-        if (wave == 0) choose(a, blockIdx.x);
-        return;
-    }
-    const int cols = hidden / 16, slot = (blockIdx.x - a.rows) / cols;
-    const int col = (blockIdx.x - a.rows) % cols * 16;
-    const int row = slot / K, k = slot % K;
-    if (!live(a, row)) return;
-    for (int i = tid; i < a.rows * E; i += kFewThreads) score[i] = ranked(a.score[i]);
-    __syncthreads();
-    // the expert of rank k: `per` lanes count those ahead of one
-    int per = 1;
-    while (per < 64 && 2 * per * E <= kFewThreads) per *= 2;
-    {
-        const double *s = score + row * E;
-        const int e = tid / per;
-        const double mine = e < E ? s[e] : 0.0;
-        int n = 0;
-        for (int i = tid % per; i < E; i += per) n += ahead(s[i], i, mine, e);
-        for (int d = 1; d < per; d <<= 1) n += __shfl_xor(n, d);
-        if (e < E && n == k) chosen = e;
-    }
-    __syncthreads();
-    const int e = chosen;
-    if (wave < kFew) {
-        int n = K;
-        if (wave < a.rows && live(a, wave)) {
-            const double *s = score + wave * E, mine = s[e];
-            n = 0;
-            for (int i = 0; i < E; i += 64)
-                n += __popcll(__ballot(i + lane < E && ahead(s[min(i + lane, E - 1)], i + lane, mine, e)));
-        }
-        if (lane == 0) rank_of[wave] = n;
-    }
-    __syncthreads();
-    for (int r = 0; r < row; ++r)
-        if (rank_of[r] < K) return;
-    const int li = lane & 15, lg = lane >> 4, nb = a.m.dim / 32;
-    const size_t w0 = ((size_t)e * hidden + col) * nb;
-    Operands<1, 2> o;
-    o.q[0] = a.m.gate_quants + w0 * 16;
-    o.q[1] = a.m.up_quants + w0 * 16;
-    o.d[0] = a.m.gate_scales + w0;
-    o.d[1] = a.m.up_scales + w0;
-    o.x = a.ximg;
-    o.row = li;
-    const int xr = rank_of[li & 7] < K ? li & 7 : row;
-    o.xo[0] = (size_t)xr * nb * 128 + (li >> 3) * 64 + lg * 16;
-    o.nb = nb;
-    o.lg = lg;
-    f32x4 acc[1][2] = {};
-    products<1, 2, WHOLE>(o, wave, kFewWaves, (nb + 3) / 4, acc);
-    red[wave][0][lane] = acc[0][0];
-    red[wave][1][lane] = acc[0][1];
-    __syncthreads();
-    // row m of x, column n: element m % 4 of lanes 16 (m / 4) + n (hi) and 32 more (lo)
-    const int m = tid >> 4, n = tid & 15;
-    if (m >= a.rows || rank_of[m] >= K) return;
-    const int from = (m >> 2) * 16 + n;
-    float g = 0.0f, u = 0.0f;
+// Tile b of `tile` pairs of one expert, counted over the experts: every wave finds
+// it from the counts (lane i has experts i * per ..), which costs it a load and a
+// scan instead of a launch that lists the tiles.  n = 0: there are fewer.
+struct Tile {
+    int e, n;
+    const int *list;
+};
+__device__ __forceinline__ Tile find_tile(const MoeArgs &a, int tile, int b) {
+    constexpr int N = kMaxExperts / 64;
+    const int lane = threadIdx.x & 63, E = a.m.n_experts, per = (E + 63) / 64;
+    int c[N], mine = 0;
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) {
-        g += red[w][0][from][m & 3] + red[w][0][from + 32][m & 3];
-        u += red[w][1][from][m & 3] + red[w][1][from + 32][m & 3];
+    for (int j = 0; j < N; ++j) {
+        c[j] = j < per && lane * per + j < E ? a.count[lane * per + j] : 0;
+        mine += (c[j] + tile - 1) / tile;
     }
-    const float sc = kUnscale * a.xscale[m];
-    a.h[((size_t)m * K + rank_of[m]) * hidden + col + n] = silu_mul(g * sc, u * sc);
+    int to = mine;
+#define CW_SCAN_STEP(ctrl, rows) to += __builtin_amdgcn_update_dpp(0, to, ctrl, rows, 0xf, true)
+    CW_SCAN_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8
+    CW_SCAN_STEP(0x112, 0xf);
+    CW_SCAN_STEP(0x114, 0xf);
+    CW_SCAN_STEP(0x118, 0xf);
+    CW_SCAN_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+    CW_SCAN_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef CW_SCAN_STEP
+    const uint64_t has = __ballot(to > b);
+    if (!has) return Tile{0, 0, nullptr};
+    const int owner = __builtin_ctzll(has);
+    int e = lane * per, left = b - (to - mine), n = 0;  // (of the owner's lane)
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int t = (c[j] + tile - 1) / tile;
+        if (!found && left < t) {
+            found = true;
+            e = lane * per + j;
+            n = c[j];
+        } else if (!found) {
+            left -= t;
+        }
+    }
+    e = __builtin_amdgcn_readlane(e, owner);
+    left = __builtin_amdgcn_readlane(left, owner);
+    n = __builtin_amdgcn_readlane(n, owner);
+    return Tile{e, min(tile, n - left * tile), a.list + (size_t)e * a.rows + left * tile};
 }
 
-// A workgroup has 16 columns of a row's y; its waves share the experts out, or
-// parts of them where there are fewer.  A wave splits its stretch of h itself, 32
-// blocks at a time under their own power of two, while their W is on its way.
-template <bool WHOLE>
-__global__ __launch_bounds__(kFewThreads) void moe_down_few_kernel(MoeArgs a) {
-    constexpr int S = 8;  // steps at a time
-    __shared__ u32x4 img[kFewWaves][S * 4 * 8];
-    __shared__ float red[kMaxTop][16];
+// A tile's pair i, its last again past the end
+__device__ __forceinline__ int pair_of(const Tile &t, int i) { return t.list[min(i, t.n - 1)]; }
+
+// A tile of pairs times a stretch of its expert's columns: of h (UP: 32 gate and the
+// same 32 up columns a set) or of z (64 columns a set).  ks waves split the sum, the
+// others take other sets.  J groups of blocks of x stay in registers per wave, MT
+// tiles of eight rows; W goes through a ring of stages (J = 0: steps of any row
+// length, through registers).  (Workgroups that take several sets one after the
+// other, asking ahead, gain nothing: 48 rows 46.4 us with one set, 45.7 with two,
+// 47.1 with three.)
+template <bool UP, int MT, int J>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(MT == 1 ? 4 : 2, MT == 1 ? 4 : 2)))
+void moe_tile_kernel(MoeArgs a, int ks) {
+    // stages of SJ groups, R of them in LDS for each wave: as many workgroups on a CU as
+    // the registers allow
+    constexpr int SJ = J == 3 ? 3 : 2, SUBS = J / SJ, R = J == 4 ? 3 : MT == 1 ? 2 : 3;
+    __shared__ __attribute__((aligned(1024))) unsigned char ring[J ? kWaves * R * Stage<SJ>::BYTES : 16];
+    __shared__ float4 red[kWaves - 1][64];
+    __shared__ int pairs[8 * MT];
+    __shared__ float scales[8 * MT];
+    const Tile tile = find_tile(a, kTile * MT, blockIdx.y);
+    if (tile.n == 0) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
-    const int K = a.m.top_k, hidden = a.m.hidden, dim = a.m.dim, nb = hidden / 32;
-    const int r = blockIdx.y, col = blockIdx.x * 16;
-    if (!live(a, r)) return;
-    const int parts = K < kFewWaves ? kFewWaves / K : 1, steps = (nb + 3) / 4;
-    const int per = (steps + parts - 1) / parts;
-    for (int u = wave; u < K * parts; u += kFewWaves) {
-        const int j = u / parts, s0 = u % parts * per, s1 = min(steps, s0 + per);
-        const int pair = r * K + j, e = a.ids[pair];
-        const float *h = a.h + (size_t)pair * hidden;
-        const size_t w0 = ((size_t)e * dim + col) * nb;
-        float total = 0.0f;
-        for (int s = s0; s < s1; s += S) {
-            u32x4 q[S];
-            uint2 d[S];
+    const int K = a.m.top_k, N = UP ? a.m.hidden : a.m.dim, nb = (UP ? a.m.dim : a.m.hidden) / 32;
+    const int cs = kWaves / ks, sets = UP ? N / 32 : (N + 63) / 64;
+    const int set = blockIdx.x * cs + wave / ks;  // (past the last: the last again, not stored)
+    const uint8_t *const img = UP ? a.ximg : a.himg;
+
+    auto w_tile = [&](int c, const uint8_t **q, const uint16_t **d) {
+        const int at = min(set, sets - 1), col = UP ? at * 32 + (c & 1) * 16 : min(at * 64 + c * 16, N - 16);
+        const size_t w0 = ((size_t)tile.e * N + col) * nb;
+        *q = (!UP ? a.m.down_quants : c < 2 ? a.m.gate_quants : a.m.up_quants) + w0 * 16;
+        *d = (!UP ? a.m.down_scales : c < 2 ? a.m.gate_scales : a.m.up_scales) + w0;
+    };
+
+    using S = Stage<SJ>;
+    constexpr int JX = J ? J : SJ;  // groups of blocks of a wave's slice of x
+    unsigned char *const mine = ring + wave * R * S::BYTES;
+    const StageLane<SJ> l = stage_lane<SJ>(lane, nb);
+    const int slices = (nb + 4 * JX - 1) / (4 * JX), rounds = (slices + ks - 1) / ks;
+    const int total = rounds * 4 * (J ? SUBS : 1);
+    // the wave's first group of blocks in a round (a wave without any goes through the
+    // row's last ones with no x)
+    auto group = [&](int t) { return min(t * ks + wave % ks, slices - 1) * JX; };
+    int it = 0, ic = 0, isub = 0, ibuf = 0;  // of the next stage to ask for
+    auto issue = [&] {
+        const uint8_t *q;
+        const uint16_t *d;
+        w_tile(ic, &q, &d);
+        // (past the row's end its last group again)
+        const int b = min(group(it) + isub * SJ, nb / 4 - 1), n = min(SJ, nb / 4 - b);
+        issue_stage<SJ>(l, q + (size_t)b * 64, d + 4 * b, n, mine + ibuf * S::BYTES);
+        ibuf = ibuf + 1 == R ? 0 : ibuf + 1;
+        if (++isub == SUBS) {
+            isub = 0;
+            if (++ic == 4) {
+                ic = 0;
+                ++it;
+            }
+        }
+    };
+    // x rows 8 m + li / 2 of the tile, hi or lo (rows past its end read nothing)
+    size_t xo[MT];
+    bool have[MT];
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const int st = min(s + i, s1 - 1), b = min(4 * st + lg, nb - 1);
-                q[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(
-                    a.m.down_quants + (w0 + (uint32_t)(li * nb + b)) * 16));
-                const uint16_t *p = a.m.down_scales + w0 + (uint32_t)(li * nb + 4 * st);
-                if constexpr (WHOLE) {
-                    d[i] = *reinterpret_cast<const uint2 *>(p);
-                } else {
-                    uint32_t v[4];
+    for (int m = 0; m < MT; ++m) {
+        have[m] = 8 * m + (li >> 1) < tile.n;
+        const int i = pair_of(tile, 8 * m + (li >> 1));
+        xo[m] = (size_t)(UP ? i / K : i) * nb * 128 + lg * 32 + (li & 1) * 16;
+    }
+
+    // The set's sums from the waves that share it, two column tiles (of h: a gate and
+    // its up tile) at a time; a lane has column li of x rows 2 lg and 2 lg + 1, hi + lo.
+    auto store = [&](const f32x4 (&acc)[4][MT]) {
+        const int part = wave % ks;
+        if (ks == 1) lds_barrier();  // (pairs and scales)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) v[t] = 4 * st + t < nb ? p[t] : 0;
-                    d[i] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const f32x4 a0 = acc[UP ? half : 2 * half][m], a1 = acc[UP ? half + 2 : 2 * half + 1][m];
+                float v[2][2] = {{a0[0] + a0[1], a0[2] + a0[3]}, {a1[0] + a1[1], a1[2] + a1[3]}};
+                if (ks > 1) {
+                    lds_barrier();  // the last reads of red
+                    if (part) red[wave / ks * (ks - 1) + part - 1][lane] = make_float4(v[0][0], v[0][1], v[1][0], v[1][1]);
+                    lds_barrier();
                 }
-            }
-            float4 ve[2], vf[2];
-            float mx = 0.0f;
+                if (part || set >= sets) continue;
+                for (int w = 0; w < ks - 1; ++w) {
+                    const float4 o = red[wave / ks * (ks - 1) + w][lane];
+                    v[0][0] += o.x;
+                    v[0][1] += o.y;
+                    v[1][0] += o.z;
+                    v[1][1] += o.w;
+                }
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int c = lane + 64 * t, b = min(4 * s + (c >> 2), nb - 1);
-                const float *x = h + 32 * b + 4 * (c & 3);
-                ve[t] = *reinterpret_cast<const float4 *>(x);
-                vf[t] = *reinterpret_cast<const float4 *>(x + 16);
-                mx = fmaxf(mx, max8(ve[t], vf[t]));
-            }
-#pragma unroll
-            for (int dd = 32; dd >= 1; dd >>= 1) mx = fmaxf(mx, __shfl_xor(mx, dd));
-            const int ex = split_exponent(mx);
-            const float sc = ldexpf(1.0f, -ex);
-            __builtin_amdgcn_wave_barrier();  // the reads of the last stretch
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int c = lane + 64 * t;
-                u32x4 hi, lo;
-                split8(ve[t], vf[t], sc, &hi, &lo);
-                img[wave][(c >> 2) * 8 + (c & 3)] = hi;
-                img[wave][(c >> 2) * 8 + 4 + (c & 3)] = lo;
-            }
-            __builtin_amdgcn_wave_barrier();
-            float acc = 0.0f;
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                if (s + i < s1) {
-                    const u32x4 w = exchange(q[i]);
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        // rows 0 .. 7 of the fragment are h's hi, 8 .. 15 its lo
-                        const u32x4 x = img[wave][(4 * i + t) * 8 + (li >> 3) * 4 + lg];
-                        const f32x4 v = mfma16(__builtin_bit_cast(f16x8, x), nibbles(w[t]),
-                                               f32x4{0.f, 0.f, 0.f, 0.f});
-                        const f16x2 d2 = __builtin_bit_cast(f16x2, t < 2 ? d[i].x : d[i].y);
-                        acc = __builtin_fmaf((float)d2[t & 1], v[0], acc);
+                for (int q = 0; q < 2; ++q) {
+                    const int i = 8 * m + 2 * lg + q;
+                    if (i >= tile.n) continue;
+                    const size_t at = (size_t)pairs[i] * N;
+                    const float sc = scales[i];
+                    if constexpr (UP) {
+                        a.h[at + set * 32 + half * 16 + li] = silu_mul(v[0][q] * sc, v[1][q] * sc);
+                    } else {
+                        const int col = set * 64 + half * 32 + li;
+                        if (col < N) a.z[at + col] = v[0][q] * sc;
+                        if (col + 16 < N) a.z[at + col + 16] = v[1][q] * sc;
                     }
                 }
             }
-            total = __builtin_fmaf(kUnscale * ldexpf(1.0f, ex), acc, total);
-        }
-        total += __shfl_xor(total, 32);
-        if (lane < 16) red[u][li] = a.p[pair] * total;
-    }
-    __syncthreads();
-    if (tid >= 16) return;
-    float y = 0.0f;
-    for (int u = 0; u < K * parts; ++u) y += red[u][tid];
-    const size_t at = (size_t)r * dim + col + tid;
-    a.y[at] = a.residual ? a.residual[at] + y : y;
-}
+    };
 
-// ---------------------------------------------------------------- more rows
-
-constexpr int kTileThreads = 256, kTileWaves = 4;
-
-// The lane's x rows of a tile: pairs of the list, the last one again past its end.
-__device__ __forceinline__ int pair_of(const MoeArgs &a, int4 tile, int i) {
-    return a.list[tile.y + min(i, tile.z - 1)];
-}
-
-// 32 columns of h of a tile of pairs; the waves split dim.
-template <int MT, bool WHOLE>
-__global__ __launch_bounds__(kTileThreads) void moe_up_tile_kernel(MoeArgs a) {
-    __shared__ f32x4 red[kTileWaves][4][64];
-    if ((int)blockIdx.y >= a.n_tiles[0]) return;
-    const int4 tile = a.tiles[blockIdx.y];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int li = lane & 15, lg = lane >> 4;
-    const int hidden = a.m.hidden, nb = a.m.dim / 32, col = blockIdx.x * 32;
-    const int e = __builtin_amdgcn_readfirstlane(tile.x);
-    Operands<MT, 4> o;
+    const int my_pair = pair_of(tile, min(tid, 8 * MT - 1));
+    const float my_scale = kUnscale * (UP ? a.xscale[my_pair / K] : a.p[my_pair] * a.hscale[my_pair]);
+    auto put_scales = [&] {
+        if (tid >= 8 * MT) return;
+        pairs[tid] = my_pair;
+        scales[tid] = my_scale;
+    };
+    f32x4 acc[4][MT] = {};
+    if constexpr (J == 0) {
+        Operands o;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const size_t w0 = ((size_t)e * hidden + col + (c & 1) * 16) * nb;
-        o.q[c] = (c < 2 ? a.m.gate_quants : a.m.up_quants) + w0 * 16;
-        o.d[c] = (c < 2 ? a.m.gate_scales : a.m.up_scales) + w0;
-    }
-    o.x = a.ximg;
-    o.row = li;
-    o.nb = nb;
-    o.lg = lg;
+        for (int c = 0; c < 4; ++c) w_tile(c, &o.q[c], &o.d[c]);
+        multiply_steps<MT>(o, img, xo, nb, wave % ks, ks, acc);
+        put_scales();
+    } else {
+        int left = total, buf = 0;
+        u32x4 x[MT][4 * J];
+        for (int t = 0; t < rounds; ++t) {
+            const int b = group(t) * 4, n = t * ks + wave % ks < slices ? min(4 * J, nb - b) : 0;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int r = pair_of(a, tile, 8 * m + (li & 7)) / a.m.top_k;
-        o.xo[m] = (size_t)r * nb * 128 + (li >> 3) * 64 + lg * 16;
-    }
-    f32x4 acc[MT][4] = {};
-    products<MT, 4, WHOLE>(o, wave, kTileWaves, (nb + 3) / 4, acc);
-    const int i = tid >> 5, n = tid & 31, from = (i >> 2) * 16 + (n & 15);
+            for (int m = 0; m < MT; ++m) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        if (m) __syncthreads();
+                for (int i = 0; i < 4 * J; ++i) x[m][i] = u32x4{0, 0, 0, 0};
+                if (have[m]) {
+                    const uint8_t *p = img + xo[m] + (size_t)b * 128;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) red[wave][c][lane] = acc[m][c];
-        __syncthreads();
-        if (8 * m + i < tile.z) {
-            float g = 0.0f, u = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kTileWaves; ++w) {
-                g += red[w][n >> 4][from][i & 3] + red[w][n >> 4][from + 32][i & 3];
-                u += red[w][2 + (n >> 4)][from][i & 3] + red[w][2 + (n >> 4)][from + 32][i & 3];
+                    for (int i = 0; i < 4 * J; ++i)
+                        if (i < n) x[m][i] = *reinterpret_cast<const u32x4 *>(p + 128 * i);
+                }
             }
-            const int pair = pair_of(a, tile, 8 * m + i);
-            const float sc = kUnscale * a.xscale[pair / a.m.top_k];
-            a.h[(size_t)pair * hidden + col + n] = silu_mul(g * sc, u * sc);
+            // (x ahead of the first stages: behind them it comes last, 48 rows 46 -> 55 us)
+            if (t == 0)
+                for (int k = 0; k < R - 1 && k < total; ++k) issue();
+            // here, or the compiler waits for x, and so for every stage that is on its
+            // way, before each stage
+            wait_vm<0>();
+            if (t == 0) put_scales();
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int sub = 0; sub < SUBS; ++sub) {
+                    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): reads of the buffer asked for next
+                    if (left >= R) {
+                        issue();
+                        wait_vm<(R - 1) * S::DMAS>();
+                    } else if (R > 3 && left == 3) {
+                        wait_vm<2 * S::DMAS>();
+                    } else if (R > 2 && left == 2) {
+                        wait_vm<S::DMAS>();
+                    } else if (R <= 4 || left == 1) {
+                        wait_vm<0>();
+                    }
+                    multiply_stage<SJ, MT>(
+                        l, mine + buf * S::BYTES,
+                        [&](int m, int i) { return __builtin_bit_cast(f16x8, x[m][4 * SJ * sub + i]); },
+                        acc[c]);
+                    --left;
+                    buf = buf + 1 == R ? 0 : buf + 1;
+                }
         }
     }
+    store(acc);
 }
 
 __global__ __launch_bounds__(256) void moe_split_kernel(MoeArgs a) {
@@ -661,53 +729,244 @@ __global__ __launch_bounds__(256) void moe_split_kernel(MoeArgs a) {
                    a.hscale + pair);
 }
 
-// Columns of z of a tile of pairs, 64 a wave; ks waves split hidden.
-template <int MT, bool WHOLE>
-__global__ __launch_bounds__(kTileThreads) void moe_down_tile_kernel(MoeArgs a, int ks) {
-    __shared__ f32x4 red[kTileWaves][4][64];
-    if ((int)blockIdx.y >= a.n_tiles[0]) return;
-    const int4 tile = a.tiles[blockIdx.y];
+// ---------------------------------------------------------------- few rows
+//
+// One row needs no lists and no launch for the choice: a workgroup has one rank of
+// the choice and 16 columns of h, and finds the expert of that rank itself.  The
+// first workgroup writes the choice down for the second product.
+
+constexpr int kRowThreads = 512, kRowWaves = kRowThreads / 64;
+
+// DMA: the row's blocks are whole groups of four, scales 8-byte aligned
+template <bool DMA>
+__global__ __launch_bounds__(kRowThreads) void moe_up_row_kernel(MoeArgs a) {
+    constexpr int J = 2, R = 4;
+    using S = Stage<J>;
+    __shared__ __attribute__((aligned(1024))) unsigned char ring[DMA ? kRowWaves * R * S::BYTES : 16];
+    __shared__ double score[kMaxExperts];
+    __shared__ float red[kRowWaves][2][16];
+    __shared__ int chosen;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int E = a.m.n_experts, hidden = a.m.hidden;
+    if (blockIdx.x == 0) {
+        choose<kRowThreads, false>(a, 0);
+        return;
+    }
+    if (!live(a, 0)) return;
+    const int cols = hidden / 16, rank = (blockIdx.x - 1) / cols, col = (blockIdx.x - 1) % cols * 16;
+    load_scores<kRowThreads>(a, 0, score);
+    __syncthreads();
+    ranks<kRowThreads>(score, E, [&](int e, int n) {
+        if (n == rank) chosen = e;
+    });
+    __syncthreads();
+    const int e = __builtin_amdgcn_readfirstlane(chosen);
+    const int li = lane & 15, lg = lane >> 4, nb = a.m.dim / 32;
+    const size_t w0 = ((size_t)e * hidden + col) * nb;
+    const uint8_t *const img = a.ximg + lg * 32 + (li & 1) * 16;
+    f32x4 acc[4][1] = {};
+    if constexpr (DMA) {
+        unsigned char *const mine = ring + wave * R * S::BYTES;
+        const StageLane<J> l = stage_lane<J>(lane, nb);
+        const int slices = (nb + 4 * J - 1) / (4 * J);
+        const int total = wave < slices ? ((slices - 1 - wave) / kRowWaves + 1) * 2 : 0;
+        auto issue = [&](int k) {  // gate, up of the wave's k / 2th slice
+            const int b = (wave + k / 2 * kRowWaves) * 4 * J;
+            issue_stage<J>(l, (k & 1 ? a.m.up_quants : a.m.gate_quants) + (w0 + b) * 16,
+                           (k & 1 ? a.m.up_scales : a.m.gate_scales) + w0 + b, min(J, (nb - b) / 4),
+                           mine + k % R * S::BYTES);
+        };
+        for (int k = 0; k < R && k < total; ++k) issue(k);
+        for (int k = 0; k < total; k += 2) {
+            const int b = (wave + k / 2 * kRowWaves) * 4 * J;
+            u32x4 x[4 * J];
+#pragma unroll
+            for (int i = 0; i < 4 * J; ++i) {
+                x[i] = u32x4{0, 0, 0, 0};
+                if (b + i < nb) x[i] = *reinterpret_cast<const u32x4 *>(img + (size_t)(b + i) * 128);
+            }
+            // (x was asked for behind them)
+            wait_vm<0>();
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                multiply_stage<J, 1>(l, mine + (k + c) % R * S::BYTES,
+                                     [&](int, int i) { return __builtin_bit_cast(f16x8, x[i]); }, acc[c]);
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+            for (int c = 0; c < 2; ++c)
+                if (k + c + R < total) issue(k + c + R);
+        }
+    } else {
+        Operands o;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            o.q[c] = (c & 1 ? a.m.up_quants : a.m.gate_quants) + w0 * 16;
+            o.d[c] = (c & 1 ? a.m.up_scales : a.m.gate_scales) + w0;
+        }
+        const size_t xo[1] = {(size_t)(lg * 32 + (li & 1) * 16)};
+        multiply_steps<1>(o, a.ximg, xo, nb, wave, kRowWaves, acc);
+    }
+    // every two rows are the row's hi and lo
+    if (lane < 16) {
+        red[wave][0][lane] = acc[0][0][0] + acc[0][0][1];
+        red[wave][1][lane] = acc[1][0][0] + acc[1][0][1];
+    }
+    __syncthreads();
+    if (tid >= 16) return;
+    float g = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) {
+        g += red[w][0][tid];
+        u += red[w][1][tid];
+    }
+    const float sc = kUnscale * a.xscale[0];
+    a.h[(size_t)rank * hidden + col + tid] = silu_mul(g * sc, u * sc);
+}
+
+// A workgroup of W waves has 16 columns of a row's y; its waves share the experts
+// out, or parts of them where there are fewer.  A stage is W's 16 rows of 16 blocks
+// and that stretch of h, which the wave splits itself under a power of two of the
+// stretch.
+template <int W, bool DMA>
+__global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
+    constexpr int J = 4, R = W == 8 ? 2 : 3;  // (160 KB of LDS)
+    using S = Stage<J>;
+    constexpr int BYTES = S::BYTES + 2048;  // h behind W
+    __shared__ __attribute__((aligned(1024))) unsigned char ring[W * R * BYTES];
+    __shared__ u32x4 img[W][16 * 8];
+    __shared__ float red[kMaxTop][16];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
-    const int dim = a.m.dim, nb = a.m.hidden / 32;
-    const int cols = 64 * (kTileWaves / ks), col0 = blockIdx.x * cols;
-    const int e = __builtin_amdgcn_readfirstlane(tile.x);
-    Operands<MT, 4> o;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const int col = min(col0 + wave / ks * 64 + 16 * c, dim - 16);
-        const size_t w0 = ((size_t)e * dim + col) * nb;
-        o.q[c] = a.m.down_quants + w0 * 16;
-        o.d[c] = a.m.down_scales + w0;
-    }
-    o.x = a.himg;
-    o.row = li;
-    o.nb = nb;
-    o.lg = lg;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-        o.xo[m] = (size_t)pair_of(a, tile, 8 * m + (li & 7)) * nb * 128 + (li >> 3) * 64 + lg * 16;
-    f32x4 acc[MT][4] = {};
-    products<MT, 4, WHOLE>(o, wave % ks, ks, (nb + 3) / 4, acc);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        if (m) __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) red[wave][c][lane] = acc[m][c];
-        __syncthreads();
-        for (int t = tid; t < 8 * cols; t += kTileThreads) {
-            const int i = t / cols, n = t % cols, from = (i >> 2) * 16 + (n & 15);
-            if (8 * m + i >= tile.z || col0 + n >= dim) continue;
-            float v = 0.0f;
-            for (int w = 0; w < ks; ++w) {
-                const f32x4 *p = red[n / 64 * ks + w][n / 16 % 4];
-                v += p[from][i & 3] + p[from + 32][i & 3];
-            }
-            const int pair = pair_of(a, tile, 8 * m + i);
-            a.z[(size_t)pair * dim + col0 + n] = a.p[pair] * (kUnscale * a.hscale[pair] * v);
+    const int K = a.m.top_k, hidden = a.m.hidden, dim = a.m.dim, nb = hidden / 32;
+    const int r = blockIdx.y, col = blockIdx.x * 16;
+    if (!live(a, r)) return;
+    const int my_id = a.ids[r * K + min(lane, K - 1)];
+    const float my_p = a.p[r * K + min(lane, K - 1)];
+    const int parts = K < W ? W / K : 1, steps = (nb + 3) / 4;
+    const int per = (steps + parts - 1) / parts;
+    unsigned char *const mine = ring + wave * R * BYTES;
+    const StageLane<J> l = stage_lane<J>(lane, nb);
+    // unit u: part u % parts of expert u / parts, steps [s0, s1)
+    auto begin = [&](int u) { return u % parts * per; };
+    auto end = [&](int u) { return min(steps, u % parts * per + per); };
+    int iu = wave, is = begin(wave), ibuf = 0;  // the next stage to ask for
+    auto skip = [&](int &u, int &s) {  // to the next unit that has steps
+        while (u < K * parts && s >= end(u)) {
+            u += W;
+            s = begin(u);
         }
+    };
+    skip(iu, is);
+    auto issue = [&] {
+        const int j = iu / parts, e = __builtin_amdgcn_readlane(my_id, j);
+        const size_t w0 = ((size_t)e * dim + col) * nb + 4 * is;
+        unsigned char *const buf = mine + ibuf * BYTES;
+        const int jn = min(J, end(iu) - is);
+        if constexpr (DMA) {
+            issue_stage<J>(l, a.m.down_quants + w0 * 16, a.m.down_scales + w0, jn, buf);
+            const float *h = a.h + ((size_t)r * K + j) * hidden + 128 * is;
+            const uint32_t off = (32 * min(lane >> 2, 4 * jn - 1) + 4 * (lane & 3)) * 4;
+            dma16u(h, off, buf + S::BYTES);
+            dma16u(h, off + 64, buf + S::BYTES + 1024);
+        }
+        ibuf = ibuf + 1 == R ? 0 : ibuf + 1;
+        is += J;
+        skip(iu, is);
+    };
+    int asked = 0, buf = 0;
+    if constexpr (DMA)
+        for (; asked < R - 1 && iu < K * parts; ++asked) issue();
+    int u = wave, s = begin(wave);
+    float total = 0.0f;
+    skip(u, s);
+    if (lane < 16)
+        for (int k = wave; k < K * parts; k += W) red[k][lane] = 0.0f;
+    while (u < K * parts) {
+        const int j = u / parts, s1 = end(u), jn = min(J, s1 - s);
+        float4 ve, vf;
+        u32x4 q[J];
+        uint2 d[J];
+        const unsigned char *const at = mine + buf * BYTES;
+        if constexpr (DMA) {
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): reads of the buffer asked for next
+            if (iu < K * parts) {
+                issue();
+                ++asked;
+            }
+            // the stages behind this one may still be on their way
+            if (asked == 3) wait_vm<2 * (S::DMAS + 2)>();
+            else if (asked == 2) wait_vm<S::DMAS + 2>();
+            else wait_vm<0>();
+            --asked;
+            ve = *reinterpret_cast<const float4 *>(at + S::BYTES + lane * 16);
+            vf = *reinterpret_cast<const float4 *>(at + S::BYTES + 1024 + lane * 16);
+            if (lane >= 16 * jn) ve = vf = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+            const int e = __builtin_amdgcn_readlane(my_id, j);
+            const size_t w0 = ((size_t)e * dim + col + li) * nb;
+#pragma unroll
+            for (int i = 0; i < J; ++i) {
+                const int st = min(s + i, s1 - 1);
+                q[i] = *reinterpret_cast<const u32x4 *>(a.m.down_quants + (w0 + min(4 * st + lg, nb - 1)) * 16);
+                uint32_t v[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) v[t] = 4 * st + t < nb ? a.m.down_scales[w0 + 4 * st + t] : 0;
+                d[i] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+            }
+            const float *h = a.h + ((size_t)r * K + j) * hidden +
+                             32 * min(4 * s + (lane >> 2), nb - 1) + 4 * (lane & 3);
+            ve = *reinterpret_cast<const float4 *>(h);
+            vf = *reinterpret_cast<const float4 *>(h + 16);
+        }
+        float mx = max8(ve, vf);
+#pragma unroll
+        for (int dd = 32; dd >= 1; dd >>= 1) mx = fmaxf(mx, __shfl_xor(mx, dd));
+        const int ex = split_exponent(mx);
+        u32x4 hi, lo;
+        split8(ve, vf, ldexpf(1.0f, -ex), &hi, &lo);
+        __builtin_amdgcn_wave_barrier();  // the reads of the last stretch
+        img[wave][lane * 2] = hi;
+        img[wave][lane * 2 + 1] = lo;
+        __builtin_amdgcn_wave_barrier();
+        // every two rows of the fragment are h's hi and lo
+        const u32x4 *const x = &img[wave][lg * 2 + (li & 1)];
+        f32x4 acc[1] = {};
+        if constexpr (DMA) {
+            multiply_stage<J, 1>(l, at,
+                                 [&](int, int i) { return __builtin_bit_cast(f16x8, x[8 * i]); }, acc);
+        } else {
+#pragma unroll
+            for (int i = 0; i < J; ++i) {
+                if (i >= jn) break;
+                const u32x4 w = exchange(q[i]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const f32x4 v = mfma16(__builtin_bit_cast(f16x8, x[8 * (4 * i + t)]), nibbles(w[t]),
+                                           f32x4{0.f, 0.f, 0.f, 0.f});
+                    const f16x2 d2 = __builtin_bit_cast(f16x2, t < 2 ? d[i].x : d[i].y);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[0][k] = __builtin_fmaf((float)d2[t & 1], v[k], acc[0][k]);
+                }
+            }
+        }
+        total = __builtin_fmaf(kUnscale * ldexpf(1.0f, ex), acc[0][0] + acc[0][1], total);
+        buf = buf + 1 == R ? 0 : buf + 1;
+        s += J;
+        if (s >= s1) {
+            const float p = __builtin_bit_cast(
+                float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, my_p), j));
+            if (lane < 16) red[u][lane] = p * total;
+            total = 0.0f;
+        }
+        skip(u, s);
     }
+    __syncthreads();
+    if (tid >= 16) return;
+    float y = 0.0f;
+    for (int k = 0; k < K * parts; ++k) y += red[k][tid];
+    const size_t o = (size_t)r * dim + col + tid;
+    a.y[o] = a.residual ? a.residual[o] + y : y;
 }
 
 // y = [residual +] the sum of a row's experts in order of their rank
@@ -727,9 +986,17 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-bool whole_steps(int in_f, const uint16_t *s) {
-    return in_f % 128 == 0 && ((uintptr_t)s & 7) == 0;
+// Rows of whole groups of four blocks, their scales 8-byte aligned
+bool whole_groups(int in_f, const uint16_t *s) { return in_f % 128 == 0 && ((uintptr_t)s & 7) == 0; }
+
+// Workgroups that share a score's sum, 64 elements a wave at least
+int score_splits(const cw_moe &m, int rows) {
+    return rows == 1 ? 1 : std::min(kMaxSplits, std::max(1, m.dim / 512));
 }
+
+// Rows whose second product goes row by row, reading an expert again for each row
+// that chose it: that saves two launches and the passes over h and z.
+bool down_by_rows(const cw_moe &m, int rows) { return rows <= 8; }
 
 // Places of the workspace, each 256-byte aligned; with base null their size.
 size_t lay_out(const cw_moe &m, int rows, char *base, MoeArgs *a) {
@@ -739,63 +1006,100 @@ size_t lay_out(const cw_moe &m, int rows, char *base, MoeArgs *a) {
         at += (bytes + 255) & ~(size_t)255;
         return p;
     };
-    const size_t K = m.top_k, pairs = (size_t)rows * K;
-    const bool lists = rows > kFew;
-    a->score = reinterpret_cast<double *>(take((size_t)rows * m.n_experts * 8));
+    const size_t pairs = (size_t)rows * m.top_k;
+    a->splits = score_splits(m, rows);
+    a->score = reinterpret_cast<double *>(take((size_t)a->splits * rows * m.n_experts * 8));
     a->ids = reinterpret_cast<int *>(take(pairs * 4));
     a->p = reinterpret_cast<float *>(take(pairs * 4));
     a->ximg = reinterpret_cast<uint8_t *>(take((size_t)rows * m.dim * 4));
     a->xscale = reinterpret_cast<float *>(take((size_t)rows * 4));
     a->h = reinterpret_cast<float *>(take(pairs * m.hidden * 4));
-    if (lists) {
+    a->count = reinterpret_cast<int *>(take((size_t)m.n_experts * 4));
+    a->list = reinterpret_cast<int *>(take((size_t)m.n_experts * rows * 4));
+    if (!down_by_rows(m, rows)) {
         a->himg = reinterpret_cast<uint8_t *>(take(pairs * m.hidden * 4));
         a->hscale = reinterpret_cast<float *>(take(pairs * 4));
         a->z = reinterpret_cast<float *>(take(pairs * m.dim * 4));
-        a->list = reinterpret_cast<int *>(take(pairs * 4));
-        a->tiles = reinterpret_cast<int4 *>(take((pairs / kTile + m.n_experts) * 16));
-        a->n_tiles = reinterpret_cast<int *>(take(4));
     }
     return at;
 }
 
-int run_few(cw_ctx *ctx, const MoeArgs &a) {
-    const int E = a.m.n_experts, K = a.m.top_k;
-    auto score = a.rows == 1 ? moe_score_few_kernel<1> : a.rows <= 4 ? moe_score_few_kernel<4>
-                                                                     : moe_score_few_kernel<kFew>;
-    CW_TRY(launch(ctx, "moe_score", score, dim3(E + a.rows), dim3(256), 0, a));
-    const bool gw = whole_steps(a.m.dim, a.m.gate_scales) && whole_steps(a.m.dim, a.m.up_scales);
-    CW_TRY(launch(ctx, "moe_up", gw ? moe_up_few_kernel<true> : moe_up_few_kernel<false>,
-                  dim3(a.rows + a.rows * K * (a.m.hidden / 16)), dim3(kFewThreads), a.rows * E * 8, a));
-    const bool dw = whole_steps(a.m.hidden, a.m.down_scales);
-    return launch(ctx, "moe_down", dw ? moe_down_few_kernel<true> : moe_down_few_kernel<false>,
-                  dim3(a.m.dim / 16, a.rows), dim3(kFewThreads), 0, a);
+int run_down_rows(cw_ctx *ctx, const MoeArgs &a) {
+    const bool dma = whole_groups(a.m.hidden, a.m.down_scales);
+    const dim3 grid(a.m.dim / 16, a.rows);
+    if (a.rows == 1)
+        return launch(ctx, "moe_down", dma ? moe_down_row_kernel<8, true> : moe_down_row_kernel<8, false>,
+                      grid, dim3(512), 0, a);
+    return launch(ctx, "moe_down", dma ? moe_down_row_kernel<4, true> : moe_down_row_kernel<4, false>,
+                  grid, dim3(256), 0, a);
 }
 
-int run_tiles(cw_ctx *ctx, const MoeArgs &a) {
+// How the waves of a workgroup divide a product: J groups of blocks a stage (0:
+// through registers) and ks waves to a sum.
+struct TilePlan {
+    int J, ks, grid;
+};
+TilePlan tile_plan(bool up, const cw_moe &m, int mt) {
+    const int nb = (up ? m.dim : m.hidden) / 32, N = up ? m.hidden : m.dim;
+    const bool dma = up ? whole_groups(m.dim, m.gate_scales) && whole_groups(m.dim, m.up_scales)
+                        : whole_groups(m.hidden, m.down_scales);
+    TilePlan p{0, nb >= 64 ? 4 : nb >= 16 ? 2 : 1, 0};
+    if (dma) {
+        // the most of the stages' blocks that exist, then the fewest rounds
+        int best = -1;
+        for (int J = mt == 4 ? 2 : 4; J >= 2; --J)
+            for (int ks = 4; ks >= 1; ks /= 2) {
+                const int rounds = ((nb + 4 * J - 1) / (4 * J) + ks - 1) / ks;
+                const int score = nb * 1000 / (rounds * ks * 4 * J) * 64 - std::min(rounds, 63);
+                if (score > best) {
+                    best = score;
+                    p.J = J;
+                    p.ks = ks;
+                }
+            }
+    }
+    const int sets = (up ? N / 32 : (N + 63) / 64), per = kWaves / p.ks;
+    p.grid = (sets + per - 1) / per;
+    return p;
+}
+
+template <bool UP, int MT>
+int launch_tiles(cw_ctx *ctx, const MoeArgs &a, int most) {
+    const TilePlan p = tile_plan(UP, a.m, MT);
+    auto fn = p.J == 0 ? moe_tile_kernel<UP, MT, 0> : moe_tile_kernel<UP, MT, 2>;
+    if constexpr (MT < 4) {
+        if (p.J == 3) fn = moe_tile_kernel<UP, MT, 3>;
+        if (p.J == 4) fn = moe_tile_kernel<UP, MT, 4>;
+    }
+    return launch(ctx, UP ? "moe_up" : "moe_down", fn, dim3(p.grid, most), dim3(kThreads), 0, a, p.ks);
+}
+
+template <bool UP>
+int launch_product(cw_ctx *ctx, const MoeArgs &a, int mt, int most) {
+    return mt == 1 ? launch_tiles<UP, 1>(ctx, a, most)
+           : mt == 2 ? launch_tiles<UP, 2>(ctx, a, most)
+                     : launch_tiles<UP, 4>(ctx, a, most);
+}
+
+int run(cw_ctx *ctx, const MoeArgs &a) {
     const int E = a.m.n_experts, K = a.m.top_k, pairs = a.rows * K;
+    if (a.rows == 1) {
+        const bool dma = whole_groups(a.m.dim, a.m.gate_scales) && whole_groups(a.m.dim, a.m.up_scales);
+        CW_TRY(launch(ctx, "moe_score", moe_score_row_kernel, dim3(E + 1), dim3(256), 0, a));
+        CW_TRY(launch(ctx, "moe_up", dma ? moe_up_row_kernel<true> : moe_up_row_kernel<false>,
+                      dim3(1 + K * (a.m.hidden / 16)), dim3(kRowThreads), 0, a));
+        return run_down_rows(ctx, a);
+    }
     const int mean = (pairs + E - 1) / E;
-    const int mt = mean <= 4 ? 1 : mean <= 12 ? 2 : 4, tile = kTile * mt;
-    const int score = (E + 15) / 16 * ((a.rows + 15) / 16);
-    CW_TRY(launch(ctx, "moe_score", moe_score_kernel, dim3(score + a.rows), dim3(1024), 0, a));
-    const bool one = a.rows <= 64;
-    CW_TRY(launch(ctx, "moe_choose", moe_choose_kernel, dim3(one ? 1 : (a.rows + 15) / 16), dim3(1024),
-                  0, a, tile, one ? 1 : 0));
-    if (!one) CW_TRY(launch(ctx, "moe_sort", moe_sort_kernel, dim3(1), dim3(1024), 0, a, tile));
-    const int most = std::min(pairs, E + pairs / tile);
-    const bool gw = whole_steps(a.m.dim, a.m.gate_scales) && whole_steps(a.m.dim, a.m.up_scales);
-    auto up = mt == 1 ? (gw ? moe_up_tile_kernel<1, true> : moe_up_tile_kernel<1, false>)
-              : mt == 2 ? (gw ? moe_up_tile_kernel<2, true> : moe_up_tile_kernel<2, false>)
-                        : (gw ? moe_up_tile_kernel<4, true> : moe_up_tile_kernel<4, false>);
-    CW_TRY(launch(ctx, "moe_up", up, dim3(a.m.hidden / 32, most), dim3(kTileThreads), 0, a));
+    const int mt = mean <= 5 ? 1 : mean <= 12 ? 2 : 4, tile = kTile * mt;
+    const int score = (E + 15) / 16 * ((a.rows + 15) / 16) * a.splits;
+    CW_TRY(launch(ctx, "moe_score", moe_score_kernel, dim3(score + a.rows), dim3(256), 0, a));
+    CW_TRY(launch(ctx, "moe_choose", moe_choose_kernel, dim3(a.rows), dim3(256), 0, a));
+    const int most = std::min(pairs, E + pairs / tile);  // tiles
+    CW_TRY(launch_product<true>(ctx, a, mt, most));
+    if (down_by_rows(a.m, a.rows)) return run_down_rows(ctx, a);
     CW_TRY(launch(ctx, "moe_split", moe_split_kernel, dim3(pairs), dim3(256), 0, a));
-    const bool dw = whole_steps(a.m.hidden, a.m.down_scales);
-    auto down = mt == 1 ? (dw ? moe_down_tile_kernel<1, true> : moe_down_tile_kernel<1, false>)
-                : mt == 2 ? (dw ? moe_down_tile_kernel<2, true> : moe_down_tile_kernel<2, false>)
-                          : (dw ? moe_down_tile_kernel<4, true> : moe_down_tile_kernel<4, false>);
-    const int steps = (a.m.hidden / 32 + 3) / 4, ks = steps >= 16 ? 4 : steps >= 4 ? 2 : 1;
-    const int cols = 64 * (kTileWaves / ks);
-    CW_TRY(launch(ctx, "moe_down", down, dim3((a.m.dim + cols - 1) / cols, most), dim3(kTileThreads),
-                  0, a, ks));
+    CW_TRY(launch_product<false>(ctx, a, mt, most));
     return launch(ctx, "moe_sum", moe_sum_kernel, dim3((a.m.dim + 1023) / 1024, a.rows), dim3(256), 0, a);
 }
 
@@ -829,7 +1133,7 @@ extern "C" int cw_moe_rows(cw_ctx *ctx, const cw_moe *moe, const float *x, int r
     CW_HIP(hipSetDevice(ctx->device));
     MoeArgs a{};
     int chunk = std::min(rows, kChunk);
-    while (chunk > kFew && lay_out(m, chunk, nullptr, &a) > kChunkBytes) chunk = std::max(kFew, chunk / 2);
+    while (chunk > kTile && lay_out(m, chunk, nullptr, &a) > kChunkBytes) chunk = std::max(kTile, chunk / 2);
     void *scratch = nullptr;
     CW_TRY(ctx_scratch(ctx, lay_out(m, chunk, nullptr, &a), &scratch));
     for (int r0 = 0; r0 < rows; r0 += chunk) {
@@ -842,7 +1146,7 @@ extern "C" int cw_moe_rows(cw_ctx *ctx, const cw_moe *moe, const float *x, int r
         a.y = y + (size_t)r0 * m.dim;
         a.experts = experts ? experts + (size_t)r0 * m.top_k : nullptr;
         a.weights = weights ? weights + (size_t)r0 * m.top_k : nullptr;
-        CW_TRY(a.rows <= kFew ? run_few(ctx, a) : run_tiles(ctx, a));
+        CW_TRY(run(ctx, a));
     }
     return CW_OK;
 }

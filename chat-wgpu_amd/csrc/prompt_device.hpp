@@ -82,10 +82,27 @@ __device__ __forceinline__ uint32_t lds_off(unsigned char *p) {
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_u8 *)p);
 }
 __device__ __forceinline__ void dma16(const void *base, uint32_t off, unsigned char *lds_dst) {
-    asm volatile("global_load_lds_dwordx4 %0, %1"
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"  // (a wait state after M0's write)
                  :
                  : "v"(off), "s"(base), "{m0}"(lds_off(lds_dst))
                  : "memory");
+}
+
+// all but the newest N of this wave's loads have completed
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Workgroup barrier on LDS data only: __syncthreads would also wait for
+// every DMA in flight
+__device__ __forceinline__ void lds_barrier() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
 }  // namespace cwi

@@ -562,7 +562,7 @@ struct Tile {
 // dma16 of lines that nobody reads again (non-temporal: 64 single rows at 4,000
 // positions 182 -> 165 us; where a second row block reads them it costs a tenth)
 __device__ __forceinline__ void dma16_once(const void *base, uint32_t off, unsigned char *lds_dst) {
-    asm volatile("global_load_lds_dwordx4 %0, %1 nt"
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"  // (a wait state after M0's write)
                  :
                  : "v"(off), "s"(base), "{m0}"(lds_off(lds_dst))
                  : "memory");
