@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void moe_score_row_kernel(MoeArgs a) {
 // matrix cores, the waves sharing it out; then the rows' images.  The first clears
 // the experts' counts.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
-__global__ __launch_bounds__(256) void moe_score_kernel(MoeArgs a) {
+__global__ __launch_bounds__(256, 2) void moe_score_kernel(MoeArgs a) {
     __shared__ double red[4][256];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int dim = a.m.dim, E = a.m.n_experts;
@@ -171,16 +171,18 @@ __global__ __launch_bounds__(256) void moe_score_kernel(MoeArgs a) {
     const float *w = a.m.router + (size_t)min(e0 + li, E - 1) * dim + 4 * lg;
     f64x4 acc = {0.0, 0.0, 0.0, 0.0};
     const int by = a.splits * 64;
-    for (int i0 = (part * 4 + wave) * 16; i0 < dim; i0 += 4 * by) {
-        float4 u[4], v[4];
+    constexpr int D = 8;  // loads in flight
+    for (int i0 = (part * 4 + wave) * 16; i0 < dim; i0 += D * by) {
+        float4 u[D], v[D];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < D; ++k) {
             const int i = i0 + k * by < dim ? i0 + k * by : i0;
             u[k] = *reinterpret_cast<const float4 *>(x + i);
             v[k] = *reinterpret_cast<const float4 *>(w + i);
         }
+        __builtin_amdgcn_sched_barrier(0);  // (all of them, before the first is waited for)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < D; ++k) {
             if (i0 + k * by >= dim) break;
             acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[k].x, (double)v[k].x, acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[k].y, (double)v[k].y, acc, 0, 0, 0);
@@ -198,30 +200,47 @@ __global__ __launch_bounds__(256) void moe_score_kernel(MoeArgs a) {
             (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
 }
 
+// Lanes to an expert when NT threads rank E of them, and the scores that they go
+// through, in whole runs of 8 (those behind E, -inf, are ahead of nothing).
+constexpr int kRun = 8, kRanked = kMaxExperts + 64 * kRun;
+__device__ __forceinline__ int rank_lanes(int NT, int E) {
+    int per = 1;
+    while (per < 64 && 2 * per * E <= NT) per *= 2;
+    return per;
+}
+
 // score[e] = row r's scores, by a workgroup of NT threads (not yet synchronised).
 template <int NT>
 __device__ __forceinline__ void load_scores(const MoeArgs &a, int r, double *score) {
-    const int E = a.m.n_experts;
-    for (int e = threadIdx.x; e < E; e += NT) {
-        double s = a.score[(size_t)r * E + e];
-        for (int i = 1; i < a.splits; ++i) s += a.score[((size_t)i * a.rows + r) * E + e];
-        score[e] = ranked(s);
+    const int E = a.m.n_experts, run = rank_lanes(NT, E) * kRun;
+    for (int e = threadIdx.x; e < (E + run - 1) / run * run; e += NT) {
+        double v[kMaxSplits];
+#pragma unroll
+        for (int i = 0; i < kMaxSplits; ++i)
+            v[i] = e < E && i < a.splits ? a.score[((size_t)i * a.rows + r) * E + e] : 0.0;
+        double s = v[0];
+#pragma unroll
+        for (int i = 1; i < kMaxSplits; ++i) s += v[i];
+        score[e] = e < E ? ranked(s) : -INFINITY;
     }
 }
 
 // f(expert, rank) for every expert, by `per` lanes each that count those ahead of
-// it (8 rounds of finding the largest of 128 took 10 us a row, this 0.3).
+// it (8 rounds of finding the largest of 128 took 10 us a row).
 template <int NT, typename F>
 __device__ __forceinline__ void ranks(const double *score, int E, F f) {
-    int per = 1;
-    while (per < 64 && 2 * per * E <= NT) per *= 2;
-    const int part = threadIdx.x % per;
+    const int per = rank_lanes(NT, E), part = threadIdx.x % per;
     for (int e0 = 0; e0 < E; e0 += NT / per) {
         const int e = e0 + threadIdx.x / per;
         const double mine = score[min(e, E - 1)];
         int n = 0;
-#pragma unroll 8
-        for (int i = part; i < E; i += per) n += ahead(score[i], i, mine, e);
+        for (int i0 = part; i0 < E; i0 += per * kRun) {
+            double v[kRun];
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) v[k] = score[i0 + k * per];
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) n += ahead(v[k], i0 + k * per, mine, e);
+        }
         for (int d = 1; d < per; d <<= 1) n += __shfl_xor(n, d);
         if (part == 0 && e < E) f(e, n);
     }
@@ -232,7 +251,7 @@ __device__ __forceinline__ void ranks(const double *score, int E, F f) {
 // tile's rows a pair becomes does not show in its result.
 template <int NT, bool LISTS>
 __device__ void choose(const MoeArgs &a, int r) {
-    __shared__ double score[kMaxExperts], term[kMaxTop], part[NT / 64];
+    __shared__ double score[kRanked], term[kMaxTop], part[NT / 64];
     __shared__ int id[kMaxTop];
     const int tid = threadIdx.x, E = a.m.n_experts, K = a.m.top_k;
     if (!live(a, r)) {
@@ -270,7 +289,7 @@ __device__ void choose(const MoeArgs &a, int r) {
     if constexpr (LISTS) a.list[(size_t)e * a.rows + atomicAdd(&a.count[e], 1)] = i;
 }
 
-__global__ __launch_bounds__(256) void moe_choose_kernel(MoeArgs a) { choose<256, true>(a, blockIdx.x); }
+__global__ __launch_bounds__(1024) void moe_choose_kernel(MoeArgs a) { choose<1024, true>(a, blockIdx.x); }
 
 // ---------------------------------------------------------------- products
 //
@@ -740,10 +759,10 @@ constexpr int kRowThreads = 512, kRowWaves = kRowThreads / 64;
 // DMA: the row's blocks are whole groups of four, scales 8-byte aligned
 template <bool DMA>
 __global__ __launch_bounds__(kRowThreads) void moe_up_row_kernel(MoeArgs a) {
-    constexpr int J = 2, R = 4;
+    constexpr int J = 2, R = 2;  // (with 4 one workgroup fits a CU: 12.6 us for 384 of them)
     using S = Stage<J>;
     __shared__ __attribute__((aligned(1024))) unsigned char ring[DMA ? kRowWaves * R * S::BYTES : 16];
-    __shared__ double score[kMaxExperts];
+    __shared__ double score[kRanked];
     __shared__ float red[kRowWaves][2][16];
     __shared__ int chosen;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -824,16 +843,16 @@ __global__ __launch_bounds__(kRowThreads) void moe_up_row_kernel(MoeArgs a) {
 }
 
 // A workgroup of W waves has 16 columns of a row's y; its waves share the experts
-// out, or parts of them where there are fewer.  A stage is W's 16 rows of 16 blocks
+// out, or parts of them where there are fewer.  A stage is W's 16 rows of 8 blocks
 // and that stretch of h, which the wave splits itself under a power of two of the
 // stretch.
 template <int W, bool DMA>
 __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
-    constexpr int J = 4, R = W == 8 ? 2 : 3;  // (160 KB of LDS)
+    constexpr int J = 2, R = 3;
     using S = Stage<J>;
-    constexpr int BYTES = S::BYTES + 2048;  // h behind W
+    constexpr int BYTES = S::BYTES + 1024;  // h behind W
     __shared__ __attribute__((aligned(1024))) unsigned char ring[W * R * BYTES];
-    __shared__ u32x4 img[W][16 * 8];
+    __shared__ u32x4 img[W][4 * J * 8];
     __shared__ float red[kMaxTop][16];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -866,9 +885,9 @@ __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
         if constexpr (DMA) {
             issue_stage<J>(l, a.m.down_quants + w0 * 16, a.m.down_scales + w0, jn, buf);
             const float *h = a.h + ((size_t)r * K + j) * hidden + 128 * is;
-            const uint32_t off = (32 * min(lane >> 2, 4 * jn - 1) + 4 * (lane & 3)) * 4;
-            dma16u(h, off, buf + S::BYTES);
-            dma16u(h, off + 64, buf + S::BYTES + 1024);
+            // lane: chunk lane % 32 (block, group), its first or its second four elements
+            dma16u(h, (32 * min(lane >> 2 & 7, 4 * jn - 1) + 4 * (lane & 3) + (lane >> 5) * 16) * 4,
+                   buf + S::BYTES);
         }
         ibuf = ibuf + 1 == R ? 0 : ibuf + 1;
         is += J;
@@ -895,13 +914,13 @@ __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
                 ++asked;
             }
             // the stages behind this one may still be on their way
-            if (asked == 3) wait_vm<2 * (S::DMAS + 2)>();
-            else if (asked == 2) wait_vm<S::DMAS + 2>();
+            if (asked == 3) wait_vm<2 * (S::DMAS + 1)>();
+            else if (asked == 2) wait_vm<S::DMAS + 1>();
             else wait_vm<0>();
             --asked;
-            ve = *reinterpret_cast<const float4 *>(at + S::BYTES + lane * 16);
-            vf = *reinterpret_cast<const float4 *>(at + S::BYTES + 1024 + lane * 16);
-            if (lane >= 16 * jn) ve = vf = make_float4(0.f, 0.f, 0.f, 0.f);
+            ve = *reinterpret_cast<const float4 *>(at + S::BYTES + (lane & 31) * 16);
+            vf = *reinterpret_cast<const float4 *>(at + S::BYTES + 512 + (lane & 31) * 16);
+            if ((lane & 31) >= 16 * jn) ve = vf = make_float4(0.f, 0.f, 0.f, 0.f);
         } else {
             const int e = __builtin_amdgcn_readlane(my_id, j);
             const size_t w0 = ((size_t)e * dim + col + li) * nb;
@@ -915,7 +934,7 @@ __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
                 d[i] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
             }
             const float *h = a.h + ((size_t)r * K + j) * hidden +
-                             32 * min(4 * s + (lane >> 2), nb - 1) + 4 * (lane & 3);
+                             32 * min(4 * s + (lane >> 2 & 7), nb - 1) + 4 * (lane & 3);
             ve = *reinterpret_cast<const float4 *>(h);
             vf = *reinterpret_cast<const float4 *>(h + 16);
         }
@@ -926,8 +945,8 @@ __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
         u32x4 hi, lo;
         split8(ve, vf, ldexpf(1.0f, -ex), &hi, &lo);
         __builtin_amdgcn_wave_barrier();  // the reads of the last stretch
-        img[wave][lane * 2] = hi;
-        img[wave][lane * 2 + 1] = lo;
+        // (both halves of the wave have the same chunks: one stores hi, the other lo)
+        img[wave][(lane & 31) * 2 + (lane >> 5)] = lane < 32 ? hi : lo;
         __builtin_amdgcn_wave_barrier();
         // every two rows of the fragment are h's hi and lo
         const u32x4 *const x = &img[wave][lg * 2 + (li & 1)];
@@ -1094,7 +1113,7 @@ int run(cw_ctx *ctx, const MoeArgs &a) {
     const int mt = mean <= 5 ? 1 : mean <= 12 ? 2 : 4, tile = kTile * mt;
     const int score = (E + 15) / 16 * ((a.rows + 15) / 16) * a.splits;
     CW_TRY(launch(ctx, "moe_score", moe_score_kernel, dim3(score + a.rows), dim3(256), 0, a));
-    CW_TRY(launch(ctx, "moe_choose", moe_choose_kernel, dim3(a.rows), dim3(256), 0, a));
+    CW_TRY(launch(ctx, "moe_choose", moe_choose_kernel, dim3(a.rows), dim3(1024), 0, a));
     const int most = std::min(pairs, E + pairs / tile);  // tiles
     CW_TRY(launch_product<true>(ctx, a, mt, most));
     if (down_by_rows(a.m, a.rows)) return run_down_rows(ctx, a);
