@@ -379,12 +379,14 @@ __device__ __forceinline__ void issue_stage(const StageLane<J> &l, const uint8_t
         dma4u(s, l.s[t] + 4 * min(l.word[t], 2 * jn - 1), buf + Stage<J>::Q + 256 * t);
 }
 
-// acc[m] += the stage times the x fragments x(m, block), which are 0 for blocks that
-// do not exist.  A block's products are scaled and added while the next one's run and
-// its weights are decoded; a group's words are read a group ahead.
-template <int J, int MT, typename X>
+// acc += the stage times the x fragments x(half, block), which are 0 for blocks that do
+// not exist.  Eight rows: their hi and lo halves are the fragment's 16
+// rows (H = 1); 16 rows: two fragments one after the other (H = 2), so that a block's
+// scale meets the sum of both.  A block's products are scaled and added while the next
+// one's run and its weights are decoded; a group's words are read a group ahead.
+template <int J, int H, typename X>
 __device__ __forceinline__ void multiply_stage(const StageLane<J> &l, const unsigned char *buf, X x,
-                                               f32x4 (&acc)[MT]) {
+                                               f32x4 &acc) {
     constexpr int L = Stage<J>::LINE;
     uint32_t w[2][4];
     uint2 d4[2];
@@ -395,46 +397,42 @@ __device__ __forceinline__ void multiply_stage(const StageLane<J> &l, const unsi
                 buf + (L == 8 ? l.at[4 * (j & 1) + i] + j / 2 * 2048 : l.at[i] + j * 1024));
         d4[j & 1] = *reinterpret_cast<const uint2 *>(buf + l.scale + 8 * j);
     };
-    f32x4 t[2][MT];
+    f32x4 t[2];
     auto add = [&](int k) {
         const uint2 s = d4[k / 4 & 1];
         const f16x2 d2 = __builtin_bit_cast(f16x2, k & 2 ? s.y : s.x);
         const float d = (float)d2[k & 1];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[m][r] = __builtin_fmaf(d, t[k & 1][m][r], acc[m][r]);
+        for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(d, t[k & 1][r], acc[r]);
     };
     f16x8 b[2];
     read(0);
     b[0] = nibbles(w[0][0]);
 #pragma unroll
     for (int k = 0; k < 4 * J; ++k) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m) t[k & 1][m] = mfma16(x(m, k), b[k & 1], f32x4{0.f, 0.f, 0.f, 0.f});
+        t[k & 1] = mfma16(x(0, k), b[k & 1], f32x4{0.f, 0.f, 0.f, 0.f});
+        if constexpr (H == 2) t[k & 1] = mfma16(x(1, k), b[k & 1], t[k & 1]);
         if (k + 1 < 4 * J) b[k + 1 & 1] = nibbles(w[(k + 1) / 4 & 1][(k + 1) & 3]);
         if (k > 0) add(k - 1);
         // (behind the last use of the scales that it replaces)
         if (k % 4 == 0 && k / 4 + 1 < J) read(k / 4 + 1);
         // (else all products come first, each in registers of its own)
-        __builtin_amdgcn_sched_group_barrier(0x008, MT, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 9 + 4 * MT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, H, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 13, 0);
     }
     add(4 * J - 1);
     // the sums are wanted here (the compiler would put them off to the next stage, and
     // keep every product until then)
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-        asm volatile("" : "+v"(acc[m][0]), "+v"(acc[m][1]), "+v"(acc[m][2]), "+v"(acc[m][3]));
+    asm volatile("" : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]));
 }
 
 // Rows that are no whole groups of four blocks, or whose scales are not 8-byte
 // aligned: a lane of the 16 x 4 (W row, k group) loads block 4 s + group of its row,
 // and the lane groups hand each other their words (two swaps of lane halves, two of
 // rows of 16).
-template <int MT>
+template <int H>
 struct Step {
-    u32x4 q[4], x[MT][4];
+    u32x4 q[4], x[H][4];
     uint2 d[4];
 };
 struct Operands {
@@ -442,9 +440,10 @@ struct Operands {
     const uint16_t *d[4];
 };
 
-template <int MT>
-__device__ __forceinline__ void load_step(const Operands &o, const uint8_t *img, const size_t (&xo)[MT],
-                                          int nb, int s, Step<MT> &f) {
+// xo: where the lane's fragment begins in a block's image, 16 bytes a half
+template <int H>
+__device__ __forceinline__ void load_step(const Operands &o, const uint8_t *img, size_t xo,
+                                          int nb, int s, Step<H> &f) {
     const int lane = threadIdx.x & 63, row = lane & 15, lg = lane >> 4;
     const int b = min(4 * s + lg, nb - 1);
 #pragma unroll
@@ -457,11 +456,11 @@ __device__ __forceinline__ void load_step(const Operands &o, const uint8_t *img,
         f.d[c] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            f.x[m][i] = *reinterpret_cast<const u32x4 *>(img + xo[m] +
-                                                         (size_t)min(4 * s + i, nb - 1) * 128);
+            f.x[h][i] = *reinterpret_cast<const u32x4 *>(img + xo + (size_t)min(4 * s + i, nb - 1) * 128 +
+                                                         h * 16);
 }
 
 // Word w of the lane groups' blocks -> block i of word `group`.
@@ -473,8 +472,8 @@ __device__ __forceinline__ u32x4 exchange(u32x4 q) {
     return u32x4{c[0], d[0], c[1], d[1]};
 }
 
-template <int MT>
-__device__ __forceinline__ void multiply_step(const Step<MT> &f, f32x4 (&acc)[4][MT]) {
+template <int H>
+__device__ __forceinline__ void multiply_step(const Step<H> &f, f32x4 (&acc)[4]) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const u32x4 w = exchange(f.q[c]);
@@ -483,38 +482,35 @@ __device__ __forceinline__ void multiply_step(const Step<MT> &f, f32x4 (&acc)[4]
             const f16x8 b = nibbles(w[i]);
             const f16x2 d2 = __builtin_bit_cast(f16x2, i < 2 ? f.d[c].x : f.d[c].y);
             const float d = (float)d2[i & 1];
+            f32x4 t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const f32x4 t = mfma16(__builtin_bit_cast(f16x8, f.x[m][i]), b, f32x4{0.f, 0.f, 0.f, 0.f});
+            for (int h = 0; h < H; ++h) t = mfma16(__builtin_bit_cast(f16x8, f.x[h][i]), b, t);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[c][m][r] = __builtin_fmaf(d, t[r], acc[c][m][r]);
-            }
+            for (int r = 0; r < 4; ++r) acc[c][r] = __builtin_fmaf(d, t[r], acc[c][r]);
         }
     }
 }
 
 // acc += the products of steps s, s + by, ...: two steps' loads in flight.
-template <int MT>
+template <int H>
 __device__ __forceinline__ void multiply_steps(const Operands &o, const uint8_t *img,
-                                               const size_t (&xo)[MT], int nb, int s, int by,
-                                               f32x4 (&acc)[4][MT]) {
+                                               size_t xo, int nb, int s, int by,
+                                               f32x4 (&acc)[4]) {
     const int n = (nb + 3) / 4;
     if (s >= n) return;
-    Step<MT> f[2];
-    load_step<MT>(o, img, xo, nb, s, f[0]);
+    Step<H> f[2];
+    load_step(o, img, xo, nb, s, f[0]);
     for (;; s += 2 * by) {
-        load_step<MT>(o, img, xo, nb, min(s + by, n - 1), f[1]);
-        multiply_step<MT>(f[0], acc);
+        load_step(o, img, xo, nb, min(s + by, n - 1), f[1]);
+        multiply_step(f[0], acc);
         if (s + by >= n) break;
-        load_step<MT>(o, img, xo, nb, min(s + 2 * by, n - 1), f[0]);
-        multiply_step<MT>(f[1], acc);
+        load_step(o, img, xo, nb, min(s + 2 * by, n - 1), f[0]);
+        multiply_step(f[1], acc);
         if (s + 2 * by >= n) break;
     }
 }
 
 // ---------------------------------------------------------------- tiles of pairs
-
-constexpr int kThreads = 256, kWaves = 4;
 
 // Tile b of `tile` pairs of one expert, counted over the experts: every wave finds
 // it from the counts (lane i has experts i * per ..), which costs it a load and a
@@ -566,179 +562,201 @@ __device__ __forceinline__ Tile find_tile(const MoeArgs &a, int tile, int b) {
 // A tile's pair i, its last again past the end
 __device__ __forceinline__ int pair_of(const Tile &t, int i) { return t.list[min(i, t.n - 1)]; }
 
-// A tile of pairs times a stretch of its expert's columns: of h (UP: 32 gate and the
-// same 32 up columns a set) or of z (64 columns a set).  ks waves split the sum, the
-// others take other sets.  J groups of blocks of x stay in registers per wave, MT
-// tiles of eight rows; W goes through a ring of stages (J = 0: steps of any row
-// length, through registers).  (Workgroups that take several sets one after the
-// other, asking ahead, gain nothing: 48 rows 46.4 us with one set, 45.7 with two,
-// 47.1 with three.)
-template <bool UP, int MT, int J>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(MT == 1 ? 4 : 2, MT == 1 ? 4 : 2)))
-void moe_tile_kernel(MoeArgs a, int ks) {
-    // stages of SJ groups, R of them in LDS for each wave: as many workgroups on a CU as
-    // the registers allow
-    constexpr int SJ = J == 3 ? 3 : 2, SUBS = J / SJ, R = J == 4 ? 3 : MT == 1 ? 2 : 3;
-    __shared__ __attribute__((aligned(1024))) unsigned char ring[J ? kWaves * R * Stage<SJ>::BYTES : 16];
-    __shared__ float4 red[kWaves - 1][64];
-    __shared__ int pairs[8 * MT];
-    __shared__ float scales[8 * MT];
-    const Tile tile = find_tile(a, kTile * MT, blockIdx.y);
+// How a tile kernel of 8 H rows and J groups of blocks of x in a wave's registers (0:
+// through registers, any row length) is laid out.  16 rows decode W half as often, but
+// have 128 B of x for 64: eight waves share a sum where four do.
+template <int H, int J>
+struct TileShape {
+    static constexpr int ROWS = kTile * H, WAVES = 4 * H;  // WAVES at most
+    // stages of SJ groups, SUBS of them a slice of x, R in LDS for each wave
+    static constexpr int SJ = J == 3 ? 3 : 2, SUBS = J / SJ, R = J == 4 ? 3 : 2;
+    static constexpr int RING = J ? WAVES * R * Stage<SJ>::BYTES : 16;
+    static constexpr int OCC = H == 2 && J == 0 ? 2 : 4;  // waves a SIMD that registers allow
+};
+
+// A tile of pairs times stretches of its expert's columns: of h (UP: 32 gate and the
+// same 32 up columns a set) or of z (64 columns a set).  ks waves split the sum, others
+// take other sets; W goes through each wave's ring of stages, x stays in registers
+// where a wave's slice of it is all it has, for `groups` sets one after the other.
+// (Eight rows take one set: with two or three the next one's W is asked for ahead, but
+// 48 rows still take 45.7 and 47.1 us, 46.4 with one.)
+template <bool UP, int H, int J>
+__global__ __launch_bounds__((TileShape<H, J>::WAVES * 64))
+__attribute__((amdgpu_waves_per_eu(TileShape<H, J>::OCC, TileShape<H, J>::OCC)))
+void moe_tile_kernel(MoeArgs a, int ks, int groups) {
+    using T = TileShape<H, J>;
+    constexpr int SJ = T::SJ, SUBS = T::SUBS, R = T::R;
+    constexpr int SET = UP ? 32 : 64;  // columns
+    using S = Stage<SJ>;
+    __shared__ __attribute__((aligned(1024))) unsigned char ring[T::RING];
+    __shared__ f32x4 red[T::WAVES][4][32 * H];
+    __shared__ int pairs[T::ROWS];
+    __shared__ float scales[T::ROWS];
+    const Tile tile = find_tile(a, T::ROWS, blockIdx.y);
     if (tile.n == 0) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
     const int K = a.m.top_k, N = UP ? a.m.hidden : a.m.dim, nb = (UP ? a.m.dim : a.m.hidden) / 32;
-    const int cs = kWaves / ks, sets = UP ? N / 32 : (N + 63) / 64;
-    const int set = blockIdx.x * cs + wave / ks;  // (past the last: the last again, not stored)
+    const int cs = (int)blockDim.x / 64 / ks, sets = (N + SET - 1) / SET;
+    const int set0 = blockIdx.x * groups * cs;
+    const int n_groups = H == 1 ? 1 : min(groups, (sets - set0 + cs - 1) / cs);
     const uint8_t *const img = UP ? a.ximg : a.himg;
 
-    auto w_tile = [&](int c, const uint8_t **q, const uint16_t **d) {
-        const int at = min(set, sets - 1), col = UP ? at * 32 + (c & 1) * 16 : min(at * 64 + c * 16, N - 16);
+    // column tile c of the wave's set of a group (past the last set: the last again,
+    // not stored)
+    auto w_tile = [&](int g, int c, const uint8_t **q, const uint16_t **d) {
+        const int set = min(set0 + g * cs + wave / ks, sets - 1);
+        const int col = UP ? set * 32 + (c & 1) * 16 : min(set * 64 + c * 16, N - 16);
         const size_t w0 = ((size_t)tile.e * N + col) * nb;
         *q = (!UP ? a.m.down_quants : c < 2 ? a.m.gate_quants : a.m.up_quants) + w0 * 16;
         *d = (!UP ? a.m.down_scales : c < 2 ? a.m.gate_scales : a.m.up_scales) + w0;
     };
 
-    using S = Stage<SJ>;
-    constexpr int JX = J ? J : SJ;  // groups of blocks of a wave's slice of x
-    unsigned char *const mine = ring + wave * R * S::BYTES;
-    const StageLane<SJ> l = stage_lane<SJ>(lane, nb);
-    const int slices = (nb + 4 * JX - 1) / (4 * JX), rounds = (slices + ks - 1) / ks;
-    const int total = rounds * 4 * (J ? SUBS : 1);
-    // the wave's first group of blocks in a round (a wave without any goes through the
-    // row's last ones with no x)
-    auto group = [&](int t) { return min(t * ks + wave % ks, slices - 1) * JX; };
-    int it = 0, ic = 0, isub = 0, ibuf = 0;  // of the next stage to ask for
-    auto issue = [&] {
-        const uint8_t *q;
-        const uint16_t *d;
-        w_tile(ic, &q, &d);
-        // (past the row's end its last group again)
-        const int b = min(group(it) + isub * SJ, nb / 4 - 1), n = min(SJ, nb / 4 - b);
-        issue_stage<SJ>(l, q + (size_t)b * 64, d + 4 * b, n, mine + ibuf * S::BYTES);
-        ibuf = ibuf + 1 == R ? 0 : ibuf + 1;
-        if (++isub == SUBS) {
-            isub = 0;
-            if (++ic == 4) {
-                ic = 0;
-                ++it;
-            }
-        }
-    };
-    // x rows 8 m + li / 2 of the tile, hi or lo (rows past its end read nothing)
-    size_t xo[MT];
-    bool have[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        have[m] = 8 * m + (li >> 1) < tile.n;
-        const int i = pair_of(tile, 8 * m + (li >> 1));
-        xo[m] = (size_t)(UP ? i / K : i) * nb * 128 + lg * 32 + (li & 1) * 16;
-    }
-
-    // The set's sums from the waves that share it, two column tiles (of h: a gate and
-    // its up tile) at a time; a lane has column li of x rows 2 lg and 2 lg + 1, hi + lo.
-    auto store = [&](const f32x4 (&acc)[4][MT]) {
-        const int part = wave % ks;
-        if (ks == 1) lds_barrier();  // (pairs and scales)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const f32x4 a0 = acc[UP ? half : 2 * half][m], a1 = acc[UP ? half + 2 : 2 * half + 1][m];
-                float v[2][2] = {{a0[0] + a0[1], a0[2] + a0[3]}, {a1[0] + a1[1], a1[2] + a1[3]}};
-                if (ks > 1) {
-                    lds_barrier();  // the last reads of red
-                    if (part) red[wave / ks * (ks - 1) + part - 1][lane] = make_float4(v[0][0], v[0][1], v[1][0], v[1][1]);
-                    lds_barrier();
-                }
-                if (part || set >= sets) continue;
-                for (int w = 0; w < ks - 1; ++w) {
-                    const float4 o = red[wave / ks * (ks - 1) + w][lane];
-                    v[0][0] += o.x;
-                    v[0][1] += o.y;
-                    v[1][0] += o.z;
-                    v[1][1] += o.w;
-                }
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int i = 8 * m + 2 * lg + q;
-                    if (i >= tile.n) continue;
-                    const size_t at = (size_t)pairs[i] * N;
-                    const float sc = scales[i];
-                    if constexpr (UP) {
-                        a.h[at + set * 32 + half * 16 + li] = silu_mul(v[0][q] * sc, v[1][q] * sc);
-                    } else {
-                        const int col = set * 64 + half * 32 + li;
-                        if (col < N) a.z[at + col] = v[0][q] * sc;
-                        if (col + 16 < N) a.z[at + col + 16] = v[1][q] * sc;
-                    }
-                }
-            }
-    };
-
-    const int my_pair = pair_of(tile, min(tid, 8 * MT - 1));
+    // x rows of the lane's fragments, hi or lo of row li / 2 or both of row li (rows past
+    // the tile's end read nothing)
+    const int row = H == 1 ? li >> 1 : li, row_pair = pair_of(tile, row);
+    const size_t xo = (size_t)(UP ? row_pair / K : row_pair) * nb * 128 + lg * 32 + (H == 1 ? (li & 1) * 16 : 0);
+    const int my_pair = pair_of(tile, min(tid, T::ROWS - 1));
     const float my_scale = kUnscale * (UP ? a.xscale[my_pair / K] : a.p[my_pair] * a.hscale[my_pair]);
     auto put_scales = [&] {
-        if (tid >= 8 * MT) return;
+        if (tid >= T::ROWS) return;
         pairs[tid] = my_pair;
         scales[tid] = my_scale;
     };
-    f32x4 acc[4][MT] = {};
+
+    // A group's sums from the waves that share them, to h or z.  Eight rows: a lane's
+    // elements are hi and lo of rows 2 lg and 2 lg + 1, of 16 rows 4 lg to 4 lg + 3.
+    auto store = [&](int g, const f32x4 (&acc)[4]) {
+        lds_barrier();  // the last reads of red
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if constexpr (H == 1)
+                reinterpret_cast<float2 *>(red[wave][c])[lane] =
+                    make_float2(acc[c][0] + acc[c][1], acc[c][2] + acc[c][3]);
+            else
+                red[wave][c][lane] = acc[c];
+        lds_barrier();
+        // a thread: P rows of one column, which one lane of each wave holds (lanes along
+        // the columns: reads of P floats each, side by side)
+        constexpr int P = H == 1 ? 2 : 4;
+        using Rows = __attribute__((ext_vector_type(P))) float;
+        const int width = SET * cs;
+        for (int t = tid; t < T::ROWS / P * width; t += (int)blockDim.x) {
+            const int i = t / width * P, s = t % width / SET, n0 = t % SET;
+            const int col = (set0 + g * cs + s) * SET + n0;
+            if (i >= tile.n) break;
+            if (col >= N) continue;
+            const int from = i / P * 16 + (n0 & 15);
+            auto sum = [&](int c) {
+                Rows v = 0.0f;
+                for (int w = 0; w < ks; ++w)
+                    v += reinterpret_cast<const Rows *>(red[s * ks + w][c])[from];
+                return v;
+            };
+            const Rows v = sum(n0 >> 4), u = UP ? sum(2 + (n0 >> 4)) : v;
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                if (i + e >= tile.n) break;
+                const size_t at = (size_t)pairs[i + e] * N + col;
+                const float scale = scales[i + e];
+                if constexpr (UP) a.h[at] = silu_mul(v[e] * scale, u[e] * scale);
+                else a.z[at] = v[e] * scale;
+            }
+        }
+    };
+
     if constexpr (J == 0) {
-        Operands o;
+        for (int g = 0; g < n_groups; ++g) {
+            Operands o;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) w_tile(c, &o.q[c], &o.d[c]);
-        multiply_steps<MT>(o, img, xo, nb, wave % ks, ks, acc);
-        put_scales();
+            for (int c = 0; c < 4; ++c) w_tile(g, c, &o.q[c], &o.d[c]);
+            f32x4 acc[4] = {};
+            multiply_steps<H>(o, img, xo, nb, wave % ks, ks, acc);
+            if (g == 0) put_scales();
+            store(g, acc);
+        }
     } else {
-        int left = total, buf = 0;
-        u32x4 x[MT][4 * J];
-        for (int t = 0; t < rounds; ++t) {
-            const int b = group(t) * 4, n = t * ks + wave % ks < slices ? min(4 * J, nb - b) : 0;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-#pragma unroll
-                for (int i = 0; i < 4 * J; ++i) x[m][i] = u32x4{0, 0, 0, 0};
-                if (have[m]) {
-                    const uint8_t *p = img + xo[m] + (size_t)b * 128;
-#pragma unroll
-                    for (int i = 0; i < 4 * J; ++i)
-                        if (i < n) x[m][i] = *reinterpret_cast<const u32x4 *>(p + 128 * i);
+        unsigned char *const mine = ring + wave * R * S::BYTES;
+        const StageLane<SJ> l = stage_lane<SJ>(lane, nb);
+        const int slices = (nb + 4 * J - 1) / (4 * J), rounds = (slices + ks - 1) / ks;
+        // the wave's first group of blocks in a round (a wave without any goes through
+        // the row's last ones with no x)
+        auto first = [&](int t) { return min(t * ks + wave % ks, slices - 1) * J; };
+        int ig = 0, it = 0, ic = 0, isub = 0, ibuf = 0;  // of the next stage to ask for
+        auto issue = [&] {
+            const uint8_t *q;
+            const uint16_t *d;
+            w_tile(ig, ic, &q, &d);
+            // (past the row's end its last group again)
+            const int b = min(first(it) + isub * SJ, nb / 4 - 1), n = min(SJ, nb / 4 - b);
+            issue_stage<SJ>(l, q + (size_t)b * 64, d + 4 * b, n, mine + ibuf * S::BYTES);
+            ibuf = ibuf + 1 == R ? 0 : ibuf + 1;
+            if (++isub == SUBS) {
+                isub = 0;
+                if (++ic == 4) {
+                    ic = 0;
+                    if (++it == rounds) {
+                        it = 0;
+                        ++ig;
+                    }
                 }
             }
-            // (x ahead of the first stages: behind them it comes last, 48 rows 46 -> 55 us)
-            if (t == 0)
-                for (int k = 0; k < R - 1 && k < total; ++k) issue();
-            // here, or the compiler waits for x, and so for every stage that is on its
-            // way, before each stage
-            wait_vm<0>();
-            if (t == 0) put_scales();
+        };
+        const int total = n_groups * rounds * 4 * SUBS;
+        int left = total, buf = 0;
+        u32x4 x[H][4 * J];
+        for (int g = 0; g < n_groups; ++g) {
+            f32x4 acc[4] = {};
+            for (int t = 0; t < rounds; ++t) {
+                if (g == 0 || rounds > 1) {
+                    const int b = first(t) * 4, n = t * ks + wave % ks < slices ? min(4 * J, nb - b) : 0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+                    for (int i = 0; i < 4 * J; ++i)
 #pragma unroll
-                for (int sub = 0; sub < SUBS; ++sub) {
-                    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): reads of the buffer asked for next
-                    if (left >= R) {
-                        issue();
-                        wait_vm<(R - 1) * S::DMAS>();
-                    } else if (R > 3 && left == 3) {
-                        wait_vm<2 * S::DMAS>();
-                    } else if (R > 2 && left == 2) {
-                        wait_vm<S::DMAS>();
-                    } else if (R <= 4 || left == 1) {
-                        wait_vm<0>();
+                        for (int h = 0; h < H; ++h) x[h][i] = u32x4{0, 0, 0, 0};
+                    if (row < tile.n) {
+                        const uint8_t *p = img + xo + (size_t)b * 128;
+#pragma unroll
+                        for (int i = 0; i < 4 * J; ++i)
+                            if (i < n)
+#pragma unroll
+                                for (int h = 0; h < H; ++h)
+                                    x[h][i] = *reinterpret_cast<const u32x4 *>(p + 128 * i + 16 * h);
                     }
-                    multiply_stage<SJ, MT>(
-                        l, mine + buf * S::BYTES,
-                        [&](int m, int i) { return __builtin_bit_cast(f16x8, x[m][4 * SJ * sub + i]); },
-                        acc[c]);
-                    --left;
-                    buf = buf + 1 == R ? 0 : buf + 1;
+                    // (x ahead of the first stages: behind them it comes last, 48 rows
+                    // 46 -> 55 us)
+                    if (g + t == 0)
+                        for (int k = 0; k < R - 1 && k < total; ++k) issue();
+                    // here, or the compiler waits for x, and so for every stage that is on
+                    // its way, before each stage
+                    wait_vm<0>();
+                    if (g + t == 0) put_scales();
                 }
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int sub = 0; sub < SUBS; ++sub) {
+                        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): reads of the buffer asked for next
+                        if (left >= R) {
+                            issue();
+                            wait_vm<(R - 1) * S::DMAS>();
+                        } else if (R == 3 && left == 2) {
+                            wait_vm<S::DMAS>();
+                        } else {
+                            wait_vm<0>();
+                        }
+                        multiply_stage<SJ, H>(
+                            l, mine + buf * S::BYTES,
+                            [&](int h, int i) { return __builtin_bit_cast(f16x8, x[h][4 * SJ * sub + i]); },
+                            acc[c]);
+                        --left;
+                        buf = buf + 1 == R ? 0 : buf + 1;
+                    }
+            }
+            store(g, acc);
         }
     }
-    store(acc);
 }
 
 __global__ __launch_bounds__(256) void moe_split_kernel(MoeArgs a) {
@@ -784,7 +802,7 @@ __global__ __launch_bounds__(kRowThreads) void moe_up_row_kernel(MoeArgs a) {
     const int li = lane & 15, lg = lane >> 4, nb = a.m.dim / 32;
     const size_t w0 = ((size_t)e * hidden + col) * nb;
     const uint8_t *const img = a.ximg + lg * 32 + (li & 1) * 16;
-    f32x4 acc[4][1] = {};
+    f32x4 acc[4] = {};
     if constexpr (DMA) {
         unsigned char *const mine = ring + wave * R * S::BYTES;
         const StageLane<J> l = stage_lane<J>(lane, nb);
@@ -822,13 +840,13 @@ __global__ __launch_bounds__(kRowThreads) void moe_up_row_kernel(MoeArgs a) {
             o.q[c] = (c & 1 ? a.m.up_quants : a.m.gate_quants) + w0 * 16;
             o.d[c] = (c & 1 ? a.m.up_scales : a.m.gate_scales) + w0;
         }
-        const size_t xo[1] = {(size_t)(lg * 32 + (li & 1) * 16)};
+        const size_t xo = lg * 32 + (li & 1) * 16;
         multiply_steps<1>(o, a.ximg, xo, nb, wave, kRowWaves, acc);
     }
     // every two rows are the row's hi and lo
     if (lane < 16) {
-        red[wave][0][lane] = acc[0][0][0] + acc[0][0][1];
-        red[wave][1][lane] = acc[1][0][0] + acc[1][0][1];
+        red[wave][0][lane] = acc[0][0] + acc[0][1];
+        red[wave][1][lane] = acc[1][0] + acc[1][1];
     }
     __syncthreads();
     if (tid >= 16) return;
@@ -950,7 +968,7 @@ __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
         __builtin_amdgcn_wave_barrier();
         // every two rows of the fragment are h's hi and lo
         const u32x4 *const x = &img[wave][lg * 2 + (li & 1)];
-        f32x4 acc[1] = {};
+        f32x4 acc = {};
         if constexpr (DMA) {
             multiply_stage<J, 1>(l, at,
                                  [&](int, int i) { return __builtin_bit_cast(f16x8, x[8 * i]); }, acc);
@@ -965,11 +983,11 @@ __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
                                            f32x4{0.f, 0.f, 0.f, 0.f});
                     const f16x2 d2 = __builtin_bit_cast(f16x2, t < 2 ? d[i].x : d[i].y);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[0][k] = __builtin_fmaf((float)d2[t & 1], v[k], acc[0][k]);
+                    for (int k = 0; k < 4; ++k) acc[k] = __builtin_fmaf((float)d2[t & 1], v[k], acc[k]);
                 }
             }
         }
-        total = __builtin_fmaf(kUnscale * ldexpf(1.0f, ex), acc[0][0] + acc[0][1], total);
+        total = __builtin_fmaf(kUnscale * ldexpf(1.0f, ex), acc[0] + acc[1], total);
         buf = buf + 1 == R ? 0 : buf + 1;
         s += J;
         if (s >= s1) {
@@ -1053,51 +1071,61 @@ int run_down_rows(cw_ctx *ctx, const MoeArgs &a) {
                   grid, dim3(256), 0, a);
 }
 
-// How the waves of a workgroup divide a product: J groups of blocks a stage (0:
-// through registers) and ks waves to a sum.
+// How the waves of a workgroup divide a product: J groups of blocks of x each (0:
+// through registers), ks waves to a sum, cs sets at a time, `groups` of those.
 struct TilePlan {
-    int J, ks, grid;
+    int J, ks, cs, groups, grid;
 };
-TilePlan tile_plan(bool up, const cw_moe &m, int mt) {
-    const int nb = (up ? m.dim : m.hidden) / 32, N = up ? m.hidden : m.dim;
+template <int H>
+TilePlan tile_plan(const cw_ctx *ctx, bool up, const cw_moe &m, int tiles) {
+    constexpr int W = 4 * H;
+    const int nb = (up ? m.dim : m.hidden) / 32, sets = up ? m.hidden / 32 : (m.dim + 63) / 64;
     const bool dma = up ? whole_groups(m.dim, m.gate_scales) && whole_groups(m.dim, m.up_scales)
                         : whole_groups(m.hidden, m.down_scales);
-    TilePlan p{0, nb >= 64 ? 4 : nb >= 16 ? 2 : 1, 0};
+    TilePlan p{0, nb >= 64 ? 4 : nb >= 16 ? 2 : 1, 1, 1, 0};
+    int rounds = 1;
     if (dma) {
-        // the most of the stages' blocks that exist, then the fewest rounds
+        // 16 rows: x of all of the sum if that fits; then the most of the waves' and the
+        // stages' blocks that exist, and the fewest rounds
         int best = -1;
-        for (int J = mt == 4 ? 2 : 4; J >= 2; --J)
-            for (int ks = 4; ks >= 1; ks /= 2) {
-                const int rounds = ((nb + 4 * J - 1) / (4 * J) + ks - 1) / ks;
-                const int score = nb * 1000 / (rounds * ks * 4 * J) * 64 - std::min(rounds, 63);
+        for (int J = H == 1 ? 4 : 2; J >= 2; --J)
+            for (int ks = W; ks >= 1; --ks) {
+                const int r = ((nb + 4 * J - 1) / (4 * J) + ks - 1) / ks;
+                const int used = nb * 1000 / (r * ks * 4 * J) * (W / ks * ks) / W;
+                const int score = (H == 2 && r == 1 ? 1 << 20 : 0) + used * 64 - std::min(r, 63);
                 if (score > best) {
                     best = score;
                     p.J = J;
                     p.ks = ks;
+                    rounds = r;
                 }
             }
     }
-    const int sets = (up ? N / 32 : (N + 63) / 64), per = kWaves / p.ks;
-    p.grid = (sets + per - 1) / per;
+    p.cs = std::max(1, std::min(W / p.ks, sets));
+    const int units = (sets + p.cs - 1) / p.cs;
+    // 16 rows' x is read again for every workgroup: no more of them than fill the chip's
+    // places (two a CU) twice (500 rows, 8 of 128 experts: once 271 us, twice 260, four
+    // times 293, one set each 495 at 800 rows for 355)
+    if (H == 2 && rounds == 1) p.groups = std::min(std::max(1, tiles * units / (4 * ctx->n_cu)), units);
+    p.grid = (units + p.groups - 1) / p.groups;
     return p;
 }
 
-template <bool UP, int MT>
-int launch_tiles(cw_ctx *ctx, const MoeArgs &a, int most) {
-    const TilePlan p = tile_plan(UP, a.m, MT);
-    auto fn = p.J == 0 ? moe_tile_kernel<UP, MT, 0> : moe_tile_kernel<UP, MT, 2>;
-    if constexpr (MT < 4) {
-        if (p.J == 3) fn = moe_tile_kernel<UP, MT, 3>;
-        if (p.J == 4) fn = moe_tile_kernel<UP, MT, 4>;
+template <bool UP, int H>
+int launch_tiles(cw_ctx *ctx, const MoeArgs &a, int most, int tiles) {
+    const TilePlan p = tile_plan<H>(ctx, UP, a.m, tiles);
+    auto fn = p.J == 0 ? moe_tile_kernel<UP, H, 0> : moe_tile_kernel<UP, H, 2>;
+    if constexpr (H == 1) {
+        if (p.J == 3) fn = moe_tile_kernel<UP, H, 3>;
+        if (p.J == 4) fn = moe_tile_kernel<UP, H, 4>;
     }
-    return launch(ctx, UP ? "moe_up" : "moe_down", fn, dim3(p.grid, most), dim3(kThreads), 0, a, p.ks);
+    return launch(ctx, UP ? "moe_up" : "moe_down", fn, dim3(p.grid, most), dim3(64 * p.ks * p.cs), 0, a,
+                  p.ks, p.groups);
 }
 
 template <bool UP>
-int launch_product(cw_ctx *ctx, const MoeArgs &a, int mt, int most) {
-    return mt == 1 ? launch_tiles<UP, 1>(ctx, a, most)
-           : mt == 2 ? launch_tiles<UP, 2>(ctx, a, most)
-                     : launch_tiles<UP, 4>(ctx, a, most);
+int launch_product(cw_ctx *ctx, const MoeArgs &a, int h, int most, int tiles) {
+    return h == 1 ? launch_tiles<UP, 1>(ctx, a, most, tiles) : launch_tiles<UP, 2>(ctx, a, most, tiles);
 }
 
 int run(cw_ctx *ctx, const MoeArgs &a) {
@@ -1110,15 +1138,19 @@ int run(cw_ctx *ctx, const MoeArgs &a) {
         return run_down_rows(ctx, a);
     }
     const int mean = (pairs + E - 1) / E;
-    const int mt = mean <= 5 ? 1 : mean <= 12 ? 2 : 4, tile = kTile * mt;
+    // Tiles of eight rows up to ten an expert, else of 16 (us with 8 and with 16; 8 of 128
+    // experts, 2048 x 768: 7 rows an expert 113, 119; 10: 136, 138; 15: 171, 160; 31: 294,
+    // 260; 2 of 8, 4096 x 12288: 8 rows 200, 212; 12: 258, 253; 40: 588, 564).
+    const int h = mean <= 10 ? 1 : 2, tile = kTile * h;
     const int score = (E + 15) / 16 * ((a.rows + 15) / 16) * a.splits;
     CW_TRY(launch(ctx, "moe_score", moe_score_kernel, dim3(score + a.rows), dim3(256), 0, a));
     CW_TRY(launch(ctx, "moe_choose", moe_choose_kernel, dim3(a.rows), dim3(1024), 0, a));
-    const int most = std::min(pairs, E + pairs / tile);  // tiles
-    CW_TRY(launch_product<true>(ctx, a, mt, most));
+    // tiles at most, and how many to expect of rows that choose evenly
+    const int most = std::min(pairs, E + pairs / tile), tiles = std::min(pairs, std::max(E, pairs / tile));
+    CW_TRY(launch_product<true>(ctx, a, h, most, tiles));
     if (down_by_rows(a.m, a.rows)) return run_down_rows(ctx, a);
     CW_TRY(launch(ctx, "moe_split", moe_split_kernel, dim3(pairs), dim3(256), 0, a));
-    CW_TRY(launch_product<false>(ctx, a, mt, most));
+    CW_TRY(launch_product<false>(ctx, a, h, most, tiles));
     return launch(ctx, "moe_sum", moe_sum_kernel, dim3((a.m.dim + 1023) / 1024, a.rows), dim3(256), 0, a);
 }
 

@@ -70,6 +70,8 @@ SHAPES = [
     (300, 160, 96, 16, 4, False),
     (33, 4096, 128, 9, 3, True),
     (21, 128, 4128, 4, 2, True),
+    (512, 256, 4096, 8, 4, True),
+    (600, 4096, 256, 8, 8, False),
 ]
 
 
