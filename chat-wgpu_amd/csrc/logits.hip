@@ -9,12 +9,13 @@
 // l_t) over v != t.  s is kept without the token's own 1, which for a likely
 // token would take all of s's digits.
 //
-// One pass over the logits.  A workgroup has a slice of a row's vocabulary and
-// counts the slice's tokens in LDS: it reads the request's whole history and
-// keeps what falls into its slice, so no count goes through memory.  Counts are
-// whole numbers and a bias is chosen by its place in the list, so the order of the
-// LDS atomics does not show.  (max, s, index) of the slices are joined by a second
-// launch in a fixed order.
+// One pass over the logits.  A workgroup has a slice of a row's vocabulary, whose
+// logits its threads ask for first and keep in registers.  It counts the slice's tokens
+// in LDS: it reads the request's whole history, eight tokens a thread in flight, and
+// keeps what falls into its slice, so no count goes through memory.  Counts are whole
+// numbers and a bias is chosen by its place in the list, so the order of the LDS
+// atomics does not show.  Each wave then has its largest logit, and one exp for each
+// other.  (max, s, index) of the slices are joined by a second launch in a fixed order.
 
 #include "paged_device.hpp"
 
@@ -37,7 +38,7 @@ struct LogitArgs {
     int vocab;
     float *out;
     size_t out_stride;
-    int slice, parts;  // tokens a workgroup takes (a multiple of 32), workgroups a row
+    int parts;         // workgroups a row
     struct Top *part;  // [rows][parts]; null: no token is wanted
     uint32_t *token;
     float *logprob;
@@ -78,128 +79,184 @@ __device__ __forceinline__ V rule(const V *p, int b, V none) {
     return p ? p[b] : none;
 }
 
-// V logits at a time: 4 where rows are 16-byte aligned and whole fours, else 1.
-template <int V>
+// The first request whose rows the batch row is among, n_seq if none; by every wave.
+__device__ __forceinline__ int owner_of(const LogitArgs &a, int br) {
+    constexpr int U = 4;
+    for (int b0 = 0; b0 < a.n_seq; b0 += 64 * U) {
+        int r0[U], r1[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int b = min(b0 + 64 * u + (int)(threadIdx.x & 63), a.n_seq - 1);
+            r0[u] = a.first_row[b];
+            r1[u] = a.first_row[b + 1];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            // (past the last request the last again)
+            const uint64_t has = __ballot(r0[u] >= 0 && r0[u] <= br && br < r1[u] && r1[u] <= a.batch_rows);
+            if (has) return min(b0 + 64 * u + __builtin_ctzll(has), a.n_seq - 1);
+        }
+    }
+    return a.n_seq;
+}
+
+// IT runs of V logits a thread, V = 4 where rows are 16-byte aligned and whole fours.
+template <int V, int IT>
 __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
-    extern __shared__ uint32_t lds[];
-    __shared__ int owner;
+    constexpr int N = V * IT, kSlice = kThreads * N;
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ Top tops[kThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const size_t row = blockIdx.y;
-    const int lo = blockIdx.x * a.slice, n = min(a.slice, a.vocab - lo);
+    const int lo = blockIdx.x * kSlice, n = min(kSlice, a.vocab - lo);
     const bool counts = a.r.tokens || a.r.node_token, biased = a.r.bias;
-    uint32_t *const count = lds, *const last = lds + (counts ? a.slice : 0);
+    uint32_t *const count = lds, *const last = lds + (counts ? kSlice : 0);
 
-    // the request whose rows the batch row is among
     const int br = a.at ? a.at[row] : (int)row;
-    if (tid == 0) owner = a.n_seq;
-    for (int v = tid; v < (counts + biased) * a.slice; v += kThreads) lds[v] = 0;
-    __syncthreads();
-    for (int b = tid; b < a.n_seq; b += kThreads) {
-        const int r0 = a.first_row[b], r1 = a.first_row[b + 1];
-        if (r0 >= 0 && r0 <= br && br < r1 && r1 <= a.batch_rows) atomicMin(&owner, b);
-    }
-    __syncthreads();
-    const int b = owner;
+    const int b = owner_of(a, br);
     if (b == a.n_seq) {
         if (a.part && tid == 0) a.part[row * a.parts + blockIdx.x].i = kPadding;
         return;
     }
-    auto add = [&](int v, bool made) {
-        if ((unsigned)(v - lo) < (unsigned)n) {
-            if (made) atomicAdd(&count[v - lo], 1u);
-            else atomicOr(&count[v - lo], kPrompt);
-        }
-    };
-    if (a.r.tokens) {
-        const int len = min(max(a.r.length[b], 0), a.r.max_len), made = rule(a.r.prompt, b, 0);
-        const int *t = a.r.tokens + (size_t)b * a.r.max_len;
-        for (int i = tid; i < len; i += kThreads) add(t[i], i >= made);
-    }
-    if (a.r.node_token) {
-        const int r0 = a.first_row[b], nodes = a.first_row[b + 1] - r0, self = br - r0;
-        for (int j = tid; j < nodes; j += kThreads) {
-            const bool sees = !a.mask ? j <= self
-                                      : j < 32 * a.mask_words &&
-                                            (a.mask[(size_t)br * a.mask_words + (j >> 5)] >> (j & 31) & 1);
-            if (sees) add(a.r.node_token[r0 + j], true);
-        }
-    }
-    if (biased) {
-        const int e0 = a.r.bias_first[b], e1 = a.r.bias_first[b + 1];
-        if (e0 >= 0 && e1 <= a.r.n_bias)
-            for (int e = e0 + tid; e < e1; e += kThreads) {
-                const int v = a.r.bias_token[e];
-                if ((unsigned)(v - lo) < (unsigned)n) atomicMax(&last[v - lo], (uint32_t)e + 1);
+    // the thread's logits: V from at(0), V from at(1), ...
+    auto at = [&](int it) { return (it * kThreads + tid) * V; };
+    const float *x = a.x + row * a.stride + lo;
+    float l[N];
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) l[it * V + j] = -INFINITY;
+        if (at(it) < n) {
+            if constexpr (V == 4) {
+                const float4 q = *reinterpret_cast<const float4 *>(x + at(it));
+                l[4 * it] = q.x;
+                l[4 * it + 1] = q.y;
+                l[4 * it + 2] = q.z;
+                l[4 * it + 3] = q.w;
+            } else {
+                l[it] = x[at(it)];
             }
+        }
     }
-    const float repeat = rule(a.r.repeat, b, 1.0f), presence = rule(a.r.presence, b, 0.0f);
-    const float frequency = rule(a.r.frequency, b, 0.0f);
+    uint32_t bits[IT];
     const uint32_t *allowed = nullptr;
     if (a.r.allowed) {
         const int k = a.r.allowed_row ? a.r.allowed_row[row] : (int)row;
         if ((unsigned)k < (unsigned)a.r.n_allowed) allowed = a.r.allowed + (size_t)k * a.r.allowed_words;
     }
-    __syncthreads();
+#pragma unroll
+    for (int it = 0; it < IT; ++it)
+        bits[it] = allowed && at(it) < n ? allowed[(lo + at(it)) >> 5] : ~0u;
 
-    const float *x = a.x + row * a.stride;
-    Top top{-INFINITY, 0.0f, kNone};
-    for (int v0 = lo + tid * V; v0 < lo + n; v0 += kThreads * V) {
-        float l[V];
-        if constexpr (V == 4) {
-            const float4 q = *reinterpret_cast<const float4 *>(x + v0);
-            l[0] = q.x;
-            l[1] = q.y;
-            l[2] = q.z;
-            l[3] = q.w;
-        } else {
-            l[0] = x[v0];
+    if (counts || biased) {
+        for (int v = tid; v < (counts + biased) * kSlice / 4; v += kThreads)
+            reinterpret_cast<uint4 *>(lds)[v] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        auto add = [&](int v, bool made) {
+            if ((unsigned)(v - lo) < (unsigned)n) {
+                if (made) atomicAdd(&count[v - lo], 1u);
+                else atomicOr(&count[v - lo], kPrompt);
+            }
+        };
+        if (a.r.tokens) {
+            constexpr int U = 8;
+            const int len = min(max(a.r.length[b], 0), a.r.max_len), made = rule(a.r.prompt, b, 0);
+            const int *t = a.r.tokens + (size_t)b * a.r.max_len;
+            for (int i = tid; i < len; i += U * kThreads) {
+                int v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = t[min(i + u * kThreads, len - 1)];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (i + u * kThreads < len) add(v[u], i + u * kThreads >= made);
+            }
         }
-        const uint32_t bits = allowed ? allowed[v0 >> 5] >> (v0 & 31) : ~0u;
-        float best = top.m;
-        int at = -1;
+        if (a.r.node_token) {
+            const int r0 = a.first_row[b], nodes = a.first_row[b + 1] - r0, self = br - r0;
+            for (int j = tid; j < nodes; j += kThreads) {
+                const bool sees =
+                    !a.mask ? j <= self
+                            : j < 32 * a.mask_words &&
+                                  (a.mask[(size_t)br * a.mask_words + (j >> 5)] >> (j & 31) & 1);
+                const int v = a.r.node_token[r0 + j];
+                if (sees) add(v, true);
+            }
+        }
+        if (biased) {
+            const int e0 = a.r.bias_first[b], e1 = a.r.bias_first[b + 1];
+            if (e0 >= 0 && e1 <= a.r.n_bias)
+                for (int e = e0 + tid; e < e1; e += kThreads) {
+                    const int v = a.r.bias_token[e];
+                    if ((unsigned)(v - lo) < (unsigned)n) atomicMax(&last[v - lo], (uint32_t)e + 1);
+                }
+        }
+        __syncthreads();
+    }
+    const float repeat = rule(a.r.repeat, b, 1.0f), presence = rule(a.r.presence, b, 0.0f);
+    const float frequency = rule(a.r.frequency, b, 0.0f);
+
+    Top top{-INFINITY, 0.0f, kNone};
+    int own = -1;  // of the thread's logits
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        const uint32_t allow = bits[it] >> ((lo + at(it)) & 31);
+        uint32_t c[V] = {}, e[V] = {};
+        if (counts)
+#pragma unroll
+            for (int j = 0; j < V; ++j) c[j] = count[at(it) + j];
+        if (biased)
+#pragma unroll
+            for (int j = 0; j < V; ++j) e[j] = last[at(it) + j];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            if (counts) {
-                const uint32_t c = count[v0 - lo + j];
-                if (c) {
-                    l[j] = l[j] > 0.0f ? l[j] / repeat : l[j] * repeat;
-                    const uint32_t made = c & ~kPrompt;
-                    if (made) l[j] = __builtin_fmaf(-frequency, (float)made, l[j]) - presence;
-                }
+            float v = l[it * V + j];
+            if (c[j]) {
+                v = v > 0.0f ? v / repeat : v * repeat;
+                const uint32_t made = c[j] & ~kPrompt;
+                if (made) v = __builtin_fmaf(-frequency, (float)made, v) - presence;
             }
-            if (biased) {
-                const uint32_t e = last[v0 - lo + j];
-                if (e) l[j] += a.r.bias[e - 1];
+            if (e[j]) v += a.r.bias[e[j] - 1];
+            if (!(allow >> j & 1)) v = -INFINITY;
+            if (v > top.m) {
+                top.m = v;
+                own = it * V + j;
             }
-            if (!(bits >> j & 1)) l[j] = -INFINITY;
-            if (l[j] > best) {
-                best = l[j];
-                at = j;
-            }
+            l[it * V + j] = v;
         }
-        if (a.out) {
-            float *o = a.out + row * a.out_stride + v0;
-            if constexpr (V == 4) *reinterpret_cast<float4 *>(o) = make_float4(l[0], l[1], l[2], l[3]);
-            else o[0] = l[0];
-        }
-        if (a.part) {
-            if (at >= 0) {
-                // (1 + s: the former largest is now one of the others)
-                if (top.i >= 0) top.s = (1.0f + top.s) * expf(top.m - best);
-                top.m = best;
-                top.i = v0 + at;
-            }
-            const float m = top.i >= 0 ? top.m : 0.0f;  // (-inf - -inf)
-#pragma unroll
-            for (int j = 0; j < V; ++j) top.s += j == at ? 0.0f : expf(l[j] - m);
+        if (a.out && at(it) < n) {
+            float *o = a.out + row * a.out_stride + lo + at(it);
+            if constexpr (V == 4)
+                *reinterpret_cast<float4 *>(o) =
+                    make_float4(l[4 * it], l[4 * it + 1], l[4 * it + 2], l[4 * it + 3]);
+            else
+                o[0] = l[it];
         }
     }
     if (!a.part) return;
-    top = wave_join(top);
-    if (lane == 0) tops[wave] = top;
+    // the wave's largest, then the others' exponentials below it
+    if (own >= 0) top.i = lo + at(own / V) + own % V;
+    int best = own >= 0 ? top.i : INT_MAX;
+    float m = top.m;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const float om = __shfl_xor(m, d);
+        const int oi = __shfl_xor(best, d);
+        if (om > m || (om == m && oi < best)) {
+            m = om;
+            best = oi;
+        }
+    }
+    if (best != top.i) own = -1;
+    const float below = best == INT_MAX ? 0.0f : m;  // (-inf - -inf)
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) s += k == own ? 0.0f : expf(l[k] - below);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+    if (lane == 0) tops[wave] = Top{m, s, best == INT_MAX ? kNone : best};
     __syncthreads();
     if (tid == 0) {
+        top = tops[0];
         for (int w = 1; w < kThreads / 64; ++w) top = join(top, tops[w]);
         a.part[row * a.parts + blockIdx.x] = top;
     }
@@ -270,18 +327,22 @@ extern "C" int cw_logits_rows(cw_ctx *ctx, const cw_logit_rules *rules, const cw
     a.out_stride = out_stride;
     a.token = token;
     a.logprob = logprob;
-    a.slice = 4096;
-    a.parts = (vocab + a.slice - 1) / a.slice;
+    const bool wide = aligned16(logits) && stride % 4 == 0 && vocab % 4 == 0 &&
+                      (!out || (aligned16(out) && out_stride % 4 == 0));
+    // Slices of 4096 tokens where they fill the chip, else of 1024.
+    const bool few = (long)rows * ((vocab + 4095) / 4096) < 2 * ctx->n_cu;
+    const int slice = few ? 1024 : 4096;
+    a.parts = (vocab + slice - 1) / slice;
     if (token || logprob) {
         void *scratch = nullptr;
         CW_TRY(ctx_scratch(ctx, (size_t)rows * a.parts * sizeof(Top), &scratch));
         a.part = static_cast<Top *>(scratch);
     }
     const int tables = (r.tokens || r.node_token ? 1 : 0) + (r.bias ? 1 : 0);
-    const bool wide = aligned16(logits) && stride % 4 == 0 && vocab % 4 == 0 &&
-                      (!out || (aligned16(out) && out_stride % 4 == 0));
-    CW_TRY(launch(ctx, "logits_rows", wide ? logits_kernel<4> : logits_kernel<1>,
-                  dim3(a.parts, rows), dim3(kThreads), tables * a.slice * 4, a));
+    CW_TRY(launch(ctx, "logits_rows",
+                  wide ? few ? logits_kernel<4, 1> : logits_kernel<4, 4>
+                       : few ? logits_kernel<1, 4> : logits_kernel<1, 16>,
+                  dim3(a.parts, rows), dim3(kThreads), tables * slice * 4, a));
     if (!a.part) return CW_OK;
     return launch(ctx, "logits_join", logits_join_kernel, dim3(rows), dim3(64), 0, a);
 }
