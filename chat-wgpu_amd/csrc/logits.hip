@@ -14,10 +14,17 @@
 // in LDS: it reads the request's whole history, eight tokens a thread in flight, and
 // keeps what falls into its slice, so no count goes through memory.  Counts are whole
 // numbers and a bias is chosen by its place in the list, so the order of the LDS
-// atomics does not show.  Each wave then has its largest logit, and one exp for each
-// other.  (max, s, index) of the slices are joined by a second launch in a fixed order.
+// atomics does not show.  Each wave then has its largest logit, and one exponential for
+// each other.  (max, s, index) of the slices are joined by a second launch in a fixed
+// order.
+//
+// What bounds it, at 151936 tokens: two launches for one row (5.4 + 4.5 us).  61 rows
+// after 4100 tokens take 20 us for 37 MB: their vector instructions alone are 11 us, the
+// counts 8 us of the whole (each of the 38 slices reads the history).  48 rows with
+// masks, biases and out take 23 us for 55 MB, 14 without the counts.
 
 #include "paged_device.hpp"
+#include "prompt_device.hpp"
 
 namespace {
 
@@ -79,25 +86,24 @@ __device__ __forceinline__ V rule(const V *p, int b, V none) {
     return p ? p[b] : none;
 }
 
+// Requests from b0 on, one a lane (past the last one the last again).
+struct Owners {
+    int r0, r1;
+};
+__device__ __forceinline__ Owners owners(const LogitArgs &a, int b0) {
+    const int b = min(b0 + (int)(threadIdx.x & 63), a.n_seq - 1);
+    return Owners{a.first_row[b], a.first_row[b + 1]};
+}
+
 // The first request whose rows the batch row is among, n_seq if none; by every wave.
-__device__ __forceinline__ int owner_of(const LogitArgs &a, int br) {
-    constexpr int U = 4;
-    for (int b0 = 0; b0 < a.n_seq; b0 += 64 * U) {
-        int r0[U], r1[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int b = min(b0 + 64 * u + (int)(threadIdx.x & 63), a.n_seq - 1);
-            r0[u] = a.first_row[b];
-            r1[u] = a.first_row[b + 1];
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            // (past the last request the last again)
-            const uint64_t has = __ballot(r0[u] >= 0 && r0[u] <= br && br < r1[u] && r1[u] <= a.batch_rows);
-            if (has) return min(b0 + 64 * u + __builtin_ctzll(has), a.n_seq - 1);
-        }
+__device__ __forceinline__ int owner_of(const LogitArgs &a, Owners o, int br) {
+    for (int b0 = 0;;) {
+        const uint64_t has = __ballot(o.r0 >= 0 && o.r0 <= br && br < o.r1 && o.r1 <= a.batch_rows);
+        if (has) return min(b0 + __builtin_ctzll(has), a.n_seq - 1);
+        b0 += 64;
+        if (b0 >= a.n_seq) return a.n_seq;
+        o = owners(a, b0);
     }
-    return a.n_seq;
 }
 
 // IT runs of V logits a thread, V = 4 where rows are 16-byte aligned and whole fours.
@@ -112,12 +118,9 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
     const bool counts = a.r.tokens || a.r.node_token, biased = a.r.bias;
     uint32_t *const count = lds, *const last = lds + (counts ? kSlice : 0);
 
+    // What is to come from memory is asked for in the order of its use.
+    const Owners first = owners(a, 0);
     const int br = a.at ? a.at[row] : (int)row;
-    const int b = owner_of(a, br);
-    if (b == a.n_seq) {
-        if (a.part && tid == 0) a.part[row * a.parts + blockIdx.x].i = kPadding;
-        return;
-    }
     // the thread's logits: V from at(0), V from at(1), ...
     auto at = [&](int it) { return (it * kThreads + tid) * V; };
     const float *x = a.x + row * a.stride + lo;
@@ -148,31 +151,39 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
     for (int it = 0; it < IT; ++it)
         bits[it] = allowed && at(it) < n ? allowed[(lo + at(it)) >> 5] : ~0u;
 
-    if (counts || biased) {
-        for (int v = tid; v < (counts + biased) * kSlice / 4; v += kThreads)
-            reinterpret_cast<uint4 *>(lds)[v] = make_uint4(0, 0, 0, 0);
-        __syncthreads();
+    const int tables = counts + biased;
+    for (int v = tid; v < tables * kSlice / 4; v += kThreads)
+        reinterpret_cast<uint4 *>(lds)[v] = make_uint4(0, 0, 0, 0);
+    const int b = owner_of(a, first, br);
+    if (b == a.n_seq) {
+        if (a.part && tid == 0) a.part[row * a.parts + blockIdx.x].i = kPadding;
+        return;
+    }
+    const float repeat = rule(a.r.repeat, b, 1.0f), presence = rule(a.r.presence, b, 0.0f);
+    const float frequency = rule(a.r.frequency, b, 0.0f);
+    const int len = a.r.tokens ? min(max(a.r.length[b], 0), a.r.max_len) : 0;
+    const int prompt = rule(a.r.prompt, b, 0);
+    const int r0 = a.first_row[b], nodes = a.first_row[b + 1] - r0, self = br - r0;
+    const int e0 = biased ? a.r.bias_first[b] : 0, e1 = biased ? a.r.bias_first[b + 1] : 0;
+    if (tables) {
+        lds_barrier();
         auto add = [&](int v, bool made) {
             if ((unsigned)(v - lo) < (unsigned)n) {
                 if (made) atomicAdd(&count[v - lo], 1u);
                 else atomicOr(&count[v - lo], kPrompt);
             }
         };
-        if (a.r.tokens) {
-            constexpr int U = 8;
-            const int len = min(max(a.r.length[b], 0), a.r.max_len), made = rule(a.r.prompt, b, 0);
-            const int *t = a.r.tokens + (size_t)b * a.r.max_len;
-            for (int i = tid; i < len; i += U * kThreads) {
-                int v[U];
+        constexpr int U = 8;
+        const int *t = a.r.tokens + (size_t)b * a.r.max_len;
+        for (int i = tid; i < len; i += U * kThreads) {
+            int v[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) v[u] = t[min(i + u * kThreads, len - 1)];
+            for (int u = 0; u < U; ++u) v[u] = t[min(i + u * kThreads, len - 1)];
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (i + u * kThreads < len) add(v[u], i + u * kThreads >= made);
-            }
+            for (int u = 0; u < U; ++u)
+                if (i + u * kThreads < len) add(v[u], i + u * kThreads >= prompt);
         }
-        if (a.r.node_token) {
-            const int r0 = a.first_row[b], nodes = a.first_row[b + 1] - r0, self = br - r0;
+        if (a.r.node_token)
             for (int j = tid; j < nodes; j += kThreads) {
                 const bool sees =
                     !a.mask ? j <= self
@@ -181,47 +192,44 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
                 const int v = a.r.node_token[r0 + j];
                 if (sees) add(v, true);
             }
-        }
-        if (biased) {
-            const int e0 = a.r.bias_first[b], e1 = a.r.bias_first[b + 1];
-            if (e0 >= 0 && e1 <= a.r.n_bias)
-                for (int e = e0 + tid; e < e1; e += kThreads) {
-                    const int v = a.r.bias_token[e];
-                    if ((unsigned)(v - lo) < (unsigned)n) atomicMax(&last[v - lo], (uint32_t)e + 1);
-                }
-        }
-        __syncthreads();
+        if (biased && e0 >= 0 && e1 <= a.r.n_bias)
+            for (int e = e0 + tid; e < e1; e += kThreads) {
+                const int v = a.r.bias_token[e];
+                if ((unsigned)(v - lo) < (unsigned)n) atomicMax(&last[v - lo], (uint32_t)e + 1);
+            }
+        lds_barrier();
     }
-    const float repeat = rule(a.r.repeat, b, 1.0f), presence = rule(a.r.presence, b, 0.0f);
-    const float frequency = rule(a.r.frequency, b, 0.0f);
 
-    Top top{-INFINITY, 0.0f, kNone};
-    int own = -1;  // of the thread's logits
+    // (no branch for the few that change: nearly every wave would take it for each logit.
+    // With inv the nearest to 1 / repeat, v inv and one step after it are v / repeat to
+    // its last bit; infinities and zeros have no step.)
+    const float inv = 1.0f / repeat;
+    float m = -INFINITY;
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
-        const uint32_t allow = bits[it] >> ((lo + at(it)) & 31);
-        uint32_t c[V] = {}, e[V] = {};
-        if (counts)
+        if (counts) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) c[j] = count[at(it) + j];
-        if (biased)
-#pragma unroll
-            for (int j = 0; j < V; ++j) e[j] = last[at(it) + j];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            float v = l[it * V + j];
-            if (c[j]) {
-                v = v > 0.0f ? v / repeat : v * repeat;
-                const uint32_t made = c[j] & ~kPrompt;
-                if (made) v = __builtin_fmaf(-frequency, (float)made, v) - presence;
+            for (int j = 0; j < V; ++j) {
+                const uint32_t c = count[at(it) + j], made = c & ~kPrompt;
+                float v = l[it * V + j];
+                const float q = v * inv, step = __builtin_fmaf(__builtin_fmaf(-q, repeat, v), inv, q);
+                const float less = step == step ? step : q;
+                v = c ? (v > 0.0f ? less : v * repeat) : v;
+                l[it * V + j] =
+                    __builtin_fmaf(made ? -frequency : 0.0f, (float)made, v) - (made ? presence : 0.0f);
             }
-            if (e[j]) v += a.r.bias[e[j] - 1];
-            if (!(allow >> j & 1)) v = -INFINITY;
-            if (v > top.m) {
-                top.m = v;
-                own = it * V + j;
+        }
+        if (biased) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const uint32_t e = last[at(it) + j];
+                if (e) l[it * V + j] += a.r.bias[e - 1];
             }
-            l[it * V + j] = v;
+        }
+        if (allowed) {
+            const uint32_t allow = bits[it] >> ((lo + at(it)) & 31);
+#pragma unroll
+            for (int j = 0; j < V; ++j) l[it * V + j] = allow >> j & 1 ? l[it * V + j] : -INFINITY;
         }
         if (a.out && at(it) < n) {
             float *o = a.out + row * a.out_stride + lo + at(it);
@@ -231,29 +239,51 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
             else
                 o[0] = l[it];
         }
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = fmaxf(m, l[it * V + j]);
     }
     if (!a.part) return;
-    // the wave's largest, then the others' exponentials below it
-    if (own >= 0) top.i = lo + at(own / V) + own % V;
-    int best = own >= 0 ? top.i : INT_MAX;
-    float m = top.m;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const float om = __shfl_xor(m, d);
-        const int oi = __shfl_xor(best, d);
-        if (om > m || (om == m && oi < best)) {
-            m = om;
-            best = oi;
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    // the wave's largest: the first of those that equal it, the others among the rest
+    Top top{m, 0.0f, kNone};
+    int same = 0;
+    if (m > -INFINITY)
+#pragma unroll
+        for (int it = IT - 1; it >= 0; --it) {
+            uint64_t is[V], any = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                is[j] = __ballot(l[it * V + j] == m);
+                any |= is[j];
+                same += __builtin_popcountll(is[j]);
+            }
+            if (any) {
+                const int from = __builtin_ctzll(any);
+                int j = V - 1;
+#pragma unroll
+                for (int k = V - 2; k >= 0; --k) j = is[k] >> from & 1 ? k : j;
+                top.i = lo + (it * kThreads + wave * 64 + from) * V + j;
+            }
         }
-    }
-    if (best != top.i) own = -1;
-    const float below = best == INT_MAX ? 0.0f : m;  // (-inf - -inf)
+    // exp(d) = (2^(d log2(e) / 2))^2, so that small ones keep their bits; log2(e) / 2 in
+    // two parts, for one rounding of the product
+    constexpr float kHi = 0x1.715476p-1f, kLo = 0x1.4ae0cp-27f;
+    const float below = top.i >= 0 ? m : 0.0f;  // (-inf - -inf)
     float s = 0.0f;
 #pragma unroll
-    for (int k = 0; k < N; ++k) s += k == own ? 0.0f : expf(l[k] - below);
+    for (int k = 0; k < N; ++k) {
+        const float d = l[k] - below;
+        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(d, kHi, d * kLo));
+        e = l[k] == m ? 0.0f : e;  // (of two infinities e is NaN)
+        s = __builtin_fmaf(e, e, s);
+    }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-    if (lane == 0) tops[wave] = Top{m, s, best == INT_MAX ? kNone : best};
+    if (lane == 0) {
+        top.s = s + (float)(same > 1 ? same - 1 : 0);
+        tops[wave] = top;
+    }
     __syncthreads();
     if (tid == 0) {
         top = tops[0];
@@ -329,7 +359,8 @@ extern "C" int cw_logits_rows(cw_ctx *ctx, const cw_logit_rules *rules, const cw
     a.logprob = logprob;
     const bool wide = aligned16(logits) && stride % 4 == 0 && vocab % 4 == 0 &&
                       (!out || (aligned16(out) && out_stride % 4 == 0));
-    // Slices of 4096 tokens where they fill the chip, else of 1024.
+    // Slices of 4096 tokens where they fill the chip twice, else of 1024 (one row of 151936
+    // after 900 tokens 5.4 us, 7.1 with 4096; 61 rows after 4100 19.9 us, 22.8 with 2048).
     const bool few = (long)rows * ((vocab + 4095) / 4096) < 2 * ctx->n_cu;
     const int slice = few ? 1024 : 4096;
     a.parts = (vocab + slice - 1) / slice;
