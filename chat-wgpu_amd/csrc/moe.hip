@@ -2,18 +2,23 @@
 // (tokens) of a step: y = [residual +] sum_e p_e Wd_e (silu(Wg_e x) * (Wu_e x))
 // over the top_k experts of a row.
 //
+// The choice hangs on the scores, so they are sums in f64 (products of f32 values are
+// exact there), and their ranks are counted, not sorted.  Rows that chose an expert
+// form its list; tiles of 8 or 16 of a list go through its matrices.
+//
 // The products run on the matrix cores like q4_gemm.hip's, x as f16 pairs hi + lo
 // under a power of two a row (22 bits), W as its nibbles (exact), a block's scale
-// after its 32 products.  Few rows meet an expert, so one 16x16x32 MFMA has eight
-// rows' hi halves and the same rows' lo halves as its 16 rows; the two sums of a
-// row meet at the end.
+// after its 32 products.  Few rows meet an expert: eight rows' hi halves and the same
+// rows' lo halves are the 16 rows of one 16x16x32 MFMA, and the two sums of a row
+// meet at the end; 16 rows take two of them one after the other.  x stays in
+// registers; W, which is read once, goes through a ring in LDS of each wave's own.
 //
-// W goes from memory to registers without LDS: a lane of the 16 x 4 (W row, k
-// group) loads whole blocks, block 4 s + g of its row, and four lane groups hand
-// each other their words (two swaps of lane halves, two of rows of 16: one
-// instruction a block), so that group g has bytes 4 g .. 4 g + 3 of each of the
-// four blocks, which is the fragment that nibbles() takes.  The x image lies as the
-// fragments are read and stays in the L2s.
+// What bounds it: the experts' weights from memory (all of 128 experts of 2,048 x 768:
+// 340 MB with their scales), 6.3 TB/s at best.  us by kernel, of 8 of 128 experts: scores, choice
+// and up in one launch, down of one row 2.5 + 8.9 + 8.4 (27 MB an expert's eight); 48 rows: scores 5,
+// choice 6, up 47, split 5, down 28, sum 5 (up alone 4.8 TB/s; loads without products
+// 40 and 23.5); 500 rows: 12, 11, 133, 7.5, 85, 9: there the vector units decode and
+// scale, 45 % of the time busy already at 48 rows.
 
 #include "prompt_device.hpp"
 
@@ -1031,9 +1036,13 @@ int score_splits(const cw_moe &m, int rows) {
     return rows == 1 ? 1 : std::min(kMaxSplits, std::max(1, m.dim / 512));
 }
 
-// Rows whose second product goes row by row, reading an expert again for each row
-// that chose it: that saves two launches and the passes over h and z.
-bool down_by_rows(const cw_moe &m, int rows) { return rows <= 8; }
+// Whether the second product goes row by row, reading an expert again for each row
+// that chose it: that saves two launches and the passes over h and z, and pays while
+// few rows meet (us by rows and by tiles; 8 of 128 experts, 2048 x 768: 2 rows 33, 36;
+// 6 rows 46, 48; 8 rows 57, 53; 2 of 8, 4096 x 12288: 2 rows 102, 101; 8 rows 220, 147).
+bool down_by_rows(const cw_moe &m, int rows) {
+    return rows == 1 || 5 * rows * m.top_k <= 2 * m.n_experts;
+}
 
 // Places of the workspace, each 256-byte aligned; with base null their size.
 size_t lay_out(const cw_moe &m, int rows, char *base, MoeArgs *a) {

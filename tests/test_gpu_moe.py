@@ -72,6 +72,8 @@ SHAPES = [
     (21, 128, 4128, 4, 2, True),
     (512, 256, 4096, 8, 4, True),
     (600, 4096, 256, 8, 8, False),
+    (6, 1024, 512, 128, 8, True),
+    (3, 160, 288, 100, 4, False),
 ]
 
 
