@@ -342,7 +342,8 @@ __device__ __forceinline__ StageLane<J> stage_lane(int lane, int nb) {
     return l;
 }
 
-// DMAs from a base that is the same in every lane, wherever the compiler has it: it
+// DMAs to an address in LDS (a number: of a pointer each would look whether it is null)
+// from a base that is the same in every lane, wherever the compiler has it: it
 // may come straight from a vector instruction, which the assembler's hazard rules
 // want five wait states after (and M0 one).
 template <typename T>
@@ -352,17 +353,17 @@ __device__ __forceinline__ const T *uniform(const T *p) {
     const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
     return reinterpret_cast<const T *>((uintptr_t)((uint64_t)hi << 32 | lo));
 }
-__device__ __forceinline__ void dma16u(const void *base, uint32_t off, unsigned char *lds_dst) {
+__device__ __forceinline__ void dma16u(const void *base, uint32_t off, uint32_t lds) {
     asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
                  :
-                 : "v"(off), "s"(uniform(static_cast<const char *>(base))), "{m0}"(lds_off(lds_dst))
+                 : "v"(off), "s"(uniform(static_cast<const char *>(base))), "{m0}"(lds)
                  : "memory");
 }
-// 4 bytes a lane, at lds_dst + 4 i
-__device__ __forceinline__ void dma4u(const void *base, uint32_t off, unsigned char *lds_dst) {
+// 4 bytes a lane, at lds + 4 i
+__device__ __forceinline__ void dma4u(const void *base, uint32_t off, uint32_t lds) {
     asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1"
                  :
-                 : "v"(off), "s"(uniform(static_cast<const char *>(base))), "{m0}"(lds_off(lds_dst))
+                 : "v"(off), "s"(uniform(static_cast<const char *>(base))), "{m0}"(lds)
                  : "memory");
 }
 
@@ -370,18 +371,22 @@ __device__ __forceinline__ void dma4u(const void *base, uint32_t off, unsigned c
 // [0, jn) exist (those behind re-read the last).
 template <int J>
 __device__ __forceinline__ void issue_stage(const StageLane<J> &l, const uint8_t *q, const uint16_t *s,
-                                            int jn, unsigned char *buf) {
+                                            int jn, uint32_t buf) {
     constexpr int L = Stage<J>::LINE;
+    const bool whole = jn == J;  // (but for a row's last stage)
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const int k = L == 8 ? j & 1 : 0, first = L == 8 ? j / 2 * 8 : j * 4;  // the line's first block
-        // (min: whole lines but for the row's last stage)
-        dma16u(q + 16 * min(first, 4 * jn - 4), l.q[k] + 16 * min(l.block[k], max(4 * jn - first, 4) - 1),
-               buf + j * 1024);
+        uint32_t off = l.q[k] + 16 * l.block[k];
+        if (!whole) off = l.q[k] + 16 * min(l.block[k], max(4 * jn - first, 4) - 1);
+        dma16u(q + 16 * (whole ? first : min(first, 4 * jn - 4)), off, buf + j * 1024);
     }
 #pragma unroll
-    for (int t = 0; t < (J > 2 ? 2 : 1); ++t)
-        dma4u(s, l.s[t] + 4 * min(l.word[t], 2 * jn - 1), buf + Stage<J>::Q + 256 * t);
+    for (int t = 0; t < (J > 2 ? 2 : 1); ++t) {
+        uint32_t off = l.s[t] + 4 * l.word[t];
+        if (!whole) off = l.s[t] + 4 * min(l.word[t], 2 * jn - 1);
+        dma4u(s, off, buf + Stage<J>::Q + 256 * t);
+    }
 }
 
 // acc += the stage times the x fragments x(half, block), which are 0 for blocks that do
@@ -608,15 +613,10 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
     const int n_groups = H == 1 ? 1 : min(groups, (sets - set0 + cs - 1) / cs);
     const uint8_t *const img = UP ? a.ximg : a.himg;
 
-    // column tile c of the wave's set of a group (past the last set: the last again,
-    // not stored)
-    auto w_tile = [&](int g, int c, const uint8_t **q, const uint16_t **d) {
-        const int set = min(set0 + g * cs + wave / ks, sets - 1);
-        const int col = UP ? set * 32 + (c & 1) * 16 : min(set * 64 + c * 16, N - 16);
-        const size_t w0 = ((size_t)tile.e * N + col) * nb;
-        *q = (!UP ? a.m.down_quants : c < 2 ? a.m.gate_quants : a.m.up_quants) + w0 * 16;
-        *d = (!UP ? a.m.down_scales : c < 2 ? a.m.gate_scales : a.m.up_scales) + w0;
-    };
+    // the first column of the wave's set of a group (past the last set the last again, not
+    // stored), and the W row of its column tile c from there
+    auto first_col = [&](int g) { return min(set0 + g * cs + wave / ks, sets - 1) * SET; };
+    auto tile_row = [&](int col, int c) { return UP ? (c & 1) * 16 : min(c * 16, N - 16 - col); };
 
     // x rows of the lane's fragments, hi or lo of row li / 2 or both of row li (rows past
     // the tile's end read nothing)
@@ -675,7 +675,12 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
         for (int g = 0; g < n_groups; ++g) {
             Operands o;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) w_tile(g, c, &o.q[c], &o.d[c]);
+            for (int c = 0; c < 4; ++c) {
+                const int col = first_col(g);
+                const size_t w0 = ((size_t)tile.e * N + col + tile_row(col, c)) * nb;
+                o.q[c] = (!UP ? a.m.down_quants : c < 2 ? a.m.gate_quants : a.m.up_quants) + w0 * 16;
+                o.d[c] = (!UP ? a.m.down_scales : c < 2 ? a.m.gate_scales : a.m.up_scales) + w0;
+            }
             f32x4 acc[4] = {};
             multiply_steps<H>(o, img, xo, nb, wave % ks, ks, acc);
             if (g == 0) put_scales();
@@ -688,25 +693,38 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
         // the wave's first group of blocks in a round (a wave without any goes through
         // the row's last ones with no x)
         auto first = [&](int t) { return min(t * ks + wave % ks, slices - 1) * J; };
-        int ig = 0, it = 0, ic = 0, isub = 0, ibuf = 0;  // of the next stage to ask for
-        auto issue = [&] {
-            const uint8_t *q;
-            const uint16_t *d;
-            w_tile(ig, ic, &q, &d);
-            // (past the row's end its last group again)
-            const int b = min(first(it) + isub * SJ, nb / 4 - 1), n = min(SJ, nb / 4 - b);
-            issue_stage<SJ>(l, q + (size_t)b * 64, d + 4 * b, n, mine + ibuf * S::BYTES);
-            ibuf = ibuf + 1 == R ? 0 : ibuf + 1;
-            if (++isub == SUBS) {
-                isub = 0;
-                if (++ic == 4) {
-                    ic = 0;
-                    if (++it == rounds) {
-                        it = 0;
-                        ++ig;
-                    }
-                }
+        // Stages are asked for R - 1 ahead, tile c = k / SUBS and sub = k % SUBS of a round,
+        // k a constant where it is called: what changes with the round alone is kept.
+        const uint32_t lds = lds_off(mine);
+        const uint8_t *q0, *q1 = nullptr;
+        const uint16_t *d0, *d1 = nullptr;
+        int ig = 0, it = 0, icol = 0, ib = 0, ibuf = 0;  // of the next stage to ask for
+        auto begin = [&] {
+            icol = first_col(ig);
+            ib = first(it);
+            const size_t w0 = ((size_t)tile.e * N + icol) * nb + 4 * ib;
+            q0 = (UP ? a.m.gate_quants : a.m.down_quants) + w0 * 16;
+            d0 = (UP ? a.m.gate_scales : a.m.down_scales) + w0;
+            if constexpr (UP) {
+                q1 = a.m.up_quants + w0 * 16;
+                d1 = a.m.up_scales + w0;
             }
+        };
+        auto issue = [&](int k) {
+            if (k == 4 * SUBS) {
+                if (++it == rounds) {
+                    it = 0;
+                    ++ig;
+                }
+                begin();
+            }
+            const int c = k / SUBS % 4, sub = k % SUBS;
+            // (past the row's end its last group again)
+            const int skip = min(sub * SJ, nb / 4 - 1 - ib), n = min(SJ, nb / 4 - ib - skip);
+            const uint32_t at = tile_row(icol, c) * nb + 4 * skip;
+            issue_stage<SJ>(l, (UP && c >= 2 ? q1 : q0) + 16 * (size_t)at, (UP && c >= 2 ? d1 : d0) + at, n,
+                            lds + ibuf * S::BYTES);
+            ibuf = ibuf + 1 == R ? 0 : ibuf + 1;
         };
         const int total = n_groups * rounds * 4 * SUBS;
         int left = total, buf = 0;
@@ -731,8 +749,11 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
                     }
                     // (x ahead of the first stages: behind them it comes last, 48 rows
                     // 46 -> 55 us)
-                    if (g + t == 0)
-                        for (int k = 0; k < R - 1 && k < total; ++k) issue();
+                    if (g + t == 0) {
+                        begin();
+#pragma unroll
+                        for (int k = 0; k < R - 1; ++k) issue(k);
+                    }
                     // here, or the compiler waits for x, and so for every stage that is on
                     // its way, before each stage
                     wait_vm<0>();
@@ -744,7 +765,7 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
                     for (int sub = 0; sub < SUBS; ++sub) {
                         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): reads of the buffer asked for next
                         if (left >= R) {
-                            issue();
+                            issue(c * SUBS + sub + R - 1);
                             wait_vm<(R - 1) * S::DMAS>();
                         } else if (R == 3 && left == 2) {
                             wait_vm<S::DMAS>();
@@ -813,11 +834,12 @@ __global__ __launch_bounds__(kRowThreads) void moe_up_row_kernel(MoeArgs a) {
         const StageLane<J> l = stage_lane<J>(lane, nb);
         const int slices = (nb + 4 * J - 1) / (4 * J);
         const int total = wave < slices ? ((slices - 1 - wave) / kRowWaves + 1) * 2 : 0;
+        const uint32_t lds = lds_off(mine);
         auto issue = [&](int k) {  // gate, up of the wave's k / 2th slice
             const int b = (wave + k / 2 * kRowWaves) * 4 * J;
             issue_stage<J>(l, (k & 1 ? a.m.up_quants : a.m.gate_quants) + (w0 + b) * 16,
                            (k & 1 ? a.m.up_scales : a.m.gate_scales) + w0 + b, min(J, (nb - b) / 4),
-                           mine + k % R * S::BYTES);
+                           lds + k % R * S::BYTES);
         };
         for (int k = 0; k < R && k < total; ++k) issue(k);
         for (int k = 0; k < total; k += 2) {
@@ -888,6 +910,7 @@ __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
     const int parts = K < W ? W / K : 1, steps = (nb + 3) / 4;
     const int per = (steps + parts - 1) / parts;
     unsigned char *const mine = ring + wave * R * BYTES;
+    const uint32_t lds = lds_off(mine);
     const StageLane<J> l = stage_lane<J>(lane, nb);
     // unit u: part u % parts of expert u / parts, steps [s0, s1)
     auto begin = [&](int u) { return u % parts * per; };
@@ -903,7 +926,7 @@ __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
     auto issue = [&] {
         const int j = iu / parts, e = __builtin_amdgcn_readlane(my_id, j);
         const size_t w0 = ((size_t)e * dim + col) * nb + 4 * is;
-        unsigned char *const buf = mine + ibuf * BYTES;
+        const uint32_t buf = lds + ibuf * BYTES;
         const int jn = min(J, end(iu) - is);
         if constexpr (DMA) {
             issue_stage<J>(l, a.m.down_quants + w0 * 16, a.m.down_scales + w0, jn, buf);
