@@ -1213,6 +1213,8 @@ extern "C" int cw_moe_rows(cw_ctx *ctx, const cw_moe *moe, const float *x, int r
                  "cw_moe_rows: x, router and quants must be 16-byte aligned");
     const size_t n = (size_t)rows * m.dim;
     CW_CHECK_ARG(x + n <= y || y + n <= x, "cw_moe_rows: x and y overlap");
+    CW_CHECK_ARG(!residual || residual == y || residual + n <= y || y + n <= residual,
+                 "cw_moe_rows: residual and y overlap");
     CW_HIP(hipSetDevice(ctx->device));
     MoeArgs a{};
     int chunk = std::min(rows, kChunk);

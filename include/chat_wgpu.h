@@ -362,9 +362,9 @@ typedef struct cw_moe {
  * cw_q4_gemm (block scales finite; x 16-byte aligned).  experts and weights
  * [rows][top_k] receive the choice in order of score, and p (NULL: not wanted).
  * positions (NULL: none): a row of a negative position is padding: what it holds
- * does not count, and nothing of it is written.  y may be residual; it must not overlap x.  A row whose x is not
- * finite gives NaN, and experts in range; other rows are not touched by it.
- * rows at most 65536. */
+ * does not count, and nothing of it is written.  y may be residual, else it overlaps
+ * neither it nor x.  A row whose x is not finite gives NaN, and experts in range;
+ * other rows are not touched by it.  rows at most 65536. */
 int cw_moe_rows(cw_ctx *ctx, const cw_moe *moe, const float *x, int rows, const int *positions,
                 const float *residual, float *y, int *experts, float *weights);
 

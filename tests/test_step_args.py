@@ -63,6 +63,7 @@ def moe_call(ctx=CTX, x=1 << 20, rows=3, pos=None, res=None, y=1 << 24, ids=None
     (dict(n_experts=64, top_k=33), "top_k=33"), (dict(normalise=2), "normalise=2"),
     (dict(x=(1 << 20) + 4), "aligned"), (dict(router=4100), "aligned"), (dict(up_quants=4104), "aligned"),
     (dict(y=1 << 20), "overlap"), (dict(y=(1 << 20) + 767), "overlap"), (dict(y=(1 << 20) - 764), "overlap"),
+    (dict(res=(1 << 24) + 4), "residual and y"), (dict(res=(1 << 24) - 764), "residual and y"),
 ])
 def test_moe_rows(kw, text):
     refused(moe_call(**kw), text)
