@@ -95,15 +95,32 @@ __device__ __forceinline__ Owners owners(const LogitArgs &a, int b0) {
     return Owners{a.first_row[b], a.first_row[b + 1]};
 }
 
-// The first request whose rows the batch row is among, n_seq if none; by every wave.
+// The request whose rows the batch row is among, n_seq if none; by every wave.  Of more
+// than 64 the 64 are looked at whose first begins at or before the row and the next 64's
+// behind it; where first_row does not ascend, all of them in turn.
 __device__ __forceinline__ int owner_of(const LogitArgs &a, Owners o, int br) {
-    for (int b0 = 0;;) {
+    auto among = [&](int b0) {
         const uint64_t has = __ballot(o.r0 >= 0 && o.r0 <= br && br < o.r1 && o.r1 <= a.batch_rows);
-        if (has) return min(b0 + __builtin_ctzll(has), a.n_seq - 1);
-        b0 += 64;
-        if (b0 >= a.n_seq) return a.n_seq;
-        o = owners(a, b0);
+        return has ? min(b0 + __builtin_ctzll(has), a.n_seq - 1) : a.n_seq;
+    };
+    int b = among(0);
+    if (b < a.n_seq || a.n_seq <= 64) return b;
+    const int lane = threadIdx.x & 63, runs = (a.n_seq + 63) / 64;
+    int run = -1;
+    for (int i = 0; i < runs; i += 64)
+        run += __builtin_popcountll(
+            __ballot(i + lane < runs && a.first_row[64 * min(i + lane, runs - 1)] <= br));
+    if (run > 0) {
+        o = owners(a, 64 * run);
+        b = among(64 * run);
+        if (b < a.n_seq) return b;
     }
+    for (int b0 = 64; b0 < a.n_seq; b0 += 64) {
+        o = owners(a, b0);
+        b = among(b0);
+        if (b < a.n_seq) return b;
+    }
+    return a.n_seq;
 }
 
 // IT runs of V logits a thread, V = 4 where rows are 16-byte aligned and whole fours.

@@ -331,3 +331,29 @@ def test_recorded(ctx, rng):
         for a, d in zip(got, (out, token, logprob)):
             assert np.array_equal(a, d.download())
     g.close()
+
+
+def test_rows_of_many_requests(ctx, rng):
+    """More requests than lanes, most without a row, and a table that does not ascend."""
+    n, vocab = 9000, 500
+    new = (rng.random(n) < 0.02).astype(int)
+    new[[0, 64, n - 1]] = 1, 3, 2
+    first = i32(np.concatenate([[0], np.cumsum(new)]))
+    rows = int(first[-1]) + 3
+    x = draw(rng, rows, vocab)
+    frequency = rng.random(n).astype(np.float32)
+    hist = i32(rng.integers(0, vocab, (n, 7)))
+    rules = cw.logit_rules(tokens=ctx.storage(hist), length=ctx.storage(i32(np.full(n, 7))), max_len=7,
+                           frequency=ctx.storage(frequency))
+    for table in (first, np.concatenate([first[:1], first[:0:-1]])):  # the second: requests 0 only
+        out = ctx.storage(np.full((rows, vocab), 7.5, np.float32))
+        ctx.logits_rows(rules, cw.batch(None, n, rows, ctx.storage(i32(table)), None, 0), ctx.storage(x),
+                        rows, vocab, out=out)
+        got = out.download()
+        for r in range(rows):
+            own = [b for b in range(n) if table[b] <= r < table[b + 1]]
+            if not own:
+                assert np.all(got[r] == 7.5)
+                continue
+            want, bound = so.logits(x[r], hist[own[0]], frequency=float(frequency[own[0]]))
+            assert np.all(np.abs(got[r] - want) <= 1.001 * bound)
