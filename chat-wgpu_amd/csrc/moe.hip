@@ -13,12 +13,15 @@
 // meet at the end; 16 rows take two of them one after the other.  x stays in
 // registers; W, which is read once, goes through a ring in LDS of each wave's own.
 //
-// What bounds it: the experts' weights from memory (all of 128 experts of 2,048 x 768:
-// 340 MB with their scales), 6.3 TB/s at best.  us by kernel, of 8 of 128 experts: scores, choice
-// and up in one launch, down of one row 2.5 + 8.9 + 8.4 (27 MB an expert's eight); 48 rows: scores 5,
-// choice 6, up 47, split 5, down 28, sum 5 (up alone 4.8 TB/s; loads without products
-// 40 and 23.5); 500 rows: 12, 11, 133, 7.5, 85, 9: there the vector units decode and
-// scale, 45 % of the time busy already at 48 rows.
+// What bounds it: the experts' weights from memory (128 of 2,048 x 768 are 340 MB with
+// their scales), which reading alone brings in at 6.3 TB/s.  Microseconds of the launches,
+// 8 of these 128 experts a row:
+//   1 row     scores 2.7, choice and up 8.8, down 8.6: launches' beginnings and ends
+//   48 rows   scores 5, choice 6, up 49 (44 at best), split 5, down 28, sum 5: up and
+//             down read at 4.3 TB/s (loads without products 40 and 23.5), the vector
+//             units, which decode and scale, 0.6 busy
+//   500 rows  scores 13, choice 11, up 139, split 8, down 99, sum 9: tiles of one
+//             expert decode its weights again; vector units 0.6, matrix cores 0.22 busy
 
 #include "prompt_device.hpp"
 
@@ -294,6 +297,8 @@ __device__ void choose(const MoeArgs &a, int r) {
     if constexpr (LISTS) a.list[(size_t)e * a.rows + atomicAdd(&a.count[e], 1)] = i;
 }
 
+// A workgroup a row: 6 us for 48 rows of 128 experts, 11 for 500 (with 512 or 256
+// threads the same: the lists' atomics, 31 on each count, and a launch).
 __global__ __launch_bounds__(1024) void moe_choose_kernel(MoeArgs a) { choose<1024, true>(a, blockIdx.x); }
 
 // ---------------------------------------------------------------- products
@@ -390,9 +395,9 @@ __device__ __forceinline__ void issue_stage(const StageLane<J> &l, const uint8_t
 }
 
 // acc += the stage times the x fragments x(half, block), which are 0 for blocks that do
-// not exist.  Eight rows: their hi and lo halves are the fragment's 16
-// rows (H = 1); 16 rows: two fragments one after the other (H = 2), so that a block's
-// scale meets the sum of both.  A block's products are scaled and added while the next
+// not exist.  Eight rows: their hi and lo halves are the fragment's 16 rows (H = 1);
+// 16 rows: two fragments one after the other (H = 2), so that a block's scale meets the
+// sum of both.  A block's products are scaled and added while the next
 // one's run and its weights are decoded; a group's words are read a group ahead.
 template <int J, int H, typename X>
 __device__ __forceinline__ void multiply_stage(const StageLane<J> &l, const unsigned char *buf, X x,
@@ -785,6 +790,8 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
     }
 }
 
+// h's images: every workgroup of the down product reads a row's, so its largest value
+// is found and it is split once.  5 us for 48 rows of 8 experts, 8 for 500 (23 MB).
 __global__ __launch_bounds__(256) void moe_split_kernel(MoeArgs a) {
     const size_t pair = blockIdx.x;
     if (a.ids[pair] < 0) return;
@@ -1034,7 +1041,8 @@ __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
     a.y[o] = a.residual ? a.residual[o] + y : y;
 }
 
-// y = [residual +] the sum of a row's experts in order of their rank
+// y = [residual +] the sum of a row's experts in order of their rank: 5 us for 48 rows of 8
+// (a launch), 9 for 500 (37 MB)
 __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
     const int r = blockIdx.y, K = a.m.top_k, dim = a.m.dim;
     const int n = (blockIdx.x * 256 + threadIdx.x) * 4;

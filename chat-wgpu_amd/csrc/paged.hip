@@ -171,6 +171,12 @@ int launch_rope(cw_ctx *ctx, const char *label, const RopeArgs &a, bool wide, bo
 // elements) hold it whole, add its squares up among themselves and rotate what
 // they hold.  A lane has four pairs (4 elements of either half, or 8 in a row), or
 // 8 elements behind rot, and keeps its angles for the heads it takes.
+//
+// What bounds it: memory, each value read and written once, and the vector units beside
+// it.  6,000 rows of 24 heads of 128 (147 MB) take 27 to 30 us, 4.9 to 5.5 TB/s, with
+// the vector units busy throughout (angles in f64, norm, rotation); 4,100 rows of 32 + 2 x
+// 8 with the write into an f16 cache 34 us (185 MB, 5.4 TB/s); 32 to 48 rows one launch,
+// 3.6 us.
 
 struct NormArgs {
     const float *q_gain, *k_gain;  // [hd]
