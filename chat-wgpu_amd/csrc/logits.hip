@@ -178,7 +178,8 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
     }
     const float repeat = rule(a.r.repeat, b, 1.0f), presence = rule(a.r.presence, b, 0.0f);
     const float frequency = rule(a.r.frequency, b, 0.0f);
-    const int len = a.r.tokens ? min(max(a.r.length[b], 0), a.r.max_len) : 0;
+    const bool penal = repeat != 1.0f || presence != 0.0f || frequency != 0.0f;
+    const int len = a.r.tokens && penal ? min(max(a.r.length[b], 0), a.r.max_len) : 0;
     const int prompt = rule(a.r.prompt, b, 0);
     const int r0 = a.first_row[b], nodes = a.first_row[b + 1] - r0, self = br - r0;
     const int e0 = biased ? a.r.bias_first[b] : 0, e1 = biased ? a.r.bias_first[b + 1] : 0;
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
             for (int u = 0; u < U; ++u)
                 if (i + u * kThreads < len) add(v[u], i + u * kThreads >= prompt);
         }
-        if (a.r.node_token)
+        if (a.r.node_token && penal)
             for (int j = tid; j < nodes; j += kThreads) {
                 const bool sees =
                     !a.mask ? j <= self
@@ -217,30 +218,39 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
         lds_barrier();
     }
 
-    // (no branch for the few that change: nearly every wave would take it for each logit.
-    // With inv the nearest to 1 / repeat, v inv and one step after it are v / repeat to
-    // its last bit; infinities and zeros have no step.)
+    // Where a wave has tokens that were seen, all its logits go through their rules: under
+    // a branch each, waves with some would take it for nearly every logit.  With inv the
+    // nearest to 1 / repeat, v inv and one step after it are v / repeat to its last bit;
+    // infinities and zeros have no step.
     const float inv = 1.0f / repeat;
     float m = -INFINITY;
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
         if (counts) {
+            uint32_t c[V], any = 0;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const uint32_t c = count[at(it) + j], made = c & ~kPrompt;
-                float v = l[it * V + j];
-                const float q = v * inv, step = __builtin_fmaf(__builtin_fmaf(-q, repeat, v), inv, q);
-                const float less = step == step ? step : q;
-                v = c ? (v > 0.0f ? less : v * repeat) : v;
-                l[it * V + j] =
-                    __builtin_fmaf(made ? -frequency : 0.0f, (float)made, v) - (made ? presence : 0.0f);
+            for (int j = 0; j < V; ++j) any |= c[j] = count[at(it) + j];
+            if (__any(any)) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const uint32_t made = c[j] & ~kPrompt;
+                    float v = l[it * V + j];
+                    const float q = v * inv, step = __builtin_fmaf(__builtin_fmaf(-q, repeat, v), inv, q);
+                    const float less = step == step ? step : q;
+                    v = c[j] ? (v > 0.0f ? less : v * repeat) : v;
+                    l[it * V + j] = __builtin_fmaf(made ? -frequency : 0.0f, (float)made, v) -
+                                    (made ? presence : 0.0f);
+                }
             }
         }
         if (biased) {
+            uint32_t e[V], any = 0;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const uint32_t e = last[at(it) + j];
-                if (e) l[it * V + j] += a.r.bias[e - 1];
+            for (int j = 0; j < V; ++j) any |= e[j] = last[at(it) + j];
+            if (__any(any)) {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (e[j]) l[it * V + j] += a.r.bias[e[j] - 1];
             }
         }
         if (allowed) {

@@ -186,6 +186,19 @@ def test_more_rows_than_go_through_together(ctx, rng):
     assert np.all(got[0][pos < 0] == 7.5)
 
 
+@pytest.mark.parametrize("rows,dim,hidden,n,k", [(2500, 32, 64, 9, 2), (700, 32, 8192, 32, 32)])
+def test_rows_in_pieces(ctx, rng, rows, dim, hidden, n, k):
+    """More rows, or larger ones, than the workspace takes at once: each piece has
+    its own positions, choices and residual, and rows that are padding."""
+    m = Layer(ctx, rng, dim, hidden, n, k)
+    x, res = (rng.standard_normal((rows, dim)).astype(np.float32) for _ in range(2))
+    pos = i32(np.where(rng.random(rows) < 0.1, -1, 3))
+    got = m.run(x, res, pos)
+    live = pos >= 0
+    m.check(x, got, res, live)
+    assert np.all(got[0][~live] == 7.5) and np.all(got[1][~live] == -7) and np.all(got[2][~live] == -7.0)
+
+
 @pytest.mark.parametrize("rows", [1, 6, 48, 300])
 def test_the_same_bits_each_time_and_replayed(ctx, rng, rows):
     """Eager, recorded and replayed beside other work, with rows that come and go."""
