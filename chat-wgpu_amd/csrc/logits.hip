@@ -19,9 +19,9 @@
 // order.
 //
 // What bounds it, at 151936 tokens: two launches for one row (5.4 + 4.5 us).  61 rows
-// after 4100 tokens take 20 us for 37 MB: their vector instructions alone are 11 us, the
-// counts 8 us of the whole (each of the 38 slices reads the history).  48 rows with
-// masks, biases and out take 23 us for 55 MB, 14 without the counts.
+// after 4100 tokens take 19.4 us for 37 MB: vector units 0.67 busy, the counts 8 us of
+// the whole (each of the 38 slices reads the history).  48 rows with masks, biases and
+// out take 20.7 us for 59 MB.
 
 #include "paged_device.hpp"
 #include "prompt_device.hpp"

@@ -235,3 +235,29 @@ def test_the_same_bits_each_time_and_replayed(ctx, rng, rows):
         assert np.array_equal(got[0][1][p >= 0], we) and np.all(got[0][0][p < 0] == 7.5)
     for g in graphs:
         g.close()
+
+
+@pytest.mark.parametrize("hidden", [4224, 4128])
+def test_experts_past_four_gigabytes(ctx, rng, hidden):
+    """The last two of 512 experts, whose quants lie past 2^32 bytes; rows of whole
+    groups of blocks and others."""
+    n, dim, k = 512, 4096, 2
+    two = Layer(ctx, rng, dim, hidden, k, k)
+    two.router = np.abs(two.router)
+    d = []
+    for scales, quants in (two.gate, two.up, two.down):
+        for a in (scales.view(np.uint16), quants):
+            big = ctx.empty((n, *a.shape[1:]), a.dtype)
+            skip = (n - k) * a[0].nbytes
+            cw.DeviceArray(ctx, a.shape, a.dtype, big.ptr + skip).upload(a)
+            d.append(big)
+        assert skip > 1 << 32
+    router = np.concatenate([np.zeros((n - k, dim), np.float32), two.router])
+    two.moe = cw.moe(dim, hidden, n, k, ctx.storage(router), *d)
+    for rows in (1, 3, 250):
+        x = (0.1 + rng.random((rows, dim))).astype(np.float32)
+        y, ids, p = two.run(x)
+        assert ids.min() == n - k
+        two.check(x, (y, ids - (n - k), p))
+    for a in d:
+        ctx.free(a)
