@@ -20,7 +20,7 @@
 //   48 rows   scores 5, choice 6, up 49 (44 at best), split 5, down 28, sum 5: up and
 //             down read at 4.3 TB/s (loads without products 40 and 23.5), the vector
 //             units, which decode and scale, 0.6 busy
-//   500 rows  scores 13, choice 11, up 139, split 8, down 99, sum 9: tiles of one
+//   500 rows  scores 13, choice 7, up 139, split 8, down 99, sum 9: tiles of one
 //             expert decode its weights again; vector units 0.6, matrix cores 0.22 busy
 
 #include "prompt_device.hpp"
@@ -31,6 +31,9 @@ using namespace cwi;
 
 constexpr int kMaxExperts = 512, kMaxTop = 32;
 constexpr int kTile = 8;       // rows of one MFMA
+// Counts lie a few words apart: atomics on one line follow one another (the choice of 500
+// rows 11 us side by side, 8.6, 7.0 and 6.6 with 2, 4 and 8; tiles read more lines).
+constexpr int kApart = 4;
 constexpr int kMaxSplits = 8;  // workgroups that share a score's sum
 constexpr int kChunk = 1024;   // rows that go through the layer together, at most
 constexpr size_t kChunkBytes = (size_t)1 << 30;  // of workspace, unless kTile rows need more
@@ -51,7 +54,7 @@ struct MoeArgs {
     float *xscale, *hscale;
     float *h;         // [rows][top_k][hidden]
     float *z;         // [rows][top_k][dim]
-    int *count;       // [n_experts]: pairs (row, choice) of each, and
+    int *count;       // [n_experts], kApart words apart: pairs (row, choice) of each, and
     int *list;        // [n_experts][rows]: those pairs, row * top_k + choice
 };
 
@@ -165,7 +168,7 @@ __global__ __launch_bounds__(256, 2) void moe_score_kernel(MoeArgs a) {
     const int et = (E + 15) / 16, rt = (a.rows + 15) / 16, tiles = et * rt;
     int b = blockIdx.x;
     if (b == 0)
-        for (int e = tid; e < E; e += 256) a.count[e] = 0;
+        for (int e = tid; e < E; e += 256) a.count[e * kApart] = 0;
     if (b >= tiles * a.splits) {
         const int r = b - tiles * a.splits;
         split_row<256>(a.x + (size_t)r * dim, dim, a.ximg + (size_t)r * dim * 4, a.xscale + r);
@@ -294,11 +297,11 @@ __device__ void choose(const MoeArgs &a, int r) {
     a.p[i] = p;
     if (a.experts) a.experts[i] = e;
     if (a.weights) a.weights[i] = p;
-    if constexpr (LISTS) a.list[(size_t)e * a.rows + atomicAdd(&a.count[e], 1)] = i;
+    if constexpr (LISTS) a.list[(size_t)e * a.rows + atomicAdd(&a.count[e * kApart], 1)] = i;
 }
 
-// A workgroup a row: 6 us for 48 rows of 128 experts, 11 for 500 (with 512 or 256
-// threads the same: the lists' atomics, 31 on each count, and a launch).
+// A workgroup a row: 6 us for 48 rows of 128 experts, 7 for 500 (5.3 without the lists'
+// atomics; with 512 or 256 threads a row the same).
 __global__ __launch_bounds__(1024) void moe_choose_kernel(MoeArgs a) { choose<1024, true>(a, blockIdx.x); }
 
 // ---------------------------------------------------------------- products
@@ -540,7 +543,7 @@ __device__ __forceinline__ Tile find_tile(const MoeArgs &a, int tile, int b) {
     int c[N], mine = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        c[j] = j < per && lane * per + j < E ? a.count[lane * per + j] : 0;
+        c[j] = j < per && lane * per + j < E ? a.count[(lane * per + j) * kApart] : 0;
         mine += (c[j] + tile - 1) / tile;
     }
     int to = mine;
@@ -1091,7 +1094,7 @@ size_t lay_out(const cw_moe &m, int rows, char *base, MoeArgs *a) {
     a->ximg = reinterpret_cast<uint8_t *>(take((size_t)rows * m.dim * 4));
     a->xscale = reinterpret_cast<float *>(take((size_t)rows * 4));
     a->h = reinterpret_cast<float *>(take(pairs * m.hidden * 4));
-    a->count = reinterpret_cast<int *>(take((size_t)m.n_experts * 4));
+    a->count = reinterpret_cast<int *>(take((size_t)m.n_experts * kApart * 4));
     a->list = reinterpret_cast<int *>(take((size_t)m.n_experts * rows * 4));
     if (!down_by_rows(m, rows)) {
         a->himg = reinterpret_cast<uint8_t *>(take(pairs * m.hidden * 4));
