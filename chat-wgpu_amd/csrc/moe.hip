@@ -16,7 +16,7 @@
 // What bounds it: the experts' weights from memory (128 of 2,048 x 768 are 340 MB with
 // their scales), which reading alone brings in at 6.3 TB/s.  Microseconds of the launches,
 // 8 of these 128 experts a row:
-//   1 row     scores 2.7, choice and up 8.8, down 8.6: launches' beginnings and ends
+//   1 row     scores 2.7, choice and up 8.8, down 8.1: launches' beginnings and ends
 //   48 rows   scores 5, choice 6, up 49 (44 at best), split 5, down 28, sum 5: up and
 //             down read at 4.3 TB/s (loads without products 40 and 23.5), the vector
 //             units, which decode and scale, 0.6 busy
@@ -897,13 +897,13 @@ __global__ __launch_bounds__(kRowThreads) void moe_up_row_kernel(MoeArgs a) {
     a.h[(size_t)rank * hidden + col + tid] = silu_mul(g * sc, u * sc);
 }
 
-// A workgroup of W waves has 16 columns of a row's y; its waves share the experts
-// out, or parts of them where there are fewer.  A stage is W's 16 rows of 8 blocks
-// and that stretch of h, which the wave splits itself under a power of two of the
-// stretch.
-template <int W, bool DMA>
-__global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
-    constexpr int J = 2, R = 3;
+// A workgroup has 16 columns of a row's y; its waves share the experts out, or parts of
+// them where there are fewer.  A stage is the columns' rows of W, 8 blocks of each, and
+// that stretch of h, which the wave splits itself under a power of two of the stretch.
+template <bool DMA>
+__global__ __launch_bounds__(kRowThreads) void moe_down_row_kernel(MoeArgs a) {
+    constexpr int W = kRowWaves, J = 2;
+    constexpr int R = 2;  // (with 3 one workgroup fits a CU: one row 8.6 us for 8.1, six 18.6 for 17.2)
     using S = Stage<J>;
     constexpr int BYTES = S::BYTES + 1024;  // h behind W
     __shared__ __attribute__((aligned(1024))) unsigned char ring[W * R * BYTES];
@@ -969,9 +969,8 @@ __global__ __launch_bounds__(W * 64) void moe_down_row_kernel(MoeArgs a) {
                 issue();
                 ++asked;
             }
-            // the stages behind this one may still be on their way
-            if (asked == 3) wait_vm<2 * (S::DMAS + 1)>();
-            else if (asked == 2) wait_vm<S::DMAS + 1>();
+            // the stage behind this one may still be on its way
+            if (asked == 2) wait_vm<S::DMAS + 1>();
             else wait_vm<0>();
             --asked;
             ve = *reinterpret_cast<const float4 *>(at + S::BYTES + (lane & 31) * 16);
@@ -1072,10 +1071,10 @@ int score_splits(const cw_moe &m, int rows) {
 
 // Whether the second product goes row by row, reading an expert again for each row
 // that chose it: that saves two launches and the passes over h and z, and pays while
-// few rows meet (us by rows and by tiles; 8 of 128 experts, 2048 x 768: 2 rows 33, 36;
-// 6 rows 46, 48; 8 rows 57, 53; 2 of 8, 4096 x 12288: 2 rows 102, 101; 8 rows 220, 147).
+// few rows meet (us by rows and by tiles; 8 of 128 experts, 2048 x 768: 2 rows 29, 36;
+// 8 rows 53, 53; 16 rows 78, 68; 2 of 8, 4096 x 12288: 2 rows 95, 98; 4 rows 131, 126).
 bool down_by_rows(const cw_moe &m, int rows) {
-    return rows == 1 || 5 * rows * m.top_k <= 2 * m.n_experts;
+    return rows == 1 || 2 * rows * m.top_k <= m.n_experts;
 }
 
 // Places of the workspace, each 256-byte aligned; with base null their size.
@@ -1106,12 +1105,8 @@ size_t lay_out(const cw_moe &m, int rows, char *base, MoeArgs *a) {
 
 int run_down_rows(cw_ctx *ctx, const MoeArgs &a) {
     const bool dma = whole_groups(a.m.hidden, a.m.down_scales);
-    const dim3 grid(a.m.dim / 16, a.rows);
-    if (a.rows == 1)
-        return launch(ctx, "moe_down", dma ? moe_down_row_kernel<8, true> : moe_down_row_kernel<8, false>,
-                      grid, dim3(512), 0, a);
-    return launch(ctx, "moe_down", dma ? moe_down_row_kernel<4, true> : moe_down_row_kernel<4, false>,
-                  grid, dim3(256), 0, a);
+    return launch(ctx, "moe_down", dma ? moe_down_row_kernel<true> : moe_down_row_kernel<false>,
+                  dim3(a.m.dim / 16, a.rows), dim3(kRowThreads), 0, a);
 }
 
 // How the waves of a workgroup divide a product: J groups of blocks of x each (0:
