@@ -448,9 +448,8 @@ __device__ __forceinline__ void multiply_stage(const StageLane<J> &l, const unsi
 // aligned: a lane of the 16 x 4 (W row, k group) loads block 4 s + group of its row,
 // and the lane groups hand each other their words (two swaps of lane halves, two of
 // rows of 16).
-template <int H>
 struct Step {
-    u32x4 q[4], x[H][4];
+    u32x4 q[4], x[4];
     uint2 d[4];
 };
 struct Operands {
@@ -458,10 +457,9 @@ struct Operands {
     const uint16_t *d[4];
 };
 
-// xo: where the lane's fragment begins in a block's image, 16 bytes a half
-template <int H>
+// xo: where the lane's fragment begins in a block's image
 __device__ __forceinline__ void load_step(const Operands &o, const uint8_t *img, size_t xo,
-                                          int nb, int s, Step<H> &f) {
+                                          int nb, int s, Step &f) {
     const int lane = threadIdx.x & 63, row = lane & 15, lg = lane >> 4;
     const int b = min(4 * s + lg, nb - 1);
 #pragma unroll
@@ -474,11 +472,8 @@ __device__ __forceinline__ void load_step(const Operands &o, const uint8_t *img,
         f.d[c] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
     }
 #pragma unroll
-    for (int h = 0; h < H; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            f.x[h][i] = *reinterpret_cast<const u32x4 *>(img + xo + (size_t)min(4 * s + i, nb - 1) * 128 +
-                                                         h * 16);
+    for (int i = 0; i < 4; ++i)
+        f.x[i] = *reinterpret_cast<const u32x4 *>(img + xo + (size_t)min(4 * s + i, nb - 1) * 128);
 }
 
 // Word w of the lane groups' blocks -> block i of word `group`.
@@ -490,8 +485,7 @@ __device__ __forceinline__ u32x4 exchange(u32x4 q) {
     return u32x4{c[0], d[0], c[1], d[1]};
 }
 
-template <int H>
-__device__ __forceinline__ void multiply_step(const Step<H> &f, f32x4 (&acc)[4]) {
+__device__ __forceinline__ void multiply_step(const Step &f, f32x4 (&acc)[4]) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const u32x4 w = exchange(f.q[c]);
@@ -500,9 +494,7 @@ __device__ __forceinline__ void multiply_step(const Step<H> &f, f32x4 (&acc)[4])
             const f16x8 b = nibbles(w[i]);
             const f16x2 d2 = __builtin_bit_cast(f16x2, i < 2 ? f.d[c].x : f.d[c].y);
             const float d = (float)d2[i & 1];
-            f32x4 t = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int h = 0; h < H; ++h) t = mfma16(__builtin_bit_cast(f16x8, f.x[h][i]), b, t);
+            const f32x4 t = mfma16(__builtin_bit_cast(f16x8, f.x[i]), b, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[c][r] = __builtin_fmaf(d, t[r], acc[c][r]);
         }
@@ -510,13 +502,12 @@ __device__ __forceinline__ void multiply_step(const Step<H> &f, f32x4 (&acc)[4])
 }
 
 // acc += the products of steps s, s + by, ...: two steps' loads in flight.
-template <int H>
 __device__ __forceinline__ void multiply_steps(const Operands &o, const uint8_t *img,
                                                size_t xo, int nb, int s, int by,
                                                f32x4 (&acc)[4]) {
     const int n = (nb + 3) / 4;
     if (s >= n) return;
-    Step<H> f[2];
+    Step f[2];
     load_step(o, img, xo, nb, s, f[0]);
     for (;; s += 2 * by) {
         load_step(o, img, xo, nb, min(s + by, n - 1), f[1]);
@@ -589,7 +580,6 @@ struct TileShape {
     // stages of SJ groups, SUBS of them a slice of x, R in LDS for each wave
     static constexpr int SJ = J == 3 ? 3 : 2, SUBS = J / SJ, R = J == 4 ? 3 : 2;
     static constexpr int RING = J ? WAVES * R * Stage<SJ>::BYTES : 16;
-    static constexpr int OCC = H == 2 && J == 0 ? 2 : 4;  // waves a SIMD that registers allow
 };
 
 // A tile of pairs times stretches of its expert's columns: of h (UP: 32 gate and the
@@ -600,7 +590,7 @@ struct TileShape {
 // 48 rows still take 45.7 and 47.1 us, 46.4 with one.)
 template <bool UP, int H, int J>
 __global__ __launch_bounds__((TileShape<H, J>::WAVES * 64))
-__attribute__((amdgpu_waves_per_eu(TileShape<H, J>::OCC, TileShape<H, J>::OCC)))
+__attribute__((amdgpu_waves_per_eu(4, 4)))
 void moe_tile_kernel(MoeArgs a, int ks, int groups) {
     using T = TileShape<H, J>;
     constexpr int SJ = T::SJ, SUBS = T::SUBS, R = T::R;
@@ -680,20 +670,19 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
     };
 
     if constexpr (J == 0) {
-        for (int g = 0; g < n_groups; ++g) {
-            Operands o;
+        static_assert(H == 1);
+        const int col = first_col(0);
+        Operands o;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int col = first_col(g);
-                const size_t w0 = ((size_t)tile.e * N + col + tile_row(col, c)) * nb;
-                o.q[c] = (!UP ? a.m.down_quants : c < 2 ? a.m.gate_quants : a.m.up_quants) + w0 * 16;
-                o.d[c] = (!UP ? a.m.down_scales : c < 2 ? a.m.gate_scales : a.m.up_scales) + w0;
-            }
-            f32x4 acc[4] = {};
-            multiply_steps<H>(o, img, xo, nb, wave % ks, ks, acc);
-            if (g == 0) put_scales();
-            store(g, acc);
+        for (int c = 0; c < 4; ++c) {
+            const size_t w0 = ((size_t)tile.e * N + col + tile_row(col, c)) * nb;
+            o.q[c] = (!UP ? a.m.down_quants : c < 2 ? a.m.gate_quants : a.m.up_quants) + w0 * 16;
+            o.d[c] = (!UP ? a.m.down_scales : c < 2 ? a.m.gate_scales : a.m.up_scales) + w0;
         }
+        f32x4 acc[4] = {};
+        multiply_steps(o, img, xo, nb, wave % ks, ks, acc);
+        put_scales();
+        store(0, acc);
     } else {
         unsigned char *const mine = ring + wave * R * S::BYTES;
         const StageLane<SJ> l = stage_lane<SJ>(lane, nb);
@@ -878,7 +867,7 @@ __global__ __launch_bounds__(kRowThreads) void moe_up_row_kernel(MoeArgs a) {
             o.d[c] = (c & 1 ? a.m.up_scales : a.m.gate_scales) + w0;
         }
         const size_t xo = lg * 32 + (li & 1) * 16;
-        multiply_steps<1>(o, a.ximg, xo, nb, wave, kRowWaves, acc);
+        multiply_steps(o, a.ximg, xo, nb, wave, kRowWaves, acc);
     }
     // every two rows are the row's hi and lo
     if (lane < 16) {
@@ -1115,12 +1104,10 @@ struct TilePlan {
     int J, ks, cs, groups, grid;
 };
 template <int H>
-TilePlan tile_plan(const cw_ctx *ctx, bool up, const cw_moe &m, int tiles) {
+TilePlan tile_plan(const cw_ctx *ctx, bool up, const cw_moe &m, bool dma, int tiles) {
     constexpr int W = 4 * H;
     const int nb = (up ? m.dim : m.hidden) / 32, sets = up ? m.hidden / 32 : (m.dim + 63) / 64;
-    const bool dma = up ? whole_groups(m.dim, m.gate_scales) && whole_groups(m.dim, m.up_scales)
-                        : whole_groups(m.hidden, m.down_scales);
-    TilePlan p{0, nb >= 64 ? 4 : nb >= 16 ? 2 : 1, 1, 1, 0};
+    TilePlan p{0, nb >= 64 ? 4 : nb >= 8 ? 2 : 1, 1, 1, 0};
     int rounds = 1;
     if (dma) {
         // 16 rows: x of all of the sum if that fits; then the most of the waves' and the
@@ -1149,21 +1136,28 @@ TilePlan tile_plan(const cw_ctx *ctx, bool up, const cw_moe &m, int tiles) {
     return p;
 }
 
-template <bool UP, int H>
-int launch_tiles(cw_ctx *ctx, const MoeArgs &a, int most, int tiles) {
-    const TilePlan p = tile_plan<H>(ctx, UP, a.m, tiles);
-    auto fn = p.J == 0 ? moe_tile_kernel<UP, H, 0> : moe_tile_kernel<UP, H, 2>;
-    if constexpr (H == 1) {
-        if (p.J == 3) fn = moe_tile_kernel<UP, H, 3>;
-        if (p.J == 4) fn = moe_tile_kernel<UP, H, 4>;
-    }
-    return launch(ctx, UP ? "moe_up" : "moe_down", fn, dim3(p.grid, most), dim3(64 * p.ks * p.cs), 0, a,
-                  p.ks, p.groups);
-}
-
+// Tiles of eight rows up to ten an expert, else of 16 (us with 8 and with 16; 8 of 128
+// experts, 2048 x 768: 7 rows an expert 113, 119; 10: 136, 138; 15: 171, 160; 31: 294,
+// 260; 2 of 8, 4096 x 12288: 8 rows 200, 212; 12: 258, 253; 40: 588, 564).  W that goes
+// through registers takes eight (with 16 of 31 an expert, 2080 x 800, up and down 214 +
+// 129 us for 197 + 116: two waves a SIMD instead of four).
 template <bool UP>
-int launch_product(cw_ctx *ctx, const MoeArgs &a, int h, int most, int tiles) {
-    return h == 1 ? launch_tiles<UP, 1>(ctx, a, most, tiles) : launch_tiles<UP, 2>(ctx, a, most, tiles);
+int launch_product(cw_ctx *ctx, const MoeArgs &a) {
+    const int E = a.m.n_experts, pairs = a.rows * a.m.top_k;
+    const bool dma = UP ? whole_groups(a.m.dim, a.m.gate_scales) && whole_groups(a.m.dim, a.m.up_scales)
+                        : whole_groups(a.m.hidden, a.m.down_scales);
+    const bool wide = dma && (pairs + E - 1) / E > 10;
+    // tiles at most, and how many to expect of rows that choose evenly
+    const int tile = wide ? 2 * kTile : kTile, most = std::min(pairs, E + pairs / tile);
+    const int tiles = std::min(pairs, std::max(E, pairs / tile));
+    const TilePlan p = wide ? tile_plan<2>(ctx, UP, a.m, dma, tiles) : tile_plan<1>(ctx, UP, a.m, dma, tiles);
+    return launch(ctx, UP ? "moe_up" : "moe_down",
+                  wide       ? moe_tile_kernel<UP, 2, 2>
+                  : p.J == 0 ? moe_tile_kernel<UP, 1, 0>
+                  : p.J == 2 ? moe_tile_kernel<UP, 1, 2>
+                  : p.J == 3 ? moe_tile_kernel<UP, 1, 3>
+                             : moe_tile_kernel<UP, 1, 4>,
+                  dim3(p.grid, most), dim3(64 * p.ks * p.cs), 0, a, p.ks, p.groups);
 }
 
 int run(cw_ctx *ctx, const MoeArgs &a) {
@@ -1175,20 +1169,13 @@ int run(cw_ctx *ctx, const MoeArgs &a) {
                       dim3(1 + K * (a.m.hidden / 16)), dim3(kRowThreads), 0, a));
         return run_down_rows(ctx, a);
     }
-    const int mean = (pairs + E - 1) / E;
-    // Tiles of eight rows up to ten an expert, else of 16 (us with 8 and with 16; 8 of 128
-    // experts, 2048 x 768: 7 rows an expert 113, 119; 10: 136, 138; 15: 171, 160; 31: 294,
-    // 260; 2 of 8, 4096 x 12288: 8 rows 200, 212; 12: 258, 253; 40: 588, 564).
-    const int h = mean <= 10 ? 1 : 2, tile = kTile * h;
     const int score = (E + 15) / 16 * ((a.rows + 15) / 16) * a.splits;
     CW_TRY(launch(ctx, "moe_score", moe_score_kernel, dim3(score + a.rows), dim3(256), 0, a));
     CW_TRY(launch(ctx, "moe_choose", moe_choose_kernel, dim3(a.rows), dim3(1024), 0, a));
-    // tiles at most, and how many to expect of rows that choose evenly
-    const int most = std::min(pairs, E + pairs / tile), tiles = std::min(pairs, std::max(E, pairs / tile));
-    CW_TRY(launch_product<true>(ctx, a, h, most, tiles));
+    CW_TRY(launch_product<true>(ctx, a));
     if (down_by_rows(a.m, a.rows)) return run_down_rows(ctx, a);
     CW_TRY(launch(ctx, "moe_split", moe_split_kernel, dim3(pairs), dim3(256), 0, a));
-    CW_TRY(launch_product<false>(ctx, a, h, most, tiles));
+    CW_TRY(launch_product<false>(ctx, a));
     return launch(ctx, "moe_sum", moe_sum_kernel, dim3((a.m.dim + 1023) / 1024, a.rows), dim3(256), 0, a);
 }
 
