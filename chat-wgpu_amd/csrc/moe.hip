@@ -375,24 +375,24 @@ __device__ __forceinline__ void dma4u(const void *base, uint32_t off, uint32_t l
                  : "memory");
 }
 
-// Asks for a stage: q and s point at the first row's first block, of which groups
-// [0, jn) exist (those behind re-read the last).
+// Asks for a stage: q and s point at the first row's first block, of which [0, n) exist
+// (for those behind the last one is read again).
 template <int J>
 __device__ __forceinline__ void issue_stage(const StageLane<J> &l, const uint8_t *q, const uint16_t *s,
-                                            int jn, uint32_t buf) {
+                                            int n, uint32_t buf) {
     constexpr int L = Stage<J>::LINE;
-    const bool whole = jn == J;  // (but for a row's last stage)
+    const bool whole = n == 4 * J;  // (but for a row's last stage)
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const int k = L == 8 ? j & 1 : 0, first = L == 8 ? j / 2 * 8 : j * 4;  // the line's first block
         uint32_t off = l.q[k] + 16 * l.block[k];
-        if (!whole) off = l.q[k] + 16 * min(l.block[k], max(4 * jn - first, 4) - 1);
-        dma16u(q + 16 * (whole ? first : min(first, 4 * jn - 4)), off, buf + j * 1024);
+        if (!whole) off = l.q[k] + 16 * min(l.block[k], n - 1 - min(first, n - 1));
+        dma16u(q + 16 * (whole ? first : min(first, n - 1)), off, buf + j * 1024);
     }
 #pragma unroll
     for (int t = 0; t < (J > 2 ? 2 : 1); ++t) {
         uint32_t off = l.s[t] + 4 * l.word[t];
-        if (!whole) off = l.s[t] + 4 * min(l.word[t], 2 * jn - 1);
+        if (!whole) off = l.s[t] + 4 * min(l.word[t], (n - 1) / 2);
         dma4u(s, off, buf + Stage<J>::Q + 256 * t);
     }
 }
@@ -444,8 +444,7 @@ __device__ __forceinline__ void multiply_stage(const StageLane<J> &l, const unsi
     asm volatile("" : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]));
 }
 
-// Rows that are no whole groups of four blocks, or whose scales are not 8-byte
-// aligned: a lane of the 16 x 4 (W row, k group) loads block 4 s + group of its row,
+// Rows of an odd number of blocks, or whose scales are not 4-byte aligned: a lane of the 16 x 4 (W row, k group) loads block 4 s + group of its row,
 // and the lane groups hand each other their words (two swaps of lane halves, two of
 // rows of 16).
 struct Step {
@@ -717,7 +716,7 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
             }
             const int c = k / SUBS % 4, sub = k % SUBS;
             // (past the row's end its last group again)
-            const int skip = min(sub * SJ, nb / 4 - 1 - ib), n = min(SJ, nb / 4 - ib - skip);
+            const int skip = min(sub * SJ, (nb + 3) / 4 - 1 - ib), n = min(4 * SJ, nb - 4 * (ib + skip));
             const uint32_t at = tile_row(icol, c) * nb + 4 * skip;
             issue_stage<SJ>(l, (UP && c >= 2 ? q1 : q0) + 16 * (size_t)at, (UP && c >= 2 ? d1 : d0) + at, n,
                             lds + ibuf * S::BYTES);
@@ -799,7 +798,7 @@ __global__ __launch_bounds__(256) void moe_split_kernel(MoeArgs a) {
 
 constexpr int kRowThreads = 512, kRowWaves = kRowThreads / 64;
 
-// DMA: the row's blocks are whole groups of four, scales 8-byte aligned
+// DMA: rows of an even number of blocks, scales 4-byte aligned
 template <bool DMA>
 __global__ __launch_bounds__(kRowThreads) void moe_up_row_kernel(MoeArgs a) {
     constexpr int J = 2, R = 2;  // (with 4 one workgroup fits a CU: 12.6 us for 384 of them)
@@ -837,7 +836,7 @@ __global__ __launch_bounds__(kRowThreads) void moe_up_row_kernel(MoeArgs a) {
         auto issue = [&](int k) {  // gate, up of the wave's k / 2th slice
             const int b = (wave + k / 2 * kRowWaves) * 4 * J;
             issue_stage<J>(l, (k & 1 ? a.m.up_quants : a.m.gate_quants) + (w0 + b) * 16,
-                           (k & 1 ? a.m.up_scales : a.m.gate_scales) + w0 + b, min(J, (nb - b) / 4),
+                           (k & 1 ? a.m.up_scales : a.m.gate_scales) + w0 + b, min(4 * J, nb - b),
                            lds + k % R * S::BYTES);
         };
         for (int k = 0; k < R && k < total; ++k) issue(k);
@@ -915,6 +914,7 @@ __global__ __launch_bounds__(kRowThreads) void moe_down_row_kernel(MoeArgs a) {
     auto begin = [&](int u) { return u % parts * per; };
     auto end = [&](int u) { return min(steps, u % parts * per + per); };
     int iu = wave, is = begin(wave), ibuf = 0;  // the next stage to ask for
+    auto blocks = [&](int u, int s) { return min(4 * min(J, end(u) - s), nb - 4 * s); };  // of a stage
     auto skip = [&](int &u, int &s) {  // to the next unit that has steps
         while (u < K * parts && s >= end(u)) {
             u += W;
@@ -926,12 +926,12 @@ __global__ __launch_bounds__(kRowThreads) void moe_down_row_kernel(MoeArgs a) {
         const int j = iu / parts, e = __builtin_amdgcn_readlane(my_id, j);
         const size_t w0 = ((size_t)e * dim + col) * nb + 4 * is;
         const uint32_t buf = lds + ibuf * BYTES;
-        const int jn = min(J, end(iu) - is);
+        const int n = blocks(iu, is);
         if constexpr (DMA) {
-            issue_stage<J>(l, a.m.down_quants + w0 * 16, a.m.down_scales + w0, jn, buf);
+            issue_stage<J>(l, a.m.down_quants + w0 * 16, a.m.down_scales + w0, n, buf);
             const float *h = a.h + ((size_t)r * K + j) * hidden + 128 * is;
             // lane: chunk lane % 32 (block, group), its first or its second four elements
-            dma16u(h, (32 * min(lane >> 2 & 7, 4 * jn - 1) + 4 * (lane & 3) + (lane >> 5) * 16) * 4,
+            dma16u(h, (32 * min(lane >> 2 & 7, n - 1) + 4 * (lane & 3) + (lane >> 5) * 16) * 4,
                    buf + S::BYTES);
         }
         ibuf = ibuf + 1 == R ? 0 : ibuf + 1;
@@ -964,7 +964,7 @@ __global__ __launch_bounds__(kRowThreads) void moe_down_row_kernel(MoeArgs a) {
             --asked;
             ve = *reinterpret_cast<const float4 *>(at + S::BYTES + (lane & 31) * 16);
             vf = *reinterpret_cast<const float4 *>(at + S::BYTES + 512 + (lane & 31) * 16);
-            if ((lane & 31) >= 16 * jn) ve = vf = make_float4(0.f, 0.f, 0.f, 0.f);
+            if ((lane & 31) >= 4 * blocks(u, s)) ve = vf = make_float4(0.f, 0.f, 0.f, 0.f);
         } else {
             const int e = __builtin_amdgcn_readlane(my_id, j);
             const size_t w0 = ((size_t)e * dim + col + li) * nb;
@@ -1050,8 +1050,8 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-// Rows of whole groups of four blocks, their scales 8-byte aligned
-bool whole_groups(int in_f, const uint16_t *s) { return in_f % 128 == 0 && ((uintptr_t)s & 7) == 0; }
+// Rows whose scales a DMA takes two at a time: an even number of blocks, 4-byte aligned
+bool in_stages(int in_f, const uint16_t *s) { return in_f % 64 == 0 && ((uintptr_t)s & 3) == 0; }
 
 // Workgroups that share a score's sum, 64 elements a wave at least
 int score_splits(const cw_moe &m, int rows) {
@@ -1093,7 +1093,7 @@ size_t lay_out(const cw_moe &m, int rows, char *base, MoeArgs *a) {
 }
 
 int run_down_rows(cw_ctx *ctx, const MoeArgs &a) {
-    const bool dma = whole_groups(a.m.hidden, a.m.down_scales);
+    const bool dma = in_stages(a.m.hidden, a.m.down_scales);
     return launch(ctx, "moe_down", dma ? moe_down_row_kernel<true> : moe_down_row_kernel<false>,
                   dim3(a.m.dim / 16, a.rows), dim3(kRowThreads), 0, a);
 }
@@ -1144,8 +1144,8 @@ TilePlan tile_plan(const cw_ctx *ctx, bool up, const cw_moe &m, bool dma, int ti
 template <bool UP>
 int launch_product(cw_ctx *ctx, const MoeArgs &a) {
     const int E = a.m.n_experts, pairs = a.rows * a.m.top_k;
-    const bool dma = UP ? whole_groups(a.m.dim, a.m.gate_scales) && whole_groups(a.m.dim, a.m.up_scales)
-                        : whole_groups(a.m.hidden, a.m.down_scales);
+    const bool dma = UP ? in_stages(a.m.dim, a.m.gate_scales) && in_stages(a.m.dim, a.m.up_scales)
+                        : in_stages(a.m.hidden, a.m.down_scales);
     const bool wide = dma && (pairs + E - 1) / E > 10;
     // tiles at most, and how many to expect of rows that choose evenly
     const int tile = wide ? 2 * kTile : kTile, most = std::min(pairs, E + pairs / tile);
@@ -1163,7 +1163,7 @@ int launch_product(cw_ctx *ctx, const MoeArgs &a) {
 int run(cw_ctx *ctx, const MoeArgs &a) {
     const int E = a.m.n_experts, K = a.m.top_k, pairs = a.rows * K;
     if (a.rows == 1) {
-        const bool dma = whole_groups(a.m.dim, a.m.gate_scales) && whole_groups(a.m.dim, a.m.up_scales);
+        const bool dma = in_stages(a.m.dim, a.m.gate_scales) && in_stages(a.m.dim, a.m.up_scales);
         CW_TRY(launch(ctx, "moe_score", moe_score_row_kernel, dim3(E + 1), dim3(256), 0, a));
         CW_TRY(launch(ctx, "moe_up", dma ? moe_up_row_kernel<true> : moe_up_row_kernel<false>,
                       dim3(1 + K * (a.m.hidden / 16)), dim3(kRowThreads), 0, a));

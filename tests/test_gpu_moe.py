@@ -164,6 +164,17 @@ def test_scales_at_any_address(ctx, rng, rows, shift):
     m.check(x, m.run(x))
 
 
+@pytest.mark.parametrize("shift", [0, 1, 2])
+@pytest.mark.parametrize("dim,hidden", [(320, 448), (1984, 832), (64, 192), (1600, 2112)])
+@pytest.mark.parametrize("rows,n,k", [(1, 9, 2), (2, 24, 5), (23, 6, 2), (90, 5, 2)])
+def test_rows_of_an_even_number_of_blocks(ctx, rng, rows, n, k, dim, hidden, shift):
+    """Rows that end within a group of four blocks, by every kernel; the last
+    expert's last blocks are the last of their arrays."""
+    m = Layer(ctx, rng, dim, hidden, n, k, shift=shift)
+    x = rng.standard_normal((rows, dim)).astype(np.float32)
+    m.check(x, m.run(x))
+
+
 @pytest.mark.parametrize("rows", [1, 6, 30, 170])
 def test_large_and_small_values(ctx, rng, rows):
     """Rows of very different sizes, and elements far below their row's largest."""
