@@ -1051,6 +1051,8 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // Rows whose scales a DMA takes two at a time: an even number of blocks, 4-byte aligned
+// (2112 x 832, 4 of 64 experts: 20 rows' up and down 30 + 16 us through the stages, 55 +
+// 26 through registers; 500 rows 154 + 58, 216 + 125).
 bool in_stages(int in_f, const uint16_t *s) { return in_f % 64 == 0 && ((uintptr_t)s & 3) == 0; }
 
 // Workgroups that share a score's sum, 64 elements a wave at least
