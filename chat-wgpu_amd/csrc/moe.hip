@@ -70,8 +70,12 @@ __device__ __forceinline__ void split8(float4 ve, float4 vf, float sc, u32x4 *hi
     const float v[8] = {ve.x, ve.z, vf.x, vf.z, ve.y, ve.w, vf.y, vf.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const float f = (k & 1) ? sc : 16.0f * sc;
-        const float t0 = v[2 * k] * f, t1 = v[2 * k + 1] * f;  // exact: powers of two
+        // (sc first: it goes up to 2^126, and 16 sc would be infinite)
+        float t0 = v[2 * k] * sc, t1 = v[2 * k + 1] * sc;
+        if (!(k & 1)) {
+            t0 *= 16.0f;
+            t1 *= 16.0f;
+        }
         const f16x2 h = {(_Float16)t0, (_Float16)t1};
         const f16x2 l = {(_Float16)(t0 - (float)h.x), (_Float16)(t1 - (float)h.y)};
         (*hi)[k] = __builtin_bit_cast(uint32_t, h);
