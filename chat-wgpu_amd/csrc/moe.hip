@@ -601,8 +601,9 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
     using S = Stage<SJ>;
     __shared__ __attribute__((aligned(1024))) unsigned char ring[T::RING];
     __shared__ f32x4 red[T::WAVES][4][32 * H];
-    __shared__ int pairs[T::ROWS];
-    __shared__ float scales[T::ROWS];
+    // the tile's pairs, the scales of their rows and (down) the experts' shares in them
+    __shared__ int pairs[64];
+    __shared__ float scales[64], shares[UP ? 1 : 64];
     const Tile tile = find_tile(a, T::ROWS, blockIdx.y);
     if (tile.n == 0) return;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -623,13 +624,15 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
     // the tile's end read nothing)
     const int row = H == 1 ? li >> 1 : li, row_pair = pair_of(tile, row);
     const size_t xo = (size_t)(UP ? row_pair / K : row_pair) * nb * 128 + lg * 32 + (H == 1 ? (li & 1) * 16 : 0);
-    const int my_pair = pair_of(tile, min(tid, T::ROWS - 1));
-    const float my_scale = kUnscale * (UP ? a.xscale[my_pair / K] : a.p[my_pair] * a.hscale[my_pair]);
-    auto put_scales = [&] {
-        if (tid >= T::ROWS) return;
-        pairs[tid] = my_pair;
-        scales[tid] = my_scale;
-    };
+    // (by DMA: values of its own to be stored once x is there would cost every thread
+    // registers through the products)
+    if (wave == 0) {
+        const int pair = pair_of(tile, lane);
+        auto at = [](void *p) { return lds_off(static_cast<unsigned char *>(p)); };
+        dma4u(tile.list, min(lane, tile.n - 1) * 4, at(pairs));
+        dma4u(UP ? a.xscale : a.hscale, (UP ? pair / K : pair) * 4, at(scales));
+        if constexpr (!UP) dma4u(a.p, pair * 4, at(shares));
+    }
 
     // A group's sums from the waves that share them, to h or z.  Eight rows: a lane's
     // elements are hi and lo of rows 2 lg and 2 lg + 1, of 16 rows 4 lg to 4 lg + 3.
@@ -665,9 +668,10 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
             for (int e = 0; e < P; ++e) {
                 if (i + e >= tile.n) break;
                 const size_t at = (size_t)pairs[i + e] * N + col;
-                const float scale = scales[i + e];
+                const float scale = kUnscale * scales[i + e];
                 if constexpr (UP) a.h[at] = silu_mul(v[e] * scale, u[e] * scale);
-                else a.z[at] = v[e] * scale;
+                // (the scale last: p times a small one would be below f32's normal range)
+                else a.z[at] = v[e] * shares[i + e] * scale;
             }
         }
     };
@@ -684,7 +688,7 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
         }
         f32x4 acc[4] = {};
         multiply_steps(o, img, xo, nb, wave % ks, ks, acc);
-        put_scales();
+        wait_vm<0>();  // the scales
         store(0, acc);
     } else {
         unsigned char *const mine = ring + wave * R * S::BYTES;
@@ -755,9 +759,8 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
                         for (int k = 0; k < R - 1; ++k) issue(k);
                     }
                     // here, or the compiler waits for x, and so for every stage that is on
-                    // its way, before each stage
+                    // its way, before each stage (and for the scales)
                     wait_vm<0>();
-                    if (g + t == 0) put_scales();
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c)

@@ -41,3 +41,15 @@ def test_rows_of_small_values(ctx, rng, rows, size, dim, hidden):
     check_small(m, x, m.run(x))
     res = rng.standard_normal((rows, dim)).astype(np.float32)
     check_small(m, x, m.run(x, res), res)
+
+
+@pytest.mark.parametrize("hidden", [128, 96])
+@pytest.mark.parametrize("rows,n", [(1, 500), (40, 500), (100, 500), (300, 70)])
+def test_small_rows_under_small_weights(ctx, rng, rows, n, hidden):
+    """h near f32's lower end, large matrices behind it, and p of 1 / n."""
+    m = Layer(ctx, rng, 64, hidden, n, 3, normalise=False)
+    m.down = so.q4(rng, n, 64, hidden, scale=90.0)
+    m.upload()
+    for size in (-56, -60, -62):
+        x = (rng.standard_normal((rows, 64)) * 2.0**size).astype(np.float32)
+        check_small(m, x, m.run(x))
