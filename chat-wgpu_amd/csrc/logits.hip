@@ -298,7 +298,8 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
     if (lane == 0) {
-        top.s = s + (float)(same > 1 ? same - 1 : 0);
+        // (m - m: of two infinities the difference is NaN, here as in join)
+        top.s = same > 1 ? s + ((float)(same - 1) + (m - m)) : s;
         tops[wave] = top;
     }
     __syncthreads();

@@ -396,8 +396,9 @@ typedef struct cw_logit_rules {
  * at[i] (NULL: i).  In this order: repeat, frequency, presence, bias, -inf where
  * not allowed, each rounded to f32.  out (NULL: not wanted; it may be logits with
  * the same stride) receives them, token[i] the index of the largest (the lowest
- * among equal ones; NaN is never it), logprob[i] its log softmax; where all are
- * -inf or NaN CW_NO_TOKEN and -inf (NULL: not wanted).  Logits that are not
+ * among equal ones; NaN is never it), logprob[i] its log softmax (NaN beside a NaN
+ * or a second +inf); where all are -inf or NaN CW_NO_TOKEN and -inf (NULL: not
+ * wanted).  Logits that are not
  * allowed do not reach the others.  A row of no request is padding: nothing of it
  * is written.  Of the batch first_row, n_seq, rows and the mask are used.  vocab
  * at most 2^24, rows at most 65535. */

@@ -2,8 +2,11 @@
 import numpy as np
 import pytest
 
+import cw
 import step_oracle as so
+from test_gpu_logits import Step
 from test_gpu_moe import Layer
+from test_gpu_paged import i32
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +56,33 @@ def test_small_rows_under_small_weights(ctx, rng, rows, n, hidden):
     for size in (-56, -60, -62):
         x = (rng.standard_normal((rows, 64)) * 2.0**size).astype(np.float32)
         check_small(m, x, m.run(x))
+
+
+# ------------------------------------------------------------------ logits
+
+@pytest.mark.parametrize("vocab", [70, 4000, 5001, 40000, 700000])
+def test_more_than_one_infinity(ctx, rng, vocab):
+    """Two logits of infinity have no log softmax, wherever they lie."""
+    at = [(3, 5), (0, 1), (2, 66), (vocab - 1, vocab - 2), (1, vocab - 1), (7, 8, 9), (vocab // 2, vocab // 2 + 4),
+          (vocab - 3,)]
+    for one in range(2):  # all rows, and each alone (slices of another size)
+        s = Step(ctx, rng, vocab, [1] * len(at), 4, nodes=False, penalties=False)
+        s.rules = cw.logit_rules()
+        x = rng.standard_normal((len(at), vocab)).astype(np.float32)
+        for i, a in enumerate(at):
+            x[i, list(a)] = np.inf
+        runs = [s.run(x[i:i + 1], rows=[i]) for i in range(len(at))] if one else [s.run(x)]
+        token, logprob = (np.concatenate([r[k] for r in runs]) for k in (1, 2))
+        assert token.tolist() == [min(a) for a in at]
+        assert np.all(np.isnan(logprob[:-1])) and logprob[-1] == 0.0
+
+
+def test_infinities_that_a_bias_makes(ctx, rng):
+    vocab = 6000
+    s = Step(ctx, rng, vocab, [1] * 3, 4, nodes=False, penalties=False, bias=2)
+    s.bias_first, s.bias_token = i32([0, 2, 4, 6]), i32([8, 10, 8, 5000, 7, 8])
+    s.bias = np.array([np.inf, np.inf, np.inf, np.inf, np.inf, 1.0], np.float32)
+    s.upload()
+    x = rng.standard_normal((3, vocab)).astype(np.float32)
+    _, token, logprob = s.run(x)
+    assert token.tolist() == [8, 8, 7] and np.all(np.isnan(logprob[:2])) and logprob[2] == 0.0
