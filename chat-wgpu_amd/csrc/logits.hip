@@ -166,9 +166,9 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
         if (a.part && tid == 0) a.part[row * a.parts + blockIdx.x].i = kPadding;
         return;
     }
-    const float repeat = rule(a.r.repeat, b, 1.0f), presence = rule(a.r.presence, b, 0.0f);
-    const float frequency = rule(a.r.frequency, b, 0.0f);
-    const bool penal = repeat != 1.0f || presence != 0.0f || frequency != 0.0f;
+    const float given = rule(a.r.repeat, b, 1.0f);
+    const float presence = rule(a.r.presence, b, 0.0f), frequency = rule(a.r.frequency, b, 0.0f);
+    const bool penal = given != 1.0f || presence != 0.0f || frequency != 0.0f;
     const int len = a.r.tokens && penal ? min(max(a.r.length[b], 0), a.r.max_len) : 0;
     const int prompt = rule(a.r.prompt, b, 0);
     const int r0 = a.first_row[b], nodes = a.first_row[b + 1] - r0, self = br - r0;
@@ -210,8 +210,12 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
 
     // Where a wave has tokens that were seen, all its logits go through their rules: under
     // a branch each, waves with some would take it for nearly every logit.  With inv the
-    // nearest to 1 / repeat, v inv and one step after it are v / repeat to its last bit;
-    // infinities and zeros have no step.
+    // nearest to 1 / repeat, v inv and one step after it are v / repeat to its last bit, as
+    // long as the remainder, 2^-24 of v, is in f32's normal range (infinities and zeros have
+    // no step; of a quotient within two steps of f32's largest v inv may be infinite).
+    // 1 / repeat is finite from 2^-126 on (compared as whole numbers, by the scalar units;
+    // dividing where it is not, or waiting for repeat further up, cost every call 1 %).
+    const float repeat = __builtin_bit_cast(float, max(__builtin_bit_cast(int, given), 0x00800000));
     const float inv = 1.0f / repeat;
     float m = -INFINITY;
 #pragma unroll

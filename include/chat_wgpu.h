@@ -379,7 +379,8 @@ typedef struct cw_logit_rules {
     const int *tokens, *length, *prompt; /* [n_seq][max_len], [n_seq], [n_seq] (NULL: no prompt) */
     int max_len;
     const int *node_token;   /* [rows of the batch] */
-    const float *repeat;     /* [n_seq], positive: l / repeat (l > 0) or l * repeat of any token seen */
+    const float *repeat;     /* [n_seq]: l / repeat (l > 0) or l * repeat of any token seen; one
+                                below 2^-126 counts as that */
     const float *presence;   /* [n_seq]: off l of a generated token */
     const float *frequency;  /* [n_seq]: off l for each time that it was generated */
     const int *bias_first;   /* [n_seq+1]: request b's biases are entries bias_first[b] .. [b+1]-1 */

@@ -86,3 +86,33 @@ def test_infinities_that_a_bias_makes(ctx, rng):
     x = rng.standard_normal((3, vocab)).astype(np.float32)
     _, token, logprob = s.run(x)
     assert token.tolist() == [8, 8, 7] and np.all(np.isnan(logprob[:2])) and logprob[2] == 0.0
+
+
+@pytest.mark.parametrize("vocab", [1000, 30001])
+def test_repeat_penalties_of_any_size(ctx, rng, vocab):
+    """l / repeat and l * repeat as f32 has them, where the nearest of 1 / repeat has
+    lost bits too.  A step off where the quotient's remainder (2^-24 of l) or the result
+    is below f32's normal range.  One below 2^-126 counts as that."""
+    repeat = np.array([STEP, 2.0**-130, 3e-39, 2.0**-128, 0.0, -1.0, 2.0**-126, 1.3e-38, 1e-20, 0.7,
+                       1.3, 1e20, 2.0**126, 1e38, 3.4e38, np.finfo(np.float32).max], np.float32)
+    n = len(repeat)
+    s = Step(ctx, rng, vocab, [1] * n, 600, nodes=False)
+    s.tokens = i32(rng.integers(0, vocab, (n, 600)))
+    s.length[:] = 600
+    s.repeat, s.presence, s.frequency = repeat, None, None
+    s.upload()
+    x = (rng.standard_normal((n, vocab)) * 2.0 ** rng.integers(-149, 120, (n, vocab))).astype(np.float32)
+    x[:, ::7] = np.float32(2.0) ** rng.integers(-149, -20, x[:, ::7].shape)
+    x[:, 1::97], x[:, 2::97], x[:, 3::97], x[:, 4::97] = np.inf, -np.inf, 0.0, -0.0
+    got = s.run(x)[0]
+    repeat = np.maximum(repeat, np.float32(2.0**-126))
+    seen = np.zeros((n, vocab), bool)
+    np.put_along_axis(seen, s.tokens, True, 1)
+    with np.errstate(all="ignore"):
+        want = np.where(seen, np.where(x > 0, x / repeat[:, None], x * repeat[:, None]), x)
+        fine = np.isfinite(want)
+        assert np.array_equal(got[~fine], want[~fine], equal_nan=True)
+        normal = fine & (np.abs(want) >= 2.0**-126) & (np.abs(x) >= 2.0**-100)
+        assert np.array_equal(got[normal], want[normal])
+        off = np.abs(got.astype(np.float64) - want)
+        assert np.all(off[fine] <= np.spacing(np.abs(want[fine])))
