@@ -232,7 +232,8 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
                     const float q = v * inv, step = __builtin_fmaf(__builtin_fmaf(-q, repeat, v), inv, q);
                     const float less = step == step ? step : q;
                     v = c[j] ? (v > 0.0f ? less : v * repeat) : v;
-                    l[it * V + j] = __builtin_fmaf(made ? -frequency : 0.0f, (float)made, v) -
+                    // (0 added would make a -0 that no rule is for 0)
+                    l[it * V + j] = __builtin_fmaf(made ? -frequency : -0.0f, (float)made, v) -
                                     (made ? presence : 0.0f);
                 }
             }

@@ -116,3 +116,20 @@ def test_repeat_penalties_of_any_size(ctx, rng, vocab):
         assert np.array_equal(got[normal], want[normal])
         off = np.abs(got.astype(np.float64) - want)
         assert np.all(off[fine] <= np.spacing(np.abs(want[fine])))
+
+
+def test_zeros_keep_their_signs(ctx, rng):
+    """A logit that no rule is for comes out as it went in."""
+    vocab = 5000
+    s = Step(ctx, rng, vocab, [1, 1], 3000, nodes=False, bias=30)
+    s.tokens %= 1000
+    s.upload()
+    x = np.where(rng.random((2, vocab)) < 0.5, -0.0, 0.0).astype(np.float32)
+    got = s.run(x)[0]
+    free = np.ones((2, vocab), bool)
+    for b in range(2):
+        free[b, s.tokens[b, :s.length[b]]] = False
+        listed = s.bias_token[s.bias_first[b]:s.bias_first[b + 1]]
+        free[b, listed[(listed >= 0) & (listed < vocab)]] = False
+    assert free.sum() > 6000
+    assert np.array_equal(got.view(np.uint32)[free], x.view(np.uint32)[free])
