@@ -184,6 +184,10 @@ struct NormArgs {
     int q_heads;  // heads under q_gain; those behind them are keys
 };
 
+// Whether a sum of squares whose mean (with eps) this is has lost nothing to f32's ends:
+// heads of values past 2^60, or far below 1 without an eps to speak of, go through f64.
+__device__ __forceinline__ bool in_range(float mean) { return mean >= 0x1p-100f && mean <= 0x1p120f; }
+
 // y and the cache rows of head h: 8 elements, 4 from i0 on and 4 from i1
 template <typename KVT, bool CACHE, bool WIDE, bool STREAM>
 __device__ __forceinline__ void put_head(const RopeArgs &a, int r, int slot, int h, int i0, int i1,
@@ -253,11 +257,25 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeArgs a, Norm
             for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(x.v[j], x.v[j], ss);
             if (!on) ss = 0.0f;
             for (int d = 1; d < G; d <<= 1) ss += __shfl_xor(ss, d);
-            const float inv = 1.0f / sqrtf(ss / (float)a.hd + n.eps);
+            const float mean = ss / (float)a.hd + n.eps;
+            if (in_range(mean)) {
+                const float inv = 1.0f / sqrtf(mean);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x.v[j] *= inv;
+            } else {
+                double sum = 0.0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum = fma((double)x.v[j], (double)x.v[j], sum);
+                if (!on) sum = 0.0;
+                for (int d = 1; d < G; d <<= 1) sum += __shfl_xor(sum, d);
+                const double inv = 1.0 / sqrt(sum / a.hd + n.eps);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x.v[j] = (float)(x.v[j] * inv);
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                x.v[j] = x.v[j] * inv * gain[i0 + j];
-                x.v[4 + j] = x.v[4 + j] * inv * gain[i1 + j];
+                x.v[j] *= gain[i0 + j];
+                x.v[4 + j] *= gain[i1 + j];
             }
             if (rotates) {
 #pragma unroll
@@ -289,8 +307,19 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_any_kernel(RopeArgs a, 
     float ss = 0.0f;
     for (int i = lane; i < a.hd; i += 64) ss = __builtin_fmaf(src[i], src[i], ss);
     for (int d = 1; d < 64; d <<= 1) ss += __shfl_xor(ss, d);
-    const float inv = 1.0f / sqrtf(ss / (float)a.hd + n.eps);
-    auto get = [&](int i) { return normed ? src[i] * inv * gain[i] : src[i]; };
+    const float mean = ss / (float)a.hd + n.eps;
+    const bool fine = in_range(mean);
+    const float inv = 1.0f / sqrtf(mean);
+    double inv64 = 0.0;
+    if (!fine) {
+        double sum = 0.0;
+        for (int i = lane; i < a.hd; i += 64) sum = fma((double)src[i], (double)src[i], sum);
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+        inv64 = 1.0 / sqrt(sum / a.hd + n.eps);
+    }
+    auto get = [&](int i) {
+        return !normed ? src[i] : (fine ? src[i] * inv : (float)(src[i] * inv64)) * gain[i];
+    };
     auto put = [&](int i, float v) {
         if (h < a.heads) {
             a.y[(size_t)r * a.y_stride + (size_t)h * a.hd + i] = v;

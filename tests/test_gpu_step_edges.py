@@ -3,10 +3,12 @@ import numpy as np
 import pytest
 
 import cw
+import paged_oracle as po
 import step_oracle as so
 from test_gpu_logits import Step
 from test_gpu_moe import Layer
-from test_gpu_paged import i32
+from test_gpu_paged import KV, LAYOUT, i32
+from test_gpu_qk_norm import gains, shifted
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +135,43 @@ def test_zeros_keep_their_signs(ctx, rng):
         free[b, listed[(listed >= 0) & (listed < vocab)]] = False
     assert free.sum() > 6000
     assert np.array_equal(got.view(np.uint32)[free], x.view(np.uint32)[free])
+
+
+# ------------------------------------------------------------------ norms
+
+@pytest.mark.parametrize("hd,rot,layout,shift", [(128, 128, "halves", 0), (64, 32, "pairs", 0), (96, 96, "pairs", 1),
+                                                 (80, 20, "halves", 0), (256, 2, "halves", 0)])
+def test_norms_of_heads_of_any_size(ctx, rng, hd, rot, layout, shift):
+    """Heads whose squares are past f32's range on either side, each head another."""
+    sizes = [-147, -120, -100, -76, -62, -51, -30, 0, 30, 58, 61, 64, 90, 120]
+    heads, rows = len(sizes), 5
+    qg, kg = gains(rng, hd)
+    pos = i32(rng.integers(0, 9000, rows))
+    spec = cw.rope_spec(rot, 1e6, LAYOUT[layout])
+    x = np.ldexp(rng.standard_normal((rows, heads, hd)), np.array(sizes)[:, None]).astype(np.float32)
+    for eps in (0.0, 1e-38, 1e-30, 1e-6):
+        xd = shifted(ctx, x, shift)
+        got = ctx.qk_norm_rope_rows(spec, xd, shifted(ctx, qg, shift), None, ctx.storage(pos), rows, heads, 0, hd,
+                                    eps).download().reshape(x.shape)
+        ref, tol = so.norm_rope(x, np.tile(qg, (heads, 1)), np.float64(np.float32(eps)), pos,
+                                po.rope_freqs(rot, 1e6, "plain"), rot, layout == "pairs", 1.0)
+        # below f32's normal range: half a step for each of the pair's two by the root's factor, that
+        # times the gain (under 3), half by the gain, the products and the sum: 5 steps
+        assert np.all(np.abs(got - ref) <= tol + 8 * STEP), (eps, float((np.abs(got - ref) / (tol + 8 * STEP)).max()))
+
+
+@pytest.mark.parametrize("hd,rot", [(128, 128), (32, 6)])
+def test_norms_of_heads_of_any_size_into_a_cache(ctx, rng, hd, rot):
+    sizes = [-140, -80, -60, 0, 62, 110]
+    kvh, rows = len(sizes), 7
+    kv_type, dt = KV["f32"]
+    x = np.ldexp(rng.standard_normal((rows, 2 * kvh, hd)), np.array(sizes * 2)[:, None]).astype(np.float32)
+    kd, vd = (ctx.storage(np.zeros((rows, kvh, hd), dt)) for _ in range(2))
+    pos, kg = i32(rng.integers(0, 9000, rows)), gains(rng, hd)[1]
+    ctx.qk_norm_rope_kv_rows(cw.rope_spec(rot, 1e6), cw.kv_pages(kd, vd, kv_type, kvh, hd, rows, 1),
+                             ctx.storage(x), None, ctx.storage(kg), ctx.storage(pos),
+                             ctx.storage(i32(np.arange(rows))), rows, 0, 0.0)
+    ref, tol = so.norm_rope(x[:, :kvh], np.tile(kg, (kvh, 1)), 0.0, pos, po.rope_freqs(rot, 1e6, "plain"), rot,
+                            False, 1.0)
+    assert np.all(np.abs(kd.download() - ref) <= tol)
+    assert np.array_equal(vd.download(), x[:, kvh:])
