@@ -354,31 +354,6 @@ __device__ __forceinline__ StageLane<J> stage_lane(int lane, int nb) {
     return l;
 }
 
-// DMAs to an address in LDS (a number: of a pointer each would look whether it is null)
-// from a base that is the same in every lane, wherever the compiler has it: it
-// may come straight from a vector instruction, which the assembler's hazard rules
-// want five wait states after (and M0 one).
-template <typename T>
-__device__ __forceinline__ const T *uniform(const T *p) {
-    const uint64_t v = (uint64_t)(uintptr_t)p;
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-    const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
-    return reinterpret_cast<const T *>((uintptr_t)((uint64_t)hi << 32 | lo));
-}
-__device__ __forceinline__ void dma16u(const void *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :
-                 : "v"(off), "s"(uniform(static_cast<const char *>(base))), "{m0}"(lds)
-                 : "memory");
-}
-// 4 bytes a lane, at lds + 4 i
-__device__ __forceinline__ void dma4u(const void *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1"
-                 :
-                 : "v"(off), "s"(uniform(static_cast<const char *>(base))), "{m0}"(lds)
-                 : "memory");
-}
-
 // Asks for a stage: q and s point at the first row's first block, of which [0, n) exist
 // (for those behind the last one is read again).
 template <int J>

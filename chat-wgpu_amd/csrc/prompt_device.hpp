@@ -81,10 +81,39 @@ typedef __attribute__((address_space(3))) unsigned char lds_u8;
 __device__ __forceinline__ uint32_t lds_off(unsigned char *p) {
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_u8 *)p);
 }
+//
+// The compiler puts none of the wait states in front of an asm that the hardware wants:
+// one after a write of M0, five after a vector instruction's write (v_readfirstlane,
+// v_readlane) of a scalar register that the DMA reads.  dma16 has the one, for bases that
+// scalar instructions made (with five a prompt of 512 tokens took 0.8 % longer);
+// tests/test_lds_dma.py looks at the built kernels for others.
 __device__ __forceinline__ void dma16(const void *base, uint32_t off, unsigned char *lds_dst) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"  // (a wait state after M0's write)
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  :
                  : "v"(off), "s"(base), "{m0}"(lds_off(lds_dst))
+                 : "memory");
+}
+
+// DMAs to an address in LDS (a number: of a pointer each would look whether it is null)
+// from a base that is the same in every lane, wherever the compiler has it: 16 bytes a
+// lane at lds + 16 i, and 4 bytes at lds + 4 i.
+template <typename T>
+__device__ __forceinline__ const T *uniform(const T *p) {
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+    return reinterpret_cast<const T *>((uintptr_t)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ void dma16u(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(off), "s"(uniform(static_cast<const char *>(base))), "{m0}"(lds)
+                 : "memory");
+}
+__device__ __forceinline__ void dma4u(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1"
+                 :
+                 : "v"(off), "s"(uniform(static_cast<const char *>(base))), "{m0}"(lds)
                  : "memory");
 }
 

@@ -560,9 +560,10 @@ struct Tile {
 };
 
 // dma16 of lines that nobody reads again (non-temporal: 64 single rows at 4,000
-// positions 182 -> 165 us; where a second row block reads them it costs a tenth)
+// positions 182 -> 165 us; where a second row block reads them it costs a tenth), with
+// dma16's wait state
 __device__ __forceinline__ void dma16_once(const void *base, uint32_t off, unsigned char *lds_dst) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"  // (a wait state after M0's write)
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
                  :
                  : "v"(off), "s"(base), "{m0}"(lds_off(lds_dst))
                  : "memory");

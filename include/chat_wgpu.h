@@ -328,8 +328,9 @@ int cw_kv_accept(cw_ctx *ctx, const cw_kv_pages *kv, const cw_batch *b, const in
  * reference's QK-norm before its RoPE, qwen3.rs:160-165): every head of n_heads
  * query and then n_kv_heads key heads of a row becomes x * inverseSqrt(sum(x^2) /
  * head_dim + eps) * gain, gain [head_dim] q_gain or k_gain, and is rotated.
- * Heads whose squares leave f32's range are normalised in f64.  Padding rows, overlaps and in-place use as in cw_rope_rows; n_heads or
- * n_kv_heads may be 0 (its gain NULL). */
+ * Heads whose squares leave f32's range are normalised in f64.  Padding rows,
+ * overlaps and in-place use as in cw_rope_rows; n_heads or n_kv_heads may be 0 (its
+ * gain NULL). */
 int cw_qk_norm_rope_rows(cw_ctx *ctx, const cw_rope_spec *spec, const float *x, size_t x_stride,
                          const float *q_gain, const float *k_gain, float eps, const int *positions,
                          int rows, int n_heads, int n_kv_heads, int head_dim, float *y,
