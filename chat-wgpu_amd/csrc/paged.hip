@@ -83,12 +83,12 @@ __device__ __forceinline__ void put_unit(float *to, const float *from) {
         *reinterpret_cast<Vec<float, V> *>(to) = *reinterpret_cast<const Vec<float, V> *>(from);
 }
 
-// Workgroup (row, part of the heads).  A unit is V pairs (a thread reads V
+// Workgroup (row, `par` of the heads).  A unit is V pairs (a thread reads V
 // elements from either half, or 2 V in a row) or V copied elements; U units make
-// a head, `par` heads a round, and a thread keeps its unit's cosines for every
-// head it takes.  V = 4 where rows are 16-byte aligned, 1 where not.  STREAM: y
-// is written past the caches.  Bound by memory: 6,000 rows of 40 heads 43 us,
-// 5.6 TB/s read and written; few rows by the launch, 4 us.
+// a head, and a thread has one unit of one head.  V = 4 where rows are 16-byte
+// aligned, 1 where not.  STREAM: y is written past the caches.  Bound by memory:
+// 6,000 rows of 40 heads 43 us, 5.6 TB/s read and written; few rows by the
+// launch, 4 us.
 template <typename KVT, int V, bool PAIRS, bool CACHE, bool STREAM = false>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a, int U, int par) {
     const int r = blockIdx.x, pos = a.positions[r];
@@ -109,39 +109,39 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a, int U, 
     const bool write = CACHE && (unsigned)slot < (unsigned)a.n_slots;
     const int heads = write ? a.heads + 2 * a.kv_heads : a.heads;
     const float *row = a.x + (size_t)r * a.x_stride;
-    for (int h = blockIdx.y * par + tid / U; h < heads; h += gridDim.y * par) {
-        const bool q = h < a.heads, k = h < a.heads + a.kv_heads;
-        if (q && !rotates && !a.copy) continue;
-        const float *src = row + (size_t)h * a.hd;
-        Vec<float, 2 * V> x;
-        read_once<V>(x.v, src + i0);
-        if (rotates) {
-            read_once<V>(x.v + V, src + i1);
-            if (k) {
+    const int h = blockIdx.y * par + tid / U;
+    if (h >= heads) return;
+    const bool q = h < a.heads, k = h < a.heads + a.kv_heads;
+    if (q && !rotates && !a.copy) return;
+    const float *src = row + (size_t)h * a.hd;
+    Vec<float, 2 * V> x;
+    read_once<V>(x.v, src + i0);
+    if (rotates) {
+        read_once<V>(x.v + V, src + i1);
+        if (k) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    float &xa = x.v[PAIRS ? 2 * j : j], &xb = x.v[PAIRS ? 2 * j + 1 : V + j];
-                    const float ya = __builtin_fmaf(xa, cs[j].x, -(xb * cs[j].y));
-                    xb = __builtin_fmaf(xb, cs[j].x, xa * cs[j].y);
-                    xa = ya;
-                }
+            for (int j = 0; j < V; ++j) {
+                float &xa = x.v[PAIRS ? 2 * j : j], &xb = x.v[PAIRS ? 2 * j + 1 : V + j];
+                const float ya = __builtin_fmaf(xa, cs[j].x, -(xb * cs[j].y));
+                xb = __builtin_fmaf(xb, cs[j].x, xa * cs[j].y);
+                xa = ya;
             }
         }
-        if (q) {
-            float *dst = a.y + (size_t)r * a.y_stride + (size_t)h * a.hd;
-            put_unit<V, STREAM>(dst + i0, x.v);
-            if (rotates) put_unit<V, STREAM>(dst + i1, x.v + V);
-        } else if constexpr (CACHE) {
-            const int g = h - a.heads - (k ? 0 : a.kv_heads);
-            KVT *dst = static_cast<KVT *>(k ? a.kc : a.vc) +
-                       ((size_t)slot * a.kv_heads + g) * a.hd;
-            Vec<KVT, 2 * V> o;
+    }
+    if (q) {
+        float *dst = a.y + (size_t)r * a.y_stride + (size_t)h * a.hd;
+        put_unit<V, STREAM>(dst + i0, x.v);
+        if (rotates) put_unit<V, STREAM>(dst + i1, x.v + V);
+    } else if constexpr (CACHE) {
+        const int g = h - a.heads - (k ? 0 : a.kv_heads);
+        KVT *dst = static_cast<KVT *>(k ? a.kc : a.vc) +
+                   ((size_t)slot * a.kv_heads + g) * a.hd;
+        Vec<KVT, 2 * V> o;
 #pragma unroll
-            for (int j = 0; j < 2 * V; ++j) o.v[j] = (KVT)x.v[j];  // f16: to nearest even
-            using O = Vec<KVT, V>;
-            *reinterpret_cast<O *>(dst + i0) = *reinterpret_cast<O *>(o.v);
-            if (rotates) *reinterpret_cast<O *>(dst + i1) = *reinterpret_cast<O *>(o.v + V);
-        }
+        for (int j = 0; j < 2 * V; ++j) o.v[j] = (KVT)x.v[j];  // f16: to nearest even
+        using O = Vec<KVT, V>;
+        *reinterpret_cast<O *>(dst + i0) = *reinterpret_cast<O *>(o.v);
+        if (rotates) *reinterpret_cast<O *>(dst + i1) = *reinterpret_cast<O *>(o.v + V);
     }
 }
 
@@ -170,7 +170,7 @@ int launch_rope(cw_ctx *ctx, const char *label, const RopeArgs &a, bool wide, bo
 // factor is the head's, so a head's G lanes (a power of two, one for every eight
 // elements) hold it whole, add its squares up among themselves and rotate what
 // they hold.  A lane has four pairs (4 elements of either half, or 8 in a row), or
-// 8 elements behind rot, and keeps its angles for the heads it takes.
+// 8 elements behind rot, of one head; every head of a row makes the row's angles anew.
 //
 // What bounds it: memory, each value read and written once, and the vector units beside
 // it.  6,000 rows of 24 heads of 128 (147 MB) take 27 to 30 us, 4.9 to 5.5 TB/s, with
@@ -237,58 +237,58 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(RopeArgs a, Norm
     const bool write = CACHE && (unsigned)slot < (unsigned)a.n_slots;
     const int heads = write ? a.heads + 2 * a.kv_heads : a.heads;
     const float *row = a.x + (size_t)r * a.x_stride;
-    for (int h = blockIdx.y * par + tid / G; h < heads; h += gridDim.y * par) {
-        const float *src = row + (size_t)h * a.hd;
-        Vec<float, 8> x;
-        if constexpr (WIDE) {
-            read_once<4>(x.v, src + i0);
-            read_once<4>(x.v + 4, src + i1);
-        } else {
+    const int h = blockIdx.y * par + tid / G;
+    if (h >= heads) return;
+    const float *src = row + (size_t)h * a.hd;
+    Vec<float, 8> x;
+    if constexpr (WIDE) {
+        read_once<4>(x.v, src + i0);
+        read_once<4>(x.v + 4, src + i1);
+    } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x.v[j] = src[i0 + j];
-                x.v[4 + j] = src[i1 + j];
-            }
+        for (int j = 0; j < 4; ++j) {
+            x.v[j] = src[i0 + j];
+            x.v[4 + j] = src[i1 + j];
         }
-        if (h < a.heads + (CACHE ? a.kv_heads : 0)) {  // (values stay as they are)
-            const float *gain = h < n.q_heads ? n.q_gain : n.k_gain;
-            float ss = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(x.v[j], x.v[j], ss);
-            if (!on) ss = 0.0f;
-            for (int d = 1; d < G; d <<= 1) ss += __shfl_xor(ss, d);
-            const float mean = ss / (float)a.hd + n.eps;
-            if (in_range(mean)) {
-                const float inv = 1.0f / sqrtf(mean);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x.v[j] *= inv;
-            } else {
-                double sum = 0.0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum = fma((double)x.v[j], (double)x.v[j], sum);
-                if (!on) sum = 0.0;
-                for (int d = 1; d < G; d <<= 1) sum += __shfl_xor(sum, d);
-                const double inv = 1.0 / sqrt(sum / a.hd + n.eps);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x.v[j] = (float)(x.v[j] * inv);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x.v[j] *= gain[i0 + j];
-                x.v[4 + j] *= gain[i1 + j];
-            }
-            if (rotates) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float &xa = x.v[PAIRS ? 2 * j : j], &xb = x.v[PAIRS ? 2 * j + 1 : 4 + j];
-                    const float ya = __builtin_fmaf(xa, cs[j].x, -(xb * cs[j].y));
-                    xb = __builtin_fmaf(xb, cs[j].x, xa * cs[j].y);
-                    xa = ya;
-                }
-            }
-        }
-        if (on) put_head<KVT, CACHE, WIDE, STREAM>(a, r, slot, h, i0, i1, x.v);
     }
+    if (h < a.heads + (CACHE ? a.kv_heads : 0)) {  // (values stay as they are)
+        const float *gain = h < n.q_heads ? n.q_gain : n.k_gain;
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(x.v[j], x.v[j], ss);
+        if (!on) ss = 0.0f;
+        for (int d = 1; d < G; d <<= 1) ss += __shfl_xor(ss, d);
+        const float mean = ss / (float)a.hd + n.eps;
+        if (in_range(mean)) {
+            const float inv = 1.0f / sqrtf(mean);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x.v[j] *= inv;
+        } else {
+            double sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum = fma((double)x.v[j], (double)x.v[j], sum);
+            if (!on) sum = 0.0;
+            for (int d = 1; d < G; d <<= 1) sum += __shfl_xor(sum, d);
+            const double inv = 1.0 / sqrt(sum / a.hd + n.eps);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x.v[j] = (float)(x.v[j] * inv);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x.v[j] *= gain[i0 + j];
+            x.v[4 + j] *= gain[i1 + j];
+        }
+        if (rotates) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float &xa = x.v[PAIRS ? 2 * j : j], &xb = x.v[PAIRS ? 2 * j + 1 : 4 + j];
+                const float ya = __builtin_fmaf(xa, cs[j].x, -(xb * cs[j].y));
+                xb = __builtin_fmaf(xb, cs[j].x, xa * cs[j].y);
+                xa = ya;
+            }
+        }
+    }
+    if (on) put_head<KVT, CACHE, WIDE, STREAM>(a, r, slot, h, i0, i1, x.v);
 }
 
 // Heads or rotated parts that are no whole eighths: a wave a head, an element or a
