@@ -18,10 +18,10 @@
 // each other.  (max, s, index) of the slices are joined by a second launch in a fixed
 // order.
 //
-// What bounds it, at 151936 tokens: two launches for one row (5.3 + 2.8 us).  61 rows
-// after 4100 tokens take 19.4 us for 37 MB: vector units 0.67 busy, the counts 8 us of
-// the whole (each of the 38 slices reads the history).  48 rows with masks, biases and
-// out take 20.7 us for 59 MB.
+// What bounds it, at 151936 tokens: for one row the latencies of two launches, one behind
+// the other (5.3 + 2.8 us).  61 rows after 4100 tokens take 19 to 20 us for 37 MB: vector
+// units 0.70 busy, the counts 8 us of the whole (each of the 38 slices reads the history).
+// 48 rows with masks, biases and out take 20.7 us for 59 MB.
 
 #include "paged_device.hpp"
 #include "prompt_device.hpp"

@@ -16,12 +16,14 @@
 // What bounds it: the experts' weights from memory (128 of 2,048 x 768 are 340 MB with
 // their scales), which reading alone brings in at 6.3 TB/s.  Microseconds of the launches,
 // 8 of these 128 experts a row:
-//   1 row     scores 2.7, choice and up 8.8, down 8.1: launches' beginnings and ends
-//   48 rows   scores 5, choice 6, up 49 (44 at best), split 5, down 28, sum 5: up and
+//   1 row     scores 2.3, choice and up 9.0, down 8.2: launches' beginnings and ends
+//   48 rows   scores 5, choice 6, up 48 (44 at best), split 5, down 28, sum 5: up and
 //             down read at 4.3 TB/s (loads without products 40 and 23.5), the vector
-//             units, which decode and scale, 0.6 busy
-//   500 rows  scores 13, choice 7, up 139, split 8, down 99, sum 9: tiles of one
-//             expert decode its weights again; vector units 0.6, matrix cores 0.22 busy
+//             units, which decode and scale, 0.6 to 0.7 busy
+//   500 rows  scores 13, choice 7, up 129 to 138, split 8, down 94 to 101, sum 9: tiles of
+//             one expert decode its weights again; vector units 0.65, matrix cores 0.24 busy
+// More than kChunk rows go through in pieces that each read and decode every expert: 4,000
+// are four of 390 us.
 
 #include "prompt_device.hpp"
 
@@ -423,9 +425,9 @@ __device__ __forceinline__ void multiply_stage(const StageLane<J> &l, const unsi
     asm volatile("" : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]));
 }
 
-// Rows of an odd number of blocks, or whose scales are not 4-byte aligned: a lane of the 16 x 4 (W row, k group) loads block 4 s + group of its row,
-// and the lane groups hand each other their words (two swaps of lane halves, two of
-// rows of 16).
+// Rows of an odd number of blocks, or whose scales are not 4-byte aligned: a lane of the
+// 16 x 4 (W row, k group) loads block 4 s + group of its row, and the lane groups hand
+// each other their words (two swaps of lane halves, two of rows of 16).
 struct Step {
     u32x4 q[4], x[4];
     uint2 d[4];
@@ -551,7 +553,8 @@ __device__ __forceinline__ int pair_of(const Tile &t, int i) { return t.list[min
 
 // How a tile kernel of 8 H rows and J groups of blocks of x in a wave's registers (0:
 // through registers, any row length) is laid out.  16 rows decode W half as often, but
-// have 128 B of x for 64: eight waves share a sum where four do.
+// have 128 B of x for 64: eight waves share a sum where four do.  At four waves a SIMD the
+// products take 125 and 126 registers of 128, without scratch.
 template <int H, int J>
 struct TileShape {
     static constexpr int ROWS = kTile * H, WAVES = 4 * H;  // WAVES at most
@@ -598,7 +601,8 @@ void moe_tile_kernel(MoeArgs a, int ks, int groups) {
     // x rows of the lane's fragments, hi or lo of row li / 2 or both of row li (rows past
     // the tile's end read nothing)
     const int row = H == 1 ? li >> 1 : li, row_pair = pair_of(tile, row);
-    const size_t xo = (size_t)(UP ? row_pair / K : row_pair) * nb * 128 + lg * 32 + (H == 1 ? (li & 1) * 16 : 0);
+    const size_t xo = (size_t)(UP ? row_pair / K : row_pair) * nb * 128 + lg * 32 +
+                      (H == 1 ? (li & 1) * 16 : 0);
     // (by DMA: values of its own to be stored once x is there would cost every thread
     // registers through the products)
     if (wave == 0) {
@@ -1033,7 +1037,7 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs a) {
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // Rows whose scales a DMA takes two at a time: an even number of blocks, 4-byte aligned
-// (2112 x 832, 4 of 64 experts: 20 rows' up and down 30 + 16 us through the stages, 55 +
+// (2112 x 832, 4 of 64 experts: 20 rows' up and down 29 + 15 us through the stages, 55 +
 // 26 through registers; 500 rows 154 + 58, 216 + 125).
 bool in_stages(int in_f, const uint16_t *s) { return in_f % 64 == 0 && ((uintptr_t)s & 3) == 0; }
 

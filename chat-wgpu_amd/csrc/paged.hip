@@ -1,6 +1,6 @@
 // Several requests in one paged KV cache: rotary rows with and without the norm
-// of each head and the cache write, block tables from request lengths, the move of accepted rows.
-// The attention over that cache is tree_attention.hip's.
+// of each head and the cache write, block tables from request lengths, the move of
+// accepted rows.  The attention over that cache is tree_attention.hip's.
 
 #include <algorithm>
 #include <cmath>
@@ -173,10 +173,10 @@ int launch_rope(cw_ctx *ctx, const char *label, const RopeArgs &a, bool wide, bo
 // 8 elements behind rot, of one head; every head of a row makes the row's angles anew.
 //
 // What bounds it: memory, each value read and written once, and the vector units beside
-// it.  6,000 rows of 24 heads of 128 (147 MB) take 27 to 30 us, 4.9 to 5.5 TB/s, with
+// it.  6,000 rows of 24 heads of 128 (147 MB) take 26 to 30 us, 4.9 to 5.6 TB/s, with
 // the vector units busy throughout (angles in f64, norm, rotation); 4,100 rows of 32 + 2 x
-// 8 with the write into an f16 cache 34 us (185 MB, 5.4 TB/s); 32 to 48 rows one launch,
-// 3.6 us.
+// 8 with the write into an f16 cache 34 us (185 MB, 5.4 TB/s), into an f32 one 37 to 39
+// (202 MB, 5.2 to 5.5 TB/s); 32 to 48 rows one launch, 3.7 us.
 
 struct NormArgs {
     const float *q_gain, *k_gain;  // [hd]

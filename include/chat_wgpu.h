@@ -358,13 +358,16 @@ typedef struct cw_moe {
 /* y[r] = [residual[r] +] sum of p_e * Wdown_e (silu(Wgate_e x[r]) * (Wup_e x[r]))
  * over the top_k experts e of the largest router scores router[e] . x[r] (the
  * lower index among equal ones), p their softmax over all experts.  Scores are
- * f64, so that the choice does not hang on rounding; products are f32, as in
- * cw_q4_gemm (block scales finite; x 16-byte aligned).  experts and weights
- * [rows][top_k] receive the choice in order of score, and p (NULL: not wanted).
- * positions (NULL: none): a row of a negative position is padding: what it holds
- * does not count, and nothing of it is written.  y may be residual, else it overlaps
- * neither it nor x.  A row whose x is not finite gives NaN, and experts in range;
- * other rows are not touched by it.  rows at most 65536. */
+ * f64, so that the choice does not hang on rounding.  Sums are f32 (block scales
+ * finite; x 16-byte aligned); for the matrix cores x and the products silu(..) *
+ * (..) are held to 22 bits under a power of two a row: elements far below their
+ * row's largest to 2^-35 of that (of the latter's rows, where few rows meet an
+ * expert, 256 neighbours are a row).  experts and weights [rows][top_k] receive the
+ * choice in order of score, and p (NULL: not wanted).  positions (NULL: none): a
+ * row of a negative position is padding: what it holds does not count, and nothing
+ * of it is written.  y may be residual, else it overlaps neither it nor x.  A row
+ * whose x is not finite gives NaN, and experts in range; other rows are not touched
+ * by it.  rows at most 65536. */
 int cw_moe_rows(cw_ctx *ctx, const cw_moe *moe, const float *x, int rows, const int *positions,
                 const float *residual, float *y, int *experts, float *weights);
 
@@ -399,10 +402,9 @@ typedef struct cw_logit_rules {
  * the same stride) receives them, token[i] the index of the largest (the lowest
  * among equal ones; NaN is never it), logprob[i] its log softmax (NaN beside a NaN
  * or a second +inf); where all are -inf or NaN CW_NO_TOKEN and -inf (NULL: not
- * wanted).  Logits that are not
- * allowed do not reach the others.  A row of no request is padding: nothing of it
- * is written.  Of the batch first_row, n_seq, rows and the mask are used.  vocab
- * at most 2^24, rows at most 65535. */
+ * wanted).  Logits that are not allowed do not reach the others.  A row of no
+ * request is padding: nothing of it is written.  Of the batch first_row, n_seq, rows
+ * and the mask are used.  vocab at most 2^24, rows at most 65535. */
 int cw_logits_rows(cw_ctx *ctx, const cw_logit_rules *rules, const cw_batch *b, const int *at,
                    const float *logits, size_t stride, int rows, int vocab, float *out,
                    size_t out_stride, uint32_t *token, float *logprob);
